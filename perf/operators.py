@@ -190,9 +190,11 @@ def _plain_attend(s):
     row = torch.arange(t, device=x.device).repeat(g)
     sees = torch.arange(n, device=x.device)[None, None] <= (s["lengths"][:, None, None] - t + row[None, :, None])
     x.masked_fill_(~sees[:, None], float("-inf"))
-    x = torch.exp(x - x.amax(-1, keepdim=True))
+    most = x.amax(-1, keepdim=True)
+    x = torch.exp(x - most)
     total = x.sum(-1, keepdim=True)
     o = torch.matmul(x, v) / total
+    out["lse"] = (most + torch.log(total)).unflatten(2, (g, t)).permute(0, 3, 1, 2, 4).reshape(b, t, h * g)
     out["out"] = o.unflatten(2, (g, t)).permute(0, 3, 1, 2, 4).reshape(b, t, h * g, d).to(s["q"].dtype)
     if s["mass"] is not None:
         at = torch.arange(n, device=x.device)[None, None]
@@ -297,10 +299,11 @@ def prepare(case, seed):
         return s
     s["cache"] = _filled(case, made, n)
     if op == "attend":
-        s["out"] = {"out": torch.empty_like(made["q"])}
+        s["out"] = {"out": torch.empty_like(made["q"]), "lse": torch.empty(b, case["rows"], case["heads"], device="cuda")}
         if case["mass"]:
             s["out"]["mass"] = torch.zeros_like(made["mass"])
-        s["call"] = s["cache"].attention_call(made["q"], s["out"]["out"], made["lengths"], scale=d ** -0.5, mass_in=made["mass"], mass_out=s["out"].get("mass"))
+        s["call"] = s["cache"].attention_call(made["q"], s["out"]["out"], made["lengths"], scale=d ** -0.5, lse=s["out"]["lse"],
+                                               mass_in=made["mass"], mass_out=s["out"].get("mass"))
     else:
         keep = case["keep"]
         s["into"] = package().KV4Cache(b, h, d, keep)
@@ -348,7 +351,7 @@ def work(case):
         return {"bytes": sum(lengths) * h * 4 + kept * (2 * row + 8 * h + 2 * h * d * 2), "flops": sum(lengths) * h}
     t, heads = case["rows"], case["heads"]
     pairs = sum(t * n - t * (t - 1) // 2 for n in lengths)
-    moved = sum(lengths) * row + 2 * b * t * heads * d * size
+    moved = sum(lengths) * row + 2 * b * t * heads * d * size + b * t * heads * 4
     if case["mass"]:
         moved += sum(lengths) * h * 8
     return {"bytes": moved, "flops": 4 * pairs * heads * d}
@@ -409,7 +412,7 @@ def exact(case, seed):
         return out
     t, heads, h, d = case["rows"], case["heads"], case["kv_heads"], case["dim"]
     g = heads // h
-    out = {"out": torch.zeros(case["seqs"], t, heads, d, dtype=torch.float64, device="cuda")}
+    out = {"out": torch.zeros(case["seqs"], t, heads, d, dtype=torch.float64, device="cuda"), "lse": torch.zeros(case["seqs"], t, heads, dtype=torch.float64, device="cuda")}
     if case["mass"]:
         out["mass"] = torch.zeros(case["seqs"], h, case["length"], dtype=torch.float64, device="cuda")
     for i, n in enumerate(made["n"]):
@@ -419,7 +422,9 @@ def exact(case, seed):
             if case["mass"]:
                 out["mass"][i, j, :n - t] = made["mass"][i, j, :n - t].double()
             for u in range(j * g, j * g + g):
-                p = torch.softmax((made["q"][i, :, u].double() @ k.T / math.sqrt(d)).masked_fill(hidden, -math.inf), -1)
+                x = (made["q"][i, :, u].double() @ k.T / math.sqrt(d)).masked_fill(hidden, -math.inf)
+                out["lse"][i, :, u] = torch.logsumexp(x, -1)
+                p = torch.softmax(x, -1)
                 out["out"][i, :, u] = p @ v
                 if case["mass"]:
                     out["mass"][i, j, :n] += p.sum(0)
