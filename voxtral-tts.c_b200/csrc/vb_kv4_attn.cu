@@ -1,0 +1,684 @@
+/*
+ * vb_kv4_attn.cu - softmax attention over the 4-bit cache, and the weight that each of its tokens was given.
+ *
+ *   s_ij = scale q_i . k_j,  out_i = sum_j exp(s_ij - lse_i) v_j,  mass_j = sum_i exp(s_ij - lse_i)
+ *
+ * The codes are exact in FP16, so the products run on FP16 warp-level MMAs (m16n8k16), tokens along M, eight
+ * (row, query head) pairs of a KV head along N:
+ *   S^T [16 tokens x 8] += K Q^T    a block of 32 at a time, whose sum is multiplied by the token's scale in fp32
+ *   O^T [16 dims x 8]   += V^T P^T  values times 2^(e - E + 13), E the largest scale of the block column so far: exact in FP16 unless a
+ *                                   token's scale is under 2^-36 of the largest, where its values are rounded to 2^-38 of that
+ * Queries are brought to [2^14, 2^15) by a power of two a row (exact), then one FP16 term (bf16, fp16: exact down to 2^-29
+ * of a row's largest) or two (fp32: 22 bits and a sign). Weights are taken against a running reference that trails the maximum by
+ * at most 2^8, times 2^7, so that FP16 holds weights from 2^15 down to 2^-24 (2^-46 with the second term, as far as its exponent goes):
+ * one term for bf16 results (11 bits against the 8 of the result), two otherwise.
+ *
+ * A warp walks tiles of 32 tokens with a maximum, sums and accumulators of its own, through a ring of its own that bulk copies
+ * fill: no barrier between warps until the end. A sequence's tokens are split over CTAs where there are few of them; the CTA that
+ * comes last at a ticket joins the parts.
+ */
+#include <algorithm>
+
+#include "vb_serve.cuh"
+
+namespace vb {
+
+namespace {
+
+constexpr int kAWarps = 8, kAThreads = 32 * kAWarps, kACols = 8, kAKeys = 32;
+constexpr int kAStatus = 61;
+constexpr float kABias = 7.0f;                /* weights times 2^7 */
+
+template <int NB>
+struct ACfg {
+    static constexpr int kDim = NB * 32;
+    static constexpr int kCodes = kAKeys * NB * 16, kScales = kAKeys * NB;      /* bytes of a tile's plane */
+    static constexpr int kStage = 2 * (kCodes + kScales);
+    static constexpr int kStages = NB <= 4 ? 3 : 2;
+    static constexpr int kRing = kAWarps * kStages * kStage;
+    static constexpr int kMerge = kAWarps * kACols * (kDim + 2) * 4;
+    static constexpr int kBig = kRing > kMerge ? kRing : kMerge;
+    static constexpr bool kWhole = kv4_whole(NB);
+    static constexpr int kVScales = kWhole ? 1 : NB;                            /* scales of a lane's part of a value row */
+};
+
+struct AttnArgs {
+    Kv4 c;
+    const int *lengths, *rows;
+    int max_rows, heads, group, splits, wide;
+    float scale;
+    float *lse;
+    const float *mass_in;
+    float *mass_out;
+    float *part;
+    unsigned *tickets;
+    int *status;
+};
+
+VB_DEVINL void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b.x), "r"(b.y));
+}
+VB_DEVINL uint32_t mat_turn(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+VB_DEVINL uint32_t half_mul(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+VB_DEVINL uint32_t half_pack(float a, float b) { return serve_pack(a, b, (const __half *)nullptr); }
+VB_DEVINL float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+/* N bytes side by side (aligned to N's largest power of two) */
+template <int N>
+VB_DEVINL void get_bytes(const uint8_t *p, uint32_t (&b)[N]) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 4; i++) {
+            const uint32_t w = reinterpret_cast<const uint32_t *>(p)[i];
+#pragma unroll
+            for (int j = 0; j < 4; j++) b[4 * i + j] = (w >> (8 * j)) & 255u;
+        }
+    } else if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 2; i++) {
+            const uint32_t w = reinterpret_cast<const uint16_t *>(p)[i];
+            b[2 * i] = w & 255u;
+            b[2 * i + 1] = w >> 8;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) b[i] = p[i];
+    }
+}
+/* N words side by side (aligned to N's largest power of two, up to four) */
+template <int N>
+VB_DEVINL void get_words(const uint8_t *p, uint32_t (&w)[N]) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 4; i++) {
+            const uint4 v = reinterpret_cast<const uint4 *>(p)[i];
+            w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+        }
+    } else if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 2; i++) {
+            const uint2 v = reinterpret_cast<const uint2 *>(p)[i];
+            w[2 * i] = v.x; w[2 * i + 1] = v.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) w[i] = reinterpret_cast<const uint32_t *>(p)[i];
+    }
+}
+/* A lane's part of a value row, 2 NB bytes, as words (the last one's upper half zero where NB is odd) */
+template <int NB>
+VB_DEVINL void get_values(const uint8_t *p, uint32_t (&w)[(NB + 1) / 2]) {
+    if constexpr (NB % 2 == 0) {
+        get_words<NB / 2>(p, w);
+    } else {
+        const uint16_t *h = reinterpret_cast<const uint16_t *>(p);
+#pragma unroll
+        for (int i = 0; i < NB / 2; i++) w[i] = h[2 * i] | ((uint32_t)h[2 * i + 1] << 16);
+        w[NB / 2] = h[NB - 1];
+    }
+}
+
+/* Eight (row, head) pairs as the B operand of K Q^T, by one warp, into q_s [block][half][term][lane]; what S is to be multiplied by
+ * to be a power of two, a column each, into mul_s. */
+template <int NB, int QT, class T>
+VB_DEVINL void make_queries(const ServeRows<T> &q, const AttnArgs &a, int seq, int kv_head, int pair0, int pairs, uint2 *q_s, float *mul_s) {
+    const int lane = threadIdx.x & 31, n = lane >> 2, t = lane & 3, pair = pair0 + n;
+    const bool real = pair < pairs;
+    const int row = real ? pair / a.group : 0, head = kv_head * a.group + (real ? pair - row * a.group : 0);
+    const T *p = q.data + seq * q.seq + row * q.row + head * q.head + t * 8;
+    float x[NB][8];
+    uint32_t most = 0;
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[b][j] = 0.0f;
+        if (real) serve_load<8>(p + b * 32, a.wide, x[b]);
+    }
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) most = max(most, __float_as_uint(x[b][j]) & 0x7fffffffu);
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    /* the largest to [2^14, 2^15); rows of zeros, or with a value that is not finite, as they are */
+    const uint32_t e = most >> 23, field = e == 0u || e == 255u ? 127u : min(268u - e, 253u);
+    const float up = __uint_as_float(field << 23), down = __uint_as_float((254u - field) << 23);
+    if (t == 0) mul_s[n] = a.scale * 1.44269504f * down;
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            float y[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) y[j] = x[b][4 * h + j] * up;
+            uint2 w = make_uint2(half_pack(y[0], y[1]), half_pack(y[2], y[3]));
+            q_s[((b * 2 + h) * QT) * 32 + lane] = w;
+            if constexpr (QT == 2) {
+                const float2 f = kv4_f2(w.x), g = kv4_f2(w.y);
+                w = make_uint2(half_pack(y[0] - f.x, y[1] - f.y), half_pack(y[2] - g.x, y[3] - g.y));
+                q_s[((b * 2 + h) * QT + 1) * 32 + lane] = w;
+            }
+        }
+}
+
+/* Scores of 16 tokens: `at` words of the lane's two tokens (g and g + 8 of them), c: tokens g, g + 8 x columns 2 t, 2 t + 1. */
+template <int NB, int QT>
+VB_DEVINL void block_scores(float (&s)[4], const uint32_t wa, const uint32_t wb, float fa, float fb, const uint2 (&q)[2][QT]) {
+    uint32_t ra[4], rb[4];
+    kv4_halves(wa, ra);
+    kv4_halves(wb, rb);
+    float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int u = 0; u < QT; u++) mma_f16(c, ra[2 * h], rb[2 * h], ra[2 * h + 1], rb[2 * h + 1], q[h][u]);
+    s[0] = fmaf(c[0], fa, s[0]);
+    s[1] = fmaf(c[1], fa, s[1]);
+    s[2] = fmaf(c[2], fb, s[2]);
+    s[3] = fmaf(c[3], fb, s[3]);
+}
+
+/* grid = (row tiles x splits, kv heads, sequences) */
+template <int NB, int PT, class T>
+__global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(const AttnArgs a, const ServeRows<T> q, const ServeRows<T> out) {
+    using Cfg = ACfg<NB>;
+    constexpr int QT = sizeof(T) == 4 ? 2 : 1, kDim = Cfg::kDim, kW = (NB + 1) / 2, kVS = Cfg::kVScales;
+    extern __shared__ __align__(128) unsigned char a_smem[];
+    __shared__ __align__(8) uint64_t full[kAWarps][Cfg::kStages];
+    __shared__ __align__(16) uint2 q_s[NB * 2 * QT * 32];
+    __shared__ float mul_s[kACols];
+    __shared__ int abort_flag, is_last;
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int split = blockIdx.x % a.splits, tile_r = blockIdx.x / a.splits, kv_head = blockIdx.y, seq = blockIdx.z;
+    const Kv4Span span = kv4_span(a.lengths, a.rows, a.max_rows, seq, a.c.capacity);
+    const int pairs = span.rows * a.group, pair0 = tile_r * kACols;
+    if (pair0 >= pairs) return;
+    const int n_pairs = min(kACols, pairs - pair0);
+    const int before = span.length - span.rows;                      /* tokens before row 0 */
+    /* tokens that the tile's last row sees, in tiles; the share of this CTA is whole rounds of its warps */
+    const int seen = max(0, before + (pair0 + n_pairs - 1) / a.group + 1);
+    const int tiles = (seen + kAKeys - 1) / kAKeys;
+    int share = (tiles + a.splits - 1) / a.splits;
+    share = max(kAWarps, (share + kAWarps - 1) / kAWarps * kAWarps);
+    const int used = max(1, (tiles + share - 1) / share);
+    if (split >= used) return;
+    const int t_begin = split * share + warp, t_end = min(tiles, (split + 1) * share);
+
+    unsigned char *ring = a_smem + warp * Cfg::kStages * Cfg::kStage;
+    const size_t row0 = a.c.row(seq, kv_head, 0);
+    auto fetch = [&](int tile, int stage) {
+        unsigned char *to = ring + stage * Cfg::kStage;
+        const size_t row = row0 + (size_t)tile * kAKeys;
+        uint64_t *bar = &full[warp][stage];
+        vb_mbar_arrive_expect_tx(bar, Cfg::kStage);
+        vb_bulk_g2s(to, a.c.k + row * (NB * 16), Cfg::kCodes, bar);
+        vb_bulk_g2s(to + Cfg::kCodes, a.c.ks + row * NB, Cfg::kScales, bar);
+        vb_bulk_g2s(to + Cfg::kCodes + Cfg::kScales, a.c.v + row * (NB * 16), Cfg::kCodes, bar);
+        vb_bulk_g2s(to + 2 * Cfg::kCodes + Cfg::kScales, a.c.vs + row * NB, Cfg::kScales, bar);
+    };
+    if (lane == 0) {
+        for (int i = 0; i < Cfg::kStages; i++) vb_mbar_init(&full[warp][i], 1);
+        vb_mbar_init_fence();
+        for (int i = 0; i < Cfg::kStages; i++)
+            if (t_begin + i * kAWarps < t_end) fetch(t_begin + i * kAWarps, i);
+    }
+    if (tid == 0) abort_flag = 0;
+    if (warp == 0) make_queries<NB, QT>(q, a, seq, kv_head, pair0, pairs, q_s, mul_s);
+    __syncthreads();
+
+    /* columns 2 t and 2 t + 1 of this lane: tokens they see, what makes their scores powers of two */
+    int sees[2];
+    float mul[2];
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+        const int col = 2 * t + u;
+        sees[u] = before + (pair0 + min(col, n_pairs - 1)) / a.group + 1;      /* columns beyond the last pair are zeros and go nowhere */
+        mul[u] = mul_s[col];
+    }
+    const int all_see = before + pair0 / a.group + 1;                /* tokens that every column sees */
+
+    float ref[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+    float o[2 * NB][4];
+#pragma unroll
+    for (int i = 0; i < 2 * NB; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) o[i][j] = 0.0f;
+    int top_scale[kVS];
+#pragma unroll
+    for (int i = 0; i < kVS; i++) top_scale[i] = 0;
+
+    int stage = 0;
+    uint32_t parity = 0;
+    for (int tile = t_begin; tile < t_end; tile += kAWarps) {
+        if (!__all_sync(0xffffffffu, vb_mbar_wait(&full[warp][stage], parity, &abort_flag))) {
+            atomicCAS(a.status, 0, kAStatus);
+            *(volatile int *)&abort_flag = 1;
+            /* what is on its way lands before the memory is used for something else */
+            volatile int stay = 0;
+            for (int i = 0; i < Cfg::kStages && tile + i * kAWarps < t_end; i++) {
+                vb_mbar_wait(&full[warp][stage], parity, &stay);
+                if (++stage == Cfg::kStages) { stage = 0; parity ^= 1u; }
+            }
+            break;
+        }
+        const unsigned char *ks = ring + stage * Cfg::kStage, *kss = ks + Cfg::kCodes, *vs = kss + Cfg::kScales, *vss = vs + Cfg::kCodes;
+        const int j0 = tile * kAKeys;
+
+        /* scores */
+        float s[2][4];
+        {
+            uint32_t w[2][2][NB], f[2][2][NB];
+#pragma unroll
+            for (int m = 0; m < 2; m++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const int key = m * 16 + u * 8 + g;
+                    get_words<NB>(ks + key * (NB * 16) + t * (NB * 4), w[m][u]);
+                    get_bytes<NB>(kss + key * NB, f[m][u]);
+                }
+#pragma unroll
+            for (int m = 0; m < 2; m++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) s[m][j] = 0.0f;
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                uint2 qf[2][QT];
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int u = 0; u < QT; u++) qf[h][u] = q_s[((b * 2 + h) * QT + u) * 32 + lane];
+#pragma unroll
+                for (int m = 0; m < 2; m++)
+                    block_scores<NB, QT>(s[m], w[m][0][b], w[m][1][b], __uint_as_float(f[m][0][b] << 23), __uint_as_float(f[m][1][b] << 23), qf);
+            }
+        }
+        const bool masked = j0 + kAKeys > all_see;
+        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                s[m][j] *= mul[j & 1];
+                if (masked && j0 + m * 16 + (j >> 1) * 8 + g >= sees[j & 1]) s[m][j] = -INFINITY;
+                top[j & 1] = fmaxf(top[j & 1], s[m][j]);
+            }
+        if (__any_sync(0xffffffffu, top[0] > ref[0] + 8.0f || top[1] > ref[1] + 8.0f)) {
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], x));
+                if (top[u] > ref[u] + 8.0f) {
+                    const float fall = exp2_fast(ref[u] - top[u]);      /* the first time: 0 */
+                    ref[u] = top[u];
+                    sum[u] *= fall;
+#pragma unroll
+                    for (int i = 0; i < 2 * NB; i++) {
+                        o[i][u] *= fall;
+                        o[i][2 + u] *= fall;
+                    }
+                }
+            }
+        }
+        /* weights, turned into the B operand of V^T P^T */
+        uint2 p[2][PT];
+        const float low0 = ref[0] > -INFINITY ? ref[0] - kABias : 0.0f, low1 = ref[1] > -INFINITY ? ref[1] - kABias : 0.0f;
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+            float e[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) e[j] = exp2_fast(s[m][j] - ((j & 1) ? low1 : low0));
+            sum[0] += e[0] + e[2];
+            sum[1] += e[1] + e[3];
+            const uint32_t h0 = half_pack(e[0], e[1]), h1 = half_pack(e[2], e[3]);
+            p[m][0] = make_uint2(mat_turn(h0), mat_turn(h1));
+            if constexpr (PT == 2) {
+                const float2 f0 = kv4_f2(h0), f1 = kv4_f2(h1);
+                p[m][1] = make_uint2(mat_turn(half_pack(e[0] - f0.x, e[1] - f0.y)), mat_turn(half_pack(e[2] - f1.x, e[3] - f1.y)));
+            }
+        }
+
+        /* values: tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of each 16 */
+        uint32_t vsc[2][4][kVS];
+        int most[kVS];
+#pragma unroll
+        for (int i = 0; i < kVS; i++) most[i] = 0;
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const int key = m * 16 + (x >> 1) * 8 + 2 * t + (x & 1);
+                if constexpr (Cfg::kWhole) vsc[m][x][0] = vss[key * NB + g * NB / 8];
+                else get_bytes<kVS>(vss + key * NB, vsc[m][x]);
+#pragma unroll
+                for (int i = 0; i < kVS; i++) {
+                    if (masked && j0 + key >= seen) vsc[m][x][i] = 0;        /* whatever lies behind the last token */
+                    most[i] = max(most[i], (int)vsc[m][x][i]);
+                }
+            }
+        bool rise = false;
+#pragma unroll
+        for (int i = 0; i < kVS; i++) rise |= most[i] > top_scale[i];
+        if (__any_sync(0xffffffffu, rise)) {
+#pragma unroll
+            for (int i = 0; i < kVS; i++) {
+                most[i] = max(most[i], __shfl_xor_sync(0xffffffffu, most[i], 1));
+                most[i] = max(most[i], __shfl_xor_sync(0xffffffffu, most[i], 2));
+                if (__any_sync(0xffffffffu, most[i] == 255)) {
+                    /* a block that is NaN: so are the columns that see it; its codes are zeros */
+                    int bad = 1 << 30;
+                    most[i] = 0;
+#pragma unroll
+                    for (int m = 0; m < 2; m++)
+#pragma unroll
+                        for (int x = 0; x < 4; x++) {
+                            if (vsc[m][x][i] == 255u) {
+                                bad = min(bad, j0 + m * 16 + (x >> 1) * 8 + 2 * t + (x & 1));
+                                vsc[m][x][i] = 0;
+                            }
+                            most[i] = max(most[i], (int)vsc[m][x][i]);
+                        }
+#pragma unroll
+                    for (int x = 1; x < 4; x <<= 1) {
+                        bad = min(bad, __shfl_xor_sync(0xffffffffu, bad, x));
+                        most[i] = max(most[i], __shfl_xor_sync(0xffffffffu, most[i], x));
+                    }
+#pragma unroll
+                    for (int r = 0; r < 2 * NB; r++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            if ((Cfg::kWhole || r / 2 == i) && bad < sees[j & 1]) o[r][j] = __uint_as_float(0x7fffffffu);
+                }
+                const int up = most[i] - top_scale[i];
+                if (up > 0) {
+                    const float fall = up > 126 ? 0.0f : __uint_as_float((uint32_t)(127 - up) << 23);
+                    top_scale[i] = most[i];
+#pragma unroll
+                    for (int r = 0; r < 2 * NB; r++)
+                        if (Cfg::kWhole || r / 2 == i) {
+#pragma unroll
+                            for (int j = 0; j < 4; j++) o[r][j] *= fall;
+                        }
+                }
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+            uint32_t f[2][kVS];
+#pragma unroll
+            for (int i = 0; i < kVS; i++)
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    const int lo = (int)vsc[m][2 * x][i] + 140 - top_scale[i], hi = (int)vsc[m][2 * x + 1][i] + 140 - top_scale[i];
+                    f[x][i] = half_pack(__uint_as_float((uint32_t)max(lo, 0) << 23), __uint_as_float((uint32_t)max(hi, 0) << 23));
+                }
+            uint32_t w[4][kW];
+#pragma unroll
+            for (int x = 0; x < 4; x++) get_values<NB>(vs + (m * 16 + (x >> 1) * 8 + 2 * t + (x & 1)) * (NB * 16) + g * (NB * 2), w[x]);
+#pragma unroll
+            for (int i = 0; i < kW; i++) {
+                uint32_t r[2][2][4];                    /* [token pair][value of the byte][byte]: the two tokens' values side by side */
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    const uint32_t wa = w[2 * x][i], wb = w[2 * x + 1][i];
+                    kv4_halves((wa & 0x0f0f0f0fu) | ((wb << 4) & 0xf0f0f0f0u), r[x][0]);
+                    kv4_halves(((wa >> 4) & 0x0f0f0f0fu) | (wb & 0xf0f0f0f0u), r[x][1]);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const int at = i * 4 + k, sc = Cfg::kWhole ? 0 : at / 2;
+                    if (at < 2 * NB) {
+                        const uint32_t a0 = half_mul(r[0][0][k], f[0][sc]), a1 = half_mul(r[0][1][k], f[0][sc]);
+                        const uint32_t a2 = half_mul(r[1][0][k], f[1][sc]), a3 = half_mul(r[1][1][k], f[1][sc]);
+#pragma unroll
+                        for (int u = 0; u < PT; u++) mma_f16(o[at], a0, a1, a2, a3, p[m][u]);
+                    }
+                }
+            }
+        }
+        __syncwarp();
+        if (lane == 0 && tile + Cfg::kStages * kAWarps < t_end) fetch(tile + Cfg::kStages * kAWarps, stage);
+        if (++stage == Cfg::kStages) { stage = 0; parity ^= 1u; }
+    }
+
+    /* the warps' parts together; sums and results lose the 2^15 that the weights may have */
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], x);
+        sum[u] *= 0x1p-15f;
+    }
+    __syncthreads();                                     /* every ring is empty */
+    float *mo = reinterpret_cast<float *>(a_smem), *mm = mo + kAWarps * kACols * kDim, *ml = mm + kAWarps * kACols;
+    if (g == 0)
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            mm[warp * kACols + 2 * t + u] = ref[u];
+            ml[warp * kACols + 2 * t + u] = sum[u];
+        }
+#pragma unroll
+    for (int i = 0; i < 2 * NB; i++) {
+        const int d = Cfg::kWhole ? g * (4 * NB) + 2 * i : 32 * (i / 2) + 4 * g + 2 * (i & 1);
+        const int e = top_scale[Cfg::kWhole ? 0 : i / 2] - 155;
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            float *to = mo + (warp * kACols + 2 * t + u) * kDim + d;
+            to[0] = ldexpf(o[i][u], e);
+            to[1] = ldexpf(o[i][2 + u], e);
+        }
+    }
+    __syncthreads();
+    const int unit = (seq * a.c.kv_heads + kv_head) * (gridDim.x / a.splits) + tile_r;
+    float *part = a.part + ((size_t)unit * a.splits + split) * kACols * (kDim + 2);
+    auto finish = [&](int col, int d, float value, float total, float reference) {
+        const int pair = pair0 + col, row = pair / a.group, head = kv_head * a.group + pair - row * a.group;
+        serve_put(out.data + seq * out.seq + row * out.row + head * out.head + d, total == 0.0f ? 0.0f : value / total);
+        if (d == 0 && a.lse)
+            a.lse[((size_t)seq * a.max_rows + row) * a.heads + head] = total == 0.0f ? -INFINITY : (reference + 8.0f + log2f(total)) * 0.69314718f;
+    };
+    for (int x = tid; x < n_pairs * kDim; x += kAThreads) {
+        const int col = x / kDim, d = x - col * kDim;
+        float reference = -INFINITY, value = 0.0f, total = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kAWarps; w++) reference = fmaxf(reference, mm[w * kACols + col]);
+#pragma unroll
+        for (int w = 0; w < kAWarps; w++) {
+            const float m = mm[w * kACols + col], f = m > -INFINITY ? exp2_fast(m - reference) : 0.0f;
+            const float l = ml[w * kACols + col];
+            total += l != 0.0f ? l * f : 0.0f;           /* NaN stays */
+            value += mo[(w * kACols + col) * kDim + d] * f;
+        }
+        if (used == 1) {
+            finish(col, d, value, total, reference);
+        } else {
+            part[col * (kDim + 2) + d] = value;
+            if (d == 0) {
+                part[col * (kDim + 2) + kDim] = reference;
+                part[col * (kDim + 2) + kDim + 1] = total;
+            }
+        }
+    }
+    if (used == 1) return;
+    /* the CTA that comes last joins the parts, in their order whoever that is */
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) {
+        is_last = atomicAdd(&a.tickets[unit], 1u) == (unsigned)used - 1u;
+        if (is_last) a.tickets[unit] = 0u;
+        __threadfence();
+    }
+    __syncthreads();
+    if (!is_last) return;
+    const float *parts = a.part + (size_t)unit * a.splits * kACols * (kDim + 2);
+    for (int x = tid; x < n_pairs * kDim; x += kAThreads) {
+        const int col = x / kDim, d = x - col * kDim;
+        float reference = -INFINITY, value = 0.0f, total = 0.0f;
+        for (int w = 0; w < used; w++) reference = fmaxf(reference, __ldcg(parts + (w * kACols + col) * (kDim + 2) + kDim));
+        for (int w = 0; w < used; w++) {
+            const float *pw = parts + (w * kACols + col) * (kDim + 2);
+            const float m = __ldcg(pw + kDim), f = m > -INFINITY ? exp2_fast(m - reference) : 0.0f, l = __ldcg(pw + kDim + 1);
+            total += l != 0.0f ? l * f : 0.0f;
+            value += __ldcg(pw + d) * f;
+        }
+        finish(col, d, value, total, reference);
+    }
+}
+
+/* mass_out of 256 tokens a CTA: the scores again, now that the rows' sums are known, with the rows in turn. No atomics. */
+template <int NB, class T>
+__global__ void __launch_bounds__(kAThreads) kv4_mass_kernel(const AttnArgs a, const ServeRows<T> q) {
+    constexpr int QT = sizeof(T) == 4 ? 2 : 1;
+    __shared__ __align__(16) uint2 q_s[NB * 2 * QT * 32];
+    __shared__ float mul_s[kACols], lse_s[kACols];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int kv_head = blockIdx.y, seq = blockIdx.z;
+    const Kv4Span span = kv4_span(a.lengths, a.rows, a.max_rows, seq, a.c.capacity);
+    const int pairs = span.rows * a.group, before = span.length - span.rows;
+    const int cta0 = blockIdx.x * kAWarps * kAKeys, j0 = cta0 + warp * kAKeys;
+    if (cta0 >= span.length) return;
+    uint32_t w[2][2][NB], f[2][2][NB];
+#pragma unroll
+    for (int m = 0; m < 2; m++)
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const size_t row = a.c.row(seq, kv_head, min(j0 + m * 16 + u * 8 + g, span.length - 1));
+            get_words<NB>(a.c.k + row * (NB * 16) + t * (NB * 4), w[m][u]);
+            get_bytes<NB>(a.c.ks + row * NB, f[m][u]);
+        }
+    float mass[2][2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
+    /* rows before this CTA's first token see none of its tokens */
+    const int first = max(0, cta0 - before) * a.group / kACols * kACols;
+    for (int pair0 = first; pair0 < pairs; pair0 += kACols) {
+        __syncthreads();
+        if (warp == 0) make_queries<NB, QT>(q, a, seq, kv_head, pair0, pairs, q_s, mul_s);
+        if (tid >= 32 && tid < 32 + kACols) {
+            const int pair = pair0 + tid - 32, row = pair / a.group;
+            const float lse = pair < pairs ? a.lse[((size_t)seq * a.max_rows + row) * a.heads + kv_head * a.group + pair - row * a.group] : 0.0f;
+            lse_s[tid - 32] = lse == -INFINITY ? INFINITY : lse * 1.44269504f;       /* a row without weights gives none */
+        }
+        __syncthreads();
+        float s[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            uint2 qf[2][QT];
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int u = 0; u < QT; u++) qf[h][u] = q_s[((b * 2 + h) * QT + u) * 32 + lane];
+#pragma unroll
+            for (int m = 0; m < 2; m++)
+                block_scores<NB, QT>(s[m], w[m][0][b], w[m][1][b], __uint_as_float(f[m][0][b] << 23), __uint_as_float(f[m][1][b] << 23), qf);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int col = 2 * t + u, pair = pair0 + col;
+            const int sees = pair < pairs ? before + pair / a.group + 1 : 0;
+            const float mul = mul_s[col], lse = lse_s[col];
+#pragma unroll
+            for (int m = 0; m < 2; m++)
+#pragma unroll
+                for (int r = 0; r < 2; r++)
+                    if (j0 + m * 16 + r * 8 + g < sees) mass[m][r] += exp2_fast(s[m][2 * r + u] * mul - lse);
+        }
+    }
+    const size_t base = ((size_t)seq * a.c.kv_heads + kv_head) * a.c.capacity;
+#pragma unroll
+    for (int m = 0; m < 2; m++)
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+            float v = mass[m][r];
+            v += __shfl_xor_sync(0xffffffffu, v, 1);
+            v += __shfl_xor_sync(0xffffffffu, v, 2);
+            const int j = j0 + m * 16 + r * 8 + g;
+            if (t == 0 && j < span.length) a.mass_out[base + j] = v + (a.mass_in && j < before ? a.mass_in[base + j] : 0.0f);
+        }
+}
+
+template <class T>
+constexpr int kWeightTerms = std::is_same<T, __nv_bfloat16>::value ? 1 : 2;
+
+template <int NB, class T>
+int attn_launch(const AttnArgs &args, const vb200_kv4_attention_t &v, const Kv4Work &work, cudaStream_t st) {
+    using Cfg = ACfg<NB>;
+    constexpr int PT = kWeightTerms<T>;
+    AttnArgs a = args;
+    const ServeRows<T> q = serve_rows<T>(v.q), out = serve_rows<T>(v.out);
+    a.wide = serve_wide(q);
+    if (a.max_rows > 0) {
+        /* as many splits as fill the GPU with what runs at once, none of them under a tile a warp */
+        const long long row_tiles = ((long long)a.max_rows * a.group + kACols - 1) / kACols;
+        const long long units = row_tiles * a.c.kv_heads * a.c.seqs, at_once = (long long)work.sm_count * (NB <= 4 ? 2 : 1);
+        const long long most = ((long long)a.c.capacity + kAKeys * kAWarps - 1) / (kAKeys * kAWarps);
+        a.splits = (int)std::max(1ll, std::min(at_once / units, most));
+        kv4_attn_kernel<NB, PT, T><<<dim3((unsigned)(row_tiles * a.splits), a.c.kv_heads, a.c.seqs), kAThreads, Cfg::kBig, st>>>(a, q, out);
+        if (serve_launched()) return -1;
+    }
+    if (a.mass_out) {
+        kv4_mass_kernel<NB, T><<<dim3((a.c.capacity + kAKeys * kAWarps - 1) / (kAKeys * kAWarps), a.c.kv_heads, a.c.seqs), kAThreads, 0, st>>>(a, q);
+        return serve_launched();
+    }
+    return 0;
+}
+
+#define VB_KV4_DIMS(blocks, call) \
+    switch (blocks) {             \
+    case 1: return call(1);       \
+    case 2: return call(2);       \
+    case 3: return call(3);       \
+    case 4: return call(4);       \
+    case 6: return call(6);       \
+    default: return call(8);      \
+    }
+
+template <class T>
+int attn_dims(const AttnArgs &a, const vb200_kv4_attention_t &v, const Kv4Work &w, cudaStream_t st) {
+#define VB_CALL(n) attn_launch<n, T>(a, v, w, st)
+    VB_KV4_DIMS(a.c.blocks, VB_CALL)
+#undef VB_CALL
+}
+
+/* Loads the kernels of a head size on the current device, and lets them have their shared memory. */
+template <int NB, class T>
+int attn_load() {
+    cudaFuncAttributes f;
+    return cudaFuncSetAttribute(kv4_attn_kernel<NB, kWeightTerms<T>, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, ACfg<NB>::kBig) == cudaSuccess &&
+                   cudaFuncGetAttributes(&f, kv4_mass_kernel<NB, T>) == cudaSuccess
+               ? 0
+               : -1;
+}
+
+} // namespace
+
+int kv4_attention_load(int blocks) {
+#define VB_CALL(n) (attn_load<n, float>() || attn_load<n, __nv_bfloat16>() || attn_load<n, __half>() ? serve_launched() | -1 : 0)
+    VB_KV4_DIMS(blocks, VB_CALL)
+#undef VB_CALL
+}
+
+int kv4_attention(const Kv4 &c, const Kv4Work &w, const vb200_kv4_attention_t &v, cudaStream_t st) {
+    AttnArgs a = {};
+    a.c = c;
+    a.lengths = v.lengths; a.rows = v.rows; a.max_rows = v.max_rows; a.heads = v.heads; a.group = v.heads / c.kv_heads;
+    a.scale = v.scale; a.lse = v.lse; a.mass_in = v.mass_in; a.mass_out = v.mass_out;
+    a.part = w.part; a.tickets = w.tickets; a.status = w.status;
+    if ((long long)a.max_rows * a.group > (1ll << 30)) return serve_fail("too many rows");
+    if (v.q.type == VB200_F32) return attn_dims<float>(a, v, w, st);
+    if (v.q.type == VB200_BF16) return attn_dims<__nv_bfloat16>(a, v, w, st);
+    return attn_dims<__half>(a, v, w, st);
+}
+
+} // namespace vb

@@ -1,0 +1,351 @@
+/*
+ * vb_logprobs.cu - log probabilities of given tokens, entropy and the largest alternatives out of rows of logits, in one pass.
+ *
+ *   m = max x,  l = sum e^(x - m),  w = sum e^(x - m) (x - m);  lse = m + log l,  entropy = log l - w / l
+ *
+ * Bound by the logits' bytes where there are many rows, by latency where there is one. A row is split over the CTAs of a cluster;
+ * a thread keeps m, l, w of what it reads, rescaled when its maximum rises. The largest values: a threshold that `top` values are known to reach (the
+ * top-th largest of the maxima that 32 groups of threads have in their first stretch) lets a few dozen values of a row through, which are
+ * collected and put in order at the end. Values are compared with their index below them, so all are different. Where more come through than
+ * the list holds (rising rows), a CTA finds its largest again by bisection, from memory: slower and as right.
+ */
+#include <algorithm>
+
+#include "vb_serve.cuh"
+
+namespace vb {
+
+namespace {
+
+constexpr int kLpThreads = 512, kLpWarps = kLpThreads / 32, kLpTop = 32, kLpList = 1024, kLpUnroll = 4, kLpMaxSplit = 8;
+
+struct LpArgs {
+    const void *x;
+    long long stride;
+    int rows, vocab, top;
+    const int *tokens;
+    float *logprobs, *entropy;
+    int *top_ids;
+    float *top_logprobs;
+};
+
+/* Order of values as order of unsigned numbers: NaN above all, -0 as 0; the earlier index is the larger of two that tie. */
+VB_DEVINL uint32_t lp_key(float v) {
+    if (v != v) return 0xffffffffu;
+    const uint32_t u = __float_as_uint(v + 0.0f);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+VB_DEVINL float lp_value(uint32_t key) {
+    return key == 0xffffffffu ? __uint_as_float(0x7fffffffu) : __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+VB_DEVINL uint64_t lp_rank(float v, int i) { return ((uint64_t)lp_key(v) << 32) | (uint32_t)~i; }
+
+struct LpSums {
+    float m, l, w;
+};
+/* b into a. A side that is empty, or nothing but -inf, adds nothing. */
+VB_DEVINL LpSums lp_join(LpSums a, LpSums b) {
+    if (b.l == 0.0f) return a;
+    if (a.l == 0.0f) return b;
+    const float m = fmaxf(a.m, b.m);
+    const float da = a.m - m, db = b.m - m, fa = __expf(da), fb = __expf(db);
+    LpSums r;
+    r.m = m;
+    r.l = a.l * fa + b.l * fb;
+    /* a side that vanishes takes its difference along: 0, not 0 * -inf */
+    r.w = (fa > 0.0f ? (a.w + a.l * da) * fa : 0.0f) + (fb > 0.0f ? (b.w + b.l * db) * fb : 0.0f);
+    return r;
+}
+
+template <class T>
+struct LpRead {
+    static constexpr int kEach = 16 / sizeof(T);
+    float v[kEach];
+    VB_DEVINL void load(const T *p) { serve_load<kEach>(p, true, v); }
+};
+
+template <class T>
+__global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpArgs a) {
+    constexpr int kEach = 16 / sizeof(T);
+    __shared__ uint64_t list[kLpList], best[kLpMaxSplit * kLpTop], group[32], threshold_s;
+    __shared__ LpSums warp_sums[kLpWarps], cta_sums[kLpMaxSplit];
+    __shared__ float token_s;
+    __shared__ int n_list, bad_s[kLpMaxSplit], counts[kLpMaxSplit];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    uint32_t split, splits;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(split));
+    asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(splits));
+    /* waited for before anything is sent to another CTA's shared memory: by then that CTA runs */
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    const int row = blockIdx.x / splits;
+    const T *x = static_cast<const T *>(a.x) + (long long)row * a.stride;
+    /* elements before the first 16-byte boundary, then whole vectors, then the rest; this CTA's share of the vectors */
+    const int head = min(a.vocab, (int)(((16 - ((uintptr_t)x & 15)) & 15) / sizeof(T)));
+    const int vectors = (a.vocab - head) / kEach, tail = head + vectors * kEach;
+    const int share = (vectors + splits - 1) / splits, v0 = min(vectors, (int)split * share), v1 = min(vectors, v0 + share);
+
+    if (tid == 0) { n_list = 0; threshold_s = 0; bad_s[0] = 0; }
+    __syncthreads();
+    LpSums sums = {-INFINITY, 0.0f, 0.0f};
+    uint64_t mine = 0;                        /* the largest of this thread's first stretch */
+    bool bad = false;                         /* NaN or +inf */
+    auto take = [&](float v) {
+        if (v > sums.m) {
+            if (v == INFINITY) { bad = true; return; }
+            const float d = sums.m - v, f = __expf(d);
+            sums.w = f > 0.0f ? (sums.w + sums.l * d) * f : 0.0f;
+            sums.l *= f;
+            sums.m = v;
+        }
+        if (v == -INFINITY) return;
+        if (v != v) { bad = true; return; }
+        const float d = v - sums.m, e = __expf(d);
+        sums.l += e;
+        sums.w = fmaf(e, d, sums.w);
+    };
+    float limit = -INFINITY;                  /* values from here on may be among the largest */
+    auto collect = [&](float v, int i) {
+        if (!(v < limit)) {
+            const uint64_t r = lp_rank(v, i);
+            if (r >= threshold_s) {
+                const int at = atomicAdd(&n_list, 1);
+                if (at < kLpList) list[at] = r;
+            }
+        }
+    };
+    const uint4 *xv = reinterpret_cast<const uint4 *>(x + head);
+    bool first = true;
+    for (int c0 = v0; c0 < v1 || first; c0 += kLpThreads * kLpUnroll) {
+        LpRead<T> r[kLpUnroll];
+#pragma unroll
+        for (int u = 0; u < kLpUnroll; u++) {
+            const int i = c0 + u * kLpThreads + tid;
+            if (i < v1) r[u].load(reinterpret_cast<const T *>(xv + i));
+        }
+        /* the elements around the vectors go with the first CTA's first stretch, one a thread */
+        float extra = 0.0f;
+        int extra_i = -1;
+        if (first && split == 0) {
+            if (tid < head) extra_i = tid;
+            else if (tid - head < a.vocab - tail) extra_i = tail + tid - head;
+            if (extra_i >= 0) extra = serve_get(x + extra_i);
+        }
+#pragma unroll
+        for (int u = 0; u < kLpUnroll; u++) {
+            const int i = c0 + u * kLpThreads + tid;
+            if (i < v1)
+#pragma unroll
+                for (int j = 0; j < kEach; j++) {
+                    take(r[u].v[j]);
+                    if (first && a.top) mine = max(mine, lp_rank(r[u].v[j], head + i * kEach + j));
+                }
+        }
+        if (extra_i >= 0) {
+            take(extra);
+            if (a.top) mine = max(mine, lp_rank(extra, extra_i));
+        }
+        if (a.top) {
+            if (first) {
+                uint64_t most = mine;
+#pragma unroll
+                for (int o = 8; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+                if ((lane & 15) == 0) group[warp * 2 + (lane >> 4)] = most;
+                __syncthreads();
+                if (warp == 0) {
+                    const uint64_t v = group[lane];
+                    int rank = 0;
+                    for (int o = 0; o < 32; o++) {
+                        const uint64_t w = group[o];
+                        rank += w > v || (w == v && o < lane);
+                    }
+                    if (rank == a.top - 1) threshold_s = v;
+                }
+                __syncthreads();
+                const uint64_t th = threshold_s;
+                limit = th == 0 ? -INFINITY : lp_value((uint32_t)(th >> 32));
+                if (limit != limit) limit = INFINITY;      /* the threshold is a NaN: only NaN reaches it */
+            }
+#pragma unroll
+            for (int u = 0; u < kLpUnroll; u++) {
+                const int i = c0 + u * kLpThreads + tid;
+                if (i < v1)
+#pragma unroll
+                    for (int j = 0; j < kEach; j++) collect(r[u].v[j], head + i * kEach + j);
+            }
+            if (extra_i >= 0) collect(extra, extra_i);
+        }
+        first = false;
+    }
+    /* this CTA's sums */
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const LpSums b = {__shfl_xor_sync(0xffffffffu, sums.m, o), __shfl_xor_sync(0xffffffffu, sums.l, o), __shfl_xor_sync(0xffffffffu, sums.w, o)};
+        sums = lane & o ? lp_join(b, sums) : lp_join(sums, b);
+    }
+    if (lane == 0) warp_sums[warp] = sums;
+    if (__any_sync(0xffffffffu, bad) && lane == 0) atomicOr(&bad_s[0], 1);
+    __syncthreads();
+    if (warp == 0) {
+        sums = lane < kLpWarps ? warp_sums[lane] : LpSums{-INFINITY, 0.0f, 0.0f};
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const LpSums b = {__shfl_xor_sync(0xffffffffu, sums.m, o), __shfl_xor_sync(0xffffffffu, sums.l, o), __shfl_xor_sync(0xffffffffu, sums.w, o)};
+            sums = lane & o ? lp_join(b, sums) : lp_join(sums, b);
+        }
+    }
+    /* this CTA's largest values, in order */
+    const int there = min(a.top, v1 - v0 > 0 || split == 0 ? (v1 - v0) * kEach + (split == 0 ? head + a.vocab - tail : 0) : 0);
+    if (a.top) {
+        int n = n_list;
+        if (n > kLpList) {
+            /* the largest rank that `there` of this CTA's values reach, a bit at a time; then those values alone */
+            uint64_t least = 0;
+            for (int bit = 63; bit >= 0; bit--) {
+                const uint64_t trial = least | (1ull << bit);
+                int reach = 0;
+                for (int i = v0 * kEach + tid; i < v1 * kEach; i += kLpThreads) reach += lp_rank(serve_get(x + head + i), head + i) >= trial;
+                if (split == 0) {
+                    if (tid < head) reach += lp_rank(serve_get(x + tid), tid) >= trial;
+                    else if (tid - head < a.vocab - tail) reach += lp_rank(serve_get(x + tail + tid - head), tail + tid - head) >= trial;
+                }
+                __syncthreads();
+                if (tid == 0) n_list = 0;
+                __syncthreads();
+                if (reach) atomicAdd(&n_list, reach);
+                __syncthreads();
+                if (n_list >= there) least = trial;
+            }
+            __syncthreads();
+            if (tid == 0) { n_list = 0; threshold_s = least; }
+            __syncthreads();
+            limit = -INFINITY;
+            for (int i = v0 * kEach + tid; i < v1 * kEach; i += kLpThreads) collect(serve_get(x + head + i), head + i);
+            if (split == 0) {
+                if (tid < head) collect(serve_get(x + tid), tid);
+                else if (tid - head < a.vocab - tail) collect(serve_get(x + tail + tid - head), tail + tid - head);
+            }
+            __syncthreads();
+            n = n_list;
+        }
+        for (int i = tid; i < n; i += kLpThreads) {
+            const uint64_t v = list[i];
+            int rank = 0;
+            for (int o = 0; o < n; o++) rank += list[o] > v;
+            if (rank < there) best[rank] = v;
+        }
+    }
+    __syncthreads();
+    /* to the cluster's first CTA */
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    if (splits > 1) {
+        if (split != 0) {
+            uint32_t to;
+            if (tid < there) {
+                asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"(vb_smem_u32(&best[split * kLpTop + tid])));
+                asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to), "l"(best[tid]) : "memory");
+            }
+            if (tid == 0) {
+                asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"(vb_smem_u32(&cta_sums[split])));
+                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(sums.m) : "memory");
+                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4), "f"(sums.l) : "memory");
+                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 8), "f"(sums.w) : "memory");
+                asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"(vb_smem_u32(&bad_s[split])));
+                asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to), "r"(bad_s[0]) : "memory");
+                asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"(vb_smem_u32(&counts[split])));
+                asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to), "r"(there) : "memory");
+            }
+        }
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (split != 0) return;
+    }
+    if (tid == 0) {
+        counts[0] = there;
+        int wrong = bad_s[0];
+        for (uint32_t c = 1; c < splits; c++) {
+            sums = lp_join(sums, cta_sums[c]);
+            wrong |= bad_s[c];
+        }
+        const float log_l = logf(sums.l);                       /* -inf for a row of nothing but -inf */
+        const float nan = __uint_as_float(0x7fffffffu);
+        const int token = a.tokens ? a.tokens[row] : -1;
+        if (a.logprobs) {
+            const bool known = token >= 0 && token < a.vocab;
+            const float v = known ? serve_get(x + token) : nan;
+            a.logprobs[row] = wrong || !known ? nan : sums.l == 0.0f ? -INFINITY : (v - sums.m) - log_l;
+        }
+        if (a.entropy) a.entropy[row] = wrong ? nan : sums.l == 0.0f ? 0.0f : log_l - sums.w / sums.l;
+        cta_sums[0] = sums;
+        token_s = wrong ? nan : log_l;
+    }
+    __syncthreads();
+    if (!a.top) return;
+    const float m = cta_sums[0].m, log_l = token_s;
+    for (int i = tid; i < (int)splits * kLpTop; i += kLpThreads) {
+        const int c = i / kLpTop, k = i - c * kLpTop;
+        if (k >= counts[c]) continue;
+        const uint64_t v = best[i];
+        int rank = k;
+        for (int o = 0; o < (int)splits; o++)
+            if (o != c)
+                for (int u = 0; u < counts[o]; u++) rank += best[o * kLpTop + u] > v;
+        if (rank < a.top) {
+            const float value = lp_value((uint32_t)(v >> 32));
+            if (a.top_ids) a.top_ids[(size_t)row * a.top + rank] = (int)~(uint32_t)v;
+            if (a.top_logprobs) a.top_logprobs[(size_t)row * a.top + rank] = value == -INFINITY && log_l == log_l ? -INFINITY : (value - m) - log_l;
+        }
+    }
+}
+
+template <class T>
+int logprobs_launch(const LpArgs &a, int sm_count, cudaStream_t st) {
+    /* a row over more CTAs while there are SMs for them, each with a stretch of its own at least */
+    constexpr int kStretch = kLpThreads * kLpUnroll * (16 / (int)sizeof(T));
+    int splits = 1;
+    while (splits < kLpMaxSplit && (long long)a.rows * splits * 2 <= 2 * sm_count && a.vocab >= splits * kStretch) splits *= 2;
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3((unsigned)a.rows * splits);
+    c.blockDim = dim3(kLpThreads);
+    c.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = splits;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    c.attrs = at;
+    c.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&c, logprobs_kernel<T>, a);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return serve_fail(cudaGetErrorString(e));
+    }
+    return 0;
+}
+
+} // namespace
+
+} // namespace vb
+
+using namespace vb;
+
+extern "C" int vb200_token_logprobs(const vb200_logprobs_t *a, void *stream) {
+    if (!a || (!a->logits && a->rows > 0)) return serve_fail("no logits");
+    if (a->type < VB200_F32 || a->type > VB200_F16) return serve_fail("logits are fp32, bf16 or fp16");
+    if ((uintptr_t)a->logits % serve_size(a->type)) return serve_fail("logits have to be aligned to their elements");
+    if (a->rows < 0 || a->rows > (1 << 27) || a->vocab < 1 || a->vocab > (1 << 30)) return serve_fail("rows have to be 0 to 2^27, vocab 1 to 2^30");
+    if (a->top < 0 || a->top > kLpTop || a->top > a->vocab) return serve_fail("top has to be 0 to 32 and at most vocab");
+    if (a->logprobs && !a->tokens) return serve_fail("logprobs needs tokens");
+    if (a->rows == 0) return 0;
+    int dev = 0, n_sm = 0, major = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess || major != 10) {
+        cudaGetLastError();
+        return serve_fail("an sm_100 GPU is required (there is no CPU fallback)");
+    }
+    if (!serve_on_device(a->logits)) return serve_fail("logits do not lie on the current device");
+    const bool tops = a->top_ids || a->top_logprobs;
+    const LpArgs l = {a->logits, a->row_stride, a->rows, a->vocab, tops ? a->top : 0, a->tokens, a->logprobs, a->entropy, a->top_ids, a->top_logprobs};
+    const cudaStream_t st = (cudaStream_t)stream;
+    if (a->type == VB200_F32) return logprobs_launch<float>(l, n_sm, st);
+    if (a->type == VB200_BF16) return logprobs_launch<__nv_bfloat16>(l, n_sm, st);
+    return logprobs_launch<__half>(l, n_sm, st);
+}
