@@ -9,7 +9,7 @@
  * collected and put in order at the end. Values are compared with their index below them, so all are different. Where more come through than
  * the list holds (rising rows), a CTA finds its largest again by bisection, from memory: slower and as right.
  */
-#include <algorithm>
+#include <type_traits>
 
 #include "vb_serve.cuh"
 
@@ -17,7 +17,10 @@ namespace vb {
 
 namespace {
 
-constexpr int kLpThreads = 512, kLpWarps = kLpThreads / 32, kLpTop = 32, kLpList = 1024, kLpUnroll = 4, kLpMaxSplit = 8;
+constexpr int kLpThreads = 512, kLpWarps = kLpThreads / 32, kLpTop = 32, kLpList = 1024, kLpMaxSplit = 8;
+/* vectors of 16 bytes that a thread takes at a time, with as many on their way: with four of BF16 it runs out of registers */
+template <class T>
+constexpr int kLpUnrolled = sizeof(T) == 4 ? 4 : 2;
 
 struct LpArgs {
     const void *x;
@@ -57,20 +60,50 @@ VB_DEVINL LpSums lp_join(LpSums a, LpSums b) {
     return r;
 }
 
+/* The larger one; NaN where either is. */
+VB_DEVINL float lp_max(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+VB_DEVINL float lp_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+/* 16 bytes of -inf: what stands in for vectors beyond a share */
 template <class T>
-struct LpRead {
-    static constexpr int kEach = 16 / sizeof(T);
-    float v[kEach];
-    VB_DEVINL void load(const T *p) { serve_load<kEach>(p, true, v); }
-};
+constexpr uint32_t kLpNothing = std::is_same<T, float>::value ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
 
 template <class T>
-__global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpArgs a) {
-    constexpr int kEach = 16 / sizeof(T);
+VB_DEVINL void lp_values(const uint4 &r, float *v) {
+    const uint32_t u[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const float2 f = serve_pair(u[j], (const T *)nullptr);
+        if constexpr (sizeof(T) == 4) v[j] = f.x;
+        else { v[2 * j] = f.x; v[2 * j + 1] = f.y; }
+    }
+}
+
+/* How many of the `n` ranks in a list, largest first, are above v. */
+VB_DEVINL int lp_above(const uint64_t *sorted, int n, uint64_t v) {
+    int lo = 0, hi = n;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (sorted[mid] > v) lo = mid + 1;
+        else hi = mid;
+    }
+    return lo;
+}
+
+template <class T>
+__global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const LpArgs a) {
+    constexpr int kEach = 16 / sizeof(T), kLpUnroll = kLpUnrolled<T>, kStep = kLpThreads * kLpUnroll;
     __shared__ uint64_t list[kLpList], best[kLpMaxSplit * kLpTop], group[32], threshold_s;
     __shared__ LpSums warp_sums[kLpWarps], cta_sums[kLpMaxSplit];
-    __shared__ float token_s;
-    __shared__ int n_list, bad_s[kLpMaxSplit], counts[kLpMaxSplit];
+    __shared__ float log_s;
+    __shared__ int n_list, bad_s[kLpMaxSplit], counts[kLpMaxSplit], ranks[kLpMaxSplit * kLpTop];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     uint32_t split, splits;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(split));
@@ -83,70 +116,98 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpArgs a) {
     const int head = min(a.vocab, (int)(((16 - ((uintptr_t)x & 15)) & 15) / sizeof(T)));
     const int vectors = (a.vocab - head) / kEach, tail = head + vectors * kEach;
     const int share = (vectors + splits - 1) / splits, v0 = min(vectors, (int)split * share), v1 = min(vectors, v0 + share);
+    const uint4 *xv = reinterpret_cast<const uint4 *>(x + head);
 
+    uint4 now[kLpUnroll], next[kLpUnroll];
+    auto fetch = [&](int c0, uint4 (&r)[kLpUnroll]) {
+#pragma unroll
+        for (int u = 0; u < kLpUnroll; u++) {
+            const int i = c0 + u * kLpThreads + tid;
+            r[u] = i < v1 ? __ldcs(xv + i) : make_uint4(kLpNothing<T>, kLpNothing<T>, kLpNothing<T>, kLpNothing<T>);
+        }
+    };
+    fetch(v0, now);
+    /* the elements around the vectors go with the first CTA's first stretch, one a thread */
+    float extra = -INFINITY, of_token = 0.0f;
+    int extra_i = -1, token = -1;
+    if (split == 0) {
+        if (tid < head) extra_i = tid;
+        else if (tid - head < a.vocab - tail) extra_i = tail + tid - head;
+        if (extra_i >= 0) extra = serve_get(x + extra_i);
+        if (tid == 0) {
+            n_list = 0;
+            if (a.tokens) token = a.tokens[row];
+            if (token >= 0 && token < a.vocab) of_token = serve_get(x + token);
+        }
+    }
     if (tid == 0) { n_list = 0; threshold_s = 0; bad_s[0] = 0; }
     __syncthreads();
+
     LpSums sums = {-INFINITY, 0.0f, 0.0f};
-    uint64_t mine = 0;                        /* the largest of this thread's first stretch */
     bool bad = false;                         /* NaN or +inf */
-    auto take = [&](float v) {
-        if (v > sums.m) {
-            if (v == INFINITY) { bad = true; return; }
-            const float d = sums.m - v, f = __expf(d);
-            sums.w = f > 0.0f ? (sums.w + sums.l * d) * f : 0.0f;
-            sums.l *= f;
-            sums.m = v;
+    /* a reference that trails the maximum by at most 8 */
+    auto raise = [&](float top) {
+        if (!(top <= sums.m + 8.0f)) {
+            if (top < INFINITY) {
+                const float d = sums.m - top, f = __expf(d);
+                sums.w = f > 0.0f ? (sums.w + sums.l * d) * f : 0.0f;
+                sums.l *= f;
+                sums.m = top;
+            } else {
+                bad = true;
+            }
         }
-        if (v == -INFINITY) return;
-        if (v != v) { bad = true; return; }
-        const float d = v - sums.m, e = __expf(d);
+    };
+    auto add = [&](float v) {
+        const float d = fmaxf(v - sums.m, -150.0f), e = lp_ex2(d * 1.44269504f);      /* -inf: 0 and 0 * -150 */
         sums.l += e;
         sums.w = fmaf(e, d, sums.w);
     };
+    uint64_t threshold = 0;
     float limit = -INFINITY;                  /* values from here on may be among the largest */
     auto collect = [&](float v, int i) {
         if (!(v < limit)) {
             const uint64_t r = lp_rank(v, i);
-            if (r >= threshold_s) {
+            if (r >= threshold) {
                 const int at = atomicAdd(&n_list, 1);
                 if (at < kLpList) list[at] = r;
             }
         }
     };
-    const uint4 *xv = reinterpret_cast<const uint4 *>(x + head);
-    bool first = true;
-    for (int c0 = v0; c0 < v1 || first; c0 += kLpThreads * kLpUnroll) {
-        LpRead<T> r[kLpUnroll];
+    for (int c0 = v0; c0 < v1 || c0 == v0; c0 += kStep) {
+        const bool first = c0 == v0;
+        if (c0 + kStep < v1) fetch(c0 + kStep, next);
+        float top = first ? extra : -INFINITY;
 #pragma unroll
         for (int u = 0; u < kLpUnroll; u++) {
-            const int i = c0 + u * kLpThreads + tid;
-            if (i < v1) r[u].load(reinterpret_cast<const T *>(xv + i));
+            float v[kEach];
+            lp_values<T>(now[u], v);
+#pragma unroll
+            for (int j = 0; j < kEach; j++) top = lp_max(top, v[j]);
         }
-        /* the elements around the vectors go with the first CTA's first stretch, one a thread */
-        float extra = 0.0f;
-        int extra_i = -1;
-        if (first && split == 0) {
-            if (tid < head) extra_i = tid;
-            else if (tid - head < a.vocab - tail) extra_i = tail + tid - head;
-            if (extra_i >= 0) extra = serve_get(x + extra_i);
-        }
+        raise(top);
+        if (first) add(extra);
 #pragma unroll
         for (int u = 0; u < kLpUnroll; u++) {
-            const int i = c0 + u * kLpThreads + tid;
-            if (i < v1)
+            float v[kEach];
+            lp_values<T>(now[u], v);
 #pragma unroll
-                for (int j = 0; j < kEach; j++) {
-                    take(r[u].v[j]);
-                    if (first && a.top) mine = max(mine, lp_rank(r[u].v[j], head + i * kEach + j));
-                }
-        }
-        if (extra_i >= 0) {
-            take(extra);
-            if (a.top) mine = max(mine, lp_rank(extra, extra_i));
+            for (int j = 0; j < kEach; j++) add(v[j]);
         }
         if (a.top) {
             if (first) {
-                uint64_t most = mine;
+                /* this thread's largest, at its first place; those of 32 groups of threads; the top-th of them */
+                uint64_t most = extra_i >= 0 ? lp_rank(extra, extra_i) : 0;
+#pragma unroll
+                for (int u = 0; u < kLpUnroll; u++) {
+                    const int i = c0 + u * kLpThreads + tid;
+                    float v[kEach];
+                    lp_values<T>(now[u], v);
+                    if (i < v1)
+#pragma unroll
+                        for (int j = 0; j < kEach; j++)
+                            if (!(v[j] < top)) most = max(most, lp_rank(v[j], head + i * kEach + j));
+                }
 #pragma unroll
                 for (int o = 8; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
                 if ((lane & 15) == 0) group[warp * 2 + (lane >> 4)] = most;
@@ -154,6 +215,7 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpArgs a) {
                 if (warp == 0) {
                     const uint64_t v = group[lane];
                     int rank = 0;
+#pragma unroll
                     for (int o = 0; o < 32; o++) {
                         const uint64_t w = group[o];
                         rank += w > v || (w == v && o < lane);
@@ -161,53 +223,58 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpArgs a) {
                     if (rank == a.top - 1) threshold_s = v;
                 }
                 __syncthreads();
-                const uint64_t th = threshold_s;
-                limit = th == 0 ? -INFINITY : lp_value((uint32_t)(th >> 32));
+                threshold = threshold_s;
+                limit = threshold == 0 ? -INFINITY : lp_value((uint32_t)(threshold >> 32));
                 if (limit != limit) limit = INFINITY;      /* the threshold is a NaN: only NaN reaches it */
+                if (extra_i >= 0) collect(extra, extra_i);
             }
+            if (!(top < limit)) {
 #pragma unroll
-            for (int u = 0; u < kLpUnroll; u++) {
-                const int i = c0 + u * kLpThreads + tid;
-                if (i < v1)
+                for (int u = 0; u < kLpUnroll; u++) {
+                    const int i = c0 + u * kLpThreads + tid;
+                    float v[kEach];
+                    lp_values<T>(now[u], v);
+                    if (i < v1)
 #pragma unroll
-                    for (int j = 0; j < kEach; j++) collect(r[u].v[j], head + i * kEach + j);
+                        for (int j = 0; j < kEach; j++) collect(v[j], head + i * kEach + j);
+                }
             }
-            if (extra_i >= 0) collect(extra, extra_i);
         }
-        first = false;
+#pragma unroll
+        for (int u = 0; u < kLpUnroll; u++) now[u] = next[u];
     }
     /* this CTA's sums */
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const LpSums b = {__shfl_xor_sync(0xffffffffu, sums.m, o), __shfl_xor_sync(0xffffffffu, sums.l, o), __shfl_xor_sync(0xffffffffu, sums.w, o)};
-        sums = lane & o ? lp_join(b, sums) : lp_join(sums, b);
-    }
-    if (lane == 0) warp_sums[warp] = sums;
-    if (__any_sync(0xffffffffu, bad) && lane == 0) atomicOr(&bad_s[0], 1);
-    __syncthreads();
-    if (warp == 0) {
-        sums = lane < kLpWarps ? warp_sums[lane] : LpSums{-INFINITY, 0.0f, 0.0f};
+    auto join_warp = [&]() {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
             const LpSums b = {__shfl_xor_sync(0xffffffffu, sums.m, o), __shfl_xor_sync(0xffffffffu, sums.l, o), __shfl_xor_sync(0xffffffffu, sums.w, o)};
             sums = lane & o ? lp_join(b, sums) : lp_join(sums, b);
         }
+    };
+    join_warp();
+    if (lane == 0) warp_sums[warp] = sums;
+    if (__any_sync(0xffffffffu, bad) && lane == 0) atomicOr(&bad_s[0], 1);
+    __syncthreads();
+    if (warp == kLpWarps - 1) {               /* the first warps have the list */
+        sums = lane < kLpWarps ? warp_sums[lane] : LpSums{-INFINITY, 0.0f, 0.0f};
+        join_warp();
+        if (lane == 0) cta_sums[0] = sums;
     }
     /* this CTA's largest values, in order */
-    const int there = min(a.top, v1 - v0 > 0 || split == 0 ? (v1 - v0) * kEach + (split == 0 ? head + a.vocab - tail : 0) : 0);
+    const int there = min(a.top, (v1 - v0) * kEach + (split == 0 ? head + a.vocab - tail : 0));
     if (a.top) {
         int n = n_list;
         if (n > kLpList) {
             /* the largest rank that `there` of this CTA's values reach, a bit at a time; then those values alone */
+            auto each = [&](auto &&f) {
+                for (int i = v0 * kEach + tid; i < v1 * kEach; i += kLpThreads) f(serve_get(x + head + i), head + i);
+                if (extra_i >= 0) f(extra, extra_i);
+            };
             uint64_t least = 0;
             for (int bit = 63; bit >= 0; bit--) {
                 const uint64_t trial = least | (1ull << bit);
                 int reach = 0;
-                for (int i = v0 * kEach + tid; i < v1 * kEach; i += kLpThreads) reach += lp_rank(serve_get(x + head + i), head + i) >= trial;
-                if (split == 0) {
-                    if (tid < head) reach += lp_rank(serve_get(x + tid), tid) >= trial;
-                    else if (tid - head < a.vocab - tail) reach += lp_rank(serve_get(x + tail + tid - head), tail + tid - head) >= trial;
-                }
+                each([&](float v, int i) { reach += lp_rank(v, i) >= trial; });
                 __syncthreads();
                 if (tid == 0) n_list = 0;
                 __syncthreads();
@@ -216,22 +283,23 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpArgs a) {
                 if (n_list >= there) least = trial;
             }
             __syncthreads();
-            if (tid == 0) { n_list = 0; threshold_s = least; }
+            if (tid == 0) n_list = 0;
             __syncthreads();
+            threshold = least;
             limit = -INFINITY;
-            for (int i = v0 * kEach + tid; i < v1 * kEach; i += kLpThreads) collect(serve_get(x + head + i), head + i);
-            if (split == 0) {
-                if (tid < head) collect(serve_get(x + tid), tid);
-                else if (tid - head < a.vocab - tail) collect(serve_get(x + tail + tid - head), tail + tid - head);
-            }
+            each(collect);
             __syncthreads();
             n = n_list;
         }
-        for (int i = tid; i < n; i += kLpThreads) {
-            const uint64_t v = list[i];
+        /* four threads count for a value */
+        for (int i = tid >> 2; i < (n + 7) / 8 * 8; i += kLpThreads / 4) {
+            const uint64_t v = i < n ? list[i] : 0;
             int rank = 0;
-            for (int o = 0; o < n; o++) rank += list[o] > v;
-            if (rank < there) best[rank] = v;
+#pragma unroll 4
+            for (int o = tid & 3; o < n; o += 4) rank += list[o] > v;
+            rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+            rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+            if ((tid & 3) == 0 && i < n && rank < there) best[rank] = v;
         }
     }
     __syncthreads();
@@ -246,9 +314,9 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpArgs a) {
             }
             if (tid == 0) {
                 asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"(vb_smem_u32(&cta_sums[split])));
-                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(sums.m) : "memory");
-                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4), "f"(sums.l) : "memory");
-                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 8), "f"(sums.w) : "memory");
+                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(cta_sums[0].m) : "memory");
+                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4), "f"(cta_sums[0].l) : "memory");
+                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 8), "f"(cta_sums[0].w) : "memory");
                 asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"(vb_smem_u32(&bad_s[split])));
                 asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to), "r"(bad_s[0]) : "memory");
                 asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"(vb_smem_u32(&counts[split])));
@@ -262,45 +330,48 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpArgs a) {
     if (tid == 0) {
         counts[0] = there;
         int wrong = bad_s[0];
+        sums = cta_sums[0];
         for (uint32_t c = 1; c < splits; c++) {
             sums = lp_join(sums, cta_sums[c]);
             wrong |= bad_s[c];
         }
         const float log_l = logf(sums.l);                       /* -inf for a row of nothing but -inf */
         const float nan = __uint_as_float(0x7fffffffu);
-        const int token = a.tokens ? a.tokens[row] : -1;
-        if (a.logprobs) {
-            const bool known = token >= 0 && token < a.vocab;
-            const float v = known ? serve_get(x + token) : nan;
-            a.logprobs[row] = wrong || !known ? nan : sums.l == 0.0f ? -INFINITY : (v - sums.m) - log_l;
-        }
+        if (a.logprobs) a.logprobs[row] = wrong || token < 0 || token >= a.vocab ? nan : sums.l == 0.0f ? -INFINITY : (of_token - sums.m) - log_l;
         if (a.entropy) a.entropy[row] = wrong ? nan : sums.l == 0.0f ? 0.0f : log_l - sums.w / sums.l;
         cta_sums[0] = sums;
-        token_s = wrong ? nan : log_l;
+        log_s = wrong ? nan : log_l;
     }
-    __syncthreads();
     if (!a.top) return;
-    const float m = cta_sums[0].m, log_l = token_s;
-    for (int i = tid; i < (int)splits * kLpTop; i += kLpThreads) {
-        const int c = i / kLpTop, k = i - c * kLpTop;
-        if (k >= counts[c]) continue;
-        const uint64_t v = best[i];
-        int rank = k;
-        for (int o = 0; o < (int)splits; o++)
-            if (o != c)
-                for (int u = 0; u < counts[o]; u++) rank += best[o * kLpTop + u] > v;
-        if (rank < a.top) {
-            const float value = lp_value((uint32_t)(v >> 32));
-            if (a.top_ids) a.top_ids[(size_t)row * a.top + rank] = (int)~(uint32_t)v;
-            if (a.top_logprobs) a.top_logprobs[(size_t)row * a.top + rank] = value == -INFINITY && log_l == log_l ? -INFINITY : (value - m) - log_l;
+    const int held = (int)splits * kLpTop;
+    for (int i = tid; i < held; i += kLpThreads) ranks[i] = i % kLpTop;
+    __syncthreads();
+    const float m = cta_sums[0].m, log_l = log_s;
+    if (splits > 1) {
+        /* a value and another CTA's list at a time */
+        for (int i = tid; i < held * (int)splits; i += kLpThreads) {
+            const int at = i / (int)splits, c = at / kLpTop, o = i - at * (int)splits;
+            if (o != c && at % kLpTop < counts[c]) {
+                const int above = lp_above(best + o * kLpTop, counts[o], best[at]);
+                if (above) atomicAdd(&ranks[at], above);
+            }
         }
+        __syncthreads();
+    }
+    for (int i = tid; i < held; i += kLpThreads) {
+        if (i % kLpTop >= counts[i / kLpTop] || ranks[i] >= a.top) continue;
+        const uint64_t v = best[i];
+        const float value = lp_value((uint32_t)(v >> 32));
+        const size_t to = (size_t)row * a.top + ranks[i];
+        if (a.top_ids) a.top_ids[to] = (int)~(uint32_t)v;
+        if (a.top_logprobs) a.top_logprobs[to] = value == -INFINITY && log_l == log_l ? -INFINITY : (value - m) - log_l;
     }
 }
 
 template <class T>
 int logprobs_launch(const LpArgs &a, int sm_count, cudaStream_t st) {
     /* a row over more CTAs while there are SMs for them, each with a stretch of its own at least */
-    constexpr int kStretch = kLpThreads * kLpUnroll * (16 / (int)sizeof(T));
+    constexpr int kStretch = kLpThreads * kLpUnrolled<T> * (16 / (int)sizeof(T));
     int splits = 1;
     while (splits < kLpMaxSplit && (long long)a.rows * splits * 2 <= 2 * sm_count && a.vocab >= splits * kStretch) splits *= 2;
     cudaLaunchConfig_t c = {};
