@@ -3,6 +3,7 @@
  * accumulated attention weight. Attention over it is in vb_kv4_attn.cu.
  */
 #include <algorithm>
+#include <limits.h>
 #include <new>
 #include <string>
 
@@ -37,97 +38,150 @@ bool serve_on_device(const void *p) {
 
 namespace {
 
-constexpr int kRowThreads = 256;
+/* One of 32, 64, 96, 128, 192, 256 values a head, as a constant */
+#define VB_KV4_DIMS(blocks, call) \
+    switch (blocks) {             \
+    case 1: return call(1);       \
+    case 2: return call(2);       \
+    case 3: return call(3);       \
+    case 4: return call(4);       \
+    case 6: return call(6);       \
+    default: return call(8);      \
+    }
+
+constexpr int kRowThreads = 256, kRowUnroll = 4;
 
 /* ------------------------------------------------------------------ rows into the cache and out of it
- * A thread has a word (8 values): four lanes make a block of 32. Both planes in one launch: blockIdx.y. Memory-bound, and at one row a
- * launch bound by its latency. */
+ * A thread has words of 8 values: four lanes make a block of 32. The words of a token (keys, then values) lie side by side in the order of
+ * threads; a CTA takes 1024 of them at a time, four a thread with their loads together. Memory-bound, and at one row a launch bound by its
+ * latency. */
 template <class T>
 struct RowsArgs {
     Kv4 c;
     const int *lengths, *rows;
     int max_rows, wide;
+    unsigned tokens;                                     /* seqs * max_rows */
     ServeRows<T> k, v;
 };
 
-template <class T, bool READ>
+template <int NB, class T, bool READ>
 __global__ void __launch_bounds__(kRowThreads) kv4_rows_kernel(const RowsArgs<T> a) {
-    const int words = a.c.blocks * 4;                    /* of a row of a head */
-    const long long total = (long long)a.c.seqs * a.max_rows * a.c.kv_heads * words;
-    const bool is_v = blockIdx.y != 0;
-    const ServeRows<T> &x = is_v ? a.v : a.k;
-    uint8_t *codes = is_v ? a.c.v : a.c.k, *scales = is_v ? a.c.vs : a.c.ks;
-    /* whole warps stay together: the four lanes of a block share its scale */
-    for (long long i0 = ((long long)blockIdx.x * kRowThreads + threadIdx.x) & ~31ll; i0 < total; i0 += (long long)gridDim.x * kRowThreads) {
-        const long long i = i0 + (threadIdx.x & 31);
-        const bool in = i < total;
-        const long long at = in ? i : total - 1;
-        const int w = (int)(at % words);
-        const long long rest = at / words;
-        const int h = (int)(rest % a.c.kv_heads);
-        const long long sr = rest / a.c.kv_heads;
-        const int r = (int)(sr % a.max_rows), s = (int)(sr / a.max_rows);
-        const Kv4Span span = kv4_span(a.lengths, a.rows, a.max_rows, s, a.c.capacity);
-        const int slot = span.length - span.rows + r;
-        const bool real = in && r < span.rows && slot >= 0;
-        T *p = x.data + s * x.seq + r * x.row + h * x.head + w * 8;
-        const size_t row = a.c.row(s, h, real ? slot : 0);
-        uint8_t *base = codes + row * (size_t)(a.c.blocks * 16);
-        float v[8];
-        if (!READ) {
+    constexpr unsigned kWords = NB * 4;                  /* of a row of a head */
+    constexpr long long kChunk = kRowThreads * kRowUnroll;
+    const unsigned plane = a.c.kv_heads * kWords, token_words = 2 * plane;
+    const long long total = (long long)a.tokens * token_words;
+    const int tid = threadIdx.x;
+    for (long long c0 = blockIdx.x * kChunk; c0 < total; c0 += gridDim.x * kChunk) {
+        const unsigned token0 = (unsigned)(c0 / token_words), off0 = (unsigned)(c0 - (long long)token0 * token_words);
+        float v[kRowUnroll][8];
+        uint32_t code[kRowUnroll], byte[kRowUnroll], w[kRowUnroll];
+        size_t row[kRowUnroll];
+        T *p[kRowUnroll];
+        bool real[kRowUnroll], is_v[kRowUnroll];
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = 0.0f;
-            if (real) serve_load<8>(p, a.wide, v);
-            /* the largest magnitude by its bits, so that a NaN is the largest of all */
-            uint32_t most = 0;
+        for (int u = 0; u < kRowUnroll; u++) {
+            const unsigned o = off0 + u * kRowThreads + tid, ahead = o / token_words, rest = o - ahead * token_words;
+            is_v[u] = rest >= plane;
+            const unsigned in_plane = is_v[u] ? rest - plane : rest, h = in_plane / kWords;
+            w[u] = in_plane - h * kWords;
+            const bool in = token0 + ahead < a.tokens;
+            const unsigned token = in ? token0 + ahead : 0, s = token / a.max_rows, r = token - s * a.max_rows;
+            const Kv4Span span = kv4_span(a.lengths, a.rows, a.max_rows, s, a.c.capacity);
+            const int slot = span.length - span.rows + (int)r;
+            real[u] = in && (int)r < span.rows && slot >= 0;
+            const ServeRows<T> &x = is_v[u] ? a.v : a.k;
+            p[u] = x.data + (long long)s * x.seq + (long long)r * x.row + (long long)h * x.head + w[u] * 8;
+            row[u] = a.c.row(s, h, real[u] ? slot : 0);
+            if (!READ) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);
-            most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-            most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-            if (!real) continue;
-            const uint32_t byte = kv4_scale(__uint_as_float(most));
-            const uint32_t code = byte == 255u ? 0u : kv4_codes(v, kv4_inverse(byte));       /* a block that is NaN: codes of zero */
-            if (is_v) {
-                uint16_t *to = reinterpret_cast<uint16_t *>(base);
-                to[kv4_value_half(2 * w, a.c.blocks)] = (uint16_t)code;
-                to[kv4_value_half(2 * w + 1, a.c.blocks)] = (uint16_t)(code >> 16);
+                for (int j = 0; j < 8; j++) v[u][j] = 0.0f;
+                if (real[u]) serve_load<8>(p[u], a.wide, v[u]);
+            } else if (real[u]) {
+                const uint8_t *base = (is_v[u] ? a.c.v : a.c.k) + row[u] * (NB * 16);
+                if (!is_v[u]) {
+                    code[u] = reinterpret_cast<const uint32_t *>(base)[kv4_key_word(w[u], NB)];
+                } else if (kv4_whole(NB)) {
+                    code[u] = reinterpret_cast<const uint32_t *>(base)[w[u]];
+                } else {
+                    const uint16_t *from = reinterpret_cast<const uint16_t *>(base);
+                    code[u] = from[kv4_value_half(2 * w[u], NB)] | ((uint32_t)from[kv4_value_half(2 * w[u] + 1, NB)] << 16);
+                }
+                byte[u] = (is_v[u] ? a.c.vs : a.c.ks)[row[u] * NB + (w[u] >> 2)];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kRowUnroll; u++) {
+            if (!READ) {
+                /* the largest magnitude by its bits, so that a NaN is the largest of all */
+                uint32_t most = 0;
+#pragma unroll
+                for (int j = 0; j < 8; j++) most = max(most, __float_as_uint(v[u][j]) & 0x7fffffffu);
+                most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                if (!real[u]) continue;
+                const uint32_t scale = kv4_scale(__uint_as_float(most));
+                const uint32_t c = scale == 255u ? 0u : kv4_codes(v[u], kv4_inverse(scale));       /* a block that is NaN: codes of zero */
+                uint8_t *base = (is_v[u] ? a.c.v : a.c.k) + row[u] * (NB * 16);
+                if (!is_v[u]) {
+                    reinterpret_cast<uint32_t *>(base)[kv4_key_word(w[u], NB)] = c;
+                } else if (kv4_whole(NB)) {
+                    reinterpret_cast<uint32_t *>(base)[w[u]] = c;
+                } else {
+                    uint16_t *to = reinterpret_cast<uint16_t *>(base);
+                    to[kv4_value_half(2 * w[u], NB)] = (uint16_t)c;
+                    to[kv4_value_half(2 * w[u] + 1, NB)] = (uint16_t)(c >> 16);
+                }
+                if ((w[u] & 3) == 0) (is_v[u] ? a.c.vs : a.c.ks)[row[u] * NB + (w[u] >> 2)] = (uint8_t)scale;
             } else {
-                reinterpret_cast<uint32_t *>(base)[kv4_key_word(w, a.c.blocks)] = code;
-            }
-            if ((w & 3) == 0) scales[row * a.c.blocks + (w >> 2)] = (uint8_t)byte;
-        } else {
-            if (!real) continue;
-            uint32_t code;
-            if (is_v) {
-                const uint16_t *from = reinterpret_cast<const uint16_t *>(base);
-                code = from[kv4_value_half(2 * w, a.c.blocks)] | ((uint32_t)from[kv4_value_half(2 * w + 1, a.c.blocks)] << 16);
-            } else {
-                code = reinterpret_cast<const uint32_t *>(base)[kv4_key_word(w, a.c.blocks)];
-            }
-            const float scale = kv4_scale_value(scales[row * a.c.blocks + (w >> 2)]);
-            uint32_t half[4];
-            kv4_halves(code, half);
+                if (!real[u]) code[u] = byte[u] = 0;
+                const float scale = kv4_scale_value(byte[u]);
+                uint32_t half[4];
+                kv4_halves(code[u], half);
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const float2 f = kv4_f2(half[j]);
-                v[2 * j] = f.x * scale;
-                v[2 * j + 1] = f.y * scale;
+                for (int j = 0; j < 4; j++) {
+                    const float2 f = kv4_f2(half[j]);
+                    v[u][2 * j] = f.x * scale;
+                    v[u][2 * j + 1] = f.y * scale;
+                }
+                if constexpr (sizeof(T) == 4) {
+                    /* two lanes' 64 bytes, 32 of them a store: whole sectors (the words of a pair are one token's and one head's) */
+                    const bool odd = tid & 1;
+                    float other[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const float give = odd ? v[u][j] : v[u][4 + j];
+                        other[j] = __shfl_xor_sync(0xffffffffu, give, 1);
+                    }
+                    if (!real[u]) continue;
+                    if (a.wide) {
+                        float4 *to = reinterpret_cast<float4 *>(p[u] - (odd ? 8 : 0)) + (odd ? 1 : 0);
+                        to[0] = odd ? make_float4(other[0], other[1], other[2], other[3]) : make_float4(v[u][0], v[u][1], v[u][2], v[u][3]);
+                        to[2] = odd ? make_float4(v[u][4], v[u][5], v[u][6], v[u][7]) : make_float4(other[0], other[1], other[2], other[3]);
+                        continue;
+                    }
+                }
+                if (real[u]) serve_store<8>(p[u], a.wide, v[u]);
             }
-            serve_store<8>(p, a.wide, v);
         }
     }
 }
 
-template <class T>
+template <int NB, class T>
 int rows_launch(const vb200_kv4 *h, const vb200_kv4_rows_t &a, bool read, cudaStream_t st) {
-    RowsArgs<T> r = {h->c, a.lengths, a.rows, a.max_rows, 0, serve_rows<T>(a.k), serve_rows<T>(a.v)};
+    RowsArgs<T> r = {h->c, a.lengths, a.rows, a.max_rows, 0, (unsigned)h->c.seqs * a.max_rows, serve_rows<T>(a.k), serve_rows<T>(a.v)};
     r.wide = serve_wide(r.k) && serve_wide(r.v);
-    const long long words = (long long)h->c.seqs * a.max_rows * h->c.kv_heads * h->c.blocks * 4;
-    const long long most = (long long)h->w.sm_count * 16;
-    const dim3 grid((unsigned)std::min((words + kRowThreads - 1) / kRowThreads, most), 2);
-    if (read) kv4_rows_kernel<T, true><<<grid, kRowThreads, 0, st>>>(r);
-    else kv4_rows_kernel<T, false><<<grid, kRowThreads, 0, st>>>(r);
+    const long long words = (long long)r.tokens * h->c.kv_heads * NB * 8, chunk = kRowThreads * kRowUnroll;
+    const unsigned grid = (unsigned)std::min((words + chunk - 1) / chunk, (long long)h->w.sm_count * 16);
+    if (read) kv4_rows_kernel<NB, T, true><<<grid, kRowThreads, 0, st>>>(r);
+    else kv4_rows_kernel<NB, T, false><<<grid, kRowThreads, 0, st>>>(r);
     return serve_launched();
+}
+
+template <class T>
+int rows_dims(const vb200_kv4 *h, const vb200_kv4_rows_t &a, bool read, cudaStream_t st) {
+#define VB_CALL(n) rows_launch<n, T>(h, a, read, st)
+    VB_KV4_DIMS(h->c.blocks, VB_CALL)
+#undef VB_CALL
 }
 
 /* ------------------------------------------------------------------ eviction */
@@ -149,12 +203,16 @@ VB_DEVINL uint32_t evict_key(float m) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int kSelThreads = 1024;
+constexpr int kSelThreads = 1024, kSelEach = 32, kSelChunk = kSelThreads * kSelEach, kSelBins = 2048;
 
-/* Which tokens stay: a CTA per sequence and head. The need-th largest key of the middle by four passes of 8 bits (counts of a
- * digit among those that share the digits before it), then the tokens in order. */
+/* Which tokens stay: a CTA per sequence and head. The need-th largest key of the middle by digits of 11, 11 and 10 bits (counts of a
+ * digit among those that share the digits before it; the first holds sign, exponent and two bits, so that masses spread over it), then
+ * the tokens in order. A thread keeps the keys of up to 32 tokens in registers; longer sequences are read again, 32768 tokens at a time.
+ */
 __global__ void __launch_bounds__(kSelThreads) kv4_select_kernel(const EvictArgs a) {
-    __shared__ int count[256], warp_sum[32][2], base[2];
+    __shared__ int count[kSelBins], warp_sum[32];
+    __shared__ uint2 place[kSelEach * 32];                /* of a warp's 32 tokens: how many stay, how many tie; then how many before them */
+    __shared__ uint2 warp_place[32];
     __shared__ uint32_t prefix;
     __shared__ int want;
     const int s = blockIdx.y, h = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -166,54 +224,118 @@ __global__ void __launch_bounds__(kSelThreads) kv4_select_kernel(const EvictArgs
     }
     const float *mass = a.mass + ((size_t)s * a.from.kv_heads + h) * a.from.capacity;
     const int lo = a.first, hi = n - a.recent;            /* the middle; it holds more than are needed of it */
+    uint32_t key[kSelEach];
+    auto read = [&](int c0) {
+#pragma unroll
+        for (int j = 0; j < kSelEach; j++) {
+            const int i = c0 + j * kSelThreads + tid;
+            if (i < n) key[j] = evict_key(mass[i]);
+            if (c0 + (j + 1) * kSelThreads >= n) break;
+        }
+    };
+    const bool once = n <= kSelChunk;
+    if (once) read(0);
     if (tid == 0) { prefix = 0; want = a.keep - a.first - a.recent; }
-    if (a.keep > a.first + a.recent) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            if (tid < 256) count[tid] = 0;
+    const bool none = a.keep == a.first + a.recent;
+    if (!none) {
+        int shift = 21;
+#pragma unroll 1
+        for (int pass = 0; pass < 3; pass++) {
+            const uint32_t mask = pass == 0 ? 0u : pass == 1 ? 0xffe00000u : 0xfffffc00u, digit = pass == 2 ? 1023u : 2047u;
+            for (int x = tid; x < kSelBins; x += kSelThreads) count[x] = 0;
             __syncthreads();
-            const uint32_t mask = shift == 24 ? 0u : ~0u << (shift + 8), p = prefix;
-            for (int i = lo + tid; i < hi; i += kSelThreads) {
-                const uint32_t key = evict_key(mass[i]);
-                if ((key & mask) == p) atomicAdd(&count[(key >> shift) & 255u], 1);
+            const uint32_t p = prefix;
+            for (int c0 = 0; c0 < n; c0 += kSelChunk) {
+                if (!once) read(c0);
+#pragma unroll
+                for (int j = 0; j < kSelEach; j++) {
+                    const int i = c0 + j * kSelThreads + tid;
+                    if (i >= lo && i < hi && (key[j] & mask) == p) atomicAdd(&count[(key[j] >> shift) & digit], 1);
+                    if (c0 + (j + 1) * kSelThreads >= n) break;
+                }
             }
             __syncthreads();
-            if (tid == 0) {
-                int left = want, d = 255;
-                for (; d > 0 && count[d] < left; d--) left -= count[d];
-                prefix = p | ((uint32_t)d << shift);
-                want = left;
+            /* thread x has bins 2047 - 2 x and 2046 - 2 x: how many lie above them */
+            const int left = want, b1 = kSelBins - 1 - 2 * tid, n1 = count[b1], n0 = count[b1 - 1];
+            int above = n1 + n0;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, above, o);
+                if (lane >= o) above += v;
+            }
+            if (lane == 31) warp_sum[warp] = above;
+            __syncthreads();
+            if (warp == 0) {
+                int v = warp_sum[lane];
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int u = __shfl_up_sync(0xffffffffu, v, o);
+                    if (lane >= o) v += u;
+                }
+                warp_sum[lane] = v;
             }
             __syncthreads();
+            above += (warp ? warp_sum[warp - 1] : 0) - n1 - n0;
+            if (above < left && left <= above + n1) { prefix = p | ((uint32_t)b1 << shift); want = left - above; }
+            else if (above + n1 < left && left <= above + n1 + n0) { prefix = p | ((uint32_t)(b1 - 1) << shift); want = left - above - n1; }
+            __syncthreads();
+            shift = pass == 0 ? 10 : 0;
         }
     }
     __syncthreads();
     /* of those equal to the threshold the first `ties` stay */
-    const bool none = a.keep == a.first + a.recent;
     const uint32_t threshold = prefix;
     const int ties = want;
-    if (tid == 0) base[0] = base[1] = 0;
-    __syncthreads();
-    for (int i0 = 0; i0 < n; i0 += kSelThreads) {
-        const int i = i0 + tid;
-        bool sure = false, tie = false;
-        if (i < n) {
-            if (i < lo || i >= hi) sure = true;
-            else if (!none) {
-                const uint32_t key = evict_key(mass[i]);
-                sure = key > threshold;
-                tie = key == threshold;
-            }
+    uint2 base = make_uint2(0, 0);                        /* stay, tie, before this chunk */
+    for (int c0 = 0; c0 < n; c0 += kSelChunk) {
+        if (!once) read(c0);
+        uint32_t stay = 0, tie = 0;                       /* a bit a token */
+#pragma unroll
+        for (int j = 0; j < kSelEach; j++) {
+            const int i = c0 + j * kSelThreads + tid;
+            const bool edge = i < lo || i >= hi;
+            const bool is_sure = i < n && (edge || (!none && key[j] > threshold)), is_tie = i < n && !edge && !none && key[j] == threshold;
+            const unsigned bs = __ballot_sync(0xffffffffu, is_sure), bt = __ballot_sync(0xffffffffu, is_tie);
+            stay |= (uint32_t)is_sure << j;
+            tie |= (uint32_t)is_tie << j;
+            if (lane == 0) place[j * 32 + warp] = make_uint2(__popc(bs), __popc(bt));
         }
-        const unsigned bt = __ballot_sync(0xffffffffu, tie), bs = __ballot_sync(0xffffffffu, sure);
-        if (lane == 0) { warp_sum[warp][0] = __popc(bs); warp_sum[warp][1] = __popc(bt); }
         __syncthreads();
-        int sures = base[0], tied = base[1];
-        for (int w = 0; w < warp; w++) { sures += warp_sum[w][0]; tied += warp_sum[w][1]; }
-        const unsigned below = (1u << lane) - 1u;
-        const int my_ties = tied + __popc(bt & below);
-        if (sure || (tie && my_ties < ties)) kept[sures + __popc(bs & below) + min(my_ties, ties)] = i;
+        {
+            uint2 v = place[tid];
+            const uint2 own = v;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned x = __shfl_up_sync(0xffffffffu, v.x, o), y = __shfl_up_sync(0xffffffffu, v.y, o);
+                if (lane >= o) { v.x += x; v.y += y; }
+            }
+            if (lane == 31) warp_place[warp] = v;
+            __syncthreads();
+            if (warp == 0) {
+                uint2 t = warp_place[lane];
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const unsigned x = __shfl_up_sync(0xffffffffu, t.x, o), y = __shfl_up_sync(0xffffffffu, t.y, o);
+                    if (lane >= o) { t.x += x; t.y += y; }
+                }
+                warp_place[lane] = t;
+            }
+            __syncthreads();
+            const uint2 ahead = warp ? warp_place[warp - 1] : make_uint2(0, 0);
+            place[tid] = make_uint2(base.x + ahead.x + v.x - own.x, base.y + ahead.y + v.y - own.y);
+            base.x += warp_place[31].x;
+            base.y += warp_place[31].y;
+        }
         __syncthreads();
-        if (tid == kSelThreads - 1) { base[0] = sures + __popc(bs); base[1] = tied + __popc(bt); }
+#pragma unroll
+        for (int j = 0; j < kSelEach; j++) {
+            if (c0 + j * kSelThreads >= n) break;
+            const bool is_sure = (stay >> j) & 1u, is_tie = (tie >> j) & 1u;
+            const unsigned bs = __ballot_sync(0xffffffffu, is_sure), bt = __ballot_sync(0xffffffffu, is_tie), below = (1u << lane) - 1u;
+            const uint2 at = place[j * 32 + warp];
+            const int tied = (int)at.y + __popc(bt & below);
+            if (is_sure || (is_tie && tied < ties)) kept[(int)at.x + __popc(bs & below) + min(tied, ties)] = c0 + j * kSelThreads + tid;
+        }
         __syncthreads();
     }
 }
@@ -260,15 +382,22 @@ __global__ void __launch_bounds__(kMoveThreads) kv4_move_kernel(const EvictArgs 
 }
 
 /* Loads the kernels on the current device: nothing is left to be loaded inside a capture. */
+template <int NB>
 int rows_load() {
     cudaFuncAttributes f;
-    const void *kernels[] = {(const void *)kv4_rows_kernel<float, false>, (const void *)kv4_rows_kernel<float, true>,
-                             (const void *)kv4_rows_kernel<__nv_bfloat16, false>, (const void *)kv4_rows_kernel<__nv_bfloat16, true>,
-                             (const void *)kv4_rows_kernel<__half, false>, (const void *)kv4_rows_kernel<__half, true>,
+    const void *kernels[] = {(const void *)kv4_rows_kernel<NB, float, false>, (const void *)kv4_rows_kernel<NB, float, true>,
+                             (const void *)kv4_rows_kernel<NB, __nv_bfloat16, false>, (const void *)kv4_rows_kernel<NB, __nv_bfloat16, true>,
+                             (const void *)kv4_rows_kernel<NB, __half, false>, (const void *)kv4_rows_kernel<NB, __half, true>,
                              (const void *)kv4_select_kernel, (const void *)kv4_move_kernel<false>, (const void *)kv4_move_kernel<true>};
     for (const void *k : kernels)
         if (cudaFuncGetAttributes(&f, k) != cudaSuccess) return serve_launched() | -1;
     return 0;
+}
+int load(int blocks) {
+    if (kv4_attention_load(blocks)) return -1;
+#define VB_CALL(n) rows_load<n>()
+    VB_KV4_DIMS(blocks, VB_CALL)
+#undef VB_CALL
 }
 
 int check_rows(const vb200_kv4 *h, const vb200_kv4_rows_t *a) {
@@ -286,9 +415,10 @@ int check_rows(const vb200_kv4 *h, const vb200_kv4_rows_t *a) {
 int rows_call(const vb200_kv4 *h, const vb200_kv4_rows_t *a, bool read, cudaStream_t st) {
     if (check_rows(h, a)) return -1;
     if (a->max_rows == 0) return 0;
-    if (a->k.type == VB200_F32) return rows_launch<float>(h, *a, read, st);
-    if (a->k.type == VB200_BF16) return rows_launch<__nv_bfloat16>(h, *a, read, st);
-    return rows_launch<__half>(h, *a, read, st);
+    if ((long long)a->max_rows * h->c.seqs > INT_MAX) return serve_fail("too many rows");
+    if (a->k.type == VB200_F32) return rows_dims<float>(h, *a, read, st);
+    if (a->k.type == VB200_BF16) return rows_dims<__nv_bfloat16>(h, *a, read, st);
+    return rows_dims<__half>(h, *a, read, st);
 }
 
 } // namespace
@@ -318,7 +448,7 @@ vb200_kv4_t *vb200_kv4_open(int seqs, int kv_heads, int head_dim, int capacity) 
     }
     vb200_kv4 *h = new (std::nothrow) vb200_kv4();
     if (!h) { serve_fail("out of memory"); return nullptr; }
-    if (rows_load() || kv4_attention_load(head_dim / 32)) {
+    if (load(head_dim / 32)) {
         delete h;
         return nullptr;
     }
