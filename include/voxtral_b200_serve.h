@@ -46,7 +46,8 @@ typedef struct {
  * that the call is about, which are the last ones; rows (device, [seqs], or NULL: max_rows of each) says how many of them are real where
  * sequences have unequal portions. Values of lengths outside [0, capacity] and of rows outside [0, max_rows] count as the nearest
  * in the range. Row r of sequence s, r < rows[s], is token lengths[s] - rows[s] + r; rows that would lie before token 0 are
- * not written by append and read, and see no key. Rows from rows[s] on are neither read nor written. */
+ * not written by append and read, and see no key. Nothing is written for rows from rows[s] on, and what they hold
+ * does not count. */
 typedef struct vb200_kv4 vb200_kv4_t;
 
 /* head_dim: 32, 64, 96, 128, 192 or 256. */

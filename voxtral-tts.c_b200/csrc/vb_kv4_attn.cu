@@ -27,6 +27,7 @@ namespace {
 
 constexpr int kAWarps = 8, kAThreads = 32 * kAWarps, kACols = 8, kAKeys = 32;
 constexpr int kAStatus = 61;
+constexpr int kAMaxSplits = 64;               /* a CTA joins them */
 constexpr float kABias = 7.0f;                /* weights times 2^7 */
 
 template <int NB>
@@ -45,7 +46,7 @@ struct ACfg {
 struct AttnArgs {
     Kv4 c;
     const int *lengths, *rows;
-    int max_rows, heads, group, splits, wide;
+    int max_rows, heads, group, splits, wide, wide_out;
     float scale;
     float *lse;
     const float *mass_in;
@@ -238,7 +239,7 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(co
             if (t_begin + i * kAWarps < t_end) fetch(t_begin + i * kAWarps, i);
     }
     if (tid == 0) abort_flag = 0;
-    if (warp == 0) make_queries<NB, QT>(q, a, seq, kv_head, pair0, pairs, q_s, mul_s);
+    if (warp == 0) make_queries<NB, QT>(q, a, seq, kv_head, pair0, a.max_rows * a.group, q_s, mul_s);
     __syncthreads();
 
     /* columns 2 t and 2 t + 1 of this lane: tokens they see, what makes their scores powers of two */
@@ -455,7 +456,8 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(co
         if (++stage == Cfg::kStages) { stage = 0; parity ^= 1u; }
     }
 
-    /* the warps' parts together; sums and results lose the 2^15 that the weights may have */
+    /* the warps' parts together, in the order of the accumulators (conflict-free, and the same place is the same result for all);
+     * sums and results lose the 2^15 that the weights may have */
 #pragma unroll
     for (int u = 0; u < 2; u++) {
 #pragma unroll
@@ -463,56 +465,81 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(co
         sum[u] *= 0x1p-15f;
     }
     __syncthreads();                                     /* every ring is empty */
-    float *mo = reinterpret_cast<float *>(a_smem), *mm = mo + kAWarps * kACols * kDim, *ml = mm + kAWarps * kACols;
-    if (g == 0)
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            mm[warp * kACols + 2 * t + u] = ref[u];
-            ml[warp * kACols + 2 * t + u] = sum[u];
-        }
+    constexpr int kUnits = 2 * NB * 32;                  /* of four results */
+    float4 *mo = reinterpret_cast<float4 *>(a_smem);
+    float2 *mm = reinterpret_cast<float2 *>(mo + kAWarps * kUnits), *ml = mm + kAWarps * 4;
+    if (g == 0) {
+        mm[warp * 4 + t] = make_float2(ref[0], ref[1]);
+        ml[warp * 4 + t] = make_float2(sum[0], sum[1]);
+    }
 #pragma unroll
     for (int i = 0; i < 2 * NB; i++) {
-        const int d = Cfg::kWhole ? g * (4 * NB) + 2 * i : 32 * (i / 2) + 4 * g + 2 * (i & 1);
-        const int e = top_scale[Cfg::kWhole ? 0 : i / 2] - 155;
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            float *to = mo + (warp * kACols + 2 * t + u) * kDim + d;
-            to[0] = ldexpf(o[i][u], e);
-            to[1] = ldexpf(o[i][2 + u], e);
-        }
+        const int e = top_scale[Cfg::kWhole ? 0 : i / 2] - 155, e0 = e >> 1;      /* in two steps: 2^e may not be a normal number */
+        const float f0 = __uint_as_float((uint32_t)(127 + e0) << 23), f1 = __uint_as_float((uint32_t)(127 + e - e0) << 23);
+        mo[(warp * 2 * NB + i) * 32 + lane] = make_float4(o[i][0] * f0 * f1, o[i][1] * f0 * f1, o[i][2] * f0 * f1, o[i][3] * f0 * f1);
     }
     __syncthreads();
     const int unit = (seq * a.c.kv_heads + kv_head) * (gridDim.x / a.splits) + tile_r;
-    float *part = a.part + ((size_t)unit * a.splits + split) * kACols * (kDim + 2);
-    auto finish = [&](int col, int d, float value, float total, float reference) {
-        const int pair = pair0 + col, row = pair / a.group, head = kv_head * a.group + pair - row * a.group;
-        serve_put(out.data + seq * out.seq + row * out.row + head * out.head + d, total == 0.0f ? 0.0f : value / total);
-        if (d == 0 && a.lse)
-            a.lse[((size_t)seq * a.max_rows + row) * a.heads + head] = total == 0.0f ? -INFINITY : (reference + 8.0f + log2f(total)) * 0.69314718f;
-    };
-    for (int x = tid; x < n_pairs * kDim; x += kAThreads) {
-        const int col = x / kDim, d = x - col * kDim;
-        float reference = -INFINITY, value = 0.0f, total = 0.0f;
+    constexpr int kPart = kACols * (kDim + 2);           /* floats of a part: results, references, sums */
+    float *parts = a.part + (size_t)unit * a.splits * kPart;
+    /* four results of columns 2 t, 2 t + 1 and dims d, d + 1, against a reference and a sum each */
+    auto finish = [&](int i, float4 v, float2 total, float2 reference) {
+        const int d = Cfg::kWhole ? g * (4 * NB) + 2 * i : 32 * (i / 2) + 4 * g + 2 * (i & 1);
 #pragma unroll
-        for (int w = 0; w < kAWarps; w++) reference = fmaxf(reference, mm[w * kACols + col]);
+        for (int u = 0; u < 2; u++) {
+            const int col = 2 * t + u, pair = pair0 + col;
+            if (col >= n_pairs) continue;
+            const float l = u ? total.y : total.x, r = u ? reference.y : reference.x, inv = l == 0.0f ? 0.0f : 1.0f / l;
+            const float x = l == 0.0f ? 0.0f : (u ? v.y : v.x) * inv, y = l == 0.0f ? 0.0f : (u ? v.w : v.z) * inv;
+            const int row = pair / a.group, head = kv_head * a.group + pair - row * a.group;
+            T *to = out.data + seq * out.seq + row * out.row + head * out.head + d;
+            if (a.wide_out) {
+                if constexpr (sizeof(T) == 4) *reinterpret_cast<float2 *>(to) = make_float2(x, y);
+                else *reinterpret_cast<uint32_t *>(to) = serve_pack(x, y, to);
+            } else {
+                serve_put(to, x);
+                serve_put(to + 1, y);
+            }
+            if (d == 0 && a.lse) a.lse[((size_t)seq * a.max_rows + row) * a.heads + head] = l == 0.0f ? -INFINITY : (r + 8.0f + log2f(l)) * 0.69314718f;
+        }
+    };
+    /* a part's factor against a reference; parts without weights have none */
+    auto factor = [](float m, float reference) { return m > -INFINITY || m != m ? exp2_fast(m - reference) : 0.0f; };
+    {
+        float2 reference = make_float2(-INFINITY, -INFINITY), total = make_float2(0.0f, 0.0f), f[kAWarps];
 #pragma unroll
         for (int w = 0; w < kAWarps; w++) {
-            const float m = mm[w * kACols + col], f = m > -INFINITY ? exp2_fast(m - reference) : 0.0f;
-            const float l = ml[w * kACols + col];
-            total += l != 0.0f ? l * f : 0.0f;           /* NaN stays */
-            value += mo[(w * kACols + col) * kDim + d] * f;
+            f[w] = mm[w * 4 + t];
+            reference.x = fmaxf(reference.x, f[w].x);
+            reference.y = fmaxf(reference.y, f[w].y);
         }
-        if (used == 1) {
-            finish(col, d, value, total, reference);
-        } else {
-            part[col * (kDim + 2) + d] = value;
-            if (d == 0) {
-                part[col * (kDim + 2) + kDim] = reference;
-                part[col * (kDim + 2) + kDim + 1] = total;
+#pragma unroll
+        for (int w = 0; w < kAWarps; w++) {
+            const float2 l = ml[w * 4 + t];
+            f[w] = make_float2(factor(f[w].x, reference.x), factor(f[w].y, reference.y));
+            total.x += l.x * f[w].x;
+            total.y += l.y * f[w].y;
+        }
+        for (int i = warp; i < 2 * NB; i += kAWarps) {
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < kAWarps; w++) {
+                const float4 x = mo[(w * 2 * NB + i) * 32 + lane];
+                v.x = fmaf(x.x, f[w].x, v.x);
+                v.y = fmaf(x.y, f[w].y, v.y);
+                v.z = fmaf(x.z, f[w].x, v.z);
+                v.w = fmaf(x.w, f[w].y, v.w);
             }
+            if (used == 1) finish(i, v, total, reference);
+            else reinterpret_cast<float4 *>(parts + split * kPart)[i * 32 + lane] = v;
+        }
+        if (used == 1) return;
+        if (warp == 0 && g == 0) {
+            float2 *to = reinterpret_cast<float2 *>(parts + split * kPart + kACols * kDim);
+            to[t] = reference;
+            to[4 + t] = total;
         }
     }
-    if (used == 1) return;
     /* the CTA that comes last joins the parts, in their order whoever that is */
     __threadfence();
     __syncthreads();
@@ -523,89 +550,162 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(co
     }
     __syncthreads();
     if (!is_last) return;
-    const float *parts = a.part + (size_t)unit * a.splits * kACols * (kDim + 2);
-    for (int x = tid; x < n_pairs * kDim; x += kAThreads) {
-        const int col = x / kDim, d = x - col * kDim;
-        float reference = -INFINITY, value = 0.0f, total = 0.0f;
-        for (int w = 0; w < used; w++) reference = fmaxf(reference, __ldcg(parts + (w * kACols + col) * (kDim + 2) + kDim));
+    float2 *ends = reinterpret_cast<float2 *>(a_smem);               /* references and sums of all parts; then factors in their place */
+    for (int x = tid; x < used * 8; x += kAThreads) ends[x] = __ldcg(reinterpret_cast<const float2 *>(parts + (x >> 3) * kPart + kACols * kDim) + (x & 7));
+    __syncthreads();
+    float2 reference = make_float2(-INFINITY, -INFINITY), total = make_float2(0.0f, 0.0f);
+    for (int w = 0; w < used; w++) {
+        const float2 m = ends[w * 8 + t];
+        reference.x = fmaxf(reference.x, m.x);
+        reference.y = fmaxf(reference.y, m.y);
+    }
+    for (int w = 0; w < used; w++) {
+        const float2 m = ends[w * 8 + t], l = ends[w * 8 + 4 + t];
+        total.x += l.x * factor(m.x, reference.x);
+        total.y += l.y * factor(m.y, reference.y);
+    }
+    for (int i = warp; i < 2 * NB; i += kAWarps) {
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
         for (int w = 0; w < used; w++) {
-            const float *pw = parts + (w * kACols + col) * (kDim + 2);
-            const float m = __ldcg(pw + kDim), f = m > -INFINITY ? exp2_fast(m - reference) : 0.0f, l = __ldcg(pw + kDim + 1);
-            total += l != 0.0f ? l * f : 0.0f;
-            value += __ldcg(pw + d) * f;
+            const float4 x = __ldcg(reinterpret_cast<const float4 *>(parts + w * kPart) + i * 32 + lane);
+            const float2 m = ends[w * 8 + t];
+            const float fx = factor(m.x, reference.x), fy = factor(m.y, reference.y);
+            v.x = fmaf(x.x, fx, v.x);
+            v.y = fmaf(x.y, fy, v.y);
+            v.z = fmaf(x.z, fx, v.z);
+            v.w = fmaf(x.w, fy, v.w);
         }
-        finish(col, d, value, total, reference);
+        finish(i, v, total, reference);
     }
 }
 
-/* mass_out of 256 tokens a CTA: the scores again, now that the rows' sums are known, with the rows in turn. No atomics. */
+/* mass_out: the scores again, now that the rows' sums are known (in the attention kernel only the last CTA of a split sequence knows them,
+ * and keeping scores takes memory for every row). A CTA has up to four tiles of tokens a warp, whose keys stay in shared memory while the
+ * (row, head) pairs come by, 64 at a time, made by a warp each. A token's weights are summed in one order: no atomics. */
+constexpr int kMTiles = 4;
+
 template <int NB, class T>
-__global__ void __launch_bounds__(kAThreads) kv4_mass_kernel(const AttnArgs a, const ServeRows<T> q) {
-    constexpr int QT = sizeof(T) == 4 ? 2 : 1;
-    __shared__ __align__(16) uint2 q_s[NB * 2 * QT * 32];
-    __shared__ float mul_s[kACols], lse_s[kACols];
+struct MCfg {
+    static constexpr int QT = sizeof(T) == 4 ? 2 : 1;
+    static constexpr int kTile = kAKeys * NB * 17;                                  /* codes, scales */
+    static constexpr int kQ = NB * 2 * QT * 32 * 8;                                 /* eight pairs */
+    static constexpr int smem(int tiles) { return kAWarps * (tiles * kTile + kQ); }
+};
+
+template <int NB, class T>
+__global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_mass_kernel(const AttnArgs a, const ServeRows<T> q, int warp_tiles) {
+    using Cfg = MCfg<NB, T>;
+    constexpr int QT = Cfg::QT;
+    extern __shared__ __align__(128) unsigned char a_smem[];
+    __shared__ __align__(8) uint64_t full[kAWarps];
+    __shared__ float mul_s[kAWarps * kACols], lse_s[kAWarps * kACols];
+    __shared__ int abort_flag;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int kv_head = blockIdx.y, seq = blockIdx.z;
     const Kv4Span span = kv4_span(a.lengths, a.rows, a.max_rows, seq, a.c.capacity);
     const int pairs = span.rows * a.group, before = span.length - span.rows;
-    const int cta0 = blockIdx.x * kAWarps * kAKeys, j0 = cta0 + warp * kAKeys;
+    const int cta0 = blockIdx.x * kAWarps * warp_tiles * kAKeys;
     if (cta0 >= span.length) return;
-    uint32_t w[2][2][NB], f[2][2][NB];
-#pragma unroll
-    for (int m = 0; m < 2; m++)
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const size_t row = a.c.row(seq, kv_head, min(j0 + m * 16 + u * 8 + g, span.length - 1));
-            get_words<NB>(a.c.k + row * (NB * 16) + t * (NB * 4), w[m][u]);
-            get_bytes<NB>(a.c.ks + row * NB, f[m][u]);
-        }
-    float mass[2][2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
-    /* rows before this CTA's first token see none of its tokens */
-    const int first = max(0, cta0 - before) * a.group / kACols * kACols;
-    for (int pair0 = first; pair0 < pairs; pair0 += kACols) {
-        __syncthreads();
-        if (warp == 0) make_queries<NB, QT>(q, a, seq, kv_head, pair0, pairs, q_s, mul_s);
-        if (tid >= 32 && tid < 32 + kACols) {
-            const int pair = pair0 + tid - 32, row = pair / a.group;
-            const float lse = pair < pairs ? a.lse[((size_t)seq * a.max_rows + row) * a.heads + kv_head * a.group + pair - row * a.group] : 0.0f;
-            lse_s[tid - 32] = lse == -INFINITY ? INFINITY : lse * 1.44269504f;       /* a row without weights gives none */
-        }
-        __syncthreads();
-        float s[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
-#pragma unroll
-        for (int b = 0; b < NB; b++) {
-            uint2 qf[2][QT];
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int u = 0; u < QT; u++) qf[h][u] = q_s[((b * 2 + h) * QT + u) * 32 + lane];
-#pragma unroll
-            for (int m = 0; m < 2; m++)
-                block_scores<NB, QT>(s[m], w[m][0][b], w[m][1][b], __uint_as_float(f[m][0][b] << 23), __uint_as_float(f[m][1][b] << 23), qf);
-        }
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const int col = 2 * t + u, pair = pair0 + col;
-            const int sees = pair < pairs ? before + pair / a.group + 1 : 0;
-            const float mul = mul_s[col], lse = lse_s[col];
-#pragma unroll
-            for (int m = 0; m < 2; m++)
-#pragma unroll
-                for (int r = 0; r < 2; r++)
-                    if (j0 + m * 16 + r * 8 + g < sees) mass[m][r] += exp2_fast(s[m][2 * r + u] * mul - lse);
+    const int tile0 = (blockIdx.x * kAWarps + warp) * warp_tiles, tiles = min(warp_tiles, (span.length + kAKeys - 1) / kAKeys - tile0);
+    unsigned char *keys = a_smem + warp * warp_tiles * Cfg::kTile;
+    uint2 *q_s = reinterpret_cast<uint2 *>(a_smem + kAWarps * warp_tiles * Cfg::kTile);
+    if (lane == 0) {
+        vb_mbar_init(&full[warp], 1);
+        vb_mbar_init_fence();
+        if (tiles > 0) {
+            const size_t row = a.c.row(seq, kv_head, tile0 * kAKeys);
+            vb_mbar_arrive_expect_tx(&full[warp], tiles * Cfg::kTile);
+            vb_bulk_g2s(keys, a.c.k + row * (NB * 16), tiles * kAKeys * NB * 16, &full[warp]);
+            vb_bulk_g2s(keys + warp_tiles * kAKeys * NB * 16, a.c.ks + row * NB, tiles * kAKeys * NB, &full[warp]);
         }
     }
+    if (tid == 0) abort_flag = 0;
+    __syncthreads();
+    float mass[kMTiles][2][2];
+#pragma unroll
+    for (int i = 0; i < kMTiles; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) mass[i][j >> 1][j & 1] = 0.0f;
+    bool here = tiles <= 0;
+    /* rows before this CTA's first token see none of its tokens */
+    for (int group0 = max(0, cta0 - before) * a.group / kACols * kACols; group0 < pairs; group0 += kAWarps * kACols) {
+        __syncthreads();                                                            /* the pairs before are done with */
+        const int made = min(kAWarps, (pairs - group0 + kACols - 1) / kACols);
+        if (warp < made) make_queries<NB, QT>(q, a, seq, kv_head, group0 + warp * kACols, pairs, q_s + warp * (Cfg::kQ / 8), mul_s + warp * kACols);
+        if (tid < kAWarps * kACols) {
+            const int pair = group0 + tid, row = pair / a.group;
+            const float lse = pair < pairs ? a.lse[((size_t)seq * a.max_rows + row) * a.heads + kv_head * a.group + pair - row * a.group] : 0.0f;
+            lse_s[tid] = lse == -INFINITY ? INFINITY : lse * 1.44269504f;           /* a row without weights gives none */
+        }
+        __syncthreads();
+        if (!here) {
+            if (!__all_sync(0xffffffffu, vb_mbar_wait(&full[warp], 0u, &abort_flag))) {
+                atomicCAS(a.status, 0, kAStatus);
+                *(volatile int *)&abort_flag = 1;
+                volatile int stay = 0;
+                vb_mbar_wait(&full[warp], 0u, &stay);
+            }
+            here = true;
+        }
+#pragma unroll
+        for (int i = 0; i < kMTiles; i++) {
+            if (i >= tiles) break;
+            const unsigned char *ks = keys + i * kAKeys * NB * 16, *kss = keys + (warp_tiles * 16 + i) * kAKeys * NB;
+            const int j0 = (tile0 + i) * kAKeys;
+            uint32_t w[2][2][NB], f[2][2][NB];
+#pragma unroll
+            for (int m = 0; m < 2; m++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const int key = m * 16 + u * 8 + g;
+                    get_words<NB>(ks + key * (NB * 16) + t * (NB * 4), w[m][u]);
+                    get_bytes<NB>(kss + key * NB, f[m][u]);
+                }
+#pragma unroll 1
+            for (int r = 0; r < made; r++) {
+                float s[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    uint2 qf[2][QT];
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+#pragma unroll
+                        for (int u = 0; u < QT; u++) qf[h][u] = q_s[r * (Cfg::kQ / 8) + ((b * 2 + h) * QT + u) * 32 + lane];
+#pragma unroll
+                    for (int m = 0; m < 2; m++)
+                        block_scores<NB, QT>(s[m], w[m][0][b], w[m][1][b], __uint_as_float(f[m][0][b] << 23), __uint_as_float(f[m][1][b] << 23), qf);
+                }
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const int col = r * kACols + 2 * t + u, pair = group0 + col;
+                    const int sees = pair < pairs ? before + pair / a.group + 1 : 0;
+                    const float mul = mul_s[col], lse = lse_s[col];
+#pragma unroll
+                    for (int m = 0; m < 2; m++)
+#pragma unroll
+                        for (int k = 0; k < 2; k++)
+                            if (j0 + m * 16 + k * 8 + g < sees) mass[i][m][k] += exp2_fast(s[m][2 * k + u] * mul - lse);
+                }
+            }
+        }
+    }
+    if (!here) vb_mbar_wait(&full[warp], 0u, &abort_flag);                          /* no rows: nothing leaves while its keys are on their way */
     const size_t base = ((size_t)seq * a.c.kv_heads + kv_head) * a.c.capacity;
 #pragma unroll
-    for (int m = 0; m < 2; m++)
+    for (int i = 0; i < kMTiles; i++) {
+        if (i >= tiles) break;
 #pragma unroll
-        for (int r = 0; r < 2; r++) {
-            float v = mass[m][r];
-            v += __shfl_xor_sync(0xffffffffu, v, 1);
-            v += __shfl_xor_sync(0xffffffffu, v, 2);
-            const int j = j0 + m * 16 + r * 8 + g;
-            if (t == 0 && j < span.length) a.mass_out[base + j] = v + (a.mass_in && j < before ? a.mass_in[base + j] : 0.0f);
-        }
+        for (int m = 0; m < 2; m++)
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                float v = mass[i][m][r];
+                v += __shfl_xor_sync(0xffffffffu, v, 1);
+                v += __shfl_xor_sync(0xffffffffu, v, 2);
+                const int j = (tile0 + i) * kAKeys + m * 16 + r * 8 + g;
+                if (t == 0 && j < span.length) a.mass_out[base + j] = v + (a.mass_in && j < before ? a.mass_in[base + j] : 0.0f);
+            }
+    }
 }
 
 template <class T>
@@ -618,17 +718,23 @@ int attn_launch(const AttnArgs &args, const vb200_kv4_attention_t &v, const Kv4W
     AttnArgs a = args;
     const ServeRows<T> q = serve_rows<T>(v.q), out = serve_rows<T>(v.out);
     a.wide = serve_wide(q);
+    a.wide_out = serve_wide(out);
     if (a.max_rows > 0) {
         /* as many splits as fill the GPU with what runs at once, none of them under a tile a warp */
         const long long row_tiles = ((long long)a.max_rows * a.group + kACols - 1) / kACols;
         const long long units = row_tiles * a.c.kv_heads * a.c.seqs, at_once = (long long)work.sm_count * (NB <= 4 ? 2 : 1);
         const long long most = ((long long)a.c.capacity + kAKeys * kAWarps - 1) / (kAKeys * kAWarps);
-        a.splits = (int)std::max(1ll, std::min(at_once / units, most));
+        a.splits = (int)std::max(1ll, std::min({at_once / units, most, (long long)kAMaxSplits}));
         kv4_attn_kernel<NB, PT, T><<<dim3((unsigned)(row_tiles * a.splits), a.c.kv_heads, a.c.seqs), kAThreads, Cfg::kBig, st>>>(a, q, out);
         if (serve_launched()) return -1;
     }
     if (a.mass_out) {
-        kv4_mass_kernel<NB, T><<<dim3((a.c.capacity + kAKeys * kAWarps - 1) / (kAKeys * kAWarps), a.c.kv_heads, a.c.seqs), kAThreads, 0, st>>>(a, q);
+        /* the more tiles a warp has, the fewer CTAs make the queries: as many as leave every SM two CTAs */
+        const long long heads = (long long)a.c.kv_heads * a.c.seqs, tiles = ((long long)a.c.capacity + kAKeys - 1) / kAKeys;
+        int warp_tiles = kMTiles;
+        while (warp_tiles > 1 && tiles / (kAWarps * warp_tiles) * heads < 2 * work.sm_count) warp_tiles >>= 1;
+        kv4_mass_kernel<NB, T><<<dim3((unsigned)((tiles + kAWarps * warp_tiles - 1) / (kAWarps * warp_tiles)), a.c.kv_heads, a.c.seqs), kAThreads,
+                                 MCfg<NB, T>::smem(warp_tiles), st>>>(a, q, warp_tiles);
         return serve_launched();
     }
     return 0;
@@ -654,9 +760,8 @@ int attn_dims(const AttnArgs &a, const vb200_kv4_attention_t &v, const Kv4Work &
 /* Loads the kernels of a head size on the current device, and lets them have their shared memory. */
 template <int NB, class T>
 int attn_load() {
-    cudaFuncAttributes f;
     return cudaFuncSetAttribute(kv4_attn_kernel<NB, kWeightTerms<T>, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, ACfg<NB>::kBig) == cudaSuccess &&
-                   cudaFuncGetAttributes(&f, kv4_mass_kernel<NB, T>) == cudaSuccess
+                   cudaFuncSetAttribute(kv4_mass_kernel<NB, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, MCfg<NB, T>::smem(kMTiles)) == cudaSuccess
                ? 0
                : -1;
 }
