@@ -7,7 +7,7 @@
 #include <new>
 #include <string>
 
-#include "vb_serve.cuh"
+#include "vb_kv4.cuh"
 
 namespace vb {
 
@@ -37,17 +37,6 @@ bool serve_on_device(const void *p) {
 }
 
 namespace {
-
-/* One of 32, 64, 96, 128, 192, 256 values a head, as a constant */
-#define VB_KV4_DIMS(blocks, call) \
-    switch (blocks) {             \
-    case 1: return call(1);       \
-    case 2: return call(2);       \
-    case 3: return call(3);       \
-    case 4: return call(4);       \
-    case 6: return call(6);       \
-    default: return call(8);      \
-    }
 
 constexpr int kRowThreads = 256, kRowUnroll = 4;
 

@@ -19,7 +19,7 @@
  */
 #include <algorithm>
 
-#include "vb_serve.cuh"
+#include "vb_kv4.cuh"
 
 namespace vb {
 
@@ -27,8 +27,8 @@ namespace {
 
 constexpr int kAWarps = 8, kAThreads = 32 * kAWarps, kACols = 8, kAKeys = 32;
 constexpr int kAStatus = 61;
+constexpr int kAMostPairs = 64;               /* of a KV head: more take the kernel of vb_kv4_prompt.cu, heads up to 128 */
 constexpr int kAMaxSplits = 64;               /* a CTA joins them */
-constexpr float kABias = 7.0f;                /* weights times 2^7 */
 
 template <int NB>
 struct ACfg {
@@ -43,19 +43,6 @@ struct ACfg {
     static constexpr int kVScales = kWhole ? 1 : NB;                            /* scales of a lane's part of a value row */
 };
 
-struct AttnArgs {
-    Kv4 c;
-    const int *lengths, *rows;
-    int max_rows, heads, group, splits, wide, wide_out;
-    float scale;
-    float *lse;
-    const float *mass_in;
-    float *mass_out;
-    float *part;
-    unsigned *tickets;
-    int *status;
-};
-
 VB_DEVINL void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -65,60 +52,6 @@ VB_DEVINL uint32_t mat_turn(uint32_t v) {
     uint32_t r;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
-}
-VB_DEVINL uint32_t half_mul(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
-VB_DEVINL uint32_t half_pack(float a, float b) { return serve_pack(a, b, (const __half *)nullptr); }
-VB_DEVINL float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-/* N bytes side by side (aligned to N's largest power of two) */
-template <int N>
-VB_DEVINL void get_bytes(const uint8_t *p, uint32_t (&b)[N]) {
-    if constexpr (N % 4 == 0) {
-#pragma unroll
-        for (int i = 0; i < N / 4; i++) {
-            const uint32_t w = reinterpret_cast<const uint32_t *>(p)[i];
-#pragma unroll
-            for (int j = 0; j < 4; j++) b[4 * i + j] = (w >> (8 * j)) & 255u;
-        }
-    } else if constexpr (N % 2 == 0) {
-#pragma unroll
-        for (int i = 0; i < N / 2; i++) {
-            const uint32_t w = reinterpret_cast<const uint16_t *>(p)[i];
-            b[2 * i] = w & 255u;
-            b[2 * i + 1] = w >> 8;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i++) b[i] = p[i];
-    }
-}
-/* N words side by side (aligned to N's largest power of two, up to four) */
-template <int N>
-VB_DEVINL void get_words(const uint8_t *p, uint32_t (&w)[N]) {
-    if constexpr (N % 4 == 0) {
-#pragma unroll
-        for (int i = 0; i < N / 4; i++) {
-            const uint4 v = reinterpret_cast<const uint4 *>(p)[i];
-            w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
-        }
-    } else if constexpr (N % 2 == 0) {
-#pragma unroll
-        for (int i = 0; i < N / 2; i++) {
-            const uint2 v = reinterpret_cast<const uint2 *>(p)[i];
-            w[2 * i] = v.x; w[2 * i + 1] = v.y;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i++) w[i] = reinterpret_cast<const uint32_t *>(p)[i];
-    }
 }
 /* A lane's part of a value row, 2 NB bytes, as words (the last one's upper half zero where NB is odd) */
 template <int NB>
@@ -136,7 +69,7 @@ VB_DEVINL void get_values(const uint8_t *p, uint32_t (&w)[(NB + 1) / 2]) {
 /* Eight (row, head) pairs as the B operand of K Q^T, by one warp, into q_s [block][half][term][lane]; what S is to be multiplied by
  * to be a power of two, a column each, into mul_s. */
 template <int NB, int QT, class T>
-VB_DEVINL void make_queries(const ServeRows<T> &q, const AttnArgs &a, int seq, int kv_head, int pair0, int pairs, uint2 *q_s, float *mul_s) {
+VB_DEVINL void make_queries(const ServeRows<T> &q, const Kv4Attn &a, int seq, int kv_head, int pair0, int pairs, uint2 *q_s, float *mul_s) {
     const int lane = threadIdx.x & 31, n = lane >> 2, t = lane & 3, pair = pair0 + n;
     const bool real = pair < pairs;
     const int row = real ? pair / a.group : 0, head = kv_head * a.group + (real ? pair - row * a.group : 0);
@@ -195,7 +128,7 @@ VB_DEVINL void block_scores(float (&s)[4], const uint32_t wa, const uint32_t wb,
 
 /* grid = (row tiles x splits, kv heads, sequences) */
 template <int NB, int PT, class T>
-__global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(const AttnArgs a, const ServeRows<T> q, const ServeRows<T> out) {
+__global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(const Kv4Attn a, const ServeRows<T> q, const ServeRows<T> out) {
     using Cfg = ACfg<NB>;
     constexpr int QT = sizeof(T) == 4 ? 2 : 1, kDim = Cfg::kDim, kW = (NB + 1) / 2, kVS = Cfg::kVScales;
     extern __shared__ __align__(128) unsigned char a_smem[];
@@ -337,7 +270,7 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(co
         }
         /* weights, turned into the B operand of V^T P^T */
         uint2 p[2][PT];
-        const float low0 = ref[0] > -INFINITY ? ref[0] - kABias : 0.0f, low1 = ref[1] > -INFINITY ? ref[1] - kABias : 0.0f;
+        const float low0 = ref[0] > -INFINITY ? ref[0] - kKv4Bias : 0.0f, low1 = ref[1] > -INFINITY ? ref[1] - kKv4Bias : 0.0f;
 #pragma unroll
         for (int m = 0; m < 2; m++) {
             float e[4];
@@ -594,7 +527,7 @@ struct MCfg {
 };
 
 template <int NB, class T>
-__global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_mass_kernel(const AttnArgs a, const ServeRows<T> q, int warp_tiles) {
+__global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_mass_kernel(const Kv4Attn a, const ServeRows<T> q, int warp_tiles) {
     using Cfg = MCfg<NB, T>;
     constexpr int QT = Cfg::QT;
     extern __shared__ __align__(128) unsigned char a_smem[];
@@ -708,18 +641,17 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_mass_kernel(co
     }
 }
 
-template <class T>
-constexpr int kWeightTerms = std::is_same<T, __nv_bfloat16>::value ? 1 : 2;
-
 template <int NB, class T>
-int attn_launch(const AttnArgs &args, const vb200_kv4_attention_t &v, const Kv4Work &work, cudaStream_t st) {
+int attn_launch(const Kv4Attn &args, const vb200_kv4_attention_t &v, const Kv4Work &work, cudaStream_t st) {
     using Cfg = ACfg<NB>;
     constexpr int PT = kWeightTerms<T>;
-    AttnArgs a = args;
+    Kv4Attn a = args;
     const ServeRows<T> q = serve_rows<T>(v.q), out = serve_rows<T>(v.out);
     a.wide = serve_wide(q);
     a.wide_out = serve_wide(out);
-    if (a.max_rows > 0) {
+    if (NB <= 4 && (long long)a.max_rows * a.group > kAMostPairs) {
+        if (kv4_prompt(a, q, out, st)) return -1;
+    } else if (a.max_rows > 0) {
         /* as many splits as fill the GPU with what runs at once, none of them under a tile a warp */
         const long long row_tiles = ((long long)a.max_rows * a.group + kACols - 1) / kACols;
         const long long units = row_tiles * a.c.kv_heads * a.c.seqs, at_once = (long long)work.sm_count * (NB <= 4 ? 2 : 1);
@@ -740,18 +672,8 @@ int attn_launch(const AttnArgs &args, const vb200_kv4_attention_t &v, const Kv4W
     return 0;
 }
 
-#define VB_KV4_DIMS(blocks, call) \
-    switch (blocks) {             \
-    case 1: return call(1);       \
-    case 2: return call(2);       \
-    case 3: return call(3);       \
-    case 4: return call(4);       \
-    case 6: return call(6);       \
-    default: return call(8);      \
-    }
-
 template <class T>
-int attn_dims(const AttnArgs &a, const vb200_kv4_attention_t &v, const Kv4Work &w, cudaStream_t st) {
+int attn_dims(const Kv4Attn &a, const vb200_kv4_attention_t &v, const Kv4Work &w, cudaStream_t st) {
 #define VB_CALL(n) attn_launch<n, T>(a, v, w, st)
     VB_KV4_DIMS(a.c.blocks, VB_CALL)
 #undef VB_CALL
@@ -769,13 +691,14 @@ int attn_load() {
 } // namespace
 
 int kv4_attention_load(int blocks) {
+    if (kv4_prompt_load(blocks)) return -1;
 #define VB_CALL(n) (attn_load<n, float>() || attn_load<n, __nv_bfloat16>() || attn_load<n, __half>() ? serve_launched() | -1 : 0)
     VB_KV4_DIMS(blocks, VB_CALL)
 #undef VB_CALL
 }
 
 int kv4_attention(const Kv4 &c, const Kv4Work &w, const vb200_kv4_attention_t &v, cudaStream_t st) {
-    AttnArgs a = {};
+    Kv4Attn a = {};
     a.c = c;
     a.lengths = v.lengths; a.rows = v.rows; a.max_rows = v.max_rows; a.heads = v.heads; a.group = v.heads / c.kv_heads;
     a.scale = v.scale; a.lse = v.lse; a.mass_in = v.mass_in; a.mass_out = v.mass_out;

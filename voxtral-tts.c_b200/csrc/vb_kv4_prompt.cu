@@ -1,0 +1,489 @@
+/*
+ * vb_kv4_prompt.cu - softmax attention over the 4-bit cache for many rows, on the 5th-generation tensor cores.
+ *
+ * A CTA owns one KV head and 128 (row, query head) pairs and walks the tokens 128 at a time:
+ *
+ *   S [128 x 128]   = Q K^T    Q in shared memory, one FP16 term (bf16, fp16) or two (fp32), rows brought to [2^14, 2^15)
+ *   O [128 x dim]  += P V      P in TMEM, in S's own columns, one term (bf16) or two; V rows [token][dim] are an MN-major operand
+ *
+ * Keys and values go from codes to FP16 on the way to shared memory, four warps for the keys and two for the values: keys times 2^(e - S + 13), S the largest
+ * scale of a warp's 32 tokens, which the softmax undoes, values times 2^(e - E + 13), E the largest scale so far, on which the
+ * accumulator is based (exact down to 2^-36 of the largest). Scores, weights, sums as in vb_kv4_attn.cu. Two warpgroups take
+ * alternate tiles with a reference, sums and an accumulator each, merged at the end, so that the tensor pipe works on one tile while the
+ * other is in its softmax.
+ *
+ * Warps: 0-3, 4-7 softmax, 8-11 keys, 12-13 values, 14 issues the MMAs. All waits are bounded.
+ */
+#include <type_traits>
+
+#include "vb_attn_tc.cuh"
+#include "vb_kv4.cuh"
+
+namespace vb {
+
+namespace {
+
+constexpr int kPRows = 128, kPKeys = 128, kPThreads = 480, kPMmaWarp = 14, kPBlock = kPKeys * 128, kPStatus = 62, kPRing = 8;
+constexpr uint32_t kPTmem = 512, kPO = 256;
+
+template <int NB, int QT>
+struct PCfg {
+    static constexpr int kD64 = (NB + 1) / 2;                                  /* blocks of 64 columns */
+    static constexpr int kSlot = kD64 * kPBlock;
+    static constexpr int kSlots = kD64 * QT >= 4 ? 2 : 3;
+    static constexpr int kQ = QT * kSlot;
+    static constexpr int kSmem = kQ + 2 * kSlots * kSlot + 1024;
+    static constexpr int kLd = NB * 32 + 4;                                    /* results on their way out: a row */
+    static_assert(kPRows * kLd * 4 + 2 * kPRows * 16 <= 2 * kSlots * kSlot, "results do not fit the rings");
+    static_assert(kSmem <= 232448 - 2048, "over what a CTA may use");
+};
+
+VB_DEVINL uint64_t p_desc_mn(uint32_t addr) {
+    uint64_t d = (uint64_t)((addr >> 4) & 0x3FFF);
+    d |= (uint64_t)(kPBlock >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+/* kind::f16 with FP16 operands, fp32 sums, 128 rows, n columns */
+VB_DEVINL uint32_t p_idesc(int n, bool mn_major) { return (1u << 4) | (mn_major ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kPRows >> 4) << 24); }
+
+/* Eight codes times a power of two to 16 bytes */
+VB_DEVINL uint4 p_halves(uint32_t w, uint32_t f) {
+    uint32_t r[4];
+    kv4_halves(w, r);
+    return make_uint4(half_mul(r[0], f), half_mul(r[1], f), half_mul(r[2], f), half_mul(r[3], f));
+}
+/* 2^(byte - top + 13) twice; byte <= top */
+VB_DEVINL uint32_t p_factor(int byte, int top) {
+    const float f = __uint_as_float((uint32_t)max(byte + 140 - top, 0) << 23);
+    return half_pack(f, f);
+}
+
+template <int NB, int PT, class T>
+__global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn a, const ServeRows<T> q, const ServeRows<T> out) {
+    constexpr int QT = sizeof(T) == 4 ? 2 : 1, kDim = NB * 32;
+    using Cfg = PCfg<NB, QT>;
+    extern __shared__ unsigned char p_smem_raw[];
+    unsigned char *base = (unsigned char *)(((uintptr_t)p_smem_raw + 1023) & ~(uintptr_t)1023);
+    unsigned char *q_s = base, *k_s = q_s + Cfg::kQ, *v_s = k_s + Cfg::kSlots * Cfg::kSlot;
+    __shared__ __align__(8) uint64_t k_full[Cfg::kSlots], k_empty[Cfg::kSlots], v_full[Cfg::kSlots], v_empty[Cfg::kSlots], s_full[2], p_full[2], o_done[2], q_full;
+    __shared__ float key_up[kPRing][4], down_s[kPRows];
+    __shared__ int value_top[kPRing], bad_s[NB], abort_s;
+    __shared__ uint32_t tmem_slot;
+    int *abort_flag = &abort_s;
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int kv_head = blockIdx.y, seq = blockIdx.z;
+    const Kv4Span span = kv4_span(a.lengths, a.rows, a.max_rows, seq, a.c.capacity);
+    const int pairs = span.rows * a.group;
+    const int pair0 = ((int)gridDim.x - 1 - (int)blockIdx.x) * kPRows;             /* the latest rows see the most tokens: they go first */
+    if (pair0 >= pairs) return;
+    const int n_pairs = min(kPRows, pairs - pair0), before = span.length - span.rows;
+    const int all_see = before + pair0 / a.group + 1, seen = max(0, before + (pair0 + n_pairs - 1) / a.group + 1);
+    const int n_tiles = (seen + kPKeys - 1) / kPKeys;
+    if (tid == 0) {
+        for (int i = 0; i < Cfg::kSlots; i++) {
+            vb_mbar_init(&k_full[i], 4);
+            vb_mbar_init(&v_full[i], 2);
+            vb_mbar_init(&k_empty[i], 1);
+            vb_mbar_init(&v_empty[i], 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            vb_mbar_init(&s_full[i], 1);
+            vb_mbar_init(&p_full[i], 128);
+            vb_mbar_init(&o_done[i], 1);
+        }
+        vb_mbar_init(&q_full, 256);
+        abort_s = 0;
+        vb_mbar_init_fence();
+    }
+    if (tid < NB) bad_s[tid] = 1 << 30;
+    if (warp == kPMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(vb_smem_u32(&tmem_slot)), "r"(kPTmem) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *(volatile uint32_t *)&tmem_slot;
+    auto give_up = [&]() {
+        atomicCAS(a.status, 0, kPStatus);
+        *(volatile int *)abort_flag = 1;
+    };
+
+    if (warp < 8) {
+        /* ---- queries: a warp has rows warp, warp + 8, ..., eight at a time, a lane the values lane + 32 i ---- */
+#pragma unroll 1
+        for (int r0 = 0; r0 < kPRows / 8; r0 += 8) {
+            float x[8][NB];
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const int pair = pair0 + warp + 8 * (r0 + u);
+                const bool real = pair < pairs;
+                const int row = real ? pair / a.group : 0, head = kv_head * a.group + (real ? pair - row * a.group : 0);
+                const T *p = q.data + seq * q.seq + row * q.row + head * q.head + lane;
+#pragma unroll
+                for (int i = 0; i < NB; i++) x[u][i] = real ? serve_get(p + 32 * i) : 0.0f;
+            }
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const int r = warp + 8 * (r0 + u);
+                uint32_t most = 0;
+#pragma unroll
+                for (int i = 0; i < NB; i++) most = max(most, __float_as_uint(x[u][i]) & 0x7fffffffu);
+                most = __reduce_max_sync(0xffffffffu, most);
+                const uint32_t e = most >> 23, field = e == 0u || e == 255u ? 127u : min(268u - e, 253u);
+                const float up = __uint_as_float(field << 23);
+                if (lane == 0) down_s[r] = __uint_as_float((254u - field) << 23);
+#pragma unroll
+                for (int i = 0; i < NB; i++) {
+                    const int d = lane + 32 * i;
+                    const uint32_t at = (uint32_t)(d >> 6) * kPBlock + at_off(r, (d & 63) >> 3) + (d & 7) * 2;
+                    const float y = x[u][i] * up;
+                    const __half hi = __float2half_rn(y);
+                    *reinterpret_cast<__half *>(q_s + at) = hi;
+                    if constexpr (QT == 2) *reinterpret_cast<__half *>(q_s + Cfg::kSlot + at) = __float2half_rn(y - __half2float(hi));
+                }
+            }
+        }
+        at_proxy_fence();
+        vb_mbar_arrive(&q_full);
+        vb_named_bar(1, 256);                                      /* down_s */
+
+        /* ---- softmax: warpgroup w takes tiles w, w + 2, ...; a thread owns pair pair0 + r ---- */
+        const int w = warp >> 2, r = tid & 127, pair = pair0 + r;
+        const bool valid = r < n_pairs;
+        const int row = valid ? pair / a.group : 0, head = kv_head * a.group + (valid ? pair - row * a.group : 0);
+        const int sees = before + (pair0 + min(r, n_pairs - 1)) / a.group + 1;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, tS = tmem + lanes + (uint32_t)(w * kPKeys), tO = tmem + lanes + kPO + (uint32_t)(w * 128);
+        const float mul = a.scale * 1.44269504f * down_s[r];
+        float ref = -INFINITY, sum = 0.0f;
+        int top_scale = 0, it = 0;
+        for (int t = w; t < n_tiles; t += 2, it++) {
+            const int j0 = t * kPKeys;
+            if (!at_warp_wait(&s_full[w], (uint32_t)it & 1u, abort_flag)) { give_up(); break; }
+            tc_fence_after();
+            const float *ups = key_up[t % kPRing];
+            const int last = sees - j0;                            /* columns before this one are seen */
+            const bool masked = j0 + kPKeys > all_see;
+            float top = -INFINITY;
+#pragma unroll 1
+            for (int c = 0; c < 4; c++) {
+                const float up = ups[c] * mul;
+                uint32_t reg[32];
+                at_ld32(tS + (uint32_t)(c * 32), reg);
+                /* the largest product, or the smallest where the factor is negative */
+                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                const uint32_t turn = __float_as_uint(up) & 0x80000000u;
+#pragma unroll
+                for (int k = 0; k < 32; k++) {
+                    const float x = __uint_as_float(reg[k] ^ turn);
+                    m4[k & 3] = fmaxf(m4[k & 3], !masked || c * 32 + k < last ? x : -INFINITY);
+                }
+                const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), f = fabsf(up);
+                if (m > -INFINITY) top = fmaxf(top, m * f);
+            }
+            /* values: the scale that this tile is based on */
+            if (!at_warp_wait(&v_full[t % Cfg::kSlots], (uint32_t)(t / Cfg::kSlots) & 1u, abort_flag)) { give_up(); break; }
+            const int now_scale = value_top[t % kPRing];
+            const bool rise = top > ref + 8.0f;
+            if (__any_sync(0xffffffffu, rise) || now_scale != top_scale) {
+                const float now = rise ? top : ref, f = rise ? exp2_fast(ref - now) : 1.0f;      /* the first time: 0 */
+                if (it > 0) {
+                    if (!at_warp_wait(&o_done[w], (uint32_t)(it - 1) & 1u, abort_flag)) { give_up(); break; }
+                    tc_fence_after();
+                    const int fall = now_scale - top_scale;
+                    const float fo = fall > 126 ? 0.0f : f * __uint_as_float((uint32_t)(127 - fall) << 23);
+#pragma unroll 1
+                    for (int c = 0; c < NB; c++) {
+                        uint32_t reg[32];
+                        at_ld32(tO + (uint32_t)(c * 32), reg);
+#pragma unroll
+                        for (int k = 0; k < 32; k++) reg[k] = __float_as_uint(__uint_as_float(reg[k]) * fo);
+                        at_st32(tO + (uint32_t)(c * 32), reg);
+                    }
+                }
+                sum *= f;
+                ref = now;
+                top_scale = now_scale;
+            }
+            const float low = ref > -INFINITY ? ref - kKv4Bias : 0.0f;      /* nothing seen yet: every weight is 2^-inf */
+            float sum4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+            for (int c = 0; c < 4; c++) {
+                const float up = ups[c] * mul;
+                uint32_t reg[32], terms[32];
+                at_ld32(tS + (uint32_t)(c * 32), reg);
+#pragma unroll
+                for (int k = 0; k < 32; k += 2) {
+                    float p[2];
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        float x = fmaf(__uint_as_float(reg[k + u]), up, -low);
+                        if (masked && c * 32 + k + u >= last) x = -INFINITY;
+                        p[u] = exp2_fast(x);
+                        sum4[(k + u) & 3] += p[u];
+                    }
+                    const uint32_t hi = half_pack(p[0], p[1]);
+                    if constexpr (PT == 2) {
+                        const float2 f = kv4_f2(hi);
+                        terms[16 + k / 2] = half_pack(p[0] - f.x, p[1] - f.y);
+                    } else {
+                        terms[16 + k / 2] = 0u;
+                    }
+                    terms[k / 2] = hi;
+                }
+                at_st32(tS + (uint32_t)(c * 32), terms);           /* 16 columns of first terms, 16 of second ones */
+            }
+            sum += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+            at_st_wait();
+            tc_fence_before();
+            vb_mbar_arrive(&p_full[w]);
+        }
+        if (it > 0 && !at_warp_wait(&o_done[w], (uint32_t)(it - 1) & 1u, abort_flag)) give_up();
+        /* both halves of the tokens, merged, each warpgroup half of the columns, by way of shared memory */
+        vb_named_bar(1, 256);                                      /* every product is done: the rings are free */
+        float4 *ends = reinterpret_cast<float4 *>(k_s);            /* 2 x 128 x (reference, sum, scale) */
+        float *rows = reinterpret_cast<float *>(k_s + 2 * kPRows * 16);
+        ends[w * kPRows + r] = make_float4(ref, sum * 0x1p-15f, __int_as_float(top_scale), 0.0f);
+        tc_fence_before();
+        vb_named_bar(1, 256);
+        tc_fence_after();
+        const float4 A = ends[r], B = ends[kPRows + r];
+        const float reference = fmaxf(A.x, B.x);
+        float fa = A.x > -INFINITY ? exp2_fast(A.x - reference) : 0.0f, fb = B.x > -INFINITY ? exp2_fast(B.x - reference) : 0.0f;
+        const float total = A.y * fa + B.y * fb, inv = total == 0.0f ? 0.0f : 1.0f / total;
+        if (w == 0 && valid && a.lse)
+            a.lse[((size_t)seq * a.max_rows + row) * a.heads + head] = total == 0.0f ? -INFINITY : (reference + 8.0f + log2f(total)) * 0.69314718f;
+        fa *= inv;
+        fb *= inv;
+        const int ea = __float_as_int(A.z) - 155, eb = __float_as_int(B.z) - 155;      /* in two steps: 2^e may not be a normal number */
+        const float a0 = __uint_as_float((uint32_t)(127 + (ea >> 1)) << 23), a1 = __uint_as_float((uint32_t)(127 + ea - (ea >> 1)) << 23);
+        const float b0 = __uint_as_float((uint32_t)(127 + (eb >> 1)) << 23), b1 = __uint_as_float((uint32_t)(127 + eb - (eb >> 1)) << 23);
+#pragma unroll 1
+        for (int c = w; c < NB; c += 2) {
+            uint32_t oa[32], ob[32];
+            const bool nan = bad_s[c] < sees;
+            if (n_tiles > 0) at_ld32(tmem + lanes + kPO + (uint32_t)(c * 32), oa);
+            if (n_tiles > 1) at_ld32(tmem + lanes + kPO + 128u + (uint32_t)(c * 32), ob);
+#pragma unroll
+            for (int k = 0; k < 32; k++) {
+                float v = 0.0f;
+                if (n_tiles > 0) v = __uint_as_float(oa[k]) * a0 * fa * a1;
+                if (n_tiles > 1) v += __uint_as_float(ob[k]) * b0 * fb * b1;
+                if (total == 0.0f) v = 0.0f;
+                oa[k] = nan ? 0x7fffffffu : __float_as_uint(v);
+            }
+#pragma unroll
+            for (int k = 0; k < 32; k += 4) *reinterpret_cast<uint4 *>(rows + r * Cfg::kLd + c * 32 + k) = make_uint4(oa[k], oa[k + 1], oa[k + 2], oa[k + 3]);
+        }
+        vb_named_bar(1, 256);
+        /* out, eight values a lane */
+        constexpr int kEights = kDim / 8;
+        for (int x = tid; x < n_pairs * kEights; x += 256) {
+            const int p = x / kEights, d = (x - p * kEights) * 8, rr = (pair0 + p) / a.group, hh = kv_head * a.group + pair0 + p - rr * a.group;
+            const float4 lo = *reinterpret_cast<const float4 *>(rows + p * Cfg::kLd + d), hi = *reinterpret_cast<const float4 *>(rows + p * Cfg::kLd + d + 4);
+            const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+            serve_store<8>(out.data + seq * out.seq + rr * out.row + hh * out.head + d, a.wide_out, v);
+        }
+    } else if (warp < 12) {
+        /* ---- keys: a warp has 32 tokens of a tile, four lanes a token (words t * NB ..: values 8 t .. of every block) ---- */
+        const int lw = warp - 8, g = lane >> 2, tq = lane & 3;
+        const size_t row0 = a.c.row(seq, kv_head, 0);
+        uint32_t words[4][NB], bytes[4][NB];
+        auto fetch = [&](int t) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const size_t row = row0 + min(t * kPKeys + lw * 32 + i * 8 + g, a.c.slots - 1);
+                get_words<NB>(a.c.k + row * (NB * 16) + tq * (NB * 4), words[i]);
+                get_bytes<NB>(a.c.ks + row * NB, bytes[i]);
+            }
+        };
+        if (n_tiles > 0) fetch(0);
+        for (int t = 0; t < n_tiles; t++) {
+            const int slot = t % Cfg::kSlots, j0 = t * kPKeys + lw * 32;
+            int most = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    if (j0 + i * 8 + g >= seen) { words[i][b] = 0; bytes[i][b] = 0; }       /* whatever lies behind the last token */
+                    if (bytes[i][b] != 255u) most = max(most, (int)bytes[i][b]);
+                }
+            most = max((int)__reduce_max_sync(0xffffffffu, (unsigned)most), 14);          /* its undoing stays a normal number */
+            if (!at_warp_wait(&k_empty[slot], ((uint32_t)(t / Cfg::kSlots) & 1u) ^ 1u, abort_flag)) { give_up(); break; }
+            unsigned char *to = k_s + slot * Cfg::kSlot;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int r = lw * 32 + i * 8 + g;
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    uint4 v = p_halves(words[i][b], p_factor((int)bytes[i][b], most));
+                    if (bytes[i][b] == 255u) v.x = 0x7fff7fffu;            /* a block that is NaN: so is the score */
+                    const int chunk = 4 * b + tq;
+                    *reinterpret_cast<uint4 *>(to + (chunk >> 3) * kPBlock + at_off(r, chunk & 7)) = v;
+                }
+            }
+            if (lane == 0) key_up[t % kPRing][lw] = __uint_as_float((uint32_t)(most - 13) << 23);
+            if (t + 1 < n_tiles) fetch(t + 1);
+            at_proxy_fence();
+            __syncwarp();
+            if (lane == 0) vb_mbar_arrive(&k_full[slot]);
+        }
+    } else if (warp < kPMmaWarp) {
+        /* ---- values: a warp has 64 tokens of a tile, a lane blocks of them ---- */
+        const int lw = warp - 12;
+        const size_t row0 = a.c.row(seq, kv_head, 0);
+        uint32_t words[2 * NB][4], byte[2 * NB], all[4][NB];
+        auto fetch = [&](int j0) {
+#pragma unroll
+            for (int i = 0; i < 2 * NB; i++) {
+                const int x = i * 32 + lane, key = x / NB, b = x - key * NB;
+                const size_t row = row0 + min(j0 + lw * 64 + key, a.c.slots - 1);
+                const unsigned char *p = a.c.v + row * (NB * 16);
+                if constexpr (kv4_whole(NB)) {
+                    get_words<4>(p + b * 16, words[i]);
+                } else {
+                    const uint16_t *h = reinterpret_cast<const uint16_t *>(p) + b;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) words[i][k] = h[2 * k * NB] | ((uint32_t)h[(2 * k + 1) * NB] << 16);
+                }
+                byte[i] = a.c.vs[row * NB + b];
+            }
+            /* all scales of the tile, four tokens a lane: every warp finds the largest for itself */
+#pragma unroll
+            for (int i = 0; i < 4; i++) get_bytes<NB>(a.c.vs + (row0 + min(j0 + lane * 4 + i, a.c.slots - 1)) * NB, all[i]);
+        };
+        int top = 0;
+        if (n_tiles > 0) fetch(0);
+        for (int t = 0; t < n_tiles; t++) {
+            const int slot = t % Cfg::kSlots, j0 = t * kPKeys;
+            int most = 0;
+            bool bad = false;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+                    if (j0 + lane * 4 + i < seen) {
+                        if (all[i][b] != 255u) most = max(most, (int)all[i][b]);
+                        else bad = true;
+                    }
+            if (__any_sync(0xffffffffu, bad) && lw == 0) {         /* blocks that are NaN: the rows that see them; their codes are zeros */
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int b = 0; b < NB; b++)
+                        if (j0 + lane * 4 + i < seen && all[i][b] == 255u) atomicMin(&bad_s[b], j0 + lane * 4 + i);
+            }
+            top = max(top, (int)__reduce_max_sync(0xffffffffu, (unsigned)most));
+            if (!at_warp_wait(&v_empty[slot], ((uint32_t)(t / Cfg::kSlots) & 1u) ^ 1u, abort_flag)) { give_up(); break; }
+            unsigned char *to = v_s + slot * Cfg::kSlot;
+#pragma unroll
+            for (int i = 0; i < 2 * NB; i++) {
+                const int x = i * 32 + lane, key = x / NB, b = x - key * NB, r = lw * 64 + key;
+                const bool none = j0 + r >= seen || byte[i] == 255u;
+                const uint32_t f = none ? 0u : p_factor((int)byte[i], top);
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const int chunk = 4 * b + k;
+                    *reinterpret_cast<uint4 *>(to + (chunk >> 3) * kPBlock + at_off(r, chunk & 7)) = p_halves(none ? 0u : words[i][k], f);
+                }
+            }
+            if (lw == 0 && lane == 0) value_top[t % kPRing] = top;
+            if (t + 1 < n_tiles) fetch((t + 1) * kPKeys);
+            at_proxy_fence();
+            __syncwarp();
+            if (lane == 0) vb_mbar_arrive(&v_full[slot]);
+        }
+    } else if (lane == 0) {
+        /* ---- MMA issuer ---- */
+        const uint32_t idesc_s = p_idesc(kPKeys, false), idesc_o = p_idesc(kDim, true);
+        const AtDesc k_desc(umma_desc_k_sw128(k_s)), q_desc(umma_desc_k_sw128(q_s)), v_desc(p_desc_mn(vb_smem_u32(v_s)));
+        bool ok = vb_mbar_wait(&q_full, 0u, abort_flag);
+        tc_fence_after();
+        auto scores = [&](int t) {
+            const int slot = t % Cfg::kSlots;
+            if (!vb_mbar_wait(&k_full[slot], (uint32_t)(t / Cfg::kSlots) & 1u, abort_flag)) return false;
+            tc_fence_after();
+            const AtDesc kd = k_desc.at(slot * (Cfg::kSlot >> 4));
+            const uint32_t d = tmem + (uint32_t)((t & 1) * kPKeys);
+#pragma unroll
+            for (int ks = 0; ks < NB * 2; ks++) {
+                const int at = (ks >> 2) * (kPBlock >> 4) + 2 * (ks & 3);
+#pragma unroll
+                for (int u = 0; u < QT; u++) at_mma_ss(d, q_desc.at(at + u * (Cfg::kSlot >> 4)), kd.at(at), idesc_s, ks + u != 0 ? 1u : 0u);
+            }
+            umma_commit(&k_empty[slot]);
+            umma_commit(&s_full[t & 1]);
+            return true;
+        };
+        ok = ok && n_tiles > 0 && scores(0);
+        if (ok && n_tiles > 1) ok = scores(1);
+        for (int t = 0; t < n_tiles && ok; t++) {
+            const int w = t & 1, slot = t % Cfg::kSlots;
+            ok = vb_mbar_wait(&v_full[slot], (uint32_t)(t / Cfg::kSlots) & 1u, abort_flag) && vb_mbar_wait(&p_full[w], (uint32_t)(t >> 1) & 1u, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            const AtDesc vd = v_desc.at(slot * (Cfg::kSlot >> 4));
+            const uint32_t d = tmem + kPO + (uint32_t)(w * 128);
+#pragma unroll
+            for (int ks = 0; ks < kPKeys / 16; ks++) {
+                const uint32_t p = tmem + (uint32_t)(w * kPKeys + (ks >> 1) * 32 + (ks & 1) * 8);
+#pragma unroll
+                for (int u = 0; u < PT; u++) at_mma_ts(d, p + u * 16, vd.at(ks * (2048 >> 4)), idesc_o, (t >> 1 | ks | u) != 0 ? 1u : 0u);
+            }
+            umma_commit(&v_empty[slot]);
+            umma_commit(&o_done[w]);
+            /* takes the columns of P once the products above have read them: MMAs of one thread run in order */
+            if (t + 2 < n_tiles) ok = scores(t + 2);
+        }
+        if (!ok && n_tiles > 0) give_up();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kPMmaWarp) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kPTmem) : "memory");
+    }
+}
+
+template <int NB, class T>
+int prompt_launch(const Kv4Attn &a, const ServeRows<T> &q, const ServeRows<T> &out, cudaStream_t st) {
+    const int tiles = (int)(((long long)a.max_rows * a.group + kPRows - 1) / kPRows);
+    kv4_prompt_kernel<NB, kWeightTerms<T>, T><<<dim3(tiles, a.c.kv_heads, a.c.seqs), kPThreads, PCfg<NB, sizeof(T) == 4 ? 2 : 1>::kSmem, st>>>(a, q, out);
+    return serve_launched();
+}
+template <int NB, class T>
+bool prompt_load() {
+    return cudaFuncSetAttribute(kv4_prompt_kernel<NB, kWeightTerms<T>, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, PCfg<NB, sizeof(T) == 4 ? 2 : 1>::kSmem) == cudaSuccess;
+}
+
+} // namespace
+
+template <class T>
+int kv4_prompt(const Kv4Attn &a, const ServeRows<T> &q, const ServeRows<T> &out, cudaStream_t st) {
+    switch (a.c.blocks) {
+    case 1: return prompt_launch<1, T>(a, q, out, st);
+    case 2: return prompt_launch<2, T>(a, q, out, st);
+    case 3: return prompt_launch<3, T>(a, q, out, st);
+    default: return prompt_launch<4, T>(a, q, out, st);
+    }
+}
+template int kv4_prompt<float>(const Kv4Attn &, const ServeRows<float> &, const ServeRows<float> &, cudaStream_t);
+template int kv4_prompt<__nv_bfloat16>(const Kv4Attn &, const ServeRows<__nv_bfloat16> &, const ServeRows<__nv_bfloat16> &, cudaStream_t);
+template int kv4_prompt<__half>(const Kv4Attn &, const ServeRows<__half> &, const ServeRows<__half> &, cudaStream_t);
+
+int kv4_prompt_load(int blocks) {
+    bool ok = true;
+    switch (blocks) {
+    case 1: ok = prompt_load<1, float>() && prompt_load<1, __nv_bfloat16>() && prompt_load<1, __half>(); break;
+    case 2: ok = prompt_load<2, float>() && prompt_load<2, __nv_bfloat16>() && prompt_load<2, __half>(); break;
+    case 3: ok = prompt_load<3, float>() && prompt_load<3, __nv_bfloat16>() && prompt_load<3, __half>(); break;
+    case 4: ok = prompt_load<4, float>() && prompt_load<4, __nv_bfloat16>() && prompt_load<4, __half>(); break;
+    }
+    return ok ? 0 : serve_launched() | -1;
+}
+
+} // namespace vb
