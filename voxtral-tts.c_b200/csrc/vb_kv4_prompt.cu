@@ -49,6 +49,11 @@ VB_DEVINL uint64_t p_desc_mn(uint32_t addr) {
 /* kind::f16 with FP16 operands, fp32 sums, 128 rows, n columns */
 VB_DEVINL uint32_t p_idesc(int n, bool mn_major) { return (1u << 4) | (mn_major ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kPRows >> 4) << 24); }
 
+VB_DEVINL void at_st16(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::VB_AT_R8(r, 0),
+                 VB_AT_R8(r, 8), "r"(taddr)
+                 : "memory");
+}
 /* Eight codes times a power of two to 16 bytes */
 VB_DEVINL uint4 p_halves(uint32_t w, uint32_t f) {
     uint32_t r[4];
@@ -135,8 +140,9 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
                 for (int i = 0; i < NB; i++) most = max(most, __float_as_uint(x[u][i]) & 0x7fffffffu);
                 most = __reduce_max_sync(0xffffffffu, most);
                 const uint32_t e = most >> 23, field = e == 0u || e == 255u ? 127u : min(268u - e, 253u);
-                const float up = __uint_as_float(field << 23);
+                float up = __uint_as_float(field << 23);
                 if (lane == 0) down_s[r] = __uint_as_float((254u - field) << 23);
+                if (a.scale < 0.0f) up = -up;                      /* the largest score is the largest product */
 #pragma unroll
                 for (int i = 0; i < NB; i++) {
                     const int d = lane + 32 * i;
@@ -158,7 +164,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
         const int row = valid ? pair / a.group : 0, head = kv_head * a.group + (valid ? pair - row * a.group : 0);
         const int sees = before + (pair0 + min(r, n_pairs - 1)) / a.group + 1;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, tS = tmem + lanes + (uint32_t)(w * kPKeys), tO = tmem + lanes + kPO + (uint32_t)(w * 128);
-        const float mul = a.scale * 1.44269504f * down_s[r];
+        const float mul = fabsf(a.scale) * 1.44269504f * down_s[r];
         float ref = -INFINITY, sum = 0.0f;
         int top_scale = 0, it = 0;
         for (int t = w; t < n_tiles; t += 2, it++) {
@@ -171,19 +177,20 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
             float top = -INFINITY;
 #pragma unroll 1
             for (int c = 0; c < 4; c++) {
-                const float up = ups[c] * mul;
                 uint32_t reg[32];
                 at_ld32(tS + (uint32_t)(c * 32), reg);
-                /* the largest product, or the smallest where the factor is negative */
-                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                const uint32_t turn = __float_as_uint(up) & 0x80000000u;
+                if (masked) {
 #pragma unroll
-                for (int k = 0; k < 32; k++) {
-                    const float x = __uint_as_float(reg[k] ^ turn);
-                    m4[k & 3] = fmaxf(m4[k & 3], !masked || c * 32 + k < last ? x : -INFINITY);
+                    for (int k = 0; k < 32; k++)
+                        if (c * 32 + k >= last) reg[k] = 0xff800000u;
                 }
-                const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), f = fabsf(up);
-                if (m > -INFINITY) top = fmaxf(top, m * f);
+                float m4[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) m4[k] = __uint_as_float(reg[k]);
+#pragma unroll
+                for (int k = 4; k < 32; k++) m4[k & 3] = fmaxf(m4[k & 3], __uint_as_float(reg[k]));
+                const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+                if (m > -INFINITY) top = fmaxf(top, m * (ups[c] * mul));
             }
             /* values: the scale that this tile is based on */
             if (!at_warp_wait(&v_full[t % Cfg::kSlots], (uint32_t)(t / Cfg::kSlots) & 1u, abort_flag)) { give_up(); break; }
@@ -210,34 +217,36 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
                 top_scale = now_scale;
             }
             const float low = ref > -INFINITY ? ref - kKv4Bias : 0.0f;      /* nothing seen yet: every weight is 2^-inf */
-            float sum4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            uint64_t sums[2] = {0, 0};
+            const uint64_t low2 = vb_f2_pack(-low, -low);
 #pragma unroll 1
             for (int c = 0; c < 4; c++) {
                 const float up = ups[c] * mul;
+                const uint64_t up2 = vb_f2_pack(up, up);
                 uint32_t reg[32], terms[32];
                 at_ld32(tS + (uint32_t)(c * 32), reg);
 #pragma unroll
                 for (int k = 0; k < 32; k += 2) {
-                    float p[2];
-#pragma unroll
-                    for (int u = 0; u < 2; u++) {
-                        float x = fmaf(__uint_as_float(reg[k + u]), up, -low);
-                        if (masked && c * 32 + k + u >= last) x = -INFINITY;
-                        p[u] = exp2_fast(x);
-                        sum4[(k + u) & 3] += p[u];
+                    float2 x = vb_f2_get(vb_f2_fma(vb_f2_pack(__uint_as_float(reg[k]), __uint_as_float(reg[k + 1])), up2, low2));
+                    if (masked) {
+                        if (c * 32 + k >= last) x.x = -INFINITY;
+                        if (c * 32 + k + 1 >= last) x.y = -INFINITY;
                     }
-                    const uint32_t hi = half_pack(p[0], p[1]);
+                    const float p0 = exp2_fast(x.x), p1 = exp2_fast(x.y);
+                    const uint64_t p = vb_f2_pack(p0, p1);
+                    sums[(k >> 1) & 1] = vb_f2_add(sums[(k >> 1) & 1], p);
+                    const uint32_t hi = half_pack(p0, p1);
+                    terms[k / 2] = hi;
                     if constexpr (PT == 2) {
                         const float2 f = kv4_f2(hi);
-                        terms[16 + k / 2] = half_pack(p[0] - f.x, p[1] - f.y);
-                    } else {
-                        terms[16 + k / 2] = 0u;
+                        terms[16 + k / 2] = half_pack(p0 - f.x, p1 - f.y);
                     }
-                    terms[k / 2] = hi;
                 }
-                at_st32(tS + (uint32_t)(c * 32), terms);           /* 16 columns of first terms, 16 of second ones */
+                if constexpr (PT == 2) at_st32(tS + (uint32_t)(c * 32), terms);      /* 16 columns of first terms, 16 of second ones */
+                else at_st16(tS + (uint32_t)(c * 32), terms);
             }
-            sum += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+            const float2 sum2 = vb_f2_get(vb_f2_add(sums[0], sums[1]));
+            sum += sum2.x + sum2.y;
             at_st_wait();
             tc_fence_before();
             vb_mbar_arrive(&p_full[w]);
