@@ -6,13 +6,13 @@
  *   S [128 x 128]   = Q K^T    Q in shared memory, one FP16 term (bf16, fp16) or two (fp32), rows brought to [2^14, 2^15)
  *   O [128 x dim]  += P V      P in TMEM, in S's own columns, one term (bf16) or two; V rows [token][dim] are an MN-major operand
  *
- * Keys and values go from codes to FP16 on the way to shared memory, four warps for the keys and two for the values: keys times 2^(e - S + 13), S the largest
+ * Keys and values go from codes to FP16 on the way to shared memory, four warps for the keys and three for the values: keys times 2^(e - S + 13), S the largest
  * scale of a warp's 32 tokens, which the softmax undoes, values times 2^(e - E + 13), E the largest scale so far, on which the
  * accumulator is based (exact down to 2^-36 of the largest). Scores, weights, sums as in vb_kv4_attn.cu. Two warpgroups take
  * alternate tiles with a reference, sums and an accumulator each, merged at the end, so that the tensor pipe works on one tile while the
  * other is in its softmax.
  *
- * Warps: 0-3, 4-7 softmax, 8-11 keys, 12-13 values, 14 issues the MMAs. All waits are bounded.
+ * Warps: 0-3, 4-7 softmax, 8-11 keys, 12-14 values, 15 issues the MMAs. All waits are bounded.
  */
 #include <type_traits>
 
@@ -23,7 +23,7 @@ namespace vb {
 
 namespace {
 
-constexpr int kPRows = 128, kPKeys = 128, kPThreads = 480, kPMmaWarp = 14, kPBlock = kPKeys * 128, kPStatus = 62, kPRing = 8;
+constexpr int kPRows = 128, kPKeys = 128, kPThreads = 512, kPMmaWarp = 15, kPBlock = kPKeys * 128, kPStatus = 62, kPRing = 8;
 constexpr uint32_t kPTmem = 512, kPO = 256;
 
 template <int NB, int QT>
@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
     if (tid == 0) {
         for (int i = 0; i < Cfg::kSlots; i++) {
             vb_mbar_init(&k_full[i], 4);
-            vb_mbar_init(&v_full[i], 2);
+            vb_mbar_init(&v_full[i], 4);
             vb_mbar_init(&k_empty[i], 1);
             vb_mbar_init(&v_empty[i], 1);
         }
@@ -303,11 +303,13 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
         const size_t row0 = a.c.row(seq, kv_head, 0);
         uint32_t words[4][NB], bytes[4][NB];
         auto fetch = [&](int t) {
+            const int j0 = t * kPKeys, end = a.c.slots - 1 - j0;             /* slots are whole tiles of 64: half of the last 128 may be none */
+            const unsigned char *codes = a.c.k + (row0 + j0) * (NB * 16), *scales = a.c.ks + (row0 + j0) * NB;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const size_t row = row0 + min(t * kPKeys + lw * 32 + i * 8 + g, a.c.slots - 1);
-                get_words<NB>(a.c.k + row * (NB * 16) + tq * (NB * 4), words[i]);
-                get_bytes<NB>(a.c.ks + row * NB, bytes[i]);
+                const int r = min(lw * 32 + i * 8 + g, end);
+                get_words<NB>(codes + r * (NB * 16) + tq * (NB * 4), words[i]);
+                get_bytes<NB>(scales + r * NB, bytes[i]);
             }
         };
         if (n_tiles > 0) fetch(0);
@@ -342,57 +344,56 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
             if (lane == 0) vb_mbar_arrive(&k_full[slot]);
         }
     } else if (warp < kPMmaWarp) {
-        /* ---- values: a warp has 64 tokens of a tile, a lane blocks of them ---- */
-        const int lw = warp - 12;
+        /* ---- values: the warps take 32 tokens in turn, a lane blocks of them ---- */
         const size_t row0 = a.c.row(seq, kv_head, 0);
-        uint32_t words[2 * NB][4], byte[2 * NB], all[4][NB];
-        auto fetch = [&](int j0) {
+        uint32_t words[NB][4], byte[NB], all[NB];
+        auto fetch = [&](int task) {
+            const int j0 = task / 4 * kPKeys, end = a.c.slots - 1 - j0;          /* slots are whole tiles of 64: half of the last 128 may be none */
+            const unsigned char *codes = a.c.v + (row0 + j0) * (NB * 16), *scales = a.c.vs + (row0 + j0) * NB;
 #pragma unroll
-            for (int i = 0; i < 2 * NB; i++) {
-                const int x = i * 32 + lane, key = x / NB, b = x - key * NB;
-                const size_t row = row0 + min(j0 + lw * 64 + key, a.c.slots - 1);
-                const unsigned char *p = a.c.v + row * (NB * 16);
+            for (int i = 0; i < NB; i++) {
+                const int x = i * 32 + lane, key = x / NB, b = x - key * NB, r = min(task % 4 * 32 + key, end);
                 if constexpr (kv4_whole(NB)) {
-                    get_words<4>(p + b * 16, words[i]);
+                    get_words<4>(codes + r * (NB * 16) + b * 16, words[i]);
                 } else {
-                    const uint16_t *h = reinterpret_cast<const uint16_t *>(p) + b;
+                    const uint16_t *h = reinterpret_cast<const uint16_t *>(codes + r * (NB * 16)) + b;
 #pragma unroll
                     for (int k = 0; k < 4; k++) words[i][k] = h[2 * k * NB] | ((uint32_t)h[(2 * k + 1) * NB] << 16);
                 }
-                byte[i] = a.c.vs[row * NB + b];
+                byte[i] = scales[r * NB + b];
             }
             /* all scales of the tile, four tokens a lane: every warp finds the largest for itself */
+            const uint32_t *four = reinterpret_cast<const uint32_t *>(scales + min(lane * 4, end - 3) * NB);
 #pragma unroll
-            for (int i = 0; i < 4; i++) get_bytes<NB>(a.c.vs + (row0 + min(j0 + lane * 4 + i, a.c.slots - 1)) * NB, all[i]);
+            for (int i = 0; i < NB; i++) all[i] = four[i];
         };
         int top = 0;
-        if (n_tiles > 0) fetch(0);
-        for (int t = 0; t < n_tiles; t++) {
-            const int slot = t % Cfg::kSlots, j0 = t * kPKeys;
+        const int tasks = n_tiles * 4;
+        if (warp - 12 < tasks) fetch(warp - 12);
+        for (int task = warp - 12; task < tasks; task += 3) {
+            const int t = task / 4, lw = task % 4, slot = t % Cfg::kSlots, j0 = t * kPKeys;
+            const int real = seen - j0;                            /* tokens of the tile that are seen */
             int most = 0;
             bool bad = false;
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+            for (int i = 0; i < NB * 4; i++) {
+                const int byte_i = (int)((all[i / 4] >> (8 * (i % 4))) & 255u);
+                const bool there = lane * 4 + i / NB < real;
+                if (there && byte_i != 255) most = max(most, byte_i);
+                bad |= there && byte_i == 255;
+            }
+            if (__any_sync(0xffffffffu, bad)) {                    /* blocks that are NaN: the rows that see them; their codes are zeros */
 #pragma unroll
-                for (int b = 0; b < NB; b++)
-                    if (j0 + lane * 4 + i < seen) {
-                        if (all[i][b] != 255u) most = max(most, (int)all[i][b]);
-                        else bad = true;
-                    }
-            if (__any_sync(0xffffffffu, bad) && lw == 0) {         /* blocks that are NaN: the rows that see them; their codes are zeros */
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int b = 0; b < NB; b++)
-                        if (j0 + lane * 4 + i < seen && all[i][b] == 255u) atomicMin(&bad_s[b], j0 + lane * 4 + i);
+                for (int i = 0; i < NB * 4; i++)
+                    if (lane * 4 + i / NB < real && ((all[i / 4] >> (8 * (i % 4))) & 255u) == 255u) atomicMin(&bad_s[i % NB], j0 + lane * 4 + i / NB);
             }
             top = max(top, (int)__reduce_max_sync(0xffffffffu, (unsigned)most));
             if (!at_warp_wait(&v_empty[slot], ((uint32_t)(t / Cfg::kSlots) & 1u) ^ 1u, abort_flag)) { give_up(); break; }
             unsigned char *to = v_s + slot * Cfg::kSlot;
 #pragma unroll
-            for (int i = 0; i < 2 * NB; i++) {
-                const int x = i * 32 + lane, key = x / NB, b = x - key * NB, r = lw * 64 + key;
-                const bool none = j0 + r >= seen || byte[i] == 255u;
+            for (int i = 0; i < NB; i++) {
+                const int x = i * 32 + lane, key = x / NB, b = x - key * NB, r = lw * 32 + key;
+                const bool none = r >= real || byte[i] == 255u;
                 const uint32_t f = none ? 0u : p_factor((int)byte[i], top);
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
@@ -401,7 +402,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
                 }
             }
             if (lw == 0 && lane == 0) value_top[t % kPRing] = top;
-            if (t + 1 < n_tiles) fetch((t + 1) * kPKeys);
+            if (task + 3 < tasks) fetch(task + 3);
             at_proxy_fence();
             __syncwarp();
             if (lane == 0) vb_mbar_arrive(&v_full[slot]);
