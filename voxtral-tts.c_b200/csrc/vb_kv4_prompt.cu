@@ -25,6 +25,9 @@ namespace {
 
 constexpr int kPRows = 128, kPKeys = 128, kPThreads = 512, kPMmaWarp = 15, kPBlock = kPKeys * 128, kPStatus = 62, kPRing = 8;
 constexpr uint32_t kPTmem = 512, kPO = 256;
+/* registers a thread at the launch, of a softmax thread and of any other: what some are given the others have given up */
+constexpr int kPRegs = 128, kPSoftRegs = 184, kPLoadRegs = 72;
+static_assert(kPThreads == 512 && 2 * kPSoftRegs + 2 * kPLoadRegs <= 4 * kPRegs, "more registers than the block is launched with");
 
 template <int NB, int QT>
 struct PCfg {
@@ -49,7 +52,27 @@ VB_DEVINL uint64_t p_desc_mn(uint32_t addr) {
 /* kind::f16 with FP16 operands, fp32 sums, 128 rows, n columns */
 VB_DEVINL uint32_t p_idesc(int n, bool mn_major) { return (1u << 4) | (mn_major ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kPRows >> 4) << 24); }
 
-VB_DEVINL void at_st16(uint32_t taddr, const uint32_t (&r)[32]) {
+/* 32 columns of this thread's TMEM lane on their way, and in place; 16 columns back */
+VB_DEVINL void p_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : VB_AT_W8(r, 0), VB_AT_W8(r, 8), VB_AT_W8(r, 16), VB_AT_W8(r, 24)
+        : "r"(taddr)
+        : "memory");
+}
+#define VB_P_RW8(r, o) "+r"((r)[o]), "+r"((r)[o + 1]), "+r"((r)[o + 2]), "+r"((r)[o + 3]), "+r"((r)[o + 4]), "+r"((r)[o + 5]), "+r"((r)[o + 6]), "+r"((r)[o + 7])
+/* (an instruction of its own for each array, none of them before the wait: an operand list has room for 30) */
+VB_DEVINL void p_ld_wait(uint32_t (&r)[4][32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int c = 0; c < 4; c++)
+#pragma unroll
+        for (int k = 0; k < 32; k += 8) asm volatile("" : VB_P_RW8(r[c], k));
+}
+template <int N>
+VB_DEVINL void p_st16(uint32_t taddr, const uint32_t (&r)[N]) {
+    static_assert(N >= 16, "");
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::VB_AT_R8(r, 0),
                  VB_AT_R8(r, 8), "r"(taddr)
                  : "memory");
@@ -118,6 +141,9 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
         *(volatile int *)abort_flag = 1;
     };
 
+    /* a softmax thread holds a row of scores: its registers from the other warps' */
+    if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPSoftRegs));
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPLoadRegs));
     if (warp < 8) {
         /* ---- queries: a warp has rows warp, warp + 8, ..., eight at a time, a lane the values lane + 32 i ---- */
 #pragma unroll 1
@@ -142,7 +168,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
                 const uint32_t e = most >> 23, field = e == 0u || e == 255u ? 127u : min(268u - e, 253u);
                 float up = __uint_as_float(field << 23);
                 if (lane == 0) down_s[r] = __uint_as_float((254u - field) << 23);
-                if (a.scale < 0.0f) up = -up;                      /* the largest score is the largest product */
+                if (a.scale <= 0.0f) up = a.scale < 0.0f ? -up : 0.0f;      /* the largest score is the largest product */
 #pragma unroll
                 for (int i = 0; i < NB; i++) {
                     const int d = lane + 32 * i;
@@ -164,7 +190,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
         const int row = valid ? pair / a.group : 0, head = kv_head * a.group + (valid ? pair - row * a.group : 0);
         const int sees = before + (pair0 + min(r, n_pairs - 1)) / a.group + 1;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, tS = tmem + lanes + (uint32_t)(w * kPKeys), tO = tmem + lanes + kPO + (uint32_t)(w * 128);
-        const float mul = fabsf(a.scale) * 1.44269504f * down_s[r];
+        /* positive, so that what is masked stays -inf: queries are zeros where the scale is */
+        const float mul = (a.scale != 0.0f ? fabsf(a.scale) * 1.44269504f : 1.0f) * down_s[r];
         float ref = -INFINITY, sum = 0.0f;
         int top_scale = 0, it = 0;
         for (int t = w; t < n_tiles; t += 2, it++) {
@@ -174,21 +201,26 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
             const float *ups = key_up[t % kPRing];
             const int last = sees - j0;                            /* columns before this one are seen */
             const bool masked = j0 + kPKeys > all_see;
-            float top = -INFINITY;
-#pragma unroll 1
-            for (int c = 0; c < 4; c++) {
-                uint32_t reg[32];
-                at_ld32(tS + (uint32_t)(c * 32), reg);
-                if (masked) {
+            /* a tile's scores in registers: 32 columns are requested behind one another, and waited for together */
+            uint32_t s[4][32];
+#pragma unroll
+            for (int c = 0; c < 4; c++) p_ld32(tS + (uint32_t)(c * 32), s[c]);
+            p_ld_wait(s);
+            if (masked) {
+#pragma unroll
+                for (int c = 0; c < 4; c++)
 #pragma unroll
                     for (int k = 0; k < 32; k++)
-                        if (c * 32 + k >= last) reg[k] = 0xff800000u;
-                }
+                        if (c * 32 + k >= last) s[c][k] = 0xff800000u;
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
                 float m4[4];
 #pragma unroll
-                for (int k = 0; k < 4; k++) m4[k] = __uint_as_float(reg[k]);
+                for (int k = 0; k < 4; k++) m4[k] = __uint_as_float(s[c][k]);
 #pragma unroll
-                for (int k = 4; k < 32; k++) m4[k & 3] = fmaxf(m4[k & 3], __uint_as_float(reg[k]));
+                for (int k = 4; k < 32; k++) m4[k & 3] = fmaxf(m4[k & 3], __uint_as_float(s[c][k]));
                 const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
                 if (m > -INFINITY) top = fmaxf(top, m * (ups[c] * mul));
             }
@@ -219,31 +251,25 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
             const float low = ref > -INFINITY ? ref - kKv4Bias : 0.0f;      /* nothing seen yet: every weight is 2^-inf */
             uint64_t sums[2] = {0, 0};
             const uint64_t low2 = vb_f2_pack(-low, -low);
-#pragma unroll 1
+#pragma unroll
             for (int c = 0; c < 4; c++) {
                 const float up = ups[c] * mul;
                 const uint64_t up2 = vb_f2_pack(up, up);
-                uint32_t reg[32], terms[32];
-                at_ld32(tS + (uint32_t)(c * 32), reg);
+                uint32_t second[PT == 2 ? 16 : 1];
 #pragma unroll
                 for (int k = 0; k < 32; k += 2) {
-                    float2 x = vb_f2_get(vb_f2_fma(vb_f2_pack(__uint_as_float(reg[k]), __uint_as_float(reg[k + 1])), up2, low2));
-                    if (masked) {
-                        if (c * 32 + k >= last) x.x = -INFINITY;
-                        if (c * 32 + k + 1 >= last) x.y = -INFINITY;
-                    }
+                    const float2 x = vb_f2_get(vb_f2_fma(vb_f2_pack(__uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1])), up2, low2));
                     const float p0 = exp2_fast(x.x), p1 = exp2_fast(x.y);
-                    const uint64_t p = vb_f2_pack(p0, p1);
-                    sums[(k >> 1) & 1] = vb_f2_add(sums[(k >> 1) & 1], p);
+                    sums[(k >> 1) & 1] = vb_f2_add(sums[(k >> 1) & 1], vb_f2_pack(p0, p1));
                     const uint32_t hi = half_pack(p0, p1);
-                    terms[k / 2] = hi;
+                    s[c][k / 2] = hi;
                     if constexpr (PT == 2) {
                         const float2 f = kv4_f2(hi);
-                        terms[16 + k / 2] = half_pack(p0 - f.x, p1 - f.y);
+                        second[k / 2] = half_pack(p0 - f.x, p1 - f.y);
                     }
                 }
-                if constexpr (PT == 2) at_st32(tS + (uint32_t)(c * 32), terms);      /* 16 columns of first terms, 16 of second ones */
-                else at_st16(tS + (uint32_t)(c * 32), terms);
+                p_st16(tS + (uint32_t)(c * 32), s[c]);             /* 16 columns of first terms, 16 of second ones */
+                if constexpr (PT == 2) p_st16(tS + (uint32_t)(c * 32 + 16), second);
             }
             const float2 sum2 = vb_f2_get(vb_f2_add(sums[0], sums[1]));
             sum += sum2.x + sum2.y;
@@ -467,6 +493,13 @@ int prompt_launch(const Kv4Attn &a, const ServeRows<T> &q, const ServeRows<T> &o
 }
 template <int NB, class T>
 bool prompt_load() {
+    /* a block launched with fewer registers than its warps ask for would wait for them for good */
+    cudaFuncAttributes f;
+    if (cudaFuncGetAttributes(&f, kv4_prompt_kernel<NB, kWeightTerms<T>, T>) != cudaSuccess) return false;
+    if (f.numRegs < kPRegs) {
+        serve_fail("the prompt kernel was built with fewer registers than it divides");
+        return false;
+    }
     return cudaFuncSetAttribute(kv4_prompt_kernel<NB, kWeightTerms<T>, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, PCfg<NB, sizeof(T) == 4 ? 2 : 1>::kSmem) == cudaSuccess;
 }
 
@@ -493,7 +526,7 @@ int kv4_prompt_load(int blocks) {
     case 3: ok = prompt_load<3, float>() && prompt_load<3, __nv_bfloat16>() && prompt_load<3, __half>(); break;
     case 4: ok = prompt_load<4, float>() && prompt_load<4, __nv_bfloat16>() && prompt_load<4, __half>(); break;
     }
-    return ok ? 0 : serve_launched() | -1;
+    return ok ? 0 : -1;
 }
 
 } // namespace vb
