@@ -145,38 +145,58 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
     if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPSoftRegs));
     else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPLoadRegs));
     if (warp < 8) {
-        /* ---- queries: a warp has rows warp, warp + 8, ..., eight at a time, a lane the values lane + 32 i ---- */
-#pragma unroll 1
-        for (int r0 = 0; r0 < kPRows / 8; r0 += 8) {
-            float x[8][NB];
+        /* ---- queries: four values a lane, NB * 8 lanes a row, so that a warp has one, two or four rows at a time; the loads of
+         * sixteen rows together ---- */
+        constexpr int kLanes = NB * 8, kSide = 32 / kLanes, kBatch = 16 / kSide;
+        const int side = lane / kLanes, d = (lane - side * kLanes) * 4;
+        const bool mine = side < kSide;
+        float x[kBatch][4];
 #pragma unroll
-            for (int u = 0; u < 8; u++) {
-                const int pair = pair0 + warp + 8 * (r0 + u);
-                const bool real = pair < pairs;
-                const int row = real ? pair / a.group : 0, head = kv_head * a.group + (real ? pair - row * a.group : 0);
-                const T *p = q.data + seq * q.seq + row * q.row + head * q.head + lane;
+        for (int u = 0; u < kBatch; u++) {
+            const int pair = pair0 + warp * 16 + u * kSide + side;
+            const bool real = mine && pair < pairs;
+            const int row = real ? pair / a.group : 0, head = kv_head * a.group + (real ? pair - row * a.group : 0);
+            const T *p = q.data + seq * q.seq + row * q.row + head * q.head + d;
 #pragma unroll
-                for (int i = 0; i < NB; i++) x[u][i] = real ? serve_get(p + 32 * i) : 0.0f;
+            for (int i = 0; i < 4; i++) x[u][i] = 0.0f;
+            if (real) {
+                if (!a.wide) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) x[u][i] = serve_get(p + i);
+                } else if constexpr (sizeof(T) == 4) {
+                    const float4 v = *reinterpret_cast<const float4 *>(p);
+                    x[u][0] = v.x; x[u][1] = v.y; x[u][2] = v.z; x[u][3] = v.w;
+                } else {
+                    const uint2 v = *reinterpret_cast<const uint2 *>(p);
+                    const float2 lo = serve_pair(v.x, p), hi = serve_pair(v.y, p);
+                    x[u][0] = lo.x; x[u][1] = lo.y; x[u][2] = hi.x; x[u][3] = hi.y;
+                }
             }
+        }
 #pragma unroll
-            for (int u = 0; u < 8; u++) {
-                const int r = warp + 8 * (r0 + u);
-                uint32_t most = 0;
+        for (int u = 0; u < kBatch; u++) {
+            const int r = warp * 16 + u * kSide + side;
+            uint32_t most = 0;
 #pragma unroll
-                for (int i = 0; i < NB; i++) most = max(most, __float_as_uint(x[u][i]) & 0x7fffffffu);
+            for (int i = 0; i < 4; i++) most = max(most, __float_as_uint(x[u][i]) & 0x7fffffffu);
+            if constexpr (kSide == 1) {
                 most = __reduce_max_sync(0xffffffffu, most);
-                const uint32_t e = most >> 23, field = e == 0u || e == 255u ? 127u : min(268u - e, 253u);
-                float up = __uint_as_float(field << 23);
-                if (lane == 0) down_s[r] = __uint_as_float((254u - field) << 23);
-                if (a.scale <= 0.0f) up = a.scale < 0.0f ? -up : 0.0f;      /* the largest score is the largest product */
+            } else {
 #pragma unroll
-                for (int i = 0; i < NB; i++) {
-                    const int d = lane + 32 * i;
-                    const uint32_t at = (uint32_t)(d >> 6) * kPBlock + at_off(r, (d & 63) >> 3) + (d & 7) * 2;
-                    const float y = x[u][i] * up;
-                    const __half hi = __float2half_rn(y);
-                    *reinterpret_cast<__half *>(q_s + at) = hi;
-                    if constexpr (QT == 2) *reinterpret_cast<__half *>(q_s + Cfg::kSlot + at) = __float2half_rn(y - __half2float(hi));
+                for (int o = 1; o < kLanes; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+            }
+            const uint32_t e = most >> 23, field = e == 0u || e == 255u ? 127u : min(268u - e, 253u);
+            float up = __uint_as_float(field << 23);
+            if (mine && d == 0) down_s[r] = __uint_as_float((254u - field) << 23);
+            if (a.scale <= 0.0f) up = a.scale < 0.0f ? -up : 0.0f;      /* the largest score is the largest product */
+            if (mine) {
+                const uint32_t at = (uint32_t)(d >> 6) * kPBlock + at_off(r, (d & 63) >> 3) + (d & 7) * 2;
+                const float y0 = x[u][0] * up, y1 = x[u][1] * up, y2 = x[u][2] * up, y3 = x[u][3] * up;
+                const uint2 hi = make_uint2(half_pack(y0, y1), half_pack(y2, y3));
+                *reinterpret_cast<uint2 *>(q_s + at) = hi;
+                if constexpr (QT == 2) {
+                    const float2 f = kv4_f2(hi.x), g = kv4_f2(hi.y);
+                    *reinterpret_cast<uint2 *>(q_s + Cfg::kSlot + at) = make_uint2(half_pack(y0 - f.x, y1 - f.y), half_pack(y2 - g.x, y3 - g.y));
                 }
             }
         }
