@@ -8,6 +8,7 @@
 #include <string>
 
 #include "vb_kv4.cuh"
+#include "vb_tc.cuh"
 
 namespace vb {
 
@@ -60,6 +61,8 @@ __global__ void __launch_bounds__(kRowThreads) kv4_rows_kernel(const RowsArgs<T>
     const unsigned plane = a.c.kv_heads * kWords, token_words = 2 * plane;
     const long long total = (long long)a.tokens * token_words;
     const int tid = threadIdx.x;
+    pdl_launch_dependents();
+    pdl_wait();
     for (long long c0 = blockIdx.x * kChunk; c0 < total; c0 += gridDim.x * kChunk) {
         const unsigned token0 = (unsigned)(c0 / token_words), off0 = (unsigned)(c0 - (long long)token0 * token_words);
         float v[kRowUnroll][8];
@@ -161,9 +164,8 @@ int rows_launch(const vb200_kv4 *h, const vb200_kv4_rows_t &a, bool read, cudaSt
     r.wide = serve_wide(r.k) && serve_wide(r.v);
     const long long words = (long long)r.tokens * h->c.kv_heads * NB * 8, chunk = kRowThreads * kRowUnroll;
     const unsigned grid = (unsigned)std::min((words + chunk - 1) / chunk, (long long)h->w.sm_count * 16);
-    if (read) kv4_rows_kernel<NB, T, true><<<grid, kRowThreads, 0, st>>>(r);
-    else kv4_rows_kernel<NB, T, false><<<grid, kRowThreads, 0, st>>>(r);
-    return serve_launched();
+    const cudaError_t e = launch_pdl(read ? kv4_rows_kernel<NB, T, true> : kv4_rows_kernel<NB, T, false>, dim3(grid), dim3(kRowThreads), 0, st, r);
+    return e == cudaSuccess ? 0 : serve_launched() | -1;
 }
 
 template <class T>
@@ -205,6 +207,8 @@ __global__ void __launch_bounds__(kSelThreads) kv4_select_kernel(const EvictArgs
     __shared__ uint32_t prefix;
     __shared__ int want;
     const int s = blockIdx.y, h = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    pdl_launch_dependents();
+    pdl_wait();
     const int n = min(max(a.lengths[s], 0), a.from.capacity);
     int *kept = a.kept + ((size_t)s * a.from.kv_heads + h) * a.keep;
     if (n <= a.keep) {
@@ -337,6 +341,8 @@ constexpr int kMoveThreads = 256;
 template <bool IN_PLACE>
 __global__ void __launch_bounds__(kMoveThreads) kv4_move_kernel(const EvictArgs a) {
     const int s = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
+    pdl_launch_dependents();
+    pdl_wait();
     const int n = min(max(a.lengths[s], 0), a.from.capacity), m = min(n, a.keep);
     if (blockIdx.x == 0 && h == 0 && tid == 0) a.new_lengths[s] = m;     /* whoever reads it later finds the same m */
     const int blocks = a.from.blocks, pieces = blocks;                   /* of 16 bytes a row and plane */
@@ -507,17 +513,17 @@ int vb200_kv4_evict(vb200_kv4_t *h, vb200_kv4_t *into, const vb200_kv4_evict_t *
     if (!serve_on_device(a->mass)) return serve_fail("mass does not lie on the current device");
     const cudaStream_t st = (cudaStream_t)stream;
     EvictArgs e = {h->c, into->c, a->lengths, a->new_lengths, a->mass, a->new_mass, a->new_mass_ld, a->kept, a->keep, a->recent, a->first, into == h};
-    kv4_select_kernel<<<dim3(h->c.kv_heads, h->c.seqs), kSelThreads, 0, st>>>(e);
-    if (serve_launched()) return -1;
+    cudaError_t err = launch_pdl(kv4_select_kernel, dim3(h->c.kv_heads, h->c.seqs), dim3(kSelThreads), 0, st, e);
+    if (err != cudaSuccess) return serve_launched() | -1;
     if (into == h) {
-        kv4_move_kernel<true><<<dim3(1, h->c.kv_heads, h->c.seqs), kMoveThreads, 0, st>>>(e);
+        err = launch_pdl(kv4_move_kernel<true>, dim3(1, h->c.kv_heads, h->c.seqs), dim3(kMoveThreads), 0, st, e);
     } else {
         const int per = kMoveThreads / (2 * h->c.blocks);
         const long long chunks = ((long long)a->keep + per - 1) / per, heads = (long long)h->c.kv_heads * h->c.seqs;
         const long long most = std::max(1ll, (long long)h->w.sm_count * 16 / heads);
-        kv4_move_kernel<false><<<dim3((unsigned)std::min(chunks, most), h->c.kv_heads, h->c.seqs), kMoveThreads, 0, st>>>(e);
+        err = launch_pdl(kv4_move_kernel<false>, dim3((unsigned)std::min(chunks, most), h->c.kv_heads, h->c.seqs), dim3(kMoveThreads), 0, st, e);
     }
-    return serve_launched();
+    return err == cudaSuccess ? 0 : serve_launched() | -1;
 }
 
 int vb200_kv4_attention(vb200_kv4_t *h, const vb200_kv4_attention_t *a, void *stream) {

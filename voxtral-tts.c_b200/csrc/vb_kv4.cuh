@@ -29,7 +29,7 @@ constexpr int kWeightTerms = std::is_same<T, __nv_bfloat16>::value ? 1 : 2;
 struct Kv4Attn {
     Kv4 c;
     const int *lengths, *rows;
-    int max_rows, heads, group, splits, wide, wide_out;
+    int max_rows, heads, group, row_tiles, split, wide, wide_out;
     float scale;
     float *lse;
     const float *mass_in;

@@ -18,8 +18,10 @@
  * comes last at a ticket joins the parts.
  */
 #include <algorithm>
+#include <limits.h>
 
 #include "vb_kv4.cuh"
+#include "vb_tc.cuh"
 
 namespace vb {
 
@@ -126,7 +128,71 @@ VB_DEVINL void block_scores(float (&s)[4], const uint32_t wa, const uint32_t wb,
     s[3] = fmaf(c[3], fb, s[3]);
 }
 
-/* grid = (row tiles x splits, kv heads, sequences) */
+/* Which (sequence, unit, split) a CTA has. A unit is eight pairs of a KV head. Where there are fewer units than CTAs that run at once,
+ * sequences are cut so that all CTAs have about the same number of tiles, by their actual lengths: the smallest share, in whole
+ * rounds of a CTA's warps, with which there are enough CTAs. (With as many splits for each sequence, four of 65536 to 131072 tokens took
+ * the time of four of 131072.) A share is two rounds at least: what joining the parts of two CTAs takes, another round takes too. */
+struct APlace {
+    int seq, unit, split, share;
+};
+VB_DEVINL APlace attn_place(const Kv4Attn &a) {
+    const int lane = threadIdx.x & 31, n_cta = gridDim.x;
+    auto tiles_of = [&](int s, int *units) {
+        const Kv4Span span = kv4_span(a.lengths, a.rows, a.max_rows, s, a.c.capacity);
+        *units = (span.rows * a.group + kACols - 1) / kACols * a.c.kv_heads;
+        return (span.length + kAKeys - 1) / kAKeys;
+    };
+    /* the first 32 sequences stay in registers; there are at most a few hundred, or every unit has a CTA of its own */
+    int units0 = 0;
+    const int tiles0 = lane < a.c.seqs ? tiles_of(lane, &units0) : 0;
+    auto total = [&](auto &&f) {
+        long long n = units0 ? (long long)f(tiles0) * units0 : 0;
+        for (int s = lane + 32; s < a.c.seqs; s += 32) {
+            int units;
+            const int tiles = tiles_of(s, &units);
+            n += (long long)f(tiles) * units;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+        return n;
+    };
+    int most = tiles0;
+    for (int s = lane + 32; s < a.c.seqs; s += 32) {
+        int units;
+        most = max(most, tiles_of(s, &units));
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+    const long long all = total([](int tiles) { return max(tiles, 1); });
+    int share = (int)max((all + n_cta - 1) / n_cta, (long long)(most + kAMaxSplits - 1) / kAMaxSplits);
+    share = max(2 * kAWarps, (share + kAWarps - 1) / kAWarps * kAWarps);
+    /* a unit's last part may be short: a little more, in steps of a sixteenth, until the CTAs are enough */
+    while (share < most && total([&](int tiles) { return max(1, (tiles + share - 1) / share); }) > n_cta)
+        share += max(kAWarps, share / 16 / kAWarps * kAWarps);
+    /* this CTA's place: sequence by sequence, all units' first parts, then their second ones */
+    int left = blockIdx.x;
+    for (int s0 = 0; s0 < a.c.seqs; s0 += 32) {
+        int units = units0, tiles = tiles0;
+        if (s0 > 0) tiles = s0 + lane < a.c.seqs ? tiles_of(s0 + lane, &units) : 0;
+        if (s0 + lane >= a.c.seqs) units = 0;
+        const int mine = units * max(1, (tiles + share - 1) / share);
+        int upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        const unsigned there = __ballot_sync(0xffffffffu, left < upto);
+        if (there) {
+            const int who = __ffs(there) - 1;
+            const int at = left - (__shfl_sync(0xffffffffu, upto, who) - __shfl_sync(0xffffffffu, mine, who)), n = __shfl_sync(0xffffffffu, units, who);
+            return {s0 + who, at % n, at / n, share};
+        }
+        left -= __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return {a.c.seqs, 0, 0, share};
+}
+
+/* grid = CTAs that run at once, or (a.split == 0) sequences x units */
 template <int NB, int PT, class T>
 __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(const Kv4Attn a, const ServeRows<T> q, const ServeRows<T> out) {
     using Cfg = ACfg<NB>;
@@ -138,20 +204,22 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(co
     __shared__ int abort_flag, is_last;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int split = blockIdx.x % a.splits, tile_r = blockIdx.x / a.splits, kv_head = blockIdx.y, seq = blockIdx.z;
+    pdl_wait();
+    pdl_launch_dependents();       /* after the wait: the masses' kernel reads what this one has waited for */
+    const APlace place = a.split ? attn_place(a) : APlace{(int)blockIdx.x / (a.row_tiles * a.c.kv_heads), (int)blockIdx.x % (a.row_tiles * a.c.kv_heads), 0, INT_MAX};
+    if (place.seq >= a.c.seqs) return;
+    const int seq = place.seq, kv_head = place.unit % a.c.kv_heads, tile_r = place.unit / a.c.kv_heads, split = place.split, share = place.share;
     const Kv4Span span = kv4_span(a.lengths, a.rows, a.max_rows, seq, a.c.capacity);
     const int pairs = span.rows * a.group, pair0 = tile_r * kACols;
     if (pair0 >= pairs) return;
     const int n_pairs = min(kACols, pairs - pair0);
     const int before = span.length - span.rows;                      /* tokens before row 0 */
-    /* tokens that the tile's last row sees, in tiles; the share of this CTA is whole rounds of its warps */
+    /* tokens that the tile's last row sees, in tiles */
     const int seen = max(0, before + (pair0 + n_pairs - 1) / a.group + 1);
     const int tiles = (seen + kAKeys - 1) / kAKeys;
-    int share = (tiles + a.splits - 1) / a.splits;
-    share = max(kAWarps, (share + kAWarps - 1) / kAWarps * kAWarps);
-    const int used = max(1, (tiles + share - 1) / share);
+    const int used = tiles <= share ? 1 : (tiles + share - 1) / share;
     if (split >= used) return;
-    const int t_begin = split * share + warp, t_end = min(tiles, (split + 1) * share);
+    const int t_begin = split * share + warp, t_end = used == 1 ? tiles : min(tiles, (split + 1) * share);
 
     unsigned char *ring = a_smem + warp * Cfg::kStages * Cfg::kStage;
     const size_t row0 = a.c.row(seq, kv_head, 0);
@@ -412,9 +480,10 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(co
         mo[(warp * 2 * NB + i) * 32 + lane] = make_float4(o[i][0] * f0 * f1, o[i][1] * f0 * f1, o[i][2] * f0 * f1, o[i][3] * f0 * f1);
     }
     __syncthreads();
-    const int unit = (seq * a.c.kv_heads + kv_head) * (gridDim.x / a.splits) + tile_r;
     constexpr int kPart = kACols * (kDim + 2);           /* floats of a part: results, references, sums */
-    float *parts = a.part + (size_t)unit * a.splits * kPart;
+    const int stride = (pairs + kACols - 1) / kACols * a.c.kv_heads, first_cta = (int)blockIdx.x - split * stride;       /* of this unit; its parts lie so many CTAs apart */
+    float *parts = a.part + (size_t)first_cta * kPart;
+    const size_t step = (size_t)stride * kPart;
     /* four results of columns 2 t, 2 t + 1 and dims d, d + 1, against a reference and a sum each */
     auto finish = [&](int i, float4 v, float2 total, float2 reference) {
         const int d = Cfg::kWhole ? g * (4 * NB) + 2 * i : 32 * (i / 2) + 4 * g + 2 * (i & 1);
@@ -464,11 +533,11 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(co
                 v.w = fmaf(x.w, f[w].y, v.w);
             }
             if (used == 1) finish(i, v, total, reference);
-            else reinterpret_cast<float4 *>(parts + split * kPart)[i * 32 + lane] = v;
+            else reinterpret_cast<float4 *>(parts + split * step)[i * 32 + lane] = v;
         }
         if (used == 1) return;
         if (warp == 0 && g == 0) {
-            float2 *to = reinterpret_cast<float2 *>(parts + split * kPart + kACols * kDim);
+            float2 *to = reinterpret_cast<float2 *>(parts + split * step + kACols * kDim);
             to[t] = reference;
             to[4 + t] = total;
         }
@@ -477,14 +546,14 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(co
     __threadfence();
     __syncthreads();
     if (tid == 0) {
-        is_last = atomicAdd(&a.tickets[unit], 1u) == (unsigned)used - 1u;
-        if (is_last) a.tickets[unit] = 0u;
+        is_last = atomicAdd(&a.tickets[first_cta], 1u) == (unsigned)used - 1u;
+        if (is_last) a.tickets[first_cta] = 0u;
         __threadfence();
     }
     __syncthreads();
     if (!is_last) return;
     float2 *ends = reinterpret_cast<float2 *>(a_smem);               /* references and sums of all parts; then factors in their place */
-    for (int x = tid; x < used * 8; x += kAThreads) ends[x] = __ldcg(reinterpret_cast<const float2 *>(parts + (x >> 3) * kPart + kACols * kDim) + (x & 7));
+    for (int x = tid; x < used * 8; x += kAThreads) ends[x] = __ldcg(reinterpret_cast<const float2 *>(parts + (x >> 3) * step + kACols * kDim) + (x & 7));
     __syncthreads();
     float2 reference = make_float2(-INFINITY, -INFINITY), total = make_float2(0.0f, 0.0f);
     for (int w = 0; w < used; w++) {
@@ -501,7 +570,7 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(co
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
         for (int w = 0; w < used; w++) {
-            const float4 x = __ldcg(reinterpret_cast<const float4 *>(parts + w * kPart) + i * 32 + lane);
+            const float4 x = __ldcg(reinterpret_cast<const float4 *>(parts + w * step) + i * 32 + lane);
             const float2 m = ends[w * 8 + t];
             const float fx = factor(m.x, reference.x), fy = factor(m.y, reference.y);
             v.x = fmaf(x.x, fx, v.x);
@@ -536,10 +605,17 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_mass_kernel(co
     __shared__ int abort_flag;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int kv_head = blockIdx.y, seq = blockIdx.z;
+    /* begins beside the end of the attention kernel, which has waited for all that is read here but the rows' sums; masses may not
+     * be written before those are waited for either */
+    const bool alone = a.max_rows == 0;
+    if (alone) pdl_wait();
     const Kv4Span span = kv4_span(a.lengths, a.rows, a.max_rows, seq, a.c.capacity);
     const int pairs = span.rows * a.group, before = span.length - span.rows;
     const int cta0 = blockIdx.x * kAWarps * warp_tiles * kAKeys;
-    if (cta0 >= span.length) return;
+    if (cta0 >= span.length) {
+        if (!alone) pdl_wait();    /* no launch is over before the ones it follows are */
+        return;
+    }
     const int tile0 = (blockIdx.x * kAWarps + warp) * warp_tiles, tiles = min(warp_tiles, (span.length + kAKeys - 1) / kAKeys - tile0);
     unsigned char *keys = a_smem + warp * warp_tiles * Cfg::kTile;
     uint2 *q_s = reinterpret_cast<uint2 *>(a_smem + kAWarps * warp_tiles * Cfg::kTile);
@@ -560,12 +636,14 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_mass_kernel(co
     for (int i = 0; i < kMTiles; i++)
 #pragma unroll
         for (int j = 0; j < 4; j++) mass[i][j >> 1][j & 1] = 0.0f;
-    bool here = tiles <= 0;
+    bool here = tiles <= 0, waited = alone;
     /* rows before this CTA's first token see none of its tokens */
     for (int group0 = max(0, cta0 - before) * a.group / kACols * kACols; group0 < pairs; group0 += kAWarps * kACols) {
         __syncthreads();                                                            /* the pairs before are done with */
         const int made = min(kAWarps, (pairs - group0 + kACols - 1) / kACols);
         if (warp < made) make_queries<NB, QT>(q, a, seq, kv_head, group0 + warp * kACols, pairs, q_s + warp * (Cfg::kQ / 8), mul_s + warp * kACols);
+        if (!waited) pdl_wait();
+        waited = true;
         if (tid < kAWarps * kACols) {
             const int pair = group0 + tid, row = pair / a.group;
             const float lse = pair < pairs ? a.lse[((size_t)seq * a.max_rows + row) * a.heads + kv_head * a.group + pair - row * a.group] : 0.0f;
@@ -623,6 +701,7 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_mass_kernel(co
             }
         }
     }
+    if (!waited) pdl_wait();
     if (!here) vb_mbar_wait(&full[warp], 0u, &abort_flag);                          /* no rows: nothing leaves while its keys are on their way */
     const size_t base = ((size_t)seq * a.c.kv_heads + kv_head) * a.c.capacity;
 #pragma unroll
@@ -652,22 +731,22 @@ int attn_launch(const Kv4Attn &args, const vb200_kv4_attention_t &v, const Kv4Wo
     if (NB <= 4 && (long long)a.max_rows * a.group > kAMostPairs) {
         if (kv4_prompt(a, q, out, st)) return -1;
     } else if (a.max_rows > 0) {
-        /* as many splits as fill the GPU with what runs at once, none of them under a tile a warp */
         const long long row_tiles = ((long long)a.max_rows * a.group + kACols - 1) / kACols;
         const long long units = row_tiles * a.c.kv_heads * a.c.seqs, at_once = (long long)work.sm_count * (NB <= 4 ? 2 : 1);
-        const long long most = ((long long)a.c.capacity + kAKeys * kAWarps - 1) / (kAKeys * kAWarps);
-        a.splits = (int)std::max(1ll, std::min({at_once / units, most, (long long)kAMaxSplits}));
-        kv4_attn_kernel<NB, PT, T><<<dim3((unsigned)(row_tiles * a.splits), a.c.kv_heads, a.c.seqs), kAThreads, Cfg::kBig, st>>>(a, q, out);
-        if (serve_launched()) return -1;
+        if (units > INT_MAX) return serve_fail("too many rows");
+        a.row_tiles = (int)row_tiles;
+        a.split = units < at_once && a.c.capacity > 2 * kAWarps * kAKeys;
+        if (launch_pdl(kv4_attn_kernel<NB, PT, T>, dim3((unsigned)(a.split ? at_once : units)), dim3(kAThreads), Cfg::kBig, st, a, q, out) != cudaSuccess)
+            return serve_launched() | -1;
     }
     if (a.mass_out) {
-        /* the more tiles a warp has, the fewer CTAs make the queries: as many as leave every SM two CTAs */
+        /* the more tiles a warp has, the fewer CTAs make the queries: as many as leave every SM one */
         const long long heads = (long long)a.c.kv_heads * a.c.seqs, tiles = ((long long)a.c.capacity + kAKeys - 1) / kAKeys;
         int warp_tiles = kMTiles;
-        while (warp_tiles > 1 && tiles / (kAWarps * warp_tiles) * heads < 2 * work.sm_count) warp_tiles >>= 1;
-        kv4_mass_kernel<NB, T><<<dim3((unsigned)((tiles + kAWarps * warp_tiles - 1) / (kAWarps * warp_tiles)), a.c.kv_heads, a.c.seqs), kAThreads,
-                                 MCfg<NB, T>::smem(warp_tiles), st>>>(a, q, warp_tiles);
-        return serve_launched();
+        while (warp_tiles > 1 && (tiles + kAWarps * warp_tiles - 1) / (kAWarps * warp_tiles) * heads < work.sm_count) warp_tiles >>= 1;
+        const dim3 grid((unsigned)((tiles + kAWarps * warp_tiles - 1) / (kAWarps * warp_tiles)), a.c.kv_heads, a.c.seqs);
+        if (launch_pdl(kv4_mass_kernel<NB, T>, grid, dim3(kAThreads), MCfg<NB, T>::smem(warp_tiles), st, a, q, warp_tiles) != cudaSuccess)
+            return serve_launched() | -1;
     }
     return 0;
 }

@@ -104,6 +104,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int kv_head = blockIdx.y, seq = blockIdx.z;
+    pdl_wait();
     const Kv4Span span = kv4_span(a.lengths, a.rows, a.max_rows, seq, a.c.capacity);
     const int pairs = span.rows * a.group;
     const int pair0 = ((int)gridDim.x - 1 - (int)blockIdx.x) * kPRows;             /* the latest rows see the most tokens: they go first */
@@ -135,6 +136,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    pdl_launch_dependents();       /* not before the allocation: a kernel that starts early must not take columns this one needs */
     const uint32_t tmem = *(volatile uint32_t *)&tmem_slot;
     auto give_up = [&]() {
         atomicCAS(a.status, 0, kPStatus);
@@ -508,8 +510,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
 template <int NB, class T>
 int prompt_launch(const Kv4Attn &a, const ServeRows<T> &q, const ServeRows<T> &out, cudaStream_t st) {
     const int tiles = (int)(((long long)a.max_rows * a.group + kPRows - 1) / kPRows);
-    kv4_prompt_kernel<NB, kWeightTerms<T>, T><<<dim3(tiles, a.c.kv_heads, a.c.seqs), kPThreads, PCfg<NB, sizeof(T) == 4 ? 2 : 1>::kSmem, st>>>(a, q, out);
-    return serve_launched();
+    const size_t smem = PCfg<NB, sizeof(T) == 4 ? 2 : 1>::kSmem;
+    return launch_pdl(kv4_prompt_kernel<NB, kWeightTerms<T>, T>, dim3(tiles, a.c.kv_heads, a.c.seqs), dim3(kPThreads), smem, st, a, q, out) == cudaSuccess ? 0 : serve_launched() | -1;
 }
 template <int NB, class T>
 bool prompt_load() {

@@ -12,6 +12,7 @@
 #include <type_traits>
 
 #include "vb_serve.cuh"
+#include "vb_tc.cuh"
 
 namespace vb {
 
@@ -110,6 +111,8 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const LpArgs a)
     asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(splits));
     /* waited for before anything is sent to another CTA's shared memory: by then that CTA runs */
     asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    pdl_launch_dependents();
+    pdl_wait();
     const int row = blockIdx.x / splits;
     const T *x = static_cast<const T *>(a.x) + (long long)row * a.stride;
     /* elements before the first 16-byte boundary, then whole vectors, then the rest; this CTA's share of the vectors */
@@ -374,17 +377,7 @@ int logprobs_launch(const LpArgs &a, int sm_count, cudaStream_t st) {
     constexpr int kStretch = kLpThreads * kLpUnrolled<T> * (16 / (int)sizeof(T));
     int splits = 1;
     while (splits < kLpMaxSplit && (long long)a.rows * splits * 2 <= 2 * sm_count && a.vocab >= splits * kStretch) splits *= 2;
-    cudaLaunchConfig_t c = {};
-    c.gridDim = dim3((unsigned)a.rows * splits);
-    c.blockDim = dim3(kLpThreads);
-    c.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = splits;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    c.attrs = at;
-    c.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&c, logprobs_kernel<T>, a);
+    const cudaError_t e = launch_pdl_cluster(logprobs_kernel<T>, splits, dim3((unsigned)a.rows * splits), dim3(kLpThreads), 0, st, a);
     if (e != cudaSuccess) {
         cudaGetLastError();
         return serve_fail(cudaGetErrorString(e));
