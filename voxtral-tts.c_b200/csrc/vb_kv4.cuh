@@ -73,6 +73,18 @@ VB_DEVINL void get_bytes(const uint8_t *p, uint32_t (&b)[N]) {
         for (int i = 0; i < N; i++) b[i] = p[i];
     }
 }
+/* N scale bytes side by side as numbers (infinity for 255: its block is zeros, so that it adds NaN). A shift to the left goes to the
+ * pipe of the multiply-adds, which has room */
+template <int N>
+VB_DEVINL void get_scales(const uint8_t *p, float (&f)[N]) {
+    constexpr int kEach = N % 4 == 0 ? 4 : N % 2 == 0 ? 2 : 1;
+#pragma unroll
+    for (int i = 0; i < N / kEach; i++) {
+        const uint32_t w = kEach == 4 ? reinterpret_cast<const uint32_t *>(p)[i] : kEach == 2 ? reinterpret_cast<const uint16_t *>(p)[i] : p[i];
+#pragma unroll
+        for (int j = 0; j < kEach; j++) f[kEach * i + j] = __uint_as_float((j < 3 ? w << (23 - 8 * j) : w >> 1) & 0x7f800000u);
+    }
+}
 /* N words side by side (aligned to N's largest power of two, up to four) */
 template <int N>
 VB_DEVINL void get_words(const uint8_t *p, uint32_t (&w)[N]) {

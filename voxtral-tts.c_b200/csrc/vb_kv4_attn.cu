@@ -50,6 +50,12 @@ VB_DEVINL void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uin
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b.x), "r"(b.y));
 }
+/* without what was there before */
+VB_DEVINL void mma_f16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b.x), "r"(b.y), "f"(0.0f));
+}
 VB_DEVINL uint32_t mat_turn(uint32_t v) {
     uint32_t r;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
@@ -92,8 +98,10 @@ VB_DEVINL void make_queries(const ServeRows<T> &q, const Kv4Attn &a, int seq, in
     most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
     /* the largest to [2^14, 2^15); rows of zeros, or with a value that is not finite, as they are */
     const uint32_t e = most >> 23, field = e == 0u || e == 255u ? 127u : min(268u - e, 253u);
-    const float up = __uint_as_float(field << 23), down = __uint_as_float((254u - field) << 23);
-    if (t == 0) mul_s[n] = a.scale * 1.44269504f * down;
+    const float down = __uint_as_float((254u - field) << 23);
+    float up = __uint_as_float(field << 23);
+    if (a.scale <= 0.0f) up = a.scale < 0.0f ? -up : 0.0f;               /* the factor is positive: the largest score is the largest product */
+    if (t == 0) mul_s[n] = (a.scale != 0.0f ? fabsf(a.scale) * 1.44269504f : 1.0f) * down;
 #pragma unroll
     for (int b = 0; b < NB; b++)
 #pragma unroll
@@ -112,20 +120,21 @@ VB_DEVINL void make_queries(const ServeRows<T> &q, const Kv4Attn &a, int seq, in
 }
 
 /* Scores of 16 tokens: `at` words of the lane's two tokens (g and g + 8 of them), c: tokens g, g + 8 x columns 2 t, 2 t + 1. */
-template <int NB, int QT>
+template <bool FIRST, int QT>
 VB_DEVINL void block_scores(float (&s)[4], const uint32_t wa, const uint32_t wb, float fa, float fb, const uint2 (&q)[2][QT]) {
     uint32_t ra[4], rb[4];
     kv4_halves(wa, ra);
     kv4_halves(wb, rb);
-    float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    float c[4];
+    mma_f16_first(c, ra[0], rb[0], ra[1], rb[1], q[0][0]);
+    if constexpr (QT == 2) mma_f16(c, ra[0], rb[0], ra[1], rb[1], q[0][1]);
 #pragma unroll
-    for (int h = 0; h < 2; h++)
+    for (int u = 0; u < QT; u++) mma_f16(c, ra[2], rb[2], ra[3], rb[3], q[1][u]);
 #pragma unroll
-        for (int u = 0; u < QT; u++) mma_f16(c, ra[2 * h], rb[2 * h], ra[2 * h + 1], rb[2 * h + 1], q[h][u]);
-    s[0] = fmaf(c[0], fa, s[0]);
-    s[1] = fmaf(c[1], fa, s[1]);
-    s[2] = fmaf(c[2], fb, s[2]);
-    s[3] = fmaf(c[3], fb, s[3]);
+    for (int j = 0; j < 4; j++) {
+        const float f = j < 2 ? fa : fb;
+        s[j] = FIRST ? c[j] * f : fmaf(c[j], f, s[j]);
+    }
 }
 
 /* Which (sequence, unit, split) a CTA has. A unit is eight pairs of a KV head. Where there are fewer units than CTAs that run at once,
@@ -284,19 +293,16 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(co
         /* scores */
         float s[2][4];
         {
-            uint32_t w[2][2][NB], f[2][2][NB];
+            uint32_t w[2][2][NB];
+            float f[2][2][NB];
 #pragma unroll
             for (int m = 0; m < 2; m++)
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
                     const int key = m * 16 + u * 8 + g;
                     get_words<NB>(ks + key * (NB * 16) + t * (NB * 4), w[m][u]);
-                    get_bytes<NB>(kss + key * NB, f[m][u]);
+                    get_scales<NB>(kss + key * NB, f[m][u]);
                 }
-#pragma unroll
-            for (int m = 0; m < 2; m++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) s[m][j] = 0.0f;
 #pragma unroll
             for (int b = 0; b < NB; b++) {
                 uint2 qf[2][QT];
@@ -306,19 +312,21 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(co
                     for (int u = 0; u < QT; u++) qf[h][u] = q_s[((b * 2 + h) * QT + u) * 32 + lane];
 #pragma unroll
                 for (int m = 0; m < 2; m++)
-                    block_scores<NB, QT>(s[m], w[m][0][b], w[m][1][b], __uint_as_float(f[m][0][b] << 23), __uint_as_float(f[m][1][b] << 23), qf);
+                    if (b == 0) block_scores<true, QT>(s[m], w[m][0][b], w[m][1][b], f[m][0][b], f[m][1][b], qf);
+                    else block_scores<false, QT>(s[m], w[m][0][b], w[m][1][b], f[m][0][b], f[m][1][b], qf);
             }
         }
         const bool masked = j0 + kAKeys > all_see;
-        float top[2] = {-INFINITY, -INFINITY};
+        if (masked) {
 #pragma unroll
-        for (int m = 0; m < 2; m++)
+            for (int m = 0; m < 2; m++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                s[m][j] *= mul[j & 1];
-                if (masked && j0 + m * 16 + (j >> 1) * 8 + g >= sees[j & 1]) s[m][j] = -INFINITY;
-                top[j & 1] = fmaxf(top[j & 1], s[m][j]);
-            }
+                for (int j = 0; j < 4; j++)
+                    if (j0 + m * 16 + (j >> 1) * 8 + g >= sees[j & 1]) s[m][j] = -INFINITY;
+        }
+        float top[2];
+#pragma unroll
+        for (int u = 0; u < 2; u++) top[u] = fmaxf(fmaxf(s[0][u], s[0][2 + u]), fmaxf(s[1][u], s[1][2 + u])) * mul[u];      /* the factors are positive */
         if (__any_sync(0xffffffffu, top[0] > ref[0] + 8.0f || top[1] > ref[1] + 8.0f)) {
 #pragma unroll
             for (int u = 0; u < 2; u++) {
@@ -343,7 +351,7 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(co
         for (int m = 0; m < 2; m++) {
             float e[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) e[j] = exp2_fast(s[m][j] - ((j & 1) ? low1 : low0));
+            for (int j = 0; j < 4; j++) e[j] = exp2_fast(fmaf(s[m][j], mul[j & 1], (j & 1) ? -low1 : -low0));
             sum[0] += e[0] + e[2];
             sum[1] += e[1] + e[3];
             const uint32_t h0 = half_pack(e[0], e[1]), h1 = half_pack(e[2], e[3]);
@@ -354,24 +362,38 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(co
             }
         }
 
-        /* values: tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of each 16 */
-        uint32_t vsc[2][4][kVS];
-        int most[kVS];
+        /* values: tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of each 16; their scale bytes in pairs, the largest and the smallest of them */
+        uint32_t vsc[2][2][kVS];
+        int most[kVS], least[kVS];
 #pragma unroll
-        for (int i = 0; i < kVS; i++) most[i] = 0;
+        for (int i = 0; i < kVS; i++) {
+            uint32_t hi = 0u, lo = 0x00ff00ffu;
 #pragma unroll
-        for (int m = 0; m < 2; m++)
+            for (int m = 0; m < 2; m++)
 #pragma unroll
-            for (int x = 0; x < 4; x++) {
-                const int key = m * 16 + (x >> 1) * 8 + 2 * t + (x & 1);
-                if constexpr (Cfg::kWhole) vsc[m][x][0] = vss[key * NB + g * NB / 8];
-                else get_bytes<kVS>(vss + key * NB, vsc[m][x]);
-#pragma unroll
-                for (int i = 0; i < kVS; i++) {
-                    if (masked && j0 + key >= seen) vsc[m][x][i] = 0;        /* whatever lies behind the last token */
-                    most[i] = max(most[i], (int)vsc[m][x][i]);
+                for (int x = 0; x < 2; x++) {
+                    const unsigned char *at = vss + (m * 16 + x * 8 + 2 * t) * NB + (Cfg::kWhole ? g * NB / 8 : i);
+                    vsc[m][x][i] = at[0] + 65536u * at[NB];
                 }
+            if (masked) {                                /* whatever lies behind the last token */
+#pragma unroll
+                for (int m = 0; m < 2; m++)
+#pragma unroll
+                    for (int x = 0; x < 2; x++) {
+                        const int key = j0 + m * 16 + x * 8 + 2 * t;
+                        vsc[m][x][i] = key + 1 < seen ? vsc[m][x][i] : key < seen ? vsc[m][x][i] & 0xffffu : 0u;
+                    }
             }
+#pragma unroll
+            for (int m = 0; m < 2; m++)
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    hi = __vmaxu2(hi, vsc[m][x][i]);
+                    lo = __vminu2(lo, vsc[m][x][i]);
+                }
+            most[i] = (int)max(hi & 0xffffu, hi >> 16);
+            least[i] = (int)min(lo & 0xffffu, lo >> 16);
+        }
         bool rise = false;
 #pragma unroll
         for (int i = 0; i < kVS; i++) rise |= most[i] > top_scale[i];
@@ -388,11 +410,14 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(co
                     for (int m = 0; m < 2; m++)
 #pragma unroll
                         for (int x = 0; x < 4; x++) {
-                            if (vsc[m][x][i] == 255u) {
+                            const uint32_t at = 16u * (x & 1), byte = (vsc[m][x >> 1][i] >> at) & 0xffffu;
+                            if (byte == 255u) {
                                 bad = min(bad, j0 + m * 16 + (x >> 1) * 8 + 2 * t + (x & 1));
-                                vsc[m][x][i] = 0;
+                                vsc[m][x >> 1][i] &= ~(0xffffu << at);
+                                least[i] = 0;
+                            } else {
+                                most[i] = max(most[i], (int)byte);
                             }
-                            most[i] = max(most[i], (int)vsc[m][x][i]);
                         }
 #pragma unroll
                     for (int x = 1; x < 4; x <<= 1) {
@@ -418,16 +443,33 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(co
                 }
             }
         }
+        /* 2^(byte - top + 13) in FP16: an exponent field of byte - top + 28, two at a time, where that is a normal number for all */
+        bool deep = false;
 #pragma unroll
-        for (int m = 0; m < 2; m++) {
-            uint32_t f[2][kVS];
+        for (int i = 0; i < kVS; i++) deep |= least[i] + 27 < top_scale[i];
+        if (!__any_sync(0xffffffffu, deep)) {
+#pragma unroll
+            for (int i = 0; i < kVS; i++) {
+                const uint32_t add = (uint32_t)(28 - top_scale[i]) * 0x04000400u;
+#pragma unroll
+                for (int m = 0; m < 2; m++)
+#pragma unroll
+                    for (int x = 0; x < 2; x++) vsc[m][x][i] = vsc[m][x][i] * 1024u + add;
+            }
+        } else {
 #pragma unroll
             for (int i = 0; i < kVS; i++)
 #pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    const int lo = (int)vsc[m][2 * x][i] + 140 - top_scale[i], hi = (int)vsc[m][2 * x + 1][i] + 140 - top_scale[i];
-                    f[x][i] = half_pack(__uint_as_float((uint32_t)max(lo, 0) << 23), __uint_as_float((uint32_t)max(hi, 0) << 23));
-                }
+                for (int m = 0; m < 2; m++)
+#pragma unroll
+                    for (int x = 0; x < 2; x++) {
+                        const int lo = (int)(vsc[m][x][i] & 0xffffu) + 140 - top_scale[i], hi = (int)(vsc[m][x][i] >> 16) + 140 - top_scale[i];
+                        vsc[m][x][i] = half_pack(__uint_as_float((uint32_t)max(lo, 0) << 23), __uint_as_float((uint32_t)max(hi, 0) << 23));
+                    }
+        }
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+            const uint32_t (&f)[2][kVS] = vsc[m];
             uint32_t w[4][kW];
 #pragma unroll
             for (int x = 0; x < 4; x++) get_values<NB>(vs + (m * 16 + (x >> 1) * 8 + 2 * t + (x & 1)) * (NB * 16) + g * (NB * 2), w[x]);
@@ -664,18 +706,19 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_mass_kernel(co
             if (i >= tiles) break;
             const unsigned char *ks = keys + i * kAKeys * NB * 16, *kss = keys + (warp_tiles * 16 + i) * kAKeys * NB;
             const int j0 = (tile0 + i) * kAKeys;
-            uint32_t w[2][2][NB], f[2][2][NB];
+            uint32_t w[2][2][NB];
+            float f[2][2][NB];
 #pragma unroll
             for (int m = 0; m < 2; m++)
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
                     const int key = m * 16 + u * 8 + g;
                     get_words<NB>(ks + key * (NB * 16) + t * (NB * 4), w[m][u]);
-                    get_bytes<NB>(kss + key * NB, f[m][u]);
+                    get_scales<NB>(kss + key * NB, f[m][u]);
                 }
 #pragma unroll 1
             for (int r = 0; r < made; r++) {
-                float s[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+                float s[2][4];
 #pragma unroll
                 for (int b = 0; b < NB; b++) {
                     uint2 qf[2][QT];
@@ -685,7 +728,8 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_mass_kernel(co
                         for (int u = 0; u < QT; u++) qf[h][u] = q_s[r * (Cfg::kQ / 8) + ((b * 2 + h) * QT + u) * 32 + lane];
 #pragma unroll
                     for (int m = 0; m < 2; m++)
-                        block_scores<NB, QT>(s[m], w[m][0][b], w[m][1][b], __uint_as_float(f[m][0][b] << 23), __uint_as_float(f[m][1][b] << 23), qf);
+                        if (b == 0) block_scores<true, QT>(s[m], w[m][0][b], w[m][1][b], f[m][0][b], f[m][1][b], qf);
+                        else block_scores<false, QT>(s[m], w[m][0][b], w[m][1][b], f[m][0][b], f[m][1][b], qf);
                 }
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
