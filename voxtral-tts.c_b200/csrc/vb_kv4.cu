@@ -42,67 +42,59 @@ namespace {
 constexpr int kRowThreads = 256, kRowUnroll = 4;
 
 /* ------------------------------------------------------------------ rows into the cache and out of it
- * A thread has words of 8 values: four lanes make a block of 32. The words of a token (keys, then values) lie side by side in the order of
- * threads; a CTA takes 1024 of them at a time, four a thread with their loads together. Memory-bound, and at one row a launch bound by its
- * latency. */
+ * A CTA has rows of one head, keys or values; a thread a word of 8 values of a row, four rows at a time with their loads together; four
+ * lanes make a block of 32. Memory-bound, and at one row a launch bound by its latency. (With words of all heads side by side, indices
+ * worked out word by word, 4097 rows of two sequences took 22 us in and 16 out.) */
 template <class T>
 struct RowsArgs {
     Kv4 c;
     const int *lengths, *rows;
     int max_rows, wide;
-    unsigned tokens;                                     /* seqs * max_rows */
     ServeRows<T> k, v;
 };
 
 template <int NB, class T, bool READ>
 __global__ void __launch_bounds__(kRowThreads) kv4_rows_kernel(const RowsArgs<T> a) {
-    constexpr unsigned kWords = NB * 4;                  /* of a row of a head */
-    constexpr long long kChunk = kRowThreads * kRowUnroll;
-    const unsigned plane = a.c.kv_heads * kWords, token_words = 2 * plane;
-    const long long total = (long long)a.tokens * token_words;
-    const int tid = threadIdx.x;
+    constexpr int kWords = NB * 4;                                       /* of a row */
+    const int kRows = (int)blockDim.x / kWords;                          /* rows side by side */
+    const int tid = threadIdx.x, w = tid % kWords, r0 = tid / kWords, h = blockIdx.y >> 1, s = blockIdx.z;
+    const bool is_v = blockIdx.y & 1;
     pdl_launch_dependents();
     pdl_wait();
-    for (long long c0 = blockIdx.x * kChunk; c0 < total; c0 += gridDim.x * kChunk) {
-        const unsigned token0 = (unsigned)(c0 / token_words), off0 = (unsigned)(c0 - (long long)token0 * token_words);
+    const Kv4Span span = kv4_span(a.lengths, a.rows, a.max_rows, s, a.c.capacity);
+    const int before = span.length - span.rows;                          /* slot of row 0 */
+    T *x = (is_v ? a.v.data + s * a.v.seq + h * a.v.head : a.k.data + s * a.k.seq + h * a.k.head) + w * 8;
+    const long long ld = is_v ? a.v.row : a.k.row;
+    const size_t row0 = a.c.row(s, h, 0);
+    uint8_t *codes = (is_v ? a.c.v : a.c.k) + row0 * (NB * 16), *scales = (is_v ? a.c.vs : a.c.ks) + row0 * NB + (w >> 2);
+    /* where this thread's word lies in a row of codes; values of 96 and 192 as two half words */
+    const int at = is_v ? kv4_value_half(2 * w, NB) * 2 : kv4_key_word(w, NB) * 4, at2 = kv4_value_half(2 * w + 1, NB) * 2;
+    const bool halves = !kv4_whole(NB) && is_v;
+    for (int c0 = blockIdx.x * (kRows * kRowUnroll); c0 < span.rows; c0 += gridDim.x * (kRows * kRowUnroll)) {
         float v[kRowUnroll][8];
-        uint32_t code[kRowUnroll], byte[kRowUnroll], w[kRowUnroll];
-        size_t row[kRowUnroll];
-        T *p[kRowUnroll];
-        bool real[kRowUnroll], is_v[kRowUnroll];
+        uint32_t code[kRowUnroll], byte[kRowUnroll];
+        bool real[kRowUnroll];
 #pragma unroll
         for (int u = 0; u < kRowUnroll; u++) {
-            const unsigned o = off0 + u * kRowThreads + tid, ahead = o / token_words, rest = o - ahead * token_words;
-            is_v[u] = rest >= plane;
-            const unsigned in_plane = is_v[u] ? rest - plane : rest, h = in_plane / kWords;
-            w[u] = in_plane - h * kWords;
-            const bool in = token0 + ahead < a.tokens;
-            const unsigned token = in ? token0 + ahead : 0, s = token / a.max_rows, r = token - s * a.max_rows;
-            const Kv4Span span = kv4_span(a.lengths, a.rows, a.max_rows, s, a.c.capacity);
-            const int slot = span.length - span.rows + (int)r;
-            real[u] = in && (int)r < span.rows && slot >= 0;
-            const ServeRows<T> &x = is_v[u] ? a.v : a.k;
-            p[u] = x.data + (long long)s * x.seq + (long long)r * x.row + (long long)h * x.head + w[u] * 8;
-            row[u] = a.c.row(s, h, real[u] ? slot : 0);
+            const int r = c0 + u * kRows + r0, slot = before + r;
+            real[u] = r0 < kRows && r < span.rows && slot >= 0;
             if (!READ) {
 #pragma unroll
                 for (int j = 0; j < 8; j++) v[u][j] = 0.0f;
-                if (real[u]) serve_load<8>(p[u], a.wide, v[u]);
-            } else if (real[u]) {
-                const uint8_t *base = (is_v[u] ? a.c.v : a.c.k) + row[u] * (NB * 16);
-                if (!is_v[u]) {
-                    code[u] = reinterpret_cast<const uint32_t *>(base)[kv4_key_word(w[u], NB)];
-                } else if (kv4_whole(NB)) {
-                    code[u] = reinterpret_cast<const uint32_t *>(base)[w[u]];
-                } else {
-                    const uint16_t *from = reinterpret_cast<const uint16_t *>(base);
-                    code[u] = from[kv4_value_half(2 * w[u], NB)] | ((uint32_t)from[kv4_value_half(2 * w[u] + 1, NB)] << 16);
+                if (real[u]) serve_load<8>(x + r * ld, a.wide, v[u]);
+            } else {
+                code[u] = byte[u] = 0;
+                if (real[u]) {
+                    const uint8_t *base = codes + (size_t)slot * (NB * 16);
+                    code[u] = halves ? *reinterpret_cast<const uint16_t *>(base + at) | ((uint32_t) * reinterpret_cast<const uint16_t *>(base + at2) << 16)
+                                     : *reinterpret_cast<const uint32_t *>(base + at);
+                    byte[u] = scales[(size_t)slot * NB];
                 }
-                byte[u] = (is_v[u] ? a.c.vs : a.c.ks)[row[u] * NB + (w[u] >> 2)];
             }
         }
 #pragma unroll
         for (int u = 0; u < kRowUnroll; u++) {
+            const int r = c0 + u * kRows + r0;
             if (!READ) {
                 /* the largest magnitude by its bits, so that a NaN is the largest of all */
                 uint32_t most = 0;
@@ -113,19 +105,15 @@ __global__ void __launch_bounds__(kRowThreads) kv4_rows_kernel(const RowsArgs<T>
                 if (!real[u]) continue;
                 const uint32_t scale = kv4_scale(__uint_as_float(most));
                 const uint32_t c = scale == 255u ? 0u : kv4_codes(v[u], kv4_inverse(scale));       /* a block that is NaN: codes of zero */
-                uint8_t *base = (is_v[u] ? a.c.v : a.c.k) + row[u] * (NB * 16);
-                if (!is_v[u]) {
-                    reinterpret_cast<uint32_t *>(base)[kv4_key_word(w[u], NB)] = c;
-                } else if (kv4_whole(NB)) {
-                    reinterpret_cast<uint32_t *>(base)[w[u]] = c;
+                uint8_t *base = codes + (size_t)(before + r) * (NB * 16);
+                if (halves) {
+                    *reinterpret_cast<uint16_t *>(base + at) = (uint16_t)c;
+                    *reinterpret_cast<uint16_t *>(base + at2) = (uint16_t)(c >> 16);
                 } else {
-                    uint16_t *to = reinterpret_cast<uint16_t *>(base);
-                    to[kv4_value_half(2 * w[u], NB)] = (uint16_t)c;
-                    to[kv4_value_half(2 * w[u] + 1, NB)] = (uint16_t)(c >> 16);
+                    *reinterpret_cast<uint32_t *>(base + at) = c;
                 }
-                if ((w[u] & 3) == 0) (is_v[u] ? a.c.vs : a.c.ks)[row[u] * NB + (w[u] >> 2)] = (uint8_t)scale;
+                if ((w & 3) == 0) scales[(size_t)(before + r) * NB] = (uint8_t)scale;
             } else {
-                if (!real[u]) code[u] = byte[u] = 0;
                 const float scale = kv4_scale_value(byte[u]);
                 uint32_t half[4];
                 kv4_halves(code[u], half);
@@ -135,8 +123,9 @@ __global__ void __launch_bounds__(kRowThreads) kv4_rows_kernel(const RowsArgs<T>
                     v[u][2 * j] = f.x * scale;
                     v[u][2 * j + 1] = f.y * scale;
                 }
+                T *p = x + r * ld;
                 if constexpr (sizeof(T) == 4) {
-                    /* two lanes' 64 bytes, 32 of them a store: whole sectors (the words of a pair are one token's and one head's) */
+                    /* two lanes' 64 bytes, 32 of them a store: whole sectors (the words of a pair are one row's) */
                     const bool odd = tid & 1;
                     float other[4];
 #pragma unroll
@@ -146,13 +135,13 @@ __global__ void __launch_bounds__(kRowThreads) kv4_rows_kernel(const RowsArgs<T>
                     }
                     if (!real[u]) continue;
                     if (a.wide) {
-                        float4 *to = reinterpret_cast<float4 *>(p[u] - (odd ? 8 : 0)) + (odd ? 1 : 0);
+                        float4 *to = reinterpret_cast<float4 *>(p - (odd ? 8 : 0)) + (odd ? 1 : 0);
                         to[0] = odd ? make_float4(other[0], other[1], other[2], other[3]) : make_float4(v[u][0], v[u][1], v[u][2], v[u][3]);
                         to[2] = odd ? make_float4(v[u][4], v[u][5], v[u][6], v[u][7]) : make_float4(other[0], other[1], other[2], other[3]);
                         continue;
                     }
                 }
-                if (real[u]) serve_store<8>(p[u], a.wide, v[u]);
+                if (real[u]) serve_store<8>(p, a.wide, v[u]);
             }
         }
     }
@@ -160,11 +149,14 @@ __global__ void __launch_bounds__(kRowThreads) kv4_rows_kernel(const RowsArgs<T>
 
 template <int NB, class T>
 int rows_launch(const vb200_kv4 *h, const vb200_kv4_rows_t &a, bool read, cudaStream_t st) {
-    RowsArgs<T> r = {h->c, a.lengths, a.rows, a.max_rows, 0, (unsigned)h->c.seqs * a.max_rows, serve_rows<T>(a.k), serve_rows<T>(a.v)};
+    RowsArgs<T> r = {h->c, a.lengths, a.rows, a.max_rows, 0, serve_rows<T>(a.k), serve_rows<T>(a.v)};
     r.wide = serve_wide(r.k) && serve_wide(r.v);
-    const long long words = (long long)r.tokens * h->c.kv_heads * NB * 8, chunk = kRowThreads * kRowUnroll;
-    const unsigned grid = (unsigned)std::min((words + chunk - 1) / chunk, (long long)h->w.sm_count * 16);
-    const cudaError_t e = launch_pdl(read ? kv4_rows_kernel<NB, T, true> : kv4_rows_kernel<NB, T, false>, dim3(grid), dim3(kRowThreads), 0, st, r);
+    /* a row or two are a warp or two: CTAs of full size take 0.9 us longer to be there */
+    const int threads = (int)std::min<long long>(kRowThreads, ((long long)a.max_rows * NB * 4 + 31) / 32 * 32), kEach = threads / (NB * 4) * kRowUnroll;
+    const long long heads = 2ll * h->c.kv_heads * h->c.seqs, chunks = (a.max_rows + kEach - 1) / kEach;
+    const long long most = std::max(1ll, (long long)h->w.sm_count * 64 / heads);
+    const dim3 grid((unsigned)std::min(chunks, most), 2 * h->c.kv_heads, h->c.seqs);
+    const cudaError_t e = launch_pdl(read ? kv4_rows_kernel<NB, T, true> : kv4_rows_kernel<NB, T, false>, grid, dim3(threads), 0, st, r);
     return e == cudaSuccess ? 0 : serve_launched() | -1;
 }
 
@@ -194,15 +186,16 @@ VB_DEVINL uint32_t evict_key(float m) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int kSelThreads = 1024, kSelEach = 32, kSelChunk = kSelThreads * kSelEach, kSelBins = 2048;
+constexpr int kSelThreads = 1024, kSelBins = 2048, kSelHeld = 40960;
 
 /* Which tokens stay: a CTA per sequence and head. The need-th largest key of the middle by digits of 11, 11 and 10 bits (counts of a
  * digit among those that share the digits before it; the first holds sign, exponent and two bits, so that masses spread over it), then
- * the tokens in order. A thread keeps the keys of up to 32 tokens in registers; longer sequences are read again, 32768 tokens at a time.
- */
+ * the tokens in order: a thread has a stretch of them, an odd number so that threads' reads fall on different banks. Keys wait in shared
+ * memory; of sequences too long for that they are read again. (With a thread's 32 keys in registers, loops unrolled over them:
+ * 17 us for 1601 tokens and 44 for 32768, most of it for fetching the code.) */
 __global__ void __launch_bounds__(kSelThreads) kv4_select_kernel(const EvictArgs a) {
+    extern __shared__ uint32_t held[];
     __shared__ int count[kSelBins], warp_sum[32];
-    __shared__ uint2 place[kSelEach * 32];                /* of a warp's 32 tokens: how many stay, how many tie; then how many before them */
     __shared__ uint2 warp_place[32];
     __shared__ uint32_t prefix;
     __shared__ int want;
@@ -217,35 +210,25 @@ __global__ void __launch_bounds__(kSelThreads) kv4_select_kernel(const EvictArgs
     }
     const float *mass = a.mass + ((size_t)s * a.from.kv_heads + h) * a.from.capacity;
     const int lo = a.first, hi = n - a.recent;            /* the middle; it holds more than are needed of it */
-    uint32_t key[kSelEach];
-    auto read = [&](int c0) {
-#pragma unroll
-        for (int j = 0; j < kSelEach; j++) {
-            const int i = c0 + j * kSelThreads + tid;
-            if (i < n) key[j] = evict_key(mass[i]);
-            if (c0 + (j + 1) * kSelThreads >= n) break;
-        }
-    };
-    const bool once = n <= kSelChunk;
-    if (once) read(0);
+    const bool hold = n <= kSelHeld;
+    auto key_of = [&](int i) { return hold ? held[i] : evict_key(mass[i]); };
+    if (hold) {
+#pragma unroll 8
+        for (int i = tid; i < n; i += kSelThreads) held[i] = evict_key(mass[i]);
+    }
+    for (int x = tid; x < kSelBins; x += kSelThreads) count[x] = 0;
     if (tid == 0) { prefix = 0; want = a.keep - a.first - a.recent; }
+    __syncthreads();
     const bool none = a.keep == a.first + a.recent;
     if (!none) {
-        int shift = 21;
 #pragma unroll 1
         for (int pass = 0; pass < 3; pass++) {
-            const uint32_t mask = pass == 0 ? 0u : pass == 1 ? 0xffe00000u : 0xfffffc00u, digit = pass == 2 ? 1023u : 2047u;
-            for (int x = tid; x < kSelBins; x += kSelThreads) count[x] = 0;
-            __syncthreads();
-            const uint32_t p = prefix;
-            for (int c0 = 0; c0 < n; c0 += kSelChunk) {
-                if (!once) read(c0);
-#pragma unroll
-                for (int j = 0; j < kSelEach; j++) {
-                    const int i = c0 + j * kSelThreads + tid;
-                    if (i >= lo && i < hi && (key[j] & mask) == p) atomicAdd(&count[(key[j] >> shift) & digit], 1);
-                    if (c0 + (j + 1) * kSelThreads >= n) break;
-                }
+            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+            const uint32_t mask = pass == 0 ? 0u : pass == 1 ? 0xffe00000u : 0xfffffc00u, digit = pass == 2 ? 1023u : 2047u, p = prefix;
+#pragma unroll 4
+            for (int i = lo + tid; i < hi; i += kSelThreads) {
+                const uint32_t key = key_of(i);
+                if ((key & mask) == p) atomicAdd(&count[(key >> shift) & digit], 1);
             }
             __syncthreads();
             /* thread x has bins 2047 - 2 x and 2046 - 2 x: how many lie above them */
@@ -257,81 +240,46 @@ __global__ void __launch_bounds__(kSelThreads) kv4_select_kernel(const EvictArgs
                 if (lane >= o) above += v;
             }
             if (lane == 31) warp_sum[warp] = above;
+            count[b1] = count[b1 - 1] = 0;                /* for the next pass */
             __syncthreads();
-            if (warp == 0) {
-                int v = warp_sum[lane];
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int u = __shfl_up_sync(0xffffffffu, v, o);
-                    if (lane >= o) v += u;
-                }
-                warp_sum[lane] = v;
-            }
-            __syncthreads();
-            above += (warp ? warp_sum[warp - 1] : 0) - n1 - n0;
+            int ahead = warp_sum[lane];
+            ahead = lane < warp ? ahead : 0;
+            above += (int)__reduce_add_sync(0xffffffffu, (unsigned)ahead) - n1 - n0;
             if (above < left && left <= above + n1) { prefix = p | ((uint32_t)b1 << shift); want = left - above; }
             else if (above + n1 < left && left <= above + n1 + n0) { prefix = p | ((uint32_t)(b1 - 1) << shift); want = left - above - n1; }
             __syncthreads();
-            shift = pass == 0 ? 10 : 0;
         }
     }
-    __syncthreads();
     /* of those equal to the threshold the first `ties` stay */
     const uint32_t threshold = prefix;
-    const int ties = want;
-    uint2 base = make_uint2(0, 0);                        /* stay, tie, before this chunk */
-    for (int c0 = 0; c0 < n; c0 += kSelChunk) {
-        if (!once) read(c0);
-        uint32_t stay = 0, tie = 0;                       /* a bit a token */
+    const int ties = want, each = ((n + kSelThreads - 1) / kSelThreads) | 1, i0 = min(n, tid * each), i1 = min(n, i0 + each);
+    uint2 here = make_uint2(0, 0);                        /* of this thread's tokens: how many stay, how many tie */
+    for (int i = i0; i < i1; i++) {
+        const uint32_t key = key_of(i);
+        const bool edge = i < lo || i >= hi;
+        here.x += edge || (!none && key > threshold);
+        here.y += !edge && !none && key == threshold;
+    }
+    uint2 upto = here;
 #pragma unroll
-        for (int j = 0; j < kSelEach; j++) {
-            const int i = c0 + j * kSelThreads + tid;
-            const bool edge = i < lo || i >= hi;
-            const bool is_sure = i < n && (edge || (!none && key[j] > threshold)), is_tie = i < n && !edge && !none && key[j] == threshold;
-            const unsigned bs = __ballot_sync(0xffffffffu, is_sure), bt = __ballot_sync(0xffffffffu, is_tie);
-            stay |= (uint32_t)is_sure << j;
-            tie |= (uint32_t)is_tie << j;
-            if (lane == 0) place[j * 32 + warp] = make_uint2(__popc(bs), __popc(bt));
-        }
-        __syncthreads();
-        {
-            uint2 v = place[tid];
-            const uint2 own = v;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const unsigned x = __shfl_up_sync(0xffffffffu, v.x, o), y = __shfl_up_sync(0xffffffffu, v.y, o);
-                if (lane >= o) { v.x += x; v.y += y; }
-            }
-            if (lane == 31) warp_place[warp] = v;
-            __syncthreads();
-            if (warp == 0) {
-                uint2 t = warp_place[lane];
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const unsigned x = __shfl_up_sync(0xffffffffu, t.x, o), y = __shfl_up_sync(0xffffffffu, t.y, o);
-                    if (lane >= o) { t.x += x; t.y += y; }
-                }
-                warp_place[lane] = t;
-            }
-            __syncthreads();
-            const uint2 ahead = warp ? warp_place[warp - 1] : make_uint2(0, 0);
-            place[tid] = make_uint2(base.x + ahead.x + v.x - own.x, base.y + ahead.y + v.y - own.y);
-            base.x += warp_place[31].x;
-            base.y += warp_place[31].y;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < kSelEach; j++) {
-            if (c0 + j * kSelThreads >= n) break;
-            const bool is_sure = (stay >> j) & 1u, is_tie = (tie >> j) & 1u;
-            const unsigned bs = __ballot_sync(0xffffffffu, is_sure), bt = __ballot_sync(0xffffffffu, is_tie), below = (1u << lane) - 1u;
-            const uint2 at = place[j * 32 + warp];
-            const int tied = (int)at.y + __popc(bt & below);
-            if (is_sure || (is_tie && tied < ties)) kept[(int)at.x + __popc(bs & below) + min(tied, ties)] = c0 + j * kSelThreads + tid;
-        }
-        __syncthreads();
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned x = __shfl_up_sync(0xffffffffu, upto.x, o), y = __shfl_up_sync(0xffffffffu, upto.y, o);
+        if (lane >= o) { upto.x += x; upto.y += y; }
+    }
+    if (lane == 31) warp_place[warp] = upto;
+    __syncthreads();
+    const uint2 t = lane < warp ? warp_place[lane] : make_uint2(0, 0);
+    int stay = (int)(upto.x - here.x + __reduce_add_sync(0xffffffffu, t.x)), tied = (int)(upto.y - here.y + __reduce_add_sync(0xffffffffu, t.y));
+    for (int i = i0; i < i1; i++) {
+        const uint32_t key = key_of(i);
+        const bool edge = i < lo || i >= hi, is_tie = !edge && !none && key == threshold;
+        const bool stays = edge || (!none && key > threshold) || (is_tie && tied < ties);
+        if (stays) kept[stay + min(tied, ties)] = i;
+        stay += stays && !is_tie;
+        tied += is_tie;
     }
 }
+size_t select_smem(int capacity) { return sizeof(uint32_t) * (size_t)std::min(capacity, kSelHeld); }
 
 /* The rows that stay into their places, in pieces of 16 bytes (codes) and a byte a block (scales). In place a CTA takes all of a
  * head, since a row's new slot may be another row's old one: rows move towards the front in order, so a stretch may be written once all
@@ -386,6 +334,7 @@ int rows_load() {
                              (const void *)kv4_select_kernel, (const void *)kv4_move_kernel<false>, (const void *)kv4_move_kernel<true>};
     for (const void *k : kernels)
         if (cudaFuncGetAttributes(&f, k) != cudaSuccess) return serve_launched() | -1;
+    if (cudaFuncSetAttribute(kv4_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)select_smem(kSelHeld)) != cudaSuccess) return serve_launched() | -1;
     return 0;
 }
 int load(int blocks) {
@@ -410,7 +359,7 @@ int check_rows(const vb200_kv4 *h, const vb200_kv4_rows_t *a) {
 int rows_call(const vb200_kv4 *h, const vb200_kv4_rows_t *a, bool read, cudaStream_t st) {
     if (check_rows(h, a)) return -1;
     if (a->max_rows == 0) return 0;
-    if ((long long)a->max_rows * h->c.seqs > INT_MAX) return serve_fail("too many rows");
+    if (a->max_rows > (1 << 30)) return serve_fail("max_rows is more than 2^30");
     if (a->k.type == VB200_F32) return rows_dims<float>(h, *a, read, st);
     if (a->k.type == VB200_BF16) return rows_dims<__nv_bfloat16>(h, *a, read, st);
     return rows_dims<__half>(h, *a, read, st);
@@ -429,8 +378,8 @@ const char *vb200_serve_error(void) { return g_serve_error.c_str(); }
 vb200_kv4_t *vb200_kv4_open(int seqs, int kv_heads, int head_dim, int capacity) {
     const bool dim_ok = head_dim == 32 || head_dim == 64 || head_dim == 96 || head_dim == 128 || head_dim == 192 || head_dim == 256;
     if (!dim_ok) { serve_fail("head_dim has to be 32, 64, 96, 128, 192 or 256"); return nullptr; }
-    if (seqs < 1 || seqs > 65535 || kv_heads < 1 || kv_heads > 65535 || capacity < 1 || capacity > (1 << 30)) {
-        serve_fail("seqs and kv_heads have to be 1 to 65535, capacity 1 to 2^30");
+    if (seqs < 1 || seqs > 65535 || kv_heads < 1 || kv_heads > 16384 || capacity < 1 || capacity > (1 << 30)) {
+        serve_fail("seqs have to be 1 to 65535, kv_heads 1 to 16384, capacity 1 to 2^30");
         return nullptr;
     }
     int dev = 0, major = 0, minor = 0, n_sm = 0;
@@ -513,7 +462,7 @@ int vb200_kv4_evict(vb200_kv4_t *h, vb200_kv4_t *into, const vb200_kv4_evict_t *
     if (!serve_on_device(a->mass)) return serve_fail("mass does not lie on the current device");
     const cudaStream_t st = (cudaStream_t)stream;
     EvictArgs e = {h->c, into->c, a->lengths, a->new_lengths, a->mass, a->new_mass, a->new_mass_ld, a->kept, a->keep, a->recent, a->first, into == h};
-    cudaError_t err = launch_pdl(kv4_select_kernel, dim3(h->c.kv_heads, h->c.seqs), dim3(kSelThreads), 0, st, e);
+    cudaError_t err = launch_pdl(kv4_select_kernel, dim3(h->c.kv_heads, h->c.seqs), dim3(kSelThreads), select_smem(h->c.capacity), st, e);
     if (err != cudaSuccess) return serve_launched() | -1;
     if (into == h) {
         err = launch_pdl(kv4_move_kernel<true>, dim3(1, h->c.kv_heads, h->c.seqs), dim3(kMoveThreads), 0, st, e);
