@@ -9,6 +9,7 @@
  * collected and put in order at the end. Values are compared with their index below them, so all are different. Where more come through than
  * the list holds (rising rows), a CTA finds its largest again by bisection, from memory: slower and as right.
  */
+#include <limits.h>
 #include <type_traits>
 
 #include "vb_serve.cuh"
@@ -47,18 +48,25 @@ VB_DEVINL uint64_t lp_rank(float v, int i) { return ((uint64_t)lp_key(v) << 32) 
 struct LpSums {
     float m, l, w;
 };
-/* b into a. A side that is empty, or nothing but -inf, adds nothing. */
-VB_DEVINL LpSums lp_join(LpSums a, LpSums b) {
-    if (b.l == 0.0f) return a;
-    if (a.l == 0.0f) return b;
-    const float m = fmaxf(a.m, b.m);
-    const float da = a.m - m, db = b.m - m, fa = __expf(da), fb = __expf(db);
-    LpSums r;
-    r.m = m;
-    r.l = a.l * fa + b.l * fb;
-    /* a side that vanishes takes its difference along: 0, not 0 * -inf */
-    r.w = (fa > 0.0f ? (a.w + a.l * da) * fa : 0.0f) + (fb > 0.0f ? (b.w + b.l * db) * fb : 0.0f);
-    return r;
+/* The same sums against a larger reference. Those of nothing stay nothing; one that vanishes takes its difference along: 0, not 0 * -inf */
+VB_DEVINL void lp_rebase(LpSums &a, float m) {
+    const float d = a.m - m, f = a.m > -INFINITY ? __expf(d) : 0.0f;
+    a.w = f > 0.0f ? (a.w + a.l * d) * f : 0.0f;
+    a.l *= f;
+    a.m = m;
+}
+/* The sums of all lanes that differ in bits below N, in every lane */
+template <int N>
+VB_DEVINL void lp_join(LpSums &a) {
+    float m = a.m;
+#pragma unroll
+    for (int o = 1; o < N; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    lp_rebase(a, m);
+#pragma unroll
+    for (int o = 1; o < N; o <<= 1) {
+        a.l += __shfl_xor_sync(0xffffffffu, a.l, o);
+        a.w += __shfl_xor_sync(0xffffffffu, a.w, o);
+    }
 }
 
 /* The larger one; NaN where either is. */
@@ -103,8 +111,7 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const LpArgs a)
     constexpr int kEach = 16 / sizeof(T), kLpUnroll = kLpUnrolled<T>, kStep = kLpThreads * kLpUnroll;
     __shared__ uint64_t list[kLpList], best[kLpMaxSplit * kLpTop], group[32], threshold_s;
     __shared__ LpSums warp_sums[kLpWarps], cta_sums[kLpMaxSplit];
-    __shared__ float log_s;
-    __shared__ int n_list, bad_s[kLpMaxSplit], counts[kLpMaxSplit], ranks[kLpMaxSplit * kLpTop];
+    __shared__ int n_list, bad_s[kLpMaxSplit], counts[kLpMaxSplit];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     uint32_t split, splits;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(split));
@@ -152,10 +159,7 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const LpArgs a)
     auto raise = [&](float top) {
         if (!(top <= sums.m + 8.0f)) {
             if (top < INFINITY) {
-                const float d = sums.m - top, f = __expf(d);
-                sums.w = f > 0.0f ? (sums.w + sums.l * d) * f : 0.0f;
-                sums.l *= f;
-                sums.m = top;
+                lp_rebase(sums, top);
             } else {
                 bad = true;
             }
@@ -180,27 +184,52 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const LpArgs a)
     for (int c0 = v0; c0 < v1 || c0 == v0; c0 += kStep) {
         const bool first = c0 == v0;
         if (c0 + kStep < v1) fetch(c0 + kStep, next);
-        float top = first ? extra : -INFINITY;
+        float top = first ? extra : -INFINITY, low = INFINITY;
 #pragma unroll
         for (int u = 0; u < kLpUnroll; u++) {
             float v[kEach];
             lp_values<T>(now[u], v);
 #pragma unroll
-            for (int j = 0; j < kEach; j++) top = lp_max(top, v[j]);
+            for (int j = 0; j < kEach; j++) {
+                top = lp_max(top, v[j]);
+                low = fminf(low, v[j]);
+            }
         }
         raise(top);
         if (first) add(extra);
+        if (low > -INFINITY) {
+            /* two at a time; nothing is infinitely far below the reference */
+            const uint64_t m2 = vb_f2_pack(-sums.m, -sums.m), log2e = vb_f2_pack(1.44269504f, 1.44269504f);
+            uint64_t l2 = 0, w2 = 0;
 #pragma unroll
-        for (int u = 0; u < kLpUnroll; u++) {
-            float v[kEach];
-            lp_values<T>(now[u], v);
+            for (int u = 0; u < kLpUnroll; u++) {
+                float v[kEach];
+                lp_values<T>(now[u], v);
 #pragma unroll
-            for (int j = 0; j < kEach; j++) add(v[j]);
+                for (int j = 0; j < kEach; j += 2) {
+                    const uint64_t d = vb_f2_add(vb_f2_pack(v[j], v[j + 1]), m2);
+                    const float2 x = vb_f2_get(vb_f2_mul(d, log2e));
+                    const uint64_t e = vb_f2_pack(lp_ex2(x.x), lp_ex2(x.y));
+                    l2 = vb_f2_add(l2, e);
+                    w2 = vb_f2_fma(e, d, w2);
+                }
+            }
+            const float2 l = vb_f2_get(l2), w = vb_f2_get(w2);
+            sums.l += l.x + l.y;
+            sums.w += w.x + w.y;
+        } else {
+#pragma unroll
+            for (int u = 0; u < kLpUnroll; u++) {
+                float v[kEach];
+                lp_values<T>(now[u], v);
+#pragma unroll
+                for (int j = 0; j < kEach; j++) add(v[j]);
+            }
         }
         if (a.top) {
             if (first) {
                 /* this thread's largest, at its first place; those of 32 groups of threads; the top-th of them */
-                uint64_t most = extra_i >= 0 ? lp_rank(extra, extra_i) : 0;
+                int at = extra_i >= 0 && !(extra < top) ? extra_i : INT_MAX;      /* not below a NaN either: one that is none is put right */
 #pragma unroll
                 for (int u = 0; u < kLpUnroll; u++) {
                     const int i = c0 + u * kLpThreads + tid;
@@ -209,8 +238,10 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const LpArgs a)
                     if (i < v1)
 #pragma unroll
                         for (int j = 0; j < kEach; j++)
-                            if (!(v[j] < top)) most = max(most, lp_rank(v[j], head + i * kEach + j));
+                            if (top == top ? v[j] == top : v[j] != v[j]) at = min(at, head + i * kEach + j);
                 }
+                if (top != top && extra_i >= 0 && at == extra_i && extra == extra) at = INT_MAX;
+                uint64_t most = at < INT_MAX ? lp_rank(top, at) : 0;
 #pragma unroll
                 for (int o = 8; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
                 if ((lane & 15) == 0) group[warp * 2 + (lane >> 4)] = most;
@@ -246,21 +277,14 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const LpArgs a)
 #pragma unroll
         for (int u = 0; u < kLpUnroll; u++) now[u] = next[u];
     }
-    /* this CTA's sums */
-    auto join_warp = [&]() {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const LpSums b = {__shfl_xor_sync(0xffffffffu, sums.m, o), __shfl_xor_sync(0xffffffffu, sums.l, o), __shfl_xor_sync(0xffffffffu, sums.w, o)};
-            sums = lane & o ? lp_join(b, sums) : lp_join(sums, b);
-        }
-    };
-    join_warp();
+    /* this CTA's sums: a warp's, then theirs */
+    lp_join<32>(sums);
     if (lane == 0) warp_sums[warp] = sums;
     if (__any_sync(0xffffffffu, bad) && lane == 0) atomicOr(&bad_s[0], 1);
     __syncthreads();
     if (warp == kLpWarps - 1) {               /* the first warps have the list */
-        sums = lane < kLpWarps ? warp_sums[lane] : LpSums{-INFINITY, 0.0f, 0.0f};
-        join_warp();
+        sums = warp_sums[lane % kLpWarps];
+        lp_join<kLpWarps>(sums);
         if (lane == 0) cta_sums[0] = sums;
     }
     /* this CTA's largest values, in order */
@@ -330,44 +354,34 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const LpArgs a)
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
         if (split != 0) return;
     }
+    if (tid == 0) counts[0] = there;
+    /* the row's sums, by every warp for itself */
+    const bool in = lane < (int)splits;
+    sums = in ? cta_sums[lane] : LpSums{-INFINITY, 0.0f, 0.0f};
+    lp_join<kLpMaxSplit>(sums);
+    sums.m = __shfl_sync(0xffffffffu, sums.m, 0);
+    sums.l = __shfl_sync(0xffffffffu, sums.l, 0);
+    const bool wrong = __any_sync(0xffffffffu, in && bad_s[in ? lane : 0] != 0);
+    const float nan = __uint_as_float(0x7fffffffu), log_l = wrong ? nan : logf(sums.l);      /* -inf for a row of nothing but -inf */
     if (tid == 0) {
-        counts[0] = there;
-        int wrong = bad_s[0];
-        sums = cta_sums[0];
-        for (uint32_t c = 1; c < splits; c++) {
-            sums = lp_join(sums, cta_sums[c]);
-            wrong |= bad_s[c];
-        }
-        const float log_l = logf(sums.l);                       /* -inf for a row of nothing but -inf */
-        const float nan = __uint_as_float(0x7fffffffu);
         if (a.logprobs) a.logprobs[row] = wrong || token < 0 || token >= a.vocab ? nan : sums.l == 0.0f ? -INFINITY : (of_token - sums.m) - log_l;
         if (a.entropy) a.entropy[row] = wrong ? nan : sums.l == 0.0f ? 0.0f : log_l - sums.w / sums.l;
-        cta_sums[0] = sums;
-        log_s = wrong ? nan : log_l;
     }
     if (!a.top) return;
-    const int held = (int)splits * kLpTop;
-    for (int i = tid; i < held; i += kLpThreads) ranks[i] = i % kLpTop;
-    __syncthreads();
-    const float m = cta_sums[0].m, log_l = log_s;
-    if (splits > 1) {
-        /* a value and another CTA's list at a time */
-        for (int i = tid; i < held * (int)splits; i += kLpThreads) {
-            const int at = i / (int)splits, c = at / kLpTop, o = i - at * (int)splits;
-            if (o != c && at % kLpTop < counts[c]) {
-                const int above = lp_above(best + o * kLpTop, counts[o], best[at]);
-                if (above) atomicAdd(&ranks[at], above);
-            }
-        }
-        __syncthreads();
-    }
-    for (int i = tid; i < held; i += kLpThreads) {
-        if (i % kLpTop >= counts[i / kLpTop] || ranks[i] >= a.top) continue;
-        const uint64_t v = best[i];
+    __syncthreads();                          /* counts[0] */
+    /* a lane a value and a list (of eight, there or not): how many of the list are above the value */
+    for (int i = tid >> 3; i < ((int)splits * a.top + 3) / 4 * 4; i += kLpThreads / 8) {
+        const int c = i % (int)splits, k = i / (int)splits, o = tid & 7;
+        const bool there_is = k < a.top && k < counts[c];
+        const uint64_t v = there_is ? best[c * kLpTop + k] : 0;
+        int rank = !there_is || o >= (int)splits ? 0 : o == c ? k : lp_above(best + o * kLpTop, counts[o], v);
+#pragma unroll
+        for (int x = 1; x < 8; x <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, x);
+        if (!there_is || o != 0 || rank >= a.top) continue;
         const float value = lp_value((uint32_t)(v >> 32));
-        const size_t to = (size_t)row * a.top + ranks[i];
+        const size_t to = (size_t)row * a.top + rank;
         if (a.top_ids) a.top_ids[to] = (int)~(uint32_t)v;
-        if (a.top_logprobs) a.top_logprobs[to] = value == -INFINITY && log_l == log_l ? -INFINITY : (value - m) - log_l;
+        if (a.top_logprobs) a.top_logprobs[to] = value == -INFINITY && log_l == log_l ? -INFINITY : (value - sums.m) - log_l;
     }
 }
 
