@@ -54,6 +54,13 @@ int vb200_lm_seq_length(vb200_lm_t *lm, int seq);
  * ([n_want][vocab]); n_want may be 0. */
 int vb200_lm_step(vb200_lm_t *lm, int seq, const int *tokens, int n, const int *want, int n_want, float *logits_out);
 
+/* Like vb200_lm_step, but what comes back of the logits at the wanted places are log probabilities, worked out on the device: of
+ * targets[i] at want[i], the entropy there (natural logarithms; may be NULL), and the `top` (0 to 32) most probable tokens with theirs, the most
+ * probable first, [n_want][top] (may be NULL where top is 0). Where vb200_lm_step copies vocab floats a place to the
+ * host, this copies 2 + 2 top. */
+int vb200_lm_score(vb200_lm_t *lm, int seq, const int *tokens, int n, const int *want, int n_want, const int *targets, int top,
+                   float *logprobs, float *entropy, int *top_ids, float *top_logprobs);
+
 /* Greedy continuation: the n prompt tokens, then n_new tokens chosen on the device (largest logit, the
  * first one on a tie) without a host round trip per token. The last one is returned but not fed. */
 int vb200_lm_generate(vb200_lm_t *lm, int seq, const int *prompt, int n, int n_new, int *out);

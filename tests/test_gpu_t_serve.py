@@ -585,3 +585,38 @@ def test_logprobs_one_output_at_a_time(pkg):
         assert torch.allclose(got.double().cpu(), w, atol=1e-4)
     assert torch.equal(ids.cpu().long(), want[2])
     pkg.token_logprobs(x[:0], tokens[:0], lp[:0])          # no rows: nothing to do
+
+
+# ---------------------------------------------------------------------------------------------- scoring with a model
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_score_of_a_language_model(pkg, dtype):
+    """What score says is what step's logits say: portions of several blocks, single tokens (launched, captured, replayed), any places."""
+    import numpy as np
+    from lm_models import attention, config, delta, tokens
+    c = config([delta(), attention()])
+    with pkg.LanguageModel(config=c, dtype=dtype, seed=3, max_tokens=400, max_seqs=2, block_rows=100) as lm:
+        t = np.asarray(tokens(c, 260, 5))
+        a, b = lm.open(), lm.open()
+        cuts = [(0, 230), (230, 231), (231, 232), (232, 233), (233, 236), (236, 260)]
+        for i, j in cuts:
+            part, top = t[i:j], min(7, c["vocab"]) if i % 2 else 0
+            want = list(range(j - i)) if j - i < 200 else [0, 5, 99, 100, 163, 164, 165, 229]
+            targets = [int(t[min(i + w + 1, 259)]) for w in want]
+            x = lm.step(a, part, want=want)
+            lp, ent, ids, tops = lm.score(b, part, want=want, targets=targets, top=top)
+            w_lp, w_ent, w_ids, w_tops = plain.logprobs(torch.from_numpy(x), torch.tensor(targets), top)
+            assert np.allclose(lp, w_lp.numpy(), atol=1e-4) and np.allclose(ent, w_ent.numpy(), atol=1e-3)
+            assert np.array_equal(ids, w_ids.numpy()) and np.allclose(tops, w_tops.numpy(), atol=1e-4)
+            assert lm.length(a) == lm.length(b) == j
+        lm.release(b)
+        b = lm.open()
+        lp, _, _, _ = lm.score(b, t[:150])
+        assert lp.shape == (149,)
+        for args in (dict(want=[3, 2], targets=[0, 0]), dict(want=[0], targets=[c["vocab"]]), dict(want=[0], targets=[-1]), dict(want=[0], targets=[0], top=33)):
+            with pytest.raises(RuntimeError):
+                lm.score(b, t[:5], **args)
+        for args in (dict(want=[0]), dict(want=[0, 1], targets=[0]), dict(want=[], targets=[])):
+            with pytest.raises(ValueError):
+                lm.score(b, t[:5], **args)
+        assert lm.length(b) == 150

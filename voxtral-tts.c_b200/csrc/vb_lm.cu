@@ -12,6 +12,7 @@
  * replayed for every position and slot.
  */
 #include "../../include/voxtral_b200_lm.h"
+#include "../../include/voxtral_b200_serve.h"
 #include "vb_lm_config.h"
 #include "vb_lm_kernels.cuh"
 #include "vb_safetensors.h"
@@ -178,6 +179,10 @@ struct vb200_lm {
     int4 *route_table = nullptr;
     bool tap_on = false;
     int tap_rows = 0;
+    /* what a scoring step makes of the wanted rows' logits: results of a block of rows, and how many of the largest */
+    struct { int *targets = nullptr, *ids = nullptr; float *logprobs = nullptr, *entropy = nullptr, *tops = nullptr; int top = 0; } score;
+    bool scoring = false;
+    int score_rows(int w0, int rows, int ld);
 
     /* one host block -> device block per launch sequence: LmDyn, tokens, wanted rows */
     int *d_in = nullptr, *h_in[2] = {};
@@ -1033,6 +1038,7 @@ int vb200_lm::enqueue(int M, int n_want, float *logits_out, bool greedy) {
             LM_DO(lm_argmax_advance(dyn(), tokens(), log, kLogCap, lg, cfg.vocab, M, st));
         } else {
             tc_reduce(logits, lg.p, lg.n, lg.stride, (size_t)nw * lg.ld, nullptr, lg.ld, st);
+            if (scoring && score_rows(w0, nw, lg.ld)) return -1;
             if (logits_out)
                 LM_CUDA(cudaMemcpy2DAsync(logits_out + (size_t)w0 * cfg.vocab, sizeof(float) * cfg.vocab, logits, sizeof(float) * lg.ld,
                                           sizeof(float) * cfg.vocab, nw, cudaMemcpyDeviceToHost, st));
@@ -1059,7 +1065,10 @@ int vb200_lm::launch(int M, int n_want, float *logits_out, bool greedy) {
         if (direct_calls[far][v]++ == 0) return enqueue(M, n_want, logits_out, greedy);
         cudaGraph_t graph = nullptr;
         LM_CUDA(cudaStreamBeginCapture(st, cudaStreamCaptureModeRelaxed));
+        const bool score_now = scoring;              /* behind the graph, which does not hold it */
+        scoring = false;
         const int rc = enqueue(M, n_want, nullptr, greedy);
+        scoring = score_now;
         const cudaError_t ee = cudaStreamEndCapture(st, &graph);
         if (rc || ee != cudaSuccess || !graph) {
             if (graph) cudaGraphDestroy(graph);
@@ -1074,9 +1083,23 @@ int vb200_lm::launch(int M, int n_want, float *logits_out, bool greedy) {
         }
     }
     LM_CUDA(cudaGraphLaunch(graph_exec, st));
+    if (v == STEP_LOGITS && scoring) return score_rows(0, 1, head.N);
     if (v == STEP_LOGITS && logits_out)
         LM_CUDA(cudaMemcpyAsync(logits_out, logits, sizeof(float) * cfg.vocab, cudaMemcpyDeviceToHost, st));
     return 0;
+}
+
+/* Log probabilities of `rows` rows of logits, the wanted rows from w0 on. */
+int vb200_lm::score_rows(int w0, int rows, int ld) {
+    vb200_logprobs_t a = {};
+    a.logits = logits; a.type = VB200_F32; a.rows = rows; a.vocab = cfg.vocab; a.row_stride = ld;
+    a.tokens = score.targets + w0; a.logprobs = score.logprobs + w0; a.entropy = score.entropy + w0;
+    a.top = score.top;
+    if (score.top) {
+        a.top_ids = score.ids + (size_t)w0 * score.top;
+        a.top_logprobs = score.tops + (size_t)w0 * score.top;
+    }
+    return vb200_token_logprobs(&a, st) ? fail(vb200_serve_error()) : 0;
 }
 
 /* Position, tokens and wanted rows of the next M rows to the device. */
@@ -1218,6 +1241,60 @@ int vb200_lm_step(vb200_lm_t *lm, int seq, const int *tokens, int n, const int *
         for (; w < n_want && want[w] < r0 + M; w++) local.push_back(want[w] - r0);
         if (lm->feed(seq, tokens + r0, M, local.data(), (int)local.size())) return -1;
         if (lm->launch(M, (int)local.size(), logits_out + (size_t)w0 * lm->cfg.vocab, false)) return -1;
+        lm->seqs[seq].length += M;
+    }
+    return lm->finish();
+}
+
+int vb200_lm_score(vb200_lm_t *lm, int seq, const int *tokens, int n, const int *want, int n_want, const int *targets, int top,
+                   float *logprobs, float *entropy, int *top_ids, float *top_logprobs) {
+    g_error.clear();
+    if (check_step(lm, seq, tokens, n)) return -1;
+    if (n_want < 1 || !want || !targets || !logprobs) return fail("scoring needs wanted places, their tokens and room for the log probabilities");
+    if (top < 0 || top > 32 || top > lm->cfg.vocab) return fail("top has to be 0 to 32 and at most the vocabulary");
+    if (top && (!top_ids || !top_logprobs)) return fail("top without buffers for it");
+    for (int i = 0; i < n_want; i++) {
+        if (want[i] < 0 || want[i] >= n || (i && want[i] <= want[i - 1])) return fail("wanted places have to ascend inside the portion");
+        if (targets[i] < 0 || targets[i] >= lm->cfg.vocab) return fail("token " + std::to_string(targets[i]) + " is outside the vocabulary");
+    }
+    if (lm->tap_on) return fail("scoring runs without the residual-stream tap");
+    auto &sc = lm->score;
+    if (!sc.targets) {
+        const size_t rows = lm->block;
+        void *p = nullptr;
+        if (cudaMalloc(&p, rows * (3 * 4 + 32 * 8)) != cudaSuccess) {
+            cudaGetLastError();
+            return fail("out of device memory for scores");
+        }
+        lm->allocs.push_back(p);
+        sc.ids = (int *)p;
+        sc.tops = (float *)(sc.ids + 32 * rows);
+        sc.logprobs = sc.tops + 32 * rows;
+        sc.entropy = sc.logprobs + rows;
+        sc.targets = (int *)(sc.entropy + rows);
+    }
+    sc.top = top;
+    int w = 0;
+    std::vector<int> local;
+    for (int r0 = 0; r0 < n; r0 += lm->block) {
+        const int M = std::min(lm->block, n - r0), w0 = w;
+        local.clear();
+        for (; w < n_want && want[w] < r0 + M; w++) local.push_back(want[w] - r0);
+        const size_t k = local.size();
+        if (lm->feed(seq, tokens + r0, M, local.data(), (int)k)) return -1;
+        if (k) LM_CUDA(cudaMemcpyAsync(sc.targets, targets + w0, sizeof(int) * k, cudaMemcpyHostToDevice, lm->st));
+        lm->scoring = k > 0;
+        const int rc = lm->launch(M, (int)k, nullptr, false);
+        lm->scoring = false;
+        if (rc) return -1;
+        if (k) {
+            LM_CUDA(cudaMemcpyAsync(logprobs + w0, sc.logprobs, sizeof(float) * k, cudaMemcpyDeviceToHost, lm->st));
+            if (entropy) LM_CUDA(cudaMemcpyAsync(entropy + w0, sc.entropy, sizeof(float) * k, cudaMemcpyDeviceToHost, lm->st));
+            if (top) {
+                LM_CUDA(cudaMemcpyAsync(top_ids + (size_t)w0 * top, sc.ids, sizeof(int) * k * top, cudaMemcpyDeviceToHost, lm->st));
+                LM_CUDA(cudaMemcpyAsync(top_logprobs + (size_t)w0 * top, sc.tops, sizeof(float) * k * top, cudaMemcpyDeviceToHost, lm->st));
+            }
+        }
         lm->seqs[seq].length += M;
     }
     return lm->finish();

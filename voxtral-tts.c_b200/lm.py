@@ -3,6 +3,7 @@
     lm = LanguageModel("model_folder")            # config.json + model.safetensors
     seq = lm.open()
     logits = lm.step(seq, tokens, want=[-1])
+    logprobs, entropy, ids, tops = lm.score(seq, tokens, top=5)
     tokens = lm.generate(seq, prompt, 64)
 
 The design is picked by config.json's "architecture". The symbols live in libvoxtral_b200.so and, for
@@ -53,6 +54,7 @@ def lm_lib(path=None):
             ("vb200_lm_seq_close", C.c_int, [vp, C.c_int]),
             ("vb200_lm_seq_length", C.c_int, [vp, C.c_int]),
             ("vb200_lm_step", C.c_int, [vp, C.c_int, vp, C.c_int, vp, C.c_int, vp]),
+            ("vb200_lm_score", C.c_int, [vp, C.c_int, vp, C.c_int, vp, C.c_int, vp, C.c_int, vp, vp, vp, vp]),
             ("vb200_lm_generate", C.c_int, [vp, C.c_int, vp, C.c_int, C.c_int, vp]),
             ("vb200_lm_last_ms", C.c_int, [vp, fp, fp]),
             ("vb200_lm_tap_enable", C.c_int, [vp, C.c_int]),
@@ -116,6 +118,21 @@ class LanguageModel:
         out = np.empty((w.size, self.info.vocab), dtype=np.float32)
         self._ok(self.L.vb200_lm_step(self.h, seq, _ptr(t), t.size, _ptr(w) if w.size else None, w.size, _ptr(out) if w.size else None))
         return out
+
+    def score(self, seq, tokens, want=None, targets=None, top=0):
+        """Feeds the next tokens like step; returns (logprobs [len(want)], entropy [len(want)], top_ids, top_logprobs [len(want), top]) of the
+        targets at the wanted places. Without want and targets: of every token of the portion but the first, each after those before it."""
+        t = _ints(tokens)
+        if (want is None) != (targets is None):
+            raise ValueError("want and targets go together")
+        w, g = (np.arange(t.size - 1, dtype=np.int32), t[1:].copy()) if want is None else (_ints([x + t.size if x < 0 else x for x in want]), _ints(targets))
+        if w.size != g.size or w.size < 1:
+            raise ValueError("as many targets as wanted places, and one at least")
+        lp, ent = np.empty(w.size, dtype=np.float32), np.empty(w.size, dtype=np.float32)
+        ids, tops = np.empty((w.size, top), dtype=np.int32), np.empty((w.size, top), dtype=np.float32)
+        self._ok(self.L.vb200_lm_score(self.h, seq, _ptr(t), t.size, _ptr(w), w.size, _ptr(g), top, _ptr(lp), _ptr(ent), _ptr(ids) if top else None,
+                                       _ptr(tops) if top else None))
+        return lp, ent, ids, tops
 
     def generate(self, seq, prompt, n_new):
         """Greedy continuation of a sequence by n_new tokens, the choice made on the device."""
