@@ -401,10 +401,10 @@ vb200_kv4_t *vb200_kv4_open(int seqs, int kv_heads, int head_dim, int capacity) 
     Kv4 &c = h->c;
     c.seqs = seqs; c.kv_heads = kv_heads; c.blocks = head_dim / 32; c.capacity = capacity;
     c.slots = (capacity + kKv4Tile - 1) / kKv4Tile * kKv4Tile;
-    /* partial results of as many CTAs as run at once, 16 rows each */
+    /* partial results of as many CTAs as run at once: two an SM of eight rows, or one of 128 */
     h->w.sm_count = n_sm;
-    h->w.n_tickets = 4 * n_sm;
-    h->w.part_floats = (size_t)4 * n_sm * 16 * (head_dim + 2);
+    h->w.n_tickets = 2 * n_sm;
+    h->w.part_floats = std::max((size_t)2 * n_sm * 8 * (head_dim + 2), kv4_prompt_floats(head_dim / 32, n_sm));
     const size_t rows = (size_t)seqs * kv_heads * c.slots, codes = rows * (size_t)(head_dim / 2), scales = rows * (size_t)c.blocks;
     const size_t work = h->w.part_floats * sizeof(float), tickets = sizeof(unsigned) * (size_t)(h->w.n_tickets + 1);
     h->bytes = 2 * codes + 2 * scales + work + tickets;

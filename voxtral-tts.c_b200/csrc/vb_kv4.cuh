@@ -4,6 +4,7 @@
 #ifndef VB_KV4_CUH
 #define VB_KV4_CUH
 
+#include <limits.h>
 #include <type_traits>
 
 #include "vb_serve.cuh"
@@ -105,10 +106,80 @@ VB_DEVINL void get_words(const uint8_t *p, uint32_t (&w)[N]) {
         for (int i = 0; i < N; i++) w[i] = reinterpret_cast<const uint32_t *>(p)[i];
     }
 }
+/* Which (sequence, unit, split) a CTA has. A unit is PAIRS (row, query head) pairs of a KV head, a share a number of tiles of TOKENS. Where
+ * there are fewer units than CTAs that run at once (a.split), sequences are cut so that all CTAs have about the same number of tiles, by
+ * their actual lengths: the smallest share, in whole rounds and `least` at least, with which there are enough CTAs. (With as many
+ * splits for each sequence, four of 65536 to 131072 tokens took the time of four of 131072.) Otherwise every unit has a CTA. */
+struct Kv4Place {
+    int seq, unit, split, share;
+};
+template <int PAIRS, int TOKENS>
+VB_DEVINL Kv4Place kv4_place(const Kv4Attn &a, int round, int least, int most_splits) {
+    if (!a.split) {
+        const int units = a.row_tiles * a.c.kv_heads;
+        return {(int)blockIdx.x / units, (int)blockIdx.x % units, 0, INT_MAX};
+    }
+    const int lane = threadIdx.x & 31, n_cta = gridDim.x;
+    auto tiles_of = [&](int s, int *units) {
+        const Kv4Span span = kv4_span(a.lengths, a.rows, a.max_rows, s, a.c.capacity);
+        *units = (span.rows * a.group + PAIRS - 1) / PAIRS * a.c.kv_heads;
+        return (span.length + TOKENS - 1) / TOKENS;
+    };
+    /* the first 32 sequences stay in registers; there are at most a few hundred, or every unit has a CTA of its own */
+    int units0 = 0;
+    const int tiles0 = lane < a.c.seqs ? tiles_of(lane, &units0) : 0;
+    auto total = [&](auto &&f) {
+        long long n = units0 ? (long long)f(tiles0) * units0 : 0;
+        for (int s = lane + 32; s < a.c.seqs; s += 32) {
+            int units;
+            const int tiles = tiles_of(s, &units);
+            n += (long long)f(tiles) * units;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+        return n;
+    };
+    int most = tiles0;
+    for (int s = lane + 32; s < a.c.seqs; s += 32) {
+        int units;
+        most = max(most, tiles_of(s, &units));
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+    const long long all = total([](int tiles) { return max(tiles, 1); });
+    int share = (int)max((all + n_cta - 1) / n_cta, (long long)(most + most_splits - 1) / most_splits);
+    share = max(least, (share + round - 1) / round * round);
+    /* a unit's last part may be short: a little more, in steps of a sixteenth, until the CTAs are enough */
+    while (share < most && total([&](int tiles) { return max(1, (tiles + share - 1) / share); }) > n_cta) share += max(round, share / 16 / round * round);
+    /* this CTA's place: sequence by sequence, all units' first parts, then their second ones */
+    int left = blockIdx.x;
+    for (int s0 = 0; s0 < a.c.seqs; s0 += 32) {
+        int units = units0, tiles = tiles0;
+        if (s0 > 0) tiles = s0 + lane < a.c.seqs ? tiles_of(s0 + lane, &units) : 0;
+        if (s0 + lane >= a.c.seqs) units = 0;
+        const int mine = units * max(1, (tiles + share - 1) / share);
+        int upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        const unsigned there = __ballot_sync(0xffffffffu, left < upto);
+        if (there) {
+            const int who = __ffs(there) - 1;
+            const int at = left - (__shfl_sync(0xffffffffu, upto, who) - __shfl_sync(0xffffffffu, mine, who)), n = __shfl_sync(0xffffffffu, units, who);
+            return {s0 + who, at % n, at / n, share};
+        }
+        left -= __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return {a.c.seqs, 0, 0, share};
+}
+
 /* Many rows, heads up to 128 (vb_kv4_prompt.cu) */
 template <class T>
-int kv4_prompt(const Kv4Attn &a, const ServeRows<T> &q, const ServeRows<T> &out, cudaStream_t st);
+int kv4_prompt(const Kv4Attn &a, const ServeRows<T> &q, const ServeRows<T> &out, int sm_count, cudaStream_t st);
 int kv4_prompt_load(int blocks);
+/* floats of partial results that it needs */
+size_t kv4_prompt_floats(int blocks, int sm_count);
 
 } // namespace vb
 

@@ -29,7 +29,6 @@ namespace {
 
 constexpr int kAWarps = 8, kAThreads = 32 * kAWarps, kACols = 8, kAKeys = 32;
 constexpr int kAStatus = 61;
-constexpr int kAMostPairs = 64;               /* of a KV head: more take the kernel of vb_kv4_prompt.cu, heads up to 128 */
 constexpr int kAMaxSplits = 64;               /* a CTA joins them */
 
 template <int NB>
@@ -137,70 +136,6 @@ VB_DEVINL void block_scores(float (&s)[4], const uint32_t wa, const uint32_t wb,
     }
 }
 
-/* Which (sequence, unit, split) a CTA has. A unit is eight pairs of a KV head. Where there are fewer units than CTAs that run at once,
- * sequences are cut so that all CTAs have about the same number of tiles, by their actual lengths: the smallest share, in whole
- * rounds of a CTA's warps, with which there are enough CTAs. (With as many splits for each sequence, four of 65536 to 131072 tokens took
- * the time of four of 131072.) A share is two rounds at least: what joining the parts of two CTAs takes, another round takes too. */
-struct APlace {
-    int seq, unit, split, share;
-};
-VB_DEVINL APlace attn_place(const Kv4Attn &a) {
-    const int lane = threadIdx.x & 31, n_cta = gridDim.x;
-    auto tiles_of = [&](int s, int *units) {
-        const Kv4Span span = kv4_span(a.lengths, a.rows, a.max_rows, s, a.c.capacity);
-        *units = (span.rows * a.group + kACols - 1) / kACols * a.c.kv_heads;
-        return (span.length + kAKeys - 1) / kAKeys;
-    };
-    /* the first 32 sequences stay in registers; there are at most a few hundred, or every unit has a CTA of its own */
-    int units0 = 0;
-    const int tiles0 = lane < a.c.seqs ? tiles_of(lane, &units0) : 0;
-    auto total = [&](auto &&f) {
-        long long n = units0 ? (long long)f(tiles0) * units0 : 0;
-        for (int s = lane + 32; s < a.c.seqs; s += 32) {
-            int units;
-            const int tiles = tiles_of(s, &units);
-            n += (long long)f(tiles) * units;
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-        return n;
-    };
-    int most = tiles0;
-    for (int s = lane + 32; s < a.c.seqs; s += 32) {
-        int units;
-        most = max(most, tiles_of(s, &units));
-    }
-    most = __reduce_max_sync(0xffffffffu, most);
-    const long long all = total([](int tiles) { return max(tiles, 1); });
-    int share = (int)max((all + n_cta - 1) / n_cta, (long long)(most + kAMaxSplits - 1) / kAMaxSplits);
-    share = max(2 * kAWarps, (share + kAWarps - 1) / kAWarps * kAWarps);
-    /* a unit's last part may be short: a little more, in steps of a sixteenth, until the CTAs are enough */
-    while (share < most && total([&](int tiles) { return max(1, (tiles + share - 1) / share); }) > n_cta)
-        share += max(kAWarps, share / 16 / kAWarps * kAWarps);
-    /* this CTA's place: sequence by sequence, all units' first parts, then their second ones */
-    int left = blockIdx.x;
-    for (int s0 = 0; s0 < a.c.seqs; s0 += 32) {
-        int units = units0, tiles = tiles0;
-        if (s0 > 0) tiles = s0 + lane < a.c.seqs ? tiles_of(s0 + lane, &units) : 0;
-        if (s0 + lane >= a.c.seqs) units = 0;
-        const int mine = units * max(1, (tiles + share - 1) / share);
-        int upto = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += v;
-        }
-        const unsigned there = __ballot_sync(0xffffffffu, left < upto);
-        if (there) {
-            const int who = __ffs(there) - 1;
-            const int at = left - (__shfl_sync(0xffffffffu, upto, who) - __shfl_sync(0xffffffffu, mine, who)), n = __shfl_sync(0xffffffffu, units, who);
-            return {s0 + who, at % n, at / n, share};
-        }
-        left -= __shfl_sync(0xffffffffu, upto, 31);
-    }
-    return {a.c.seqs, 0, 0, share};
-}
-
 /* grid = CTAs that run at once, or (a.split == 0) sequences x units */
 template <int NB, int PT, class T>
 __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(const Kv4Attn a, const ServeRows<T> q, const ServeRows<T> out) {
@@ -215,7 +150,7 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(co
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     pdl_wait();
     pdl_launch_dependents();       /* after the wait: the masses' kernel reads what this one has waited for */
-    const APlace place = a.split ? attn_place(a) : APlace{(int)blockIdx.x / (a.row_tiles * a.c.kv_heads), (int)blockIdx.x % (a.row_tiles * a.c.kv_heads), 0, INT_MAX};
+    const Kv4Place place = kv4_place<kACols, kAKeys>(a, kAWarps, 2 * kAWarps, kAMaxSplits);
     if (place.seq >= a.c.seqs) return;
     const int seq = place.seq, kv_head = place.unit % a.c.kv_heads, tile_r = place.unit / a.c.kv_heads, split = place.split, share = place.share;
     const Kv4Span span = kv4_span(a.lengths, a.rows, a.max_rows, seq, a.c.capacity);
@@ -772,8 +707,14 @@ int attn_launch(const Kv4Attn &args, const vb200_kv4_attention_t &v, const Kv4Wo
     const ServeRows<T> q = serve_rows<T>(v.q), out = serve_rows<T>(v.out);
     a.wide = serve_wide(q);
     a.wide_out = serve_wide(out);
-    if (NB <= 4 && (long long)a.max_rows * a.group > kAMostPairs) {
-        if (kv4_prompt(a, q, out, st)) return -1;
+    /* Eight pairs against n tokens cost 32 ps n here and 128 pairs 181 ps n on the tensor cores' kernel, which takes 17 us more to begin
+     * and to join (fp32, heads of 128; the other types and sizes cross at about the same place). Measured, here and there in us: 8 heads, 1024
+     * tokens, 128 and 512 pairs each 15, 30 and 29, 38; 8192 tokens, 64 and 128 pairs 30, 34 and 50, 40; 65536 tokens, 32 and 64 pairs 83, 100 and
+     * 168, 102; 64 heads, 1024 tokens, 64 and 128 pairs 30, 37 and 51, 47. The tokens are the cache's room for them: lengths are not
+     * known here. */
+    const long long pairs = (long long)a.max_rows * a.group, room = (long long)a.c.capacity * a.c.kv_heads * a.c.seqs;
+    if (NB <= 4 && (double)room * (double)((pairs + 7) / 8 - 6 * ((pairs + 127) / 128)) > 550e3) {
+        if (kv4_prompt(a, q, out, work.sm_count, st)) return -1;
     } else if (a.max_rows > 0) {
         const long long row_tiles = ((long long)a.max_rows * a.group + kACols - 1) / kACols;
         const long long units = row_tiles * a.c.kv_heads * a.c.seqs, at_once = (long long)work.sm_count * (NB <= 4 ? 2 : 1);

@@ -24,6 +24,7 @@ namespace vb {
 namespace {
 
 constexpr int kPRows = 128, kPKeys = 128, kPThreads = 512, kPMmaWarp = 15, kPBlock = kPKeys * 128, kPStatus = 62, kPRing = 8;
+constexpr int kPLeast = 2;                    /* tiles of a part at least */
 constexpr uint32_t kPTmem = 512, kPO = 256;
 /* registers a thread at the launch, of a softmax thread and of any other: what some are given the others have given up */
 constexpr int kPRegs = 128, kPSoftRegs = 184, kPLoadRegs = 72;
@@ -36,6 +37,7 @@ struct PCfg {
     static constexpr int kSlots = kD64 * QT >= 4 ? 2 : 3;
     static constexpr int kQ = QT * kSlot;
     static constexpr int kSmem = kQ + 2 * kSlots * kSlot + 1024;
+    static constexpr int kPart = kPRows * (NB * 32 + 2);                       /* floats of a part: results, references and sums */
     static constexpr int kLd = NB * 32 + 4;                                    /* results on their way out: a row */
     static_assert(kPRows * kLd * 4 + 2 * kPRows * 16 <= 2 * kSlots * kSlot, "results do not fit the rings");
     static_assert(kSmem <= 232448 - 2048, "over what a CTA may use");
@@ -103,15 +105,21 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
     int *abort_flag = &abort_s;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int kv_head = blockIdx.y, seq = blockIdx.z;
     pdl_wait();
+    const Kv4Place place = kv4_place<kPRows, kPKeys>(a, 1, kPLeast, kPRows);
+    if (place.seq >= a.c.seqs) return;
+    const int seq = place.seq, kv_head = place.unit % a.c.kv_heads;
     const Kv4Span span = kv4_span(a.lengths, a.rows, a.max_rows, seq, a.c.capacity);
     const int pairs = span.rows * a.group;
-    const int pair0 = ((int)gridDim.x - 1 - (int)blockIdx.x) * kPRows;             /* the latest rows see the most tokens: they go first */
-    if (pair0 >= pairs) return;
+    const int row_tiles = (pairs + kPRows - 1) / kPRows, tile_r = row_tiles - 1 - place.unit / a.c.kv_heads;      /* the latest rows see the most tokens: they go first */
+    if (tile_r < 0) return;
+    const int pair0 = tile_r * kPRows;
     const int n_pairs = min(kPRows, pairs - pair0), before = span.length - span.rows;
     const int all_see = before + pair0 / a.group + 1, seen = max(0, before + (pair0 + n_pairs - 1) / a.group + 1);
-    const int n_tiles = (seen + kPKeys - 1) / kPKeys;
+    /* this CTA's tiles of tokens: all, or a part */
+    const int tiles = (seen + kPKeys - 1) / kPKeys, used = tiles <= place.share ? 1 : (tiles + place.share - 1) / place.share;
+    if (place.split >= used) return;
+    const int first_tile = used == 1 ? 0 : place.split * place.share, n_tiles = used == 1 ? tiles : min(tiles, first_tile + place.share) - first_tile;
     if (tid == 0) {
         for (int i = 0; i < Cfg::kSlots; i++) {
             vb_mbar_init(&k_full[i], 4);
@@ -217,7 +225,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
         float ref = -INFINITY, sum = 0.0f;
         int top_scale = 0, it = 0;
         for (int t = w; t < n_tiles; t += 2, it++) {
-            const int j0 = t * kPKeys;
+            const int j0 = (first_tile + t) * kPKeys;
             if (!at_warp_wait(&s_full[w], (uint32_t)it & 1u, abort_flag)) { give_up(); break; }
             tc_fence_after();
             const float *ups = key_up[t % kPRing];
@@ -311,8 +319,11 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
         const float4 A = ends[r], B = ends[kPRows + r];
         const float reference = fmaxf(A.x, B.x);
         float fa = A.x > -INFINITY ? exp2_fast(A.x - reference) : 0.0f, fb = B.x > -INFINITY ? exp2_fast(B.x - reference) : 0.0f;
-        const float total = A.y * fa + B.y * fb, inv = total == 0.0f ? 0.0f : 1.0f / total;
-        if (w == 0 && valid && a.lse)
+        const float total = A.y * fa + B.y * fb, inv = used > 1 ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
+        float *part = a.part + (size_t)blockIdx.x * PCfg<NB, QT>::kPart;
+        if (used > 1) {
+            if (w == 0) reinterpret_cast<float2 *>(part + kPRows * kDim)[r] = make_float2(reference, total);
+        } else if (w == 0 && valid && a.lse)
             a.lse[((size_t)seq * a.max_rows + row) * a.heads + head] = total == 0.0f ? -INFINITY : (reference + 8.0f + log2f(total)) * 0.69314718f;
         fa *= inv;
         fb *= inv;
@@ -330,7 +341,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
                 float v = 0.0f;
                 if (n_tiles > 0) v = __uint_as_float(oa[k]) * a0 * fa * a1;
                 if (n_tiles > 1) v += __uint_as_float(ob[k]) * b0 * fb * b1;
-                if (total == 0.0f) v = 0.0f;
+                if (total == 0.0f) v = 0.0f;               /* nothing seen */
                 oa[k] = nan ? 0x7fffffffu : __float_as_uint(v);
             }
 #pragma unroll
@@ -342,6 +353,11 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
         for (int x = tid; x < n_pairs * kEights; x += 256) {
             const int p = x / kEights, d = (x - p * kEights) * 8, rr = (pair0 + p) / a.group, hh = kv_head * a.group + pair0 + p - rr * a.group;
             const float4 lo = *reinterpret_cast<const float4 *>(rows + p * Cfg::kLd + d), hi = *reinterpret_cast<const float4 *>(rows + p * Cfg::kLd + d + 4);
+            if (used > 1) {
+                reinterpret_cast<float4 *>(part + p * kDim + d)[0] = lo;
+                reinterpret_cast<float4 *>(part + p * kDim + d)[1] = hi;
+                continue;
+            }
             const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
             serve_store<8>(out.data + seq * out.seq + rr * out.row + hh * out.head + d, a.wide_out, v);
         }
@@ -351,7 +367,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
         const size_t row0 = a.c.row(seq, kv_head, 0);
         uint32_t words[4][NB], bytes[4][NB];
         auto fetch = [&](int t) {
-            const int j0 = t * kPKeys, end = a.c.slots - 1 - j0;             /* slots are whole tiles of 64: half of the last 128 may be none */
+            const int j0 = (first_tile + t) * kPKeys, end = a.c.slots - 1 - j0;             /* slots are whole tiles of 64: half of the last 128 may be none */
             const unsigned char *codes = a.c.k + (row0 + j0) * (NB * 16), *scales = a.c.ks + (row0 + j0) * NB;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -362,7 +378,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
         };
         if (n_tiles > 0) fetch(0);
         for (int t = 0; t < n_tiles; t++) {
-            const int slot = t % Cfg::kSlots, j0 = t * kPKeys + lw * 32;
+            const int slot = t % Cfg::kSlots, j0 = (first_tile + t) * kPKeys + lw * 32;
             int most = 0;
 #pragma unroll
             for (int i = 0; i < 4; i++)
@@ -396,7 +412,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
         const size_t row0 = a.c.row(seq, kv_head, 0);
         uint32_t words[NB][4], byte[NB], all[NB];
         auto fetch = [&](int task) {
-            const int j0 = task / 4 * kPKeys, end = a.c.slots - 1 - j0;          /* slots are whole tiles of 64: half of the last 128 may be none */
+            const int j0 = (first_tile + task / 4) * kPKeys, end = a.c.slots - 1 - j0;          /* slots are whole tiles of 64: half of the last 128 may be none */
             const unsigned char *codes = a.c.v + (row0 + j0) * (NB * 16), *scales = a.c.vs + (row0 + j0) * NB;
 #pragma unroll
             for (int i = 0; i < NB; i++) {
@@ -419,7 +435,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
         const int tasks = n_tiles * 4;
         if (warp - 12 < tasks) fetch(warp - 12);
         for (int task = warp - 12; task < tasks; task += 3) {
-            const int t = task / 4, lw = task % 4, slot = t % Cfg::kSlots, j0 = t * kPKeys;
+            const int t = task / 4, lw = task % 4, slot = t % Cfg::kSlots, j0 = (first_tile + t) * kPKeys;
             const int real = seen - j0;                            /* tokens of the tile that are seen */
             int most = 0;
             bool bad = false;
@@ -507,17 +523,77 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
     }
 }
 
+/* The parts of cut sequences together: a CTA takes a share of the rows of the unit that the CTA of its number had a part of, a warp a row. */
+constexpr int kJThreads = 256;
 template <int NB, class T>
-int prompt_launch(const Kv4Attn &a, const ServeRows<T> &q, const ServeRows<T> &out, cudaStream_t st) {
-    const int tiles = (int)(((long long)a.max_rows * a.group + kPRows - 1) / kPRows);
+__global__ void __launch_bounds__(kJThreads) kv4_join_kernel(const Kv4Attn a, const ServeRows<T> out) {
+    constexpr int kDim = NB * 32, kPart = kPRows * (kDim + 2);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_wait();
+    const Kv4Place place = kv4_place<kPRows, kPKeys>(a, 1, kPLeast, kPRows);
+    if (place.seq >= a.c.seqs) return;
+    const int seq = place.seq, kv_head = place.unit % a.c.kv_heads;
+    const Kv4Span span = kv4_span(a.lengths, a.rows, a.max_rows, seq, a.c.capacity);
+    const int pairs = span.rows * a.group, row_tiles = (pairs + kPRows - 1) / kPRows, tile_r = row_tiles - 1 - place.unit / a.c.kv_heads;
+    if (tile_r < 0) return;
+    const int pair0 = tile_r * kPRows, n_pairs = min(kPRows, pairs - pair0), before = span.length - span.rows;
+    const int seen = max(0, before + (pair0 + n_pairs - 1) / a.group + 1), tiles = (seen + kPKeys - 1) / kPKeys;
+    const int used = tiles <= place.share ? 1 : (tiles + place.share - 1) / place.share;
+    if (used == 1 || place.split >= used) return;
+    const int units = row_tiles * a.c.kv_heads;
+    const float *parts = a.part + (size_t)((int)blockIdx.x - place.split * units) * kPart;
+    const size_t step = (size_t)units * kPart;
+    for (int p = place.split + warp * used; p < n_pairs; p += kJThreads / 32 * used) {
+        auto end = [&](int x) { return __ldcg(reinterpret_cast<const float2 *>(parts + x * step + kPRows * kDim) + p); };
+        float reference = -INFINITY, total = 0.0f;
+        for (int x = lane; x < used; x += 32) reference = fmaxf(reference, end(x).x);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) reference = fmaxf(reference, __shfl_xor_sync(0xffffffffu, reference, o));
+        float v[NB];
+#pragma unroll
+        for (int i = 0; i < NB; i++) v[i] = 0.0f;
+        for (int x0 = 0; x0 < used; x0 += 32) {
+            const float2 e = x0 + lane < used ? end(x0 + lane) : make_float2(-INFINITY, 0.0f);
+            const float mine = e.x > -INFINITY ? exp2_fast(e.x - reference) : 0.0f;
+            float sum = e.y * mine;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            total += sum;
+            const int n = min(32, used - x0);
+#pragma unroll 4
+            for (int x = 0; x < n; x++) {
+                const float f = __shfl_sync(0xffffffffu, mine, x);
+                const float *row = parts + (x0 + x) * step + p * kDim + lane * NB;
+#pragma unroll
+                for (int i = 0; i < NB; i++) v[i] = fmaf(__ldcg(row + i), f, v[i]);
+            }
+        }
+        const int pair = pair0 + p, row = pair / a.group, head = kv_head * a.group + pair - row * a.group;
+        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+        T *to = out.data + seq * out.seq + row * out.row + head * out.head + lane * NB;
+#pragma unroll
+        for (int i = 0; i < NB; i++) serve_put(to + i, total == 0.0f ? 0.0f : v[i] * inv);
+        if (lane == 0 && a.lse) a.lse[((size_t)seq * a.max_rows + row) * a.heads + head] = total == 0.0f ? -INFINITY : (reference + 8.0f + log2f(total)) * 0.69314718f;
+    }
+}
+
+template <int NB, class T>
+int prompt_launch(Kv4Attn a, const ServeRows<T> &q, const ServeRows<T> &out, int sm_count, cudaStream_t st) {
+    const long long row_tiles = ((long long)a.max_rows * a.group + kPRows - 1) / kPRows, units = row_tiles * a.c.kv_heads * a.c.seqs;
+    if (units > INT_MAX) return serve_fail("too many rows");
+    a.row_tiles = (int)row_tiles;
+    a.split = units < sm_count && a.c.capacity > kPLeast * kPKeys;
+    const dim3 grid((unsigned)(a.split ? sm_count : units));
     const size_t smem = PCfg<NB, sizeof(T) == 4 ? 2 : 1>::kSmem;
-    return launch_pdl(kv4_prompt_kernel<NB, kWeightTerms<T>, T>, dim3(tiles, a.c.kv_heads, a.c.seqs), dim3(kPThreads), smem, st, a, q, out) == cudaSuccess ? 0 : serve_launched() | -1;
+    if (launch_pdl(kv4_prompt_kernel<NB, kWeightTerms<T>, T>, grid, dim3(kPThreads), smem, st, a, q, out) != cudaSuccess) return serve_launched() | -1;
+    if (a.split && launch_pdl(kv4_join_kernel<NB, T>, grid, dim3(kJThreads), 0, st, a, out) != cudaSuccess) return serve_launched() | -1;
+    return 0;
 }
 template <int NB, class T>
 bool prompt_load() {
     /* a block launched with fewer registers than its warps ask for would wait for them for good */
     cudaFuncAttributes f;
-    if (cudaFuncGetAttributes(&f, kv4_prompt_kernel<NB, kWeightTerms<T>, T>) != cudaSuccess) return false;
+    if (cudaFuncGetAttributes(&f, kv4_join_kernel<NB, T>) != cudaSuccess || cudaFuncGetAttributes(&f, kv4_prompt_kernel<NB, kWeightTerms<T>, T>) != cudaSuccess) return false;
     if (f.numRegs < kPRegs) {
         serve_fail("the prompt kernel was built with fewer registers than it divides");
         return false;
@@ -528,17 +604,19 @@ bool prompt_load() {
 } // namespace
 
 template <class T>
-int kv4_prompt(const Kv4Attn &a, const ServeRows<T> &q, const ServeRows<T> &out, cudaStream_t st) {
+int kv4_prompt(const Kv4Attn &a, const ServeRows<T> &q, const ServeRows<T> &out, int sm_count, cudaStream_t st) {
     switch (a.c.blocks) {
-    case 1: return prompt_launch<1, T>(a, q, out, st);
-    case 2: return prompt_launch<2, T>(a, q, out, st);
-    case 3: return prompt_launch<3, T>(a, q, out, st);
-    default: return prompt_launch<4, T>(a, q, out, st);
+    case 1: return prompt_launch<1, T>(a, q, out, sm_count, st);
+    case 2: return prompt_launch<2, T>(a, q, out, sm_count, st);
+    case 3: return prompt_launch<3, T>(a, q, out, sm_count, st);
+    default: return prompt_launch<4, T>(a, q, out, sm_count, st);
     }
 }
-template int kv4_prompt<float>(const Kv4Attn &, const ServeRows<float> &, const ServeRows<float> &, cudaStream_t);
-template int kv4_prompt<__nv_bfloat16>(const Kv4Attn &, const ServeRows<__nv_bfloat16> &, const ServeRows<__nv_bfloat16> &, cudaStream_t);
-template int kv4_prompt<__half>(const Kv4Attn &, const ServeRows<__half> &, const ServeRows<__half> &, cudaStream_t);
+template int kv4_prompt<float>(const Kv4Attn &, const ServeRows<float> &, const ServeRows<float> &, int, cudaStream_t);
+template int kv4_prompt<__nv_bfloat16>(const Kv4Attn &, const ServeRows<__nv_bfloat16> &, const ServeRows<__nv_bfloat16> &, int, cudaStream_t);
+template int kv4_prompt<__half>(const Kv4Attn &, const ServeRows<__half> &, const ServeRows<__half> &, int, cudaStream_t);
+
+size_t kv4_prompt_floats(int blocks, int sm_count) { return blocks <= 4 ? (size_t)sm_count * kPRows * (blocks * 32 + 2) : 0; }
 
 int kv4_prompt_load(int blocks) {
     bool ok = true;
