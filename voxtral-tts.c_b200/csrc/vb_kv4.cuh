@@ -109,7 +109,8 @@ VB_DEVINL void get_words(const uint8_t *p, uint32_t (&w)[N]) {
 /* Which (sequence, unit, split) a CTA has. A unit is PAIRS (row, query head) pairs of a KV head, a share a number of tiles of TOKENS. Where
  * there are fewer units than CTAs that run at once (a.split), sequences are cut so that all CTAs have about the same number of tiles, by
  * their actual lengths: the smallest share, in whole rounds and `least` at least, with which there are enough CTAs. (With as many
- * splits for each sequence, four of 65536 to 131072 tokens took the time of four of 131072.) Otherwise every unit has a CTA. */
+ * splits for each sequence, four of 65536 to 131072 tokens took the time of four of 131072.) Otherwise every unit has a CTA. `round` is a
+ * power of two. */
 struct Kv4Place {
     int seq, unit, split, share;
 };
@@ -128,28 +129,32 @@ VB_DEVINL Kv4Place kv4_place(const Kv4Attn &a, int round, int least, int most_sp
     /* the first 32 sequences stay in registers; there are at most a few hundred, or every unit has a CTA of its own */
     int units0 = 0;
     const int tiles0 = lane < a.c.seqs ? tiles_of(lane, &units0) : 0;
-    auto total = [&](auto &&f) {
-        long long n = units0 ? (long long)f(tiles0) * units0 : 0;
+    int most = tiles0;
+    float work = (float)max(tiles0, 1) * (float)units0;
+    for (int s = lane + 32; s < a.c.seqs; s += 32) {
+        int units;
+        const int tiles = tiles_of(s, &units);
+        most = max(most, tiles);
+        work += (float)max(tiles, 1) * (float)units;
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) work += __shfl_xor_sync(0xffffffffu, work, o);
+    /* a quotient to within one: no more is asked of it, but to be the same for every CTA */
+    auto quotient = [](int x, int by) { return (int)__fdividef((float)x, (float)by); };
+    int share = max((int)__fdividef(work, (float)n_cta), quotient(most, most_splits)) + 1;
+    share = max(least, (share + round - 1) & -round);
+    /* a unit's last part may be short: a little more, in steps of a sixteenth, until the CTAs are enough */
+    while (share < most) {
+        unsigned n = units0 * (unsigned)max(1, (tiles0 + share - 1) / share);
         for (int s = lane + 32; s < a.c.seqs; s += 32) {
             int units;
             const int tiles = tiles_of(s, &units);
-            n += (long long)f(tiles) * units;
+            n += units * (unsigned)max(1, (tiles + share - 1) / share);
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-        return n;
-    };
-    int most = tiles0;
-    for (int s = lane + 32; s < a.c.seqs; s += 32) {
-        int units;
-        most = max(most, tiles_of(s, &units));
+        if ((int)__reduce_add_sync(0xffffffffu, n) <= n_cta && (most + share - 1) / share <= most_splits) break;
+        share += max(round, (share >> 4) & -round);
     }
-    most = __reduce_max_sync(0xffffffffu, most);
-    const long long all = total([](int tiles) { return max(tiles, 1); });
-    int share = (int)max((all + n_cta - 1) / n_cta, (long long)(most + most_splits - 1) / most_splits);
-    share = max(least, (share + round - 1) / round * round);
-    /* a unit's last part may be short: a little more, in steps of a sixteenth, until the CTAs are enough */
-    while (share < most && total([&](int tiles) { return max(1, (tiles + share - 1) / share); }) > n_cta) share += max(round, share / 16 / round * round);
     /* this CTA's place: sequence by sequence, all units' first parts, then their second ones */
     int left = blockIdx.x;
     for (int s0 = 0; s0 < a.c.seqs; s0 += 32) {

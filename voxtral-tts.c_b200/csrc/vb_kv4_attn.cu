@@ -73,50 +73,69 @@ VB_DEVINL void get_values(const uint8_t *p, uint32_t (&w)[(NB + 1) / 2]) {
     }
 }
 
-/* Eight (row, head) pairs as the B operand of K Q^T, by one warp, into q_s [block][half][term][lane]; what S is to be multiplied by
- * to be a power of two, a column each, into mul_s. */
-template <int NB, int QT, class T>
-VB_DEVINL void make_queries(const ServeRows<T> &q, const Kv4Attn &a, int seq, int kv_head, int pair0, int pairs, uint2 *q_s, float *mul_s) {
-    const int lane = threadIdx.x & 31, n = lane >> 2, t = lane & 3, pair = pair0 + n;
-    const bool real = pair < pairs;
-    const int row = real ? pair / a.group : 0, head = kv_head * a.group + (real ? pair - row * a.group : 0);
-    const T *p = q.data + seq * q.seq + row * q.row + head * q.head + t * 8;
-    float x[NB][8];
-    uint32_t most = 0;
+/* Eight (row, head) pairs are the B operand of K Q^T, in q_s [block][half][term][lane]: column n by warp n, four values a lane. (All of
+ * them by one warp: 3450 clocks until they were there, with fp32 heads of 128.) What S is to be multiplied by to be a power of two goes into
+ * mul_s. Loads first, so that other things can be begun while they are on their way. */
+template <int NB, class T>
+struct QueryColumn {
+    static constexpr int kGroups = NB * 8, kEach = (kGroups + 31) / 32;
+    float x[kEach][4];
+    VB_DEVINL void load(const ServeRows<T> &q, const Kv4Attn &a, int seq, int kv_head, int pair, int pairs) {
+        const int lane = threadIdx.x & 31;
+        const bool real = pair < pairs;
+        const int row = real ? pair / a.group : 0, head = kv_head * a.group + (real ? pair - row * a.group : 0);
+        const T *p = q.data + seq * q.seq + row * q.row + head * q.head;
 #pragma unroll
-    for (int b = 0; b < NB; b++) {
+        for (int i = 0; i < kEach; i++) {
+            const int at = lane + 32 * i;
 #pragma unroll
-        for (int j = 0; j < 8; j++) x[b][j] = 0.0f;
-        if (real) serve_load<8>(p + b * 32, a.wide, x[b]);
-    }
+            for (int j = 0; j < 4; j++) x[i][j] = 0.0f;
+            if (!real || at >= kGroups) continue;
+            if (!a.wide) {
 #pragma unroll
-    for (int b = 0; b < NB; b++)
-#pragma unroll
-        for (int j = 0; j < 8; j++) most = max(most, __float_as_uint(x[b][j]) & 0x7fffffffu);
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-    /* the largest to [2^14, 2^15); rows of zeros, or with a value that is not finite, as they are */
-    const uint32_t e = most >> 23, field = e == 0u || e == 255u ? 127u : min(268u - e, 253u);
-    const float down = __uint_as_float((254u - field) << 23);
-    float up = __uint_as_float(field << 23);
-    if (a.scale <= 0.0f) up = a.scale < 0.0f ? -up : 0.0f;               /* the factor is positive: the largest score is the largest product */
-    if (t == 0) mul_s[n] = (a.scale != 0.0f ? fabsf(a.scale) * 1.44269504f : 1.0f) * down;
-#pragma unroll
-    for (int b = 0; b < NB; b++)
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            float y[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) y[j] = x[b][4 * h + j] * up;
-            uint2 w = make_uint2(half_pack(y[0], y[1]), half_pack(y[2], y[3]));
-            q_s[((b * 2 + h) * QT) * 32 + lane] = w;
-            if constexpr (QT == 2) {
-                const float2 f = kv4_f2(w.x), g = kv4_f2(w.y);
-                w = make_uint2(half_pack(y[0] - f.x, y[1] - f.y), half_pack(y[2] - g.x, y[3] - g.y));
-                q_s[((b * 2 + h) * QT + 1) * 32 + lane] = w;
+                for (int j = 0; j < 4; j++) x[i][j] = serve_get(p + at * 4 + j);
+            } else if constexpr (sizeof(T) == 4) {
+                const float4 v = reinterpret_cast<const float4 *>(p)[at];
+                x[i][0] = v.x; x[i][1] = v.y; x[i][2] = v.z; x[i][3] = v.w;
+            } else {
+                const uint2 v = reinterpret_cast<const uint2 *>(p)[at];
+                const float2 lo = serve_pair(v.x, p), hi = serve_pair(v.y, p);
+                x[i][0] = lo.x; x[i][1] = lo.y; x[i][2] = hi.x; x[i][3] = hi.y;
             }
         }
-}
+    }
+    template <int QT>
+    VB_DEVINL void put(const Kv4Attn &a, int n, uint2 *q_s, float *mul_s) {
+        const int lane = threadIdx.x & 31;
+        uint32_t most = 0;
+#pragma unroll
+        for (int i = 0; i < kEach; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) most = max(most, __float_as_uint(x[i][j]) & 0x7fffffffu);
+        most = __reduce_max_sync(0xffffffffu, most);
+        /* the largest to [2^14, 2^15); rows of zeros, or with a value that is not finite, as they are */
+        const uint32_t e = most >> 23, field = e == 0u || e == 255u ? 127u : min(268u - e, 253u);
+        const float down = __uint_as_float((254u - field) << 23);
+        float up = __uint_as_float(field << 23);
+        if (a.scale <= 0.0f) up = a.scale < 0.0f ? -up : 0.0f;       /* the factor is positive: the largest score is the largest product */
+        if (lane == 0) mul_s[n] = (a.scale != 0.0f ? fabsf(a.scale) * 1.44269504f : 1.0f) * down;
+#pragma unroll
+        for (int i = 0; i < kEach; i++) {
+            const int at = lane + 32 * i;                             /* 8 blocks + 2 t + half */
+            if (at >= kGroups) continue;
+            uint2 *to = q_s + (((at >> 3) * 2 + (at & 1)) * QT) * 32 + n * 4 + ((at >> 1) & 3);
+            float y[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) y[j] = x[i][j] * up;
+            const uint2 w = make_uint2(half_pack(y[0], y[1]), half_pack(y[2], y[3]));
+            to[0] = w;
+            if constexpr (QT == 2) {
+                const float2 f = kv4_f2(w.x), g = kv4_f2(w.y);
+                to[32] = make_uint2(half_pack(y[0] - f.x, y[1] - f.y), half_pack(y[2] - g.x, y[3] - g.y));
+            }
+        }
+    }
+};
 
 /* Scores of 16 tokens: `at` words of the lane's two tokens (g and g + 8 of them), c: tokens g, g + 8 x columns 2 t, 2 t + 1. */
 template <bool FIRST, int QT>
@@ -152,7 +171,9 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(co
     pdl_launch_dependents();       /* after the wait: the masses' kernel reads what this one has waited for */
     const Kv4Place place = kv4_place<kACols, kAKeys>(a, kAWarps, 2 * kAWarps, kAMaxSplits);
     if (place.seq >= a.c.seqs) return;
-    const int seq = place.seq, kv_head = place.unit % a.c.kv_heads, tile_r = place.unit / a.c.kv_heads, split = place.split, share = place.share;
+    const int seq = place.seq, tile_r = place.unit / a.c.kv_heads, kv_head = place.unit - tile_r * a.c.kv_heads, split = place.split, share = place.share;
+    QueryColumn<NB, T> column;
+    column.load(q, a, seq, kv_head, tile_r * kACols + warp, a.max_rows * a.group);
     const Kv4Span span = kv4_span(a.lengths, a.rows, a.max_rows, seq, a.c.capacity);
     const int pairs = span.rows * a.group, pair0 = tile_r * kACols;
     if (pair0 >= pairs) return;
@@ -184,7 +205,7 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(co
             if (t_begin + i * kAWarps < t_end) fetch(t_begin + i * kAWarps, i);
     }
     if (tid == 0) abort_flag = 0;
-    if (warp == 0) make_queries<NB, QT>(q, a, seq, kv_head, pair0, a.max_rows * a.group, q_s, mul_s);
+    column.template put<QT>(a, warp, q_s, mul_s);
     __syncthreads();
 
     /* columns 2 t and 2 t + 1 of this lane: tokens they see, what makes their scores powers of two */
@@ -561,7 +582,7 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(co
 
 /* mass_out: the scores again, now that the rows' sums are known (in the attention kernel only the last CTA of a split sequence knows them,
  * and keeping scores takes memory for every row). A CTA has up to four tiles of tokens a warp, whose keys stay in shared memory while the
- * (row, head) pairs come by, 64 at a time, made by a warp each. A token's weights are summed in one order: no atomics. */
+ * (row, head) pairs come by, 64 at a time, a column of eight by each warp. A token's weights are summed in one order: no atomics. */
 constexpr int kMTiles = 4;
 
 template <int NB, class T>
@@ -618,7 +639,12 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_mass_kernel(co
     for (int group0 = max(0, cta0 - before) * a.group / kACols * kACols; group0 < pairs; group0 += kAWarps * kACols) {
         __syncthreads();                                                            /* the pairs before are done with */
         const int made = min(kAWarps, (pairs - group0 + kACols - 1) / kACols);
-        if (warp < made) make_queries<NB, QT>(q, a, seq, kv_head, group0 + warp * kACols, pairs, q_s + warp * (Cfg::kQ / 8), mul_s + warp * kACols);
+#pragma unroll 1
+        for (int r = 0; r < made; r++) {
+            QueryColumn<NB, T> column;
+            column.load(q, a, seq, kv_head, group0 + r * kACols + warp, pairs);
+            column.template put<QT>(a, warp, q_s + r * (Cfg::kQ / 8), mul_s + r * kACols);
+        }
         if (!waited) pdl_wait();
         waited = true;
         if (tid < kAWarps * kACols) {
