@@ -12,7 +12,7 @@
  * alternate tiles with a reference, sums and an accumulator each, merged at the end, so that the tensor pipe works on one tile while the
  * other is in its softmax.
  *
- * Warps: 0-3, 4-7 softmax, 8-11 keys, 12-14 values, 15 issues the MMAs. All waits are bounded.
+ * Warps: 0-7, 8-15 softmax, 16-19 keys, 20-22 values, 23 issues the MMAs. All waits are bounded.
  */
 #include <type_traits>
 
@@ -23,24 +23,20 @@ namespace vb {
 
 namespace {
 
-constexpr int kPRows = 128, kPKeys = 128, kPThreads = 512, kPMmaWarp = 15, kPBlock = kPKeys * 128, kPStatus = 62, kPRing = 8;
+constexpr int kPRows = 128, kPKeys = 128, kPSoft = 512, kPThreads = 768, kPMmaWarp = 23, kPBlock = kPKeys * 128, kPStatus = 62, kPRing = 8;
 constexpr int kPLeast = 2;                    /* tiles of a part at least */
 constexpr uint32_t kPTmem = 512, kPO = 256;
-/* registers a thread at the launch, of a softmax thread and of any other: what some are given the others have given up */
-constexpr int kPRegs = 128, kPSoftRegs = 184, kPLoadRegs = 72;
-static_assert(kPThreads == 512 && 2 * kPSoftRegs + 2 * kPLoadRegs <= 4 * kPRegs, "more registers than the block is launched with");
-
 template <int NB, int QT>
 struct PCfg {
     static constexpr int kD64 = (NB + 1) / 2;                                  /* blocks of 64 columns */
     static constexpr int kSlot = kD64 * kPBlock;
-    static constexpr int kSlots = kD64 * QT >= 4 ? 2 : 3;
+    static constexpr int kSlots = kD64 >= 2 ? 2 : 3;
     static constexpr int kQ = QT * kSlot;
     static constexpr int kSmem = kQ + 2 * kSlots * kSlot + 1024;
     static constexpr int kPart = kPRows * (NB * 32 + 2);                       /* floats of a part: results, references and sums */
     static constexpr int kLd = NB * 32 + 4;                                    /* results on their way out: a row */
-    static_assert(kPRows * kLd * 4 + 2 * kPRows * 16 <= 2 * kSlots * kSlot, "results do not fit the rings");
-    static_assert(kSmem <= 232448 - 2048, "over what a CTA may use");
+    static_assert(kPRows * kLd * 4 + 4 * kPRows * 16 <= 2 * kSlots * kSlot, "results do not fit the rings");
+    static_assert(kSmem <= 232448 - 4096, "over what a CTA may use");
 };
 
 VB_DEVINL uint64_t p_desc_mn(uint32_t addr) {
@@ -54,24 +50,7 @@ VB_DEVINL uint64_t p_desc_mn(uint32_t addr) {
 /* kind::f16 with FP16 operands, fp32 sums, 128 rows, n columns */
 VB_DEVINL uint32_t p_idesc(int n, bool mn_major) { return (1u << 4) | (mn_major ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kPRows >> 4) << 24); }
 
-/* 32 columns of this thread's TMEM lane on their way, and in place; 16 columns back */
-VB_DEVINL void p_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : VB_AT_W8(r, 0), VB_AT_W8(r, 8), VB_AT_W8(r, 16), VB_AT_W8(r, 24)
-        : "r"(taddr)
-        : "memory");
-}
-#define VB_P_RW8(r, o) "+r"((r)[o]), "+r"((r)[o + 1]), "+r"((r)[o + 2]), "+r"((r)[o + 3]), "+r"((r)[o + 4]), "+r"((r)[o + 5]), "+r"((r)[o + 6]), "+r"((r)[o + 7])
-/* (an instruction of its own for each array, none of them before the wait: an operand list has room for 30) */
-VB_DEVINL void p_ld_wait(uint32_t (&r)[4][32]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int c = 0; c < 4; c++)
-#pragma unroll
-        for (int k = 0; k < 32; k += 8) asm volatile("" : VB_P_RW8(r[c], k));
-}
+/* 16 columns of this thread's TMEM lane */
 template <int N>
 VB_DEVINL void p_st16(uint32_t taddr, const uint32_t (&r)[N]) {
     static_assert(N >= 16, "");
@@ -99,7 +78,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
     unsigned char *base = (unsigned char *)(((uintptr_t)p_smem_raw + 1023) & ~(uintptr_t)1023);
     unsigned char *q_s = base, *k_s = q_s + Cfg::kQ, *v_s = k_s + Cfg::kSlots * Cfg::kSlot;
     __shared__ __align__(8) uint64_t k_full[Cfg::kSlots], k_empty[Cfg::kSlots], v_full[Cfg::kSlots], v_empty[Cfg::kSlots], s_full[2], p_full[2], o_done[2], q_full;
-    __shared__ float key_up[kPRing][4], down_s[kPRows];
+    __shared__ float key_up[kPRing][4], down_s[kPRows], top_s[2][2][kPRows];
     __shared__ int value_top[kPRing], bad_s[NB], abort_s;
     __shared__ uint32_t tmem_slot;
     int *abort_flag = &abort_s;
@@ -129,10 +108,10 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
         }
         for (int i = 0; i < 2; i++) {
             vb_mbar_init(&s_full[i], 1);
-            vb_mbar_init(&p_full[i], 128);
+            vb_mbar_init(&p_full[i], 256);
             vb_mbar_init(&o_done[i], 1);
         }
-        vb_mbar_init(&q_full, 256);
+        vb_mbar_init(&q_full, kPSoft);
         abort_s = 0;
         vb_mbar_init_fence();
     }
@@ -151,19 +130,16 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
         *(volatile int *)abort_flag = 1;
     };
 
-    /* a softmax thread holds a row of scores: its registers from the other warps' */
-    if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPSoftRegs));
-    else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPLoadRegs));
-    if (warp < 8) {
+    if (warp < kPSoft / 32) {
         /* ---- queries: four values a lane, NB * 8 lanes a row, so that a warp has one, two or four rows at a time; the loads of
-         * sixteen rows together ---- */
-        constexpr int kLanes = NB * 8, kSide = 32 / kLanes, kBatch = 16 / kSide;
+         * its eight rows together ---- */
+        constexpr int kLanes = NB * 8, kSide = 32 / kLanes, kBatch = 8 / kSide;
         const int side = lane / kLanes, d = (lane - side * kLanes) * 4;
         const bool mine = side < kSide;
         float x[kBatch][4];
 #pragma unroll
         for (int u = 0; u < kBatch; u++) {
-            const int pair = pair0 + warp * 16 + u * kSide + side;
+            const int pair = pair0 + warp * 8 + u * kSide + side;
             const bool real = mine && pair < pairs;
             const int row = real ? pair / a.group : 0, head = kv_head * a.group + (real ? pair - row * a.group : 0);
             const T *p = q.data + seq * q.seq + row * q.row + head * q.head + d;
@@ -185,7 +161,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
         }
 #pragma unroll
         for (int u = 0; u < kBatch; u++) {
-            const int r = warp * 16 + u * kSide + side;
+            const int r = warp * 8 + u * kSide + side;
             uint32_t most = 0;
 #pragma unroll
             for (int i = 0; i < 4; i++) most = max(most, __float_as_uint(x[u][i]) & 0x7fffffffu);
@@ -212,10 +188,10 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
         }
         at_proxy_fence();
         vb_mbar_arrive(&q_full);
-        vb_named_bar(1, 256);                                      /* down_s */
+        vb_named_bar(1, kPSoft);                                   /* down_s */
 
-        /* ---- softmax: warpgroup w takes tiles w, w + 2, ...; a thread owns pair pair0 + r ---- */
-        const int w = warp >> 2, r = tid & 127, pair = pair0 + r;
+        /* ---- softmax: two warpgroups take tiles w, w + 2, ...; a thread has half of the columns of pair pair0 + r ---- */
+        const int wg = warp >> 2, w = wg >> 1, half = wg & 1, r = tid & 127, pair = pair0 + r;
         const bool valid = r < n_pairs;
         const int row = valid ? pair / a.group : 0, head = kv_head * a.group + (valid ? pair - row * a.group : 0);
         const int sees = before + (pair0 + min(r, n_pairs - 1)) / a.group + 1;
@@ -231,29 +207,29 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
             const float *ups = key_up[t % kPRing];
             const int last = sees - j0;                            /* columns before this one are seen */
             const bool masked = j0 + kPKeys > all_see;
-            /* a tile's scores in registers: 32 columns are requested behind one another, and waited for together */
-            uint32_t s[4][32];
-#pragma unroll
-            for (int c = 0; c < 4; c++) p_ld32(tS + (uint32_t)(c * 32), s[c]);
-            p_ld_wait(s);
-            if (masked) {
-#pragma unroll
-                for (int c = 0; c < 4; c++)
-#pragma unroll
-                    for (int k = 0; k < 32; k++)
-                        if (c * 32 + k >= last) s[c][k] = 0xff800000u;
-            }
             float top = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
+            for (int c = 0; c < 2; c++) {
+                uint32_t reg[32];
+                const int column = half * 64 + c * 32;
+                at_ld32(tS + (uint32_t)column, reg);
+                if (masked) {
+#pragma unroll
+                    for (int k = 0; k < 32; k++)
+                        if (column + k >= last) reg[k] = 0xff800000u;
+                }
                 float m4[4];
 #pragma unroll
-                for (int k = 0; k < 4; k++) m4[k] = __uint_as_float(s[c][k]);
+                for (int k = 0; k < 4; k++) m4[k] = __uint_as_float(reg[k]);
 #pragma unroll
-                for (int k = 4; k < 32; k++) m4[k & 3] = fmaxf(m4[k & 3], __uint_as_float(s[c][k]));
+                for (int k = 4; k < 32; k++) m4[k & 3] = fmaxf(m4[k & 3], __uint_as_float(reg[k]));
                 const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-                if (m > -INFINITY) top = fmaxf(top, m * (ups[c] * mul));
+                if (m > -INFINITY) top = fmaxf(top, m * (ups[half * 2 + c] * mul));
             }
+            /* the other half's: it has been read by then when it is written again, since the next tile's scores wait for both halves */
+            top_s[w][half][r] = top;
+            vb_named_bar(2 + w, 256);
+            top = fmaxf(top, top_s[w][half ^ 1][r]);
             /* values: the scale that this tile is based on */
             if (!at_warp_wait(&v_full[t % Cfg::kSlots], (uint32_t)(t / Cfg::kSlots) & 1u, abort_flag)) { give_up(); break; }
             const int now_scale = value_top[t % kPRing];
@@ -266,7 +242,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
                     const int fall = now_scale - top_scale;
                     const float fo = fall > 126 ? 0.0f : f * __uint_as_float((uint32_t)(127 - fall) << 23);
 #pragma unroll 1
-                    for (int c = 0; c < NB; c++) {
+                    for (int c = half; c < NB; c += 2) {
                         uint32_t reg[32];
                         at_ld32(tO + (uint32_t)(c * 32), reg);
 #pragma unroll
@@ -282,24 +258,31 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
             uint64_t sums[2] = {0, 0};
             const uint64_t low2 = vb_f2_pack(-low, -low);
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                const float up = ups[c] * mul;
+            for (int c = 0; c < 2; c++) {
+                const int column = half * 64 + c * 32;
+                const float up = ups[half * 2 + c] * mul;
                 const uint64_t up2 = vb_f2_pack(up, up);
-                uint32_t second[PT == 2 ? 16 : 1];
+                uint32_t s[32], second[PT == 2 ? 16 : 1];
+                at_ld32(tS + (uint32_t)column, s);
+                if (masked) {
+#pragma unroll
+                    for (int k = 0; k < 32; k++)
+                        if (column + k >= last) s[k] = 0xff800000u;
+                }
 #pragma unroll
                 for (int k = 0; k < 32; k += 2) {
-                    const float2 x = vb_f2_get(vb_f2_fma(vb_f2_pack(__uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1])), up2, low2));
+                    const float2 x = vb_f2_get(vb_f2_fma(vb_f2_pack(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), up2, low2));
                     const float p0 = exp2_fast(x.x), p1 = exp2_fast(x.y);
                     sums[(k >> 1) & 1] = vb_f2_add(sums[(k >> 1) & 1], vb_f2_pack(p0, p1));
                     const uint32_t hi = half_pack(p0, p1);
-                    s[c][k / 2] = hi;
+                    s[k / 2] = hi;
                     if constexpr (PT == 2) {
                         const float2 f = kv4_f2(hi);
                         second[k / 2] = half_pack(p0 - f.x, p1 - f.y);
                     }
                 }
-                p_st16(tS + (uint32_t)(c * 32), s[c]);             /* 16 columns of first terms, 16 of second ones */
-                if constexpr (PT == 2) p_st16(tS + (uint32_t)(c * 32 + 16), second);
+                p_st16(tS + (uint32_t)column, s);                  /* 16 columns of first terms, 16 of second ones */
+                if constexpr (PT == 2) p_st16(tS + (uint32_t)(column + 16), second);
             }
             const float2 sum2 = vb_f2_get(vb_f2_add(sums[0], sums[1]));
             sum += sum2.x + sum2.y;
@@ -308,22 +291,24 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
             vb_mbar_arrive(&p_full[w]);
         }
         if (it > 0 && !at_warp_wait(&o_done[w], (uint32_t)(it - 1) & 1u, abort_flag)) give_up();
-        /* both halves of the tokens, merged, each warpgroup half of the columns, by way of shared memory */
-        vb_named_bar(1, 256);                                      /* every product is done: the rings are free */
-        float4 *ends = reinterpret_cast<float4 *>(k_s);            /* 2 x 128 x (reference, sum, scale) */
-        float *rows = reinterpret_cast<float *>(k_s + 2 * kPRows * 16);
-        ends[w * kPRows + r] = make_float4(ref, sum * 0x1p-15f, __int_as_float(top_scale), 0.0f);
+        /* the tiles of either pair of warpgroups, merged, a warpgroup a block of 32 columns, by way of shared memory */
+        vb_named_bar(1, kPSoft);                                     /* every product is done: the rings are free */
+        float4 *ends = reinterpret_cast<float4 *>(k_s);            /* 4 x 128 x (reference, sum, scale) */
+        float *rows = reinterpret_cast<float *>(k_s + 4 * kPRows * 16);
+        ends[wg * kPRows + r] = make_float4(ref, sum * 0x1p-15f, __int_as_float(top_scale), 0.0f);
         tc_fence_before();
-        vb_named_bar(1, 256);
+        vb_named_bar(1, kPSoft);
         tc_fence_after();
-        const float4 A = ends[r], B = ends[kPRows + r];
+        float4 A = ends[r], B = ends[2 * kPRows + r];
+        A.y += ends[kPRows + r].y;
+        B.y += ends[3 * kPRows + r].y;
         const float reference = fmaxf(A.x, B.x);
         float fa = A.x > -INFINITY ? exp2_fast(A.x - reference) : 0.0f, fb = B.x > -INFINITY ? exp2_fast(B.x - reference) : 0.0f;
         const float total = A.y * fa + B.y * fb, inv = used > 1 ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
         float *part = a.part + (size_t)blockIdx.x * PCfg<NB, QT>::kPart;
         if (used > 1) {
-            if (w == 0) reinterpret_cast<float2 *>(part + kPRows * kDim)[r] = make_float2(reference, total);
-        } else if (w == 0 && valid && a.lse)
+            if (wg == 0) reinterpret_cast<float2 *>(part + kPRows * kDim)[r] = make_float2(reference, total);
+        } else if (wg == 0 && valid && a.lse)
             a.lse[((size_t)seq * a.max_rows + row) * a.heads + head] = total == 0.0f ? -INFINITY : (reference + 8.0f + log2f(total)) * 0.69314718f;
         fa *= inv;
         fb *= inv;
@@ -331,7 +316,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
         const float a0 = __uint_as_float((uint32_t)(127 + (ea >> 1)) << 23), a1 = __uint_as_float((uint32_t)(127 + ea - (ea >> 1)) << 23);
         const float b0 = __uint_as_float((uint32_t)(127 + (eb >> 1)) << 23), b1 = __uint_as_float((uint32_t)(127 + eb - (eb >> 1)) << 23);
 #pragma unroll 1
-        for (int c = w; c < NB; c += 2) {
+        for (int c = wg; c < NB; c += kPSoft / 128) {
             uint32_t oa[32], ob[32];
             const bool nan = bad_s[c] < sees;
             if (n_tiles > 0) at_ld32(tmem + lanes + kPO + (uint32_t)(c * 32), oa);
@@ -347,10 +332,10 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
 #pragma unroll
             for (int k = 0; k < 32; k += 4) *reinterpret_cast<uint4 *>(rows + r * Cfg::kLd + c * 32 + k) = make_uint4(oa[k], oa[k + 1], oa[k + 2], oa[k + 3]);
         }
-        vb_named_bar(1, 256);
+        vb_named_bar(1, kPSoft);
         /* out, eight values a lane */
         constexpr int kEights = kDim / 8;
-        for (int x = tid; x < n_pairs * kEights; x += 256) {
+        for (int x = tid; x < n_pairs * kEights; x += kPSoft) {
             const int p = x / kEights, d = (x - p * kEights) * 8, rr = (pair0 + p) / a.group, hh = kv_head * a.group + pair0 + p - rr * a.group;
             const float4 lo = *reinterpret_cast<const float4 *>(rows + p * Cfg::kLd + d), hi = *reinterpret_cast<const float4 *>(rows + p * Cfg::kLd + d + 4);
             if (used > 1) {
@@ -361,9 +346,9 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
             const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
             serve_store<8>(out.data + seq * out.seq + rr * out.row + hh * out.head + d, a.wide_out, v);
         }
-    } else if (warp < 12) {
+    } else if (warp < 20) {
         /* ---- keys: a warp has 32 tokens of a tile, four lanes a token (words t * NB ..: values 8 t .. of every block) ---- */
-        const int lw = warp - 8, g = lane >> 2, tq = lane & 3;
+        const int lw = warp - 16, g = lane >> 2, tq = lane & 3;
         const size_t row0 = a.c.row(seq, kv_head, 0);
         uint32_t words[4][NB], bytes[4][NB];
         auto fetch = [&](int t) {
@@ -433,8 +418,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
         };
         int top = 0;
         const int tasks = n_tiles * 4;
-        if (warp - 12 < tasks) fetch(warp - 12);
-        for (int task = warp - 12; task < tasks; task += 3) {
+        if (warp - 20 < tasks) fetch(warp - 20);
+        for (int task = warp - 20; task < tasks; task += 3) {
             const int t = task / 4, lw = task % 4, slot = t % Cfg::kSlots, j0 = (first_tile + t) * kPKeys;
             const int real = seen - j0;                            /* tokens of the tile that are seen */
             int most = 0;
@@ -591,13 +576,8 @@ int prompt_launch(Kv4Attn a, const ServeRows<T> &q, const ServeRows<T> &out, int
 }
 template <int NB, class T>
 bool prompt_load() {
-    /* a block launched with fewer registers than its warps ask for would wait for them for good */
     cudaFuncAttributes f;
-    if (cudaFuncGetAttributes(&f, kv4_join_kernel<NB, T>) != cudaSuccess || cudaFuncGetAttributes(&f, kv4_prompt_kernel<NB, kWeightTerms<T>, T>) != cudaSuccess) return false;
-    if (f.numRegs < kPRegs) {
-        serve_fail("the prompt kernel was built with fewer registers than it divides");
-        return false;
-    }
+    if (cudaFuncGetAttributes(&f, kv4_join_kernel<NB, T>) != cudaSuccess) return false;
     return cudaFuncSetAttribute(kv4_prompt_kernel<NB, kWeightTerms<T>, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, PCfg<NB, sizeof(T) == 4 ? 2 : 1>::kSmem) == cudaSuccess;
 }
 
