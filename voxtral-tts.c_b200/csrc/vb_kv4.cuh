@@ -31,6 +31,7 @@ struct Kv4Attn {
     Kv4 c;
     const int *lengths, *rows;
     int max_rows, heads, group, row_tiles, split, wide, wide_out;
+    int tail0, tail_units, tail_parts;       /* of vb_kv4_prompt.cu */
     float scale;
     float *lse;
     const float *mass_in;

@@ -14,7 +14,7 @@
  *
  * Warps: 0-7, 8-15 softmax, 16-19 keys, 20-22 values, 23 issues the MMAs. All waits are bounded.
  */
-#include <type_traits>
+#include <algorithm>
 
 #include "vb_attn_tc.cuh"
 #include "vb_kv4.cuh"
@@ -24,7 +24,7 @@ namespace vb {
 namespace {
 
 constexpr int kPRows = 128, kPKeys = 128, kPSoft = 512, kPThreads = 768, kPMmaWarp = 23, kPBlock = kPKeys * 128, kPStatus = 62, kPRing = 8;
-constexpr int kPLeast = 2;                    /* tiles of a part at least */
+constexpr int kPLeast = 2, kPTailParts = 8;   /* tiles of a part at least; parts of a unit of the last round at most */
 constexpr uint32_t kPTmem = 512, kPO = 256;
 template <int NB, int QT>
 struct PCfg {
@@ -70,6 +70,44 @@ VB_DEVINL uint32_t p_factor(int byte, int top) {
     return half_pack(f, f);
 }
 
+/* What a CTA has: a unit's tiles of tokens, or the split-th part of them, and where its part lies and those beside it. */
+struct PWork {
+    int seq, kv_head, pair0, n_pairs, before, seen, used, split, first_tile, n_tiles, slot, stride;
+    Kv4Span span;
+};
+/* Where there are fewer units than SMs, CTAs have shares of the work (kv4_place). Otherwise a CTA has a unit, but the units that would be
+ * alone in a last round are cut into a.tail_parts (304 units of 24 to 33 tiles on 148 SMs: 206 us with three rounds). False: nothing. */
+VB_DEVINL bool p_work(const Kv4Attn &a, int block, PWork &p) {
+    int unit, share = INT_MAX, parts = 0;
+    if (a.split) {
+        const Kv4Place place = kv4_place<kPRows, kPKeys>(a, 1, kPLeast, kPRows);
+        p.seq = place.seq; unit = place.unit; p.split = place.split; share = place.share; p.slot = block;
+    } else {
+        const int i = block - a.tail0, u = i < 0 ? block : a.tail0 + i % a.tail_units, units = a.row_tiles * a.c.kv_heads;
+        p.seq = u / units;
+        unit = u - p.seq * units;
+        p.slot = i;
+        p.split = i < 0 ? 0 : i / a.tail_units;
+        parts = i < 0 ? 0 : a.tail_parts;
+    }
+    if (p.seq >= a.c.seqs) return false;
+    p.span = kv4_span(a.lengths, a.rows, a.max_rows, p.seq, a.c.capacity);
+    const int pairs = p.span.rows * a.group, row_tiles = (pairs + kPRows - 1) / kPRows, u = unit / a.c.kv_heads, tile_r = row_tiles - 1 - u;
+    if (tile_r < 0) return false;                                  /* the latest rows see the most tokens: they go first */
+    p.kv_head = unit - u * a.c.kv_heads;
+    p.stride = a.split ? row_tiles * a.c.kv_heads : a.tail_units;
+    p.pair0 = tile_r * kPRows;
+    p.n_pairs = min(kPRows, pairs - p.pair0);
+    p.before = p.span.length - p.span.rows;
+    p.seen = max(0, p.before + (p.pair0 + p.n_pairs - 1) / a.group + 1);
+    const int tiles = (p.seen + kPKeys - 1) / kPKeys;
+    if (parts) share = max(kPLeast, (tiles + parts - 1) / parts);
+    p.used = tiles <= share ? 1 : (tiles + share - 1) / share;
+    p.first_tile = p.used == 1 ? 0 : p.split * share;
+    p.n_tiles = p.used == 1 ? tiles : min(tiles, p.first_tile + share) - p.first_tile;
+    return p.split < p.used;
+}
+
 template <int NB, int PT, class T>
 __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn a, const ServeRows<T> q, const ServeRows<T> out) {
     constexpr int QT = sizeof(T) == 4 ? 2 : 1, kDim = NB * 32;
@@ -85,20 +123,11 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     pdl_wait();
-    const Kv4Place place = kv4_place<kPRows, kPKeys>(a, 1, kPLeast, kPRows);
-    if (place.seq >= a.c.seqs) return;
-    const int seq = place.seq, kv_head = place.unit % a.c.kv_heads;
-    const Kv4Span span = kv4_span(a.lengths, a.rows, a.max_rows, seq, a.c.capacity);
-    const int pairs = span.rows * a.group;
-    const int row_tiles = (pairs + kPRows - 1) / kPRows, tile_r = row_tiles - 1 - place.unit / a.c.kv_heads;      /* the latest rows see the most tokens: they go first */
-    if (tile_r < 0) return;
-    const int pair0 = tile_r * kPRows;
-    const int n_pairs = min(kPRows, pairs - pair0), before = span.length - span.rows;
-    const int all_see = before + pair0 / a.group + 1, seen = max(0, before + (pair0 + n_pairs - 1) / a.group + 1);
-    /* this CTA's tiles of tokens: all, or a part */
-    const int tiles = (seen + kPKeys - 1) / kPKeys, used = tiles <= place.share ? 1 : (tiles + place.share - 1) / place.share;
-    if (place.split >= used) return;
-    const int first_tile = used == 1 ? 0 : place.split * place.share, n_tiles = used == 1 ? tiles : min(tiles, first_tile + place.share) - first_tile;
+    PWork work;
+    if (!p_work(a, blockIdx.x, work)) return;
+    const int seq = work.seq, kv_head = work.kv_head, pair0 = work.pair0, n_pairs = work.n_pairs, pairs = pair0 + n_pairs, before = work.before, seen = work.seen;
+    const int first_tile = work.first_tile, n_tiles = work.n_tiles, used = work.used;
+    const int all_see = before + pair0 / a.group + 1;
     if (tid == 0) {
         for (int i = 0; i < Cfg::kSlots; i++) {
             vb_mbar_init(&k_full[i], 4);
@@ -305,7 +334,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
         const float reference = fmaxf(A.x, B.x);
         float fa = A.x > -INFINITY ? exp2_fast(A.x - reference) : 0.0f, fb = B.x > -INFINITY ? exp2_fast(B.x - reference) : 0.0f;
         const float total = A.y * fa + B.y * fb, inv = used > 1 ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
-        float *part = a.part + (size_t)blockIdx.x * PCfg<NB, QT>::kPart;
+        float *part = a.part + (size_t)work.slot * PCfg<NB, QT>::kPart;
         if (used > 1) {
             if (wg == 0) reinterpret_cast<float2 *>(part + kPRows * kDim)[r] = make_float2(reference, total);
         } else if (wg == 0 && valid && a.lse)
@@ -515,20 +544,12 @@ __global__ void __launch_bounds__(kJThreads) kv4_join_kernel(const Kv4Attn a, co
     constexpr int kDim = NB * 32, kPart = kPRows * (kDim + 2);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_wait();
-    const Kv4Place place = kv4_place<kPRows, kPKeys>(a, 1, kPLeast, kPRows);
-    if (place.seq >= a.c.seqs) return;
-    const int seq = place.seq, kv_head = place.unit % a.c.kv_heads;
-    const Kv4Span span = kv4_span(a.lengths, a.rows, a.max_rows, seq, a.c.capacity);
-    const int pairs = span.rows * a.group, row_tiles = (pairs + kPRows - 1) / kPRows, tile_r = row_tiles - 1 - place.unit / a.c.kv_heads;
-    if (tile_r < 0) return;
-    const int pair0 = tile_r * kPRows, n_pairs = min(kPRows, pairs - pair0), before = span.length - span.rows;
-    const int seen = max(0, before + (pair0 + n_pairs - 1) / a.group + 1), tiles = (seen + kPKeys - 1) / kPKeys;
-    const int used = tiles <= place.share ? 1 : (tiles + place.share - 1) / place.share;
-    if (used == 1 || place.split >= used) return;
-    const int units = row_tiles * a.c.kv_heads;
-    const float *parts = a.part + (size_t)((int)blockIdx.x - place.split * units) * kPart;
-    const size_t step = (size_t)units * kPart;
-    for (int p = place.split + warp * used; p < n_pairs; p += kJThreads / 32 * used) {
+    PWork work;
+    if (!p_work(a, blockIdx.x + (a.split ? 0 : a.tail0), work) || work.used == 1) return;
+    const int seq = work.seq, kv_head = work.kv_head, pair0 = work.pair0, n_pairs = work.n_pairs, used = work.used, split = work.split;
+    const float *parts = a.part + (size_t)(work.slot - split * work.stride) * kPart;
+    const size_t step = (size_t)work.stride * kPart;
+    for (int p = split + warp * used; p < n_pairs; p += kJThreads / 32 * used) {
         auto end = [&](int x) { return __ldcg(reinterpret_cast<const float2 *>(parts + x * step + kPRows * kDim) + p); };
         float reference = -INFINITY, total = 0.0f;
         for (int x = lane; x < used; x += 32) reference = fmaxf(reference, end(x).x);
@@ -568,10 +589,16 @@ int prompt_launch(Kv4Attn a, const ServeRows<T> &q, const ServeRows<T> &out, int
     if (units > INT_MAX) return serve_fail("too many rows");
     a.row_tiles = (int)row_tiles;
     a.split = units < sm_count && a.c.capacity > kPLeast * kPKeys;
-    const dim3 grid((unsigned)(a.split ? sm_count : units));
+    /* a part of at least four tiles: beginning and ending take as long as five */
+    const int rest = (int)(units % sm_count), most = std::min(kPTailParts, a.c.capacity / (4 * kPKeys));
+    a.tail_parts = !a.split && units > sm_count && rest > 0 ? std::min(sm_count / rest, most) : 1;
+    a.tail_units = a.tail_parts > 1 ? rest : 1;
+    a.tail0 = a.tail_parts > 1 ? (int)units - rest : INT_MAX;
+    const unsigned tail = a.tail_parts > 1 ? (unsigned)(rest * a.tail_parts) : 0u;
+    const dim3 grid((unsigned)(a.split ? sm_count : tail ? units - rest + tail : units));
     const size_t smem = PCfg<NB, sizeof(T) == 4 ? 2 : 1>::kSmem;
     if (launch_pdl(kv4_prompt_kernel<NB, kWeightTerms<T>, T>, grid, dim3(kPThreads), smem, st, a, q, out) != cudaSuccess) return serve_launched() | -1;
-    if (a.split && launch_pdl(kv4_join_kernel<NB, T>, grid, dim3(kJThreads), 0, st, a, out) != cudaSuccess) return serve_launched() | -1;
+    if ((a.split || tail) && launch_pdl(kv4_join_kernel<NB, T>, a.split ? grid : dim3(tail), dim3(kJThreads), 0, st, a, out) != cudaSuccess) return serve_launched() | -1;
     return 0;
 }
 template <int NB, class T>
