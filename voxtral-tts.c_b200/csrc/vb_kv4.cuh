@@ -183,6 +183,8 @@ VB_DEVINL Kv4Place kv4_place(const Kv4Attn &a, int round, int least, int most_sp
 /* Many rows, heads up to 128 (vb_kv4_prompt.cu) */
 template <class T>
 int kv4_prompt(const Kv4Attn &a, const ServeRows<T> &q, const ServeRows<T> &out, int sm_count, cudaStream_t st);
+template <class T>
+int kv4_mass_many(const Kv4Attn &a, const ServeRows<T> &q, cudaStream_t st);
 int kv4_prompt_load(int blocks);
 /* floats of partial results that it needs */
 size_t kv4_prompt_floats(int blocks, int sm_count);

@@ -583,7 +583,7 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(co
 /* mass_out: the scores again, now that the rows' sums are known (in the attention kernel only the last CTA of a split sequence knows them,
  * and keeping scores takes memory for every row). A CTA has up to four tiles of tokens a warp, whose keys stay in shared memory while the
  * (row, head) pairs come by, 64 at a time, a column of eight by each warp. A token's weights are summed in one order: no atomics. */
-constexpr int kMTiles = 4;
+constexpr int kMTiles = 4, kMMostPairs = 64;      /* of a KV head: more take the kernel of vb_kv4_prompt.cu, heads up to 128 */
 
 template <int NB, class T>
 struct MCfg {
@@ -750,6 +750,7 @@ int attn_launch(const Kv4Attn &args, const vb200_kv4_attention_t &v, const Kv4Wo
         if (launch_pdl(kv4_attn_kernel<NB, PT, T>, dim3((unsigned)(a.split ? at_once : units)), dim3(kAThreads), Cfg::kBig, st, a, q, out) != cudaSuccess)
             return serve_launched() | -1;
     }
+    if (a.mass_out && NB <= 4 && pairs > kMMostPairs) return kv4_mass_many(a, q, st);
     if (a.mass_out) {
         /* the more tiles a warp has, the fewer CTAs make the queries: as many as leave every SM one */
         const long long heads = (long long)a.c.kv_heads * a.c.seqs, tiles = ((long long)a.c.capacity + kAKeys - 1) / kAKeys;

@@ -23,7 +23,7 @@ namespace vb {
 
 namespace {
 
-constexpr int kPRows = 128, kPKeys = 128, kPSoft = 512, kPThreads = 768, kPMmaWarp = 23, kPBlock = kPKeys * 128, kPStatus = 62, kPRing = 8;
+constexpr int kPRows = 128, kPKeys = 128, kPSoft = 512, kPMmaWarp = 23, kPThreads = 32 * (kPMmaWarp + 1), kPBlock = kPKeys * 128, kPStatus = 62, kPRing = 8;
 constexpr int kPLeast = 2, kPTailParts = 8;   /* tiles of a part at least; parts of a unit of the last round at most */
 constexpr uint32_t kPTmem = 512, kPO = 256;
 template <int NB, int QT>
@@ -583,6 +583,250 @@ __global__ void __launch_bounds__(kJThreads) kv4_join_kernel(const Kv4Attn a, co
     }
 }
 
+/* ------------------------------------------------------------------ the weight of each token, for many rows
+ *   S^T [128 tokens x 128 pairs] = K Q^T,  mass_j = sum over pairs of exp(S_j - lse), a thread per token
+ * A CTA has 128 tokens of a KV head, whose keys stay in shared memory; the pairs that see them come by 128 at a time: eight warps bring
+ * queries to FP16, one issues the products, two warpgroups take alternate tiles of pairs. A token's weights are summed in one order.
+ * 1024 rows of 32 heads over 4096 tokens: 840 us on warp-level MMAs (vb_kv4_attn.cu), whose keys are decoded again for every eight pairs. */
+constexpr int kWMmaWarp = 16, kWThreads = 32 * (kWMmaWarp + 1), kWSlots = 2, kWStatus = 63, kWRing = 4;
+constexpr uint32_t kWTmem = 256;
+
+template <int NB, int QT>
+struct WCfg {
+    static constexpr int kSlot = (NB + 1) / 2 * kPBlock;
+    static constexpr int kSmem = kSlot + kWSlots * QT * kSlot + 1024;
+};
+
+template <int NB, class T>
+__global__ void __launch_bounds__(kWThreads, 1) kv4_mass_many_kernel(const Kv4Attn a, const ServeRows<T> q) {
+    constexpr int QT = sizeof(T) == 4 ? 2 : 1;
+    using Cfg = WCfg<NB, QT>;
+    extern __shared__ unsigned char p_smem_raw[];
+    unsigned char *base = (unsigned char *)(((uintptr_t)p_smem_raw + 1023) & ~(uintptr_t)1023);
+    unsigned char *k_s = base, *q_s = k_s + Cfg::kSlot;
+    __shared__ __align__(8) uint64_t q_full[kWSlots], q_empty[kWSlots], s_full[2], s_empty[2], k_full;
+    __shared__ __align__(16) float2 pair_s[kWRing][kPRows];                 /* of a pair: what S is multiplied by, its lse in powers of two */
+    __shared__ float sum_s[kPKeys];
+    __shared__ int abort_s;
+    __shared__ uint32_t tmem_slot;
+    int *abort_flag = &abort_s;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kv_head = blockIdx.y, seq = blockIdx.z, tok0 = blockIdx.x * kPKeys;
+    /* begins beside the end of the attention's kernels, which have waited for all that is read here but lse; masses may not be written
+     * before those are waited for either */
+    const Kv4Span span = kv4_span(a.lengths, a.rows, a.max_rows, seq, a.c.capacity);
+    const int pairs = span.rows * a.group, before = span.length - span.rows;
+    if (tok0 >= span.length) {
+        pdl_wait();                /* no launch is over before the ones it follows are */
+        return;
+    }
+    /* rows before this CTA's first token see none of its tokens */
+    const int first = (int)min((long long)pairs, (long long)max(0, tok0 - before) * a.group) / kPRows * kPRows, n_tiles = (pairs - first + kPRows - 1) / kPRows;
+    if (tid == 0) {
+        for (int i = 0; i < kWSlots; i++) {
+            vb_mbar_init(&q_full[i], 8);
+            vb_mbar_init(&q_empty[i], 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            vb_mbar_init(&s_full[i], 1);
+            vb_mbar_init(&s_empty[i], 128);
+        }
+        vb_mbar_init(&k_full, 8);
+        abort_s = 0;
+        vb_mbar_init_fence();
+    }
+    if (warp == kWMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(vb_smem_u32(&tmem_slot)), "r"(kWTmem) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *(volatile uint32_t *)&tmem_slot;
+    auto give_up = [&]() {
+        atomicCAS(a.status, 0, kWStatus);
+        *(volatile int *)abort_flag = 1;
+    };
+
+    if (warp < 8) {
+        /* ---- keys: a warp has 16 tokens, four lanes a token; a token's scales against the largest of its 16 ---- */
+        const int g = lane >> 2, tq = lane & 3;
+        const size_t row0 = a.c.row(seq, kv_head, 0);
+        __shared__ float key_up[8];
+        uint32_t words[2][NB], bytes[2][NB];
+        int most = 0;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int j = tok0 + warp * 16 + i * 8 + g;
+            const size_t row = row0 + min(j, a.c.slots - 1);
+            get_words<NB>(a.c.k + row * (NB * 16) + tq * (NB * 4), words[i]);
+            get_bytes<NB>(a.c.ks + row * NB, bytes[i]);
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                if (j >= span.length) { words[i][b] = 0; bytes[i][b] = 0; }
+                if (bytes[i][b] != 255u) most = max(most, (int)bytes[i][b]);
+            }
+        }
+        most = max((int)__reduce_max_sync(0xffffffffu, (unsigned)most), 14);              /* its undoing stays a normal number */
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                uint4 v = p_halves(words[i][b], p_factor((int)bytes[i][b], most));
+                if (bytes[i][b] == 255u) v.x = 0x7fff7fffu;                /* a block that is NaN: so is the score */
+                const int chunk = 4 * b + tq;
+                *reinterpret_cast<uint4 *>(k_s + (chunk >> 3) * kPBlock + at_off(warp * 16 + i * 8 + g, chunk & 7)) = v;
+            }
+        if (lane == 0) key_up[warp] = __uint_as_float((uint32_t)(most - 13) << 23);
+        at_proxy_fence();
+        __syncwarp();
+        if (lane == 0) vb_mbar_arrive(&k_full);
+        vb_named_bar(1, 256);
+
+        /* ---- sums: warpgroup w takes tiles w, w + 2, ... of pairs, a thread token tok0 + r ---- */
+        const int w = warp >> 2, r = tid & 127, j = tok0 + r;
+        const uint32_t tS = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(w * kPRows);
+        const float up = key_up[r >> 4];
+        const uint64_t up2 = vb_f2_pack(up, up);
+        uint64_t sums[2] = {0, 0};
+        int it = 0;
+        for (int t = w; t < n_tiles; t += 2, it++) {
+            const int pair0 = first + t * kPRows;
+            /* columns from this one on see the token; all of the warp's see all, and are pairs, or not */
+            const long long from = (long long)(j - before) * a.group - pair0;
+            const int c0 = (int)max(0ll, min((long long)kPRows, from)), c1 = min(kPRows, pairs - pair0);
+            const bool masked = __any_sync(0xffffffffu, c0 > 0) || c1 < kPRows;
+            if (!at_warp_wait(&s_full[w], (uint32_t)it & 1u, abort_flag)) { give_up(); break; }
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < 4; c++) {
+                uint32_t s[32];
+                at_ld32(tS + (uint32_t)(c * 32), s);
+                const float4 *of = reinterpret_cast<const float4 *>(&pair_s[t % kWRing][c * 32]);
+#pragma unroll
+                for (int k = 0; k < 32; k += 2) {
+                    const float4 p = of[k / 2];
+                    const float2 x = vb_f2_get(vb_f2_fma(vb_f2_mul(vb_f2_pack(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), up2), vb_f2_pack(p.x, p.z), vb_f2_pack(-p.y, -p.w)));
+                    float e0 = exp2_fast(x.x), e1 = exp2_fast(x.y);
+                    if (masked) {
+                        if (c * 32 + k < c0 || c * 32 + k >= c1) e0 = 0.0f;
+                        if (c * 32 + k + 1 < c0 || c * 32 + k + 1 >= c1) e1 = 0.0f;
+                    }
+                    sums[(k >> 1) & 1] = vb_f2_add(sums[(k >> 1) & 1], vb_f2_pack(e0, e1));
+                }
+            }
+            tc_fence_before();
+            vb_mbar_arrive(&s_empty[w]);
+        }
+        const float2 both = vb_f2_get(vb_f2_add(sums[0], sums[1]));
+        const float sum = both.x + both.y;
+        if (w == 1) sum_s[r] = sum;
+        vb_named_bar(1, 256);
+        if (w == 0 && j < span.length) {
+            pdl_wait();
+            const size_t at = ((size_t)seq * a.c.kv_heads + kv_head) * a.c.capacity + j;
+            a.mass_out[at] = sum + sum_s[r] + (a.mass_in && j < before ? a.mass_in[at] : 0.0f);
+        }
+    } else if (warp < kWMmaWarp) {
+        /* ---- queries: a warp has 16 pairs of a tile, NB * 8 lanes a pair, as in the attention ---- */
+        constexpr int kLanes = NB * 8, kSide = 32 / kLanes, kBatch = 16 / kSide < 8 ? 16 / kSide : 8;
+        const int lw = warp - 8, side = lane / kLanes, d = (lane - side * kLanes) * 4;
+        const bool mine = side < kSide;
+        pdl_wait();                                                        /* lse */
+        for (int t = 0; t < n_tiles; t++) {
+            const int slot = t % kWSlots;
+            bool waited = false;
+#pragma unroll 1
+            for (int b0 = 0; b0 < 16 / kSide; b0 += kBatch) {
+                float x[kBatch][4], lse[kBatch];
+#pragma unroll
+                for (int u = 0; u < kBatch; u++) {
+                    const int pair = first + t * kPRows + lw * 16 + (b0 + u) * kSide + side;
+                    const bool real = mine && pair < pairs;
+                    const int row = real ? pair / a.group : 0, head = kv_head * a.group + (real ? pair - row * a.group : 0);
+                    const T *p = q.data + seq * q.seq + row * q.row + head * q.head + d;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) x[u][i] = 0.0f;
+                    lse[u] = real ? a.lse[((size_t)seq * a.max_rows + row) * a.heads + head] : 0.0f;
+                    if (real) {
+                        if (!a.wide) {
+#pragma unroll
+                            for (int i = 0; i < 4; i++) x[u][i] = serve_get(p + i);
+                        } else if constexpr (sizeof(T) == 4) {
+                            const float4 v = *reinterpret_cast<const float4 *>(p);
+                            x[u][0] = v.x; x[u][1] = v.y; x[u][2] = v.z; x[u][3] = v.w;
+                        } else {
+                            const uint2 v = *reinterpret_cast<const uint2 *>(p);
+                            const float2 lo = serve_pair(v.x, p), hi = serve_pair(v.y, p);
+                            x[u][0] = lo.x; x[u][1] = lo.y; x[u][2] = hi.x; x[u][3] = hi.y;
+                        }
+                    }
+                }
+                if (!waited) {
+                    if (!at_warp_wait(&q_empty[slot], ((uint32_t)(t / kWSlots) & 1u) ^ 1u, abort_flag)) { give_up(); break; }
+                    waited = true;
+                }
+#pragma unroll
+                for (int u = 0; u < kBatch; u++) {
+                    const int r = lw * 16 + (b0 + u) * kSide + side;
+                    uint32_t most = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) most = max(most, __float_as_uint(x[u][i]) & 0x7fffffffu);
+                    if constexpr (kSide == 1) {
+                        most = __reduce_max_sync(0xffffffffu, most);
+                    } else {
+#pragma unroll
+                        for (int o = 1; o < kLanes; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+                    }
+                    const uint32_t e = most >> 23, field = e == 0u || e == 255u ? 127u : min(268u - e, 253u);
+                    const float up = __uint_as_float(field << 23);
+                    if (!mine) continue;
+                    if (d == 0)          /* a row without weights gives none */
+                        pair_s[t % kWRing][r] = make_float2(a.scale * 1.44269504f * __uint_as_float((254u - field) << 23), lse[u] == -INFINITY ? INFINITY : lse[u] * 1.44269504f);
+                    unsigned char *to = q_s + slot * (QT * Cfg::kSlot) + (d >> 6) * kPBlock + at_off(r, (d & 63) >> 3) + (d & 7) * 2;
+                    const float y0 = x[u][0] * up, y1 = x[u][1] * up, y2 = x[u][2] * up, y3 = x[u][3] * up;
+                    const uint2 hi = make_uint2(half_pack(y0, y1), half_pack(y2, y3));
+                    *reinterpret_cast<uint2 *>(to) = hi;
+                    if constexpr (QT == 2) {
+                        const float2 f = kv4_f2(hi.x), g = kv4_f2(hi.y);
+                        *reinterpret_cast<uint2 *>(to + Cfg::kSlot) = make_uint2(half_pack(y0 - f.x, y1 - f.y), half_pack(y2 - g.x, y3 - g.y));
+                    }
+                }
+            }
+            if (!waited) break;
+            at_proxy_fence();
+            __syncwarp();
+            if (lane == 0) vb_mbar_arrive(&q_full[slot]);
+        }
+    } else if (lane == 0) {
+        /* ---- MMA issuer ---- */
+        const uint32_t idesc = p_idesc(kPRows, false);
+        const AtDesc k_desc(umma_desc_k_sw128(k_s)), q_desc(umma_desc_k_sw128(q_s));
+        bool ok = vb_mbar_wait(&k_full, 0u, abort_flag);
+        for (int t = 0; t < n_tiles && ok; t++) {
+            const int slot = t % kWSlots, w = t & 1;
+            ok = vb_mbar_wait(&q_full[slot], (uint32_t)(t / kWSlots) & 1u, abort_flag) && vb_mbar_wait(&s_empty[w], ((uint32_t)(t >> 1) & 1u) ^ 1u, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            const AtDesc qd = q_desc.at(slot * (QT * Cfg::kSlot >> 4));
+#pragma unroll
+            for (int ks = 0; ks < NB * 2; ks++) {
+                const int at = (ks >> 2) * (kPBlock >> 4) + 2 * (ks & 3);
+#pragma unroll
+                for (int u = 0; u < QT; u++) at_mma_ss(tmem + (uint32_t)(w * kPRows), k_desc.at(at), qd.at(at + u * (Cfg::kSlot >> 4)), idesc, ks + u != 0 ? 1u : 0u);
+            }
+            umma_commit(&q_empty[slot]);
+            umma_commit(&s_full[w]);
+        }
+        if (!ok) give_up();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kWMmaWarp) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kWTmem) : "memory");
+    }
+}
+
 template <int NB, class T>
 int prompt_launch(Kv4Attn a, const ServeRows<T> &q, const ServeRows<T> &out, int sm_count, cudaStream_t st) {
     const long long row_tiles = ((long long)a.max_rows * a.group + kPRows - 1) / kPRows, units = row_tiles * a.c.kv_heads * a.c.seqs;
@@ -602,9 +846,16 @@ int prompt_launch(Kv4Attn a, const ServeRows<T> &q, const ServeRows<T> &out, int
     return 0;
 }
 template <int NB, class T>
+int mass_many_launch(const Kv4Attn &a, const ServeRows<T> &q, cudaStream_t st) {
+    const dim3 grid((unsigned)(((long long)a.c.capacity + kPKeys - 1) / kPKeys), a.c.kv_heads, a.c.seqs);
+    const size_t smem = WCfg<NB, sizeof(T) == 4 ? 2 : 1>::kSmem;
+    return launch_pdl(kv4_mass_many_kernel<NB, T>, grid, dim3(kWThreads), smem, st, a, q) == cudaSuccess ? 0 : serve_launched() | -1;
+}
+template <int NB, class T>
 bool prompt_load() {
     cudaFuncAttributes f;
     if (cudaFuncGetAttributes(&f, kv4_join_kernel<NB, T>) != cudaSuccess) return false;
+    if (cudaFuncSetAttribute(kv4_mass_many_kernel<NB, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, WCfg<NB, sizeof(T) == 4 ? 2 : 1>::kSmem) != cudaSuccess) return false;
     return cudaFuncSetAttribute(kv4_prompt_kernel<NB, kWeightTerms<T>, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, PCfg<NB, sizeof(T) == 4 ? 2 : 1>::kSmem) == cudaSuccess;
 }
 
@@ -619,6 +870,18 @@ int kv4_prompt(const Kv4Attn &a, const ServeRows<T> &q, const ServeRows<T> &out,
     default: return prompt_launch<4, T>(a, q, out, sm_count, st);
     }
 }
+template <class T>
+int kv4_mass_many(const Kv4Attn &a, const ServeRows<T> &q, cudaStream_t st) {
+    switch (a.c.blocks) {
+    case 1: return mass_many_launch<1, T>(a, q, st);
+    case 2: return mass_many_launch<2, T>(a, q, st);
+    case 3: return mass_many_launch<3, T>(a, q, st);
+    default: return mass_many_launch<4, T>(a, q, st);
+    }
+}
+template int kv4_mass_many<float>(const Kv4Attn &, const ServeRows<float> &, cudaStream_t);
+template int kv4_mass_many<__nv_bfloat16>(const Kv4Attn &, const ServeRows<__nv_bfloat16> &, cudaStream_t);
+template int kv4_mass_many<__half>(const Kv4Attn &, const ServeRows<__half> &, cudaStream_t);
 template int kv4_prompt<float>(const Kv4Attn &, const ServeRows<float> &, const ServeRows<float> &, int, cudaStream_t);
 template int kv4_prompt<__nv_bfloat16>(const Kv4Attn &, const ServeRows<__nv_bfloat16> &, const ServeRows<__nv_bfloat16> &, int, cudaStream_t);
 template int kv4_prompt<__half>(const Kv4Attn &, const ServeRows<__half> &, const ServeRows<__half> &, int, cudaStream_t);
