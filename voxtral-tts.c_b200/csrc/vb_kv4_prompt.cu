@@ -728,71 +728,74 @@ __global__ void __launch_bounds__(kWThreads, 1) kv4_mass_many_kernel(const Kv4At
         }
     } else if (warp < kWMmaWarp) {
         /* ---- queries: a warp has 16 pairs of a tile, NB * 8 lanes a pair, as in the attention ---- */
-        constexpr int kLanes = NB * 8, kSide = 32 / kLanes, kBatch = 16 / kSide < 8 ? 16 / kSide : 8;
+        constexpr int kLanes = NB * 8, kSide = 32 / kLanes, kBatch = 16 / kSide;
         const int lw = warp - 8, side = lane / kLanes, d = (lane - side * kLanes) * 4;
         const bool mine = side < kSide;
         pdl_wait();                                                        /* lse */
         for (int t = 0; t < n_tiles; t++) {
-            const int slot = t % kWSlots;
-            bool waited = false;
-#pragma unroll 1
-            for (int b0 = 0; b0 < 16 / kSide; b0 += kBatch) {
-                float x[kBatch][4], lse[kBatch];
+            const int slot = t % kWSlots, p0 = first + t * kPRows + lw * 16;
+            float x[kBatch][4], lse = 0.0f;
+            /* a place on from pair to pair: a division for each took longer than the rest */
+            int in_row = (p0 + side) / a.group;
+            const T *p = q.data + seq * q.seq + in_row * q.row + kv_head * a.group * q.head + d;
+            in_row = p0 + side - in_row * a.group;
+            p += in_row * q.head;
 #pragma unroll
-                for (int u = 0; u < kBatch; u++) {
-                    const int pair = first + t * kPRows + lw * 16 + (b0 + u) * kSide + side;
-                    const bool real = mine && pair < pairs;
-                    const int row = real ? pair / a.group : 0, head = kv_head * a.group + (real ? pair - row * a.group : 0);
-                    const T *p = q.data + seq * q.seq + row * q.row + head * q.head + d;
+            for (int u = 0; u < kBatch; u++) {
+                const bool real = mine && p0 + u * kSide + side < pairs;
 #pragma unroll
-                    for (int i = 0; i < 4; i++) x[u][i] = 0.0f;
-                    lse[u] = real ? a.lse[((size_t)seq * a.max_rows + row) * a.heads + head] : 0.0f;
-                    if (real) {
-                        if (!a.wide) {
+                for (int i = 0; i < 4; i++) x[u][i] = 0.0f;
+                if (real) {
+                    if (!a.wide) {
 #pragma unroll
-                            for (int i = 0; i < 4; i++) x[u][i] = serve_get(p + i);
-                        } else if constexpr (sizeof(T) == 4) {
-                            const float4 v = *reinterpret_cast<const float4 *>(p);
-                            x[u][0] = v.x; x[u][1] = v.y; x[u][2] = v.z; x[u][3] = v.w;
-                        } else {
-                            const uint2 v = *reinterpret_cast<const uint2 *>(p);
-                            const float2 lo = serve_pair(v.x, p), hi = serve_pair(v.y, p);
-                            x[u][0] = lo.x; x[u][1] = lo.y; x[u][2] = hi.x; x[u][3] = hi.y;
-                        }
-                    }
-                }
-                if (!waited) {
-                    if (!at_warp_wait(&q_empty[slot], ((uint32_t)(t / kWSlots) & 1u) ^ 1u, abort_flag)) { give_up(); break; }
-                    waited = true;
-                }
-#pragma unroll
-                for (int u = 0; u < kBatch; u++) {
-                    const int r = lw * 16 + (b0 + u) * kSide + side;
-                    uint32_t most = 0;
-#pragma unroll
-                    for (int i = 0; i < 4; i++) most = max(most, __float_as_uint(x[u][i]) & 0x7fffffffu);
-                    if constexpr (kSide == 1) {
-                        most = __reduce_max_sync(0xffffffffu, most);
+                        for (int i = 0; i < 4; i++) x[u][i] = serve_get(p + i);
+                    } else if constexpr (sizeof(T) == 4) {
+                        const float4 v = *reinterpret_cast<const float4 *>(p);
+                        x[u][0] = v.x; x[u][1] = v.y; x[u][2] = v.z; x[u][3] = v.w;
                     } else {
-#pragma unroll
-                        for (int o = 1; o < kLanes; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+                        const uint2 v = *reinterpret_cast<const uint2 *>(p);
+                        const float2 lo = serve_pair(v.x, p), hi = serve_pair(v.y, p);
+                        x[u][0] = lo.x; x[u][1] = lo.y; x[u][2] = hi.x; x[u][3] = hi.y;
                     }
-                    const uint32_t e = most >> 23, field = e == 0u || e == 255u ? 127u : min(268u - e, 253u);
-                    const float up = __uint_as_float(field << 23);
-                    if (!mine) continue;
-                    if (d == 0)          /* a row without weights gives none */
-                        pair_s[t % kWRing][r] = make_float2(a.scale * 1.44269504f * __uint_as_float((254u - field) << 23), lse[u] == -INFINITY ? INFINITY : lse[u] * 1.44269504f);
-                    unsigned char *to = q_s + slot * (QT * Cfg::kSlot) + (d >> 6) * kPBlock + at_off(r, (d & 63) >> 3) + (d & 7) * 2;
-                    const float y0 = x[u][0] * up, y1 = x[u][1] * up, y2 = x[u][2] * up, y3 = x[u][3] * up;
-                    const uint2 hi = make_uint2(half_pack(y0, y1), half_pack(y2, y3));
-                    *reinterpret_cast<uint2 *>(to) = hi;
-                    if constexpr (QT == 2) {
-                        const float2 f = kv4_f2(hi.x), g = kv4_f2(hi.y);
-                        *reinterpret_cast<uint2 *>(to + Cfg::kSlot) = make_uint2(half_pack(y0 - f.x, y1 - f.y), half_pack(y2 - g.x, y3 - g.y));
-                    }
+                }
+                in_row += kSide;
+                p += kSide * q.head;
+                while (in_row >= a.group) {
+                    in_row -= a.group;
+                    p += q.row - a.group * q.head;
                 }
             }
-            if (!waited) break;
+            if (lane < 16 && p0 + lane < pairs) {
+                const int row = (p0 + lane) / a.group;
+                lse = a.lse[((size_t)seq * a.max_rows + row) * a.heads + kv_head * a.group + p0 + lane - row * a.group];
+            }
+            if (!at_warp_wait(&q_empty[slot], ((uint32_t)(t / kWSlots) & 1u) ^ 1u, abort_flag)) { give_up(); break; }
+            if (lane < 16) pair_s[t % kWRing][lw * 16 + lane].y = lse == -INFINITY ? INFINITY : lse * 1.44269504f;       /* a row without weights gives none */
+#pragma unroll
+            for (int u = 0; u < kBatch; u++) {
+                const int r = lw * 16 + u * kSide + side;
+                uint32_t most = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) most = max(most, __float_as_uint(x[u][i]) & 0x7fffffffu);
+                if constexpr (kSide == 1) {
+                    most = __reduce_max_sync(0xffffffffu, most);
+                } else {
+#pragma unroll
+                    for (int o = 1; o < kLanes; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+                }
+                const uint32_t e = most >> 23, field = e == 0u || e == 255u ? 127u : min(268u - e, 253u);
+                const float up = __uint_as_float(field << 23);
+                if (!mine) continue;
+                if (d == 0) pair_s[t % kWRing][r].x = a.scale * 1.44269504f * __uint_as_float((254u - field) << 23);
+                unsigned char *to = q_s + slot * (QT * Cfg::kSlot) + (d >> 6) * kPBlock + at_off(r, (d & 63) >> 3) + (d & 7) * 2;
+                const float y0 = x[u][0] * up, y1 = x[u][1] * up, y2 = x[u][2] * up, y3 = x[u][3] * up;
+                const uint2 hi = make_uint2(half_pack(y0, y1), half_pack(y2, y3));
+                *reinterpret_cast<uint2 *>(to) = hi;
+                if constexpr (QT == 2) {
+                    const float2 f = kv4_f2(hi.x), g = kv4_f2(hi.y);
+                    *reinterpret_cast<uint2 *>(to + Cfg::kSlot) = make_uint2(half_pack(y0 - f.x, y1 - f.y), half_pack(y2 - g.x, y3 - g.y));
+                }
+            }
             at_proxy_fence();
             __syncwarp();
             if (lane == 0) vb_mbar_arrive(&q_full[slot]);
