@@ -192,7 +192,7 @@ def test_a_few_rows(pkg, heads, kv_heads, dim, rows, lengths, dtype):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("heads,kv_heads,dim,rows,length", [(8, 2, 128, 150, 150), (8, 8, 64, 65, 400), (4, 2, 96, 130, 190), (6, 2, 192, 70, 333), (2, 1, 256, 90, 100),
-                                                          (16, 1, 32, 64, 77), (5, 1, 128, 257, 1025), (32, 32, 64, 129, 200), (4, 2, 128, 100, 1500), (4, 4, 96, 66, 900), (32, 32, 32, 129, 2100)])
+                                                          (16, 1, 32, 64, 77), (5, 1, 128, 257, 1025), (32, 32, 64, 129, 200), (4, 2, 128, 100, 1500), (4, 4, 96, 66, 900), (32, 32, 32, 129, 2100), (27, 27, 32, 129, 2100)])
 def test_portions_of_a_prompt(pkg, heads, kv_heads, dim, rows, length, dtype):
     g = _gen(rows * dim)
     t = TYPES[dtype]

@@ -79,7 +79,7 @@ VB_DEVINL void get_values(const uint8_t *p, uint32_t (&w)[(NB + 1) / 2]) {
 template <int NB, class T>
 struct QueryColumn {
     static constexpr int kGroups = NB * 8, kEach = (kGroups + 31) / 32;
-    float x[kEach][4];
+    ServeRaw4<T> raw[kEach];
     VB_DEVINL void load(const ServeRows<T> &q, const Kv4Attn &a, int seq, int kv_head, int pair, int pairs) {
         const int lane = threadIdx.x & 31;
         const bool real = pair < pairs;
@@ -88,20 +88,8 @@ struct QueryColumn {
 #pragma unroll
         for (int i = 0; i < kEach; i++) {
             const int at = lane + 32 * i;
-#pragma unroll
-            for (int j = 0; j < 4; j++) x[i][j] = 0.0f;
-            if (!real || at >= kGroups) continue;
-            if (!a.wide) {
-#pragma unroll
-                for (int j = 0; j < 4; j++) x[i][j] = serve_get(p + at * 4 + j);
-            } else if constexpr (sizeof(T) == 4) {
-                const float4 v = reinterpret_cast<const float4 *>(p)[at];
-                x[i][0] = v.x; x[i][1] = v.y; x[i][2] = v.z; x[i][3] = v.w;
-            } else {
-                const uint2 v = reinterpret_cast<const uint2 *>(p)[at];
-                const float2 lo = serve_pair(v.x, p), hi = serve_pair(v.y, p);
-                x[i][0] = lo.x; x[i][1] = lo.y; x[i][2] = hi.x; x[i][3] = hi.y;
-            }
+            raw[i].none();
+            if (real && at < kGroups) raw[i].load(p + at * 4, a.wide);
         }
     }
     template <int QT>
@@ -109,9 +97,11 @@ struct QueryColumn {
         const int lane = threadIdx.x & 31;
         uint32_t most = 0;
 #pragma unroll
-        for (int i = 0; i < kEach; i++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) most = max(most, __float_as_uint(x[i][j]) & 0x7fffffffu);
+        for (int i = 0; i < kEach; i++) {
+            const float4 x = raw[i].get();
+            most = max(max(most, __float_as_uint(x.x) & 0x7fffffffu), __float_as_uint(x.y) & 0x7fffffffu);
+            most = max(max(most, __float_as_uint(x.z) & 0x7fffffffu), __float_as_uint(x.w) & 0x7fffffffu);
+        }
         most = __reduce_max_sync(0xffffffffu, most);
         /* the largest to [2^14, 2^15); rows of zeros, or with a value that is not finite, as they are */
         const uint32_t e = most >> 23, field = e == 0u || e == 255u ? 127u : min(268u - e, 253u);
@@ -124,9 +114,8 @@ struct QueryColumn {
             const int at = lane + 32 * i;                             /* 8 blocks + 2 t + half */
             if (at >= kGroups) continue;
             uint2 *to = q_s + (((at >> 3) * 2 + (at & 1)) * QT) * 32 + n * 4 + ((at >> 1) & 3);
-            float y[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) y[j] = x[i][j] * up;
+            const float4 x = raw[i].get();
+            const float y[4] = {x.x * up, x.y * up, x.z * up, x.w * up};
             const uint2 w = make_uint2(half_pack(y[0], y[1]), half_pack(y[2], y[3]));
             to[0] = w;
             if constexpr (QT == 2) {

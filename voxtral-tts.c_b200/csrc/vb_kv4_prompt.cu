@@ -165,35 +165,21 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
         constexpr int kLanes = NB * 8, kSide = 32 / kLanes, kBatch = 8 / kSide;
         const int side = lane / kLanes, d = (lane - side * kLanes) * 4;
         const bool mine = side < kSide;
-        float x[kBatch][4];
+        ServeRaw4<T> raw[kBatch];
 #pragma unroll
         for (int u = 0; u < kBatch; u++) {
             const int pair = pair0 + warp * 8 + u * kSide + side;
             const bool real = mine && pair < pairs;
             const int row = real ? pair / a.group : 0, head = kv_head * a.group + (real ? pair - row * a.group : 0);
             const T *p = q.data + seq * q.seq + row * q.row + head * q.head + d;
-#pragma unroll
-            for (int i = 0; i < 4; i++) x[u][i] = 0.0f;
-            if (real) {
-                if (!a.wide) {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) x[u][i] = serve_get(p + i);
-                } else if constexpr (sizeof(T) == 4) {
-                    const float4 v = *reinterpret_cast<const float4 *>(p);
-                    x[u][0] = v.x; x[u][1] = v.y; x[u][2] = v.z; x[u][3] = v.w;
-                } else {
-                    const uint2 v = *reinterpret_cast<const uint2 *>(p);
-                    const float2 lo = serve_pair(v.x, p), hi = serve_pair(v.y, p);
-                    x[u][0] = lo.x; x[u][1] = lo.y; x[u][2] = hi.x; x[u][3] = hi.y;
-                }
-            }
+            raw[u].none();
+            if (real) raw[u].load(p, a.wide);
         }
 #pragma unroll
         for (int u = 0; u < kBatch; u++) {
             const int r = warp * 8 + u * kSide + side;
-            uint32_t most = 0;
-#pragma unroll
-            for (int i = 0; i < 4; i++) most = max(most, __float_as_uint(x[u][i]) & 0x7fffffffu);
+            const float4 x = raw[u].get();
+            uint32_t most = max(max(__float_as_uint(x.x) & 0x7fffffffu, __float_as_uint(x.y) & 0x7fffffffu), max(__float_as_uint(x.z) & 0x7fffffffu, __float_as_uint(x.w) & 0x7fffffffu));
             if constexpr (kSide == 1) {
                 most = __reduce_max_sync(0xffffffffu, most);
             } else {
@@ -206,7 +192,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
             if (a.scale <= 0.0f) up = a.scale < 0.0f ? -up : 0.0f;      /* the largest score is the largest product */
             if (mine) {
                 const uint32_t at = (uint32_t)(d >> 6) * kPBlock + at_off(r, (d & 63) >> 3) + (d & 7) * 2;
-                const float y0 = x[u][0] * up, y1 = x[u][1] * up, y2 = x[u][2] * up, y3 = x[u][3] * up;
+                const float y0 = x.x * up, y1 = x.y * up, y2 = x.z * up, y3 = x.w * up;
                 const uint2 hi = make_uint2(half_pack(y0, y1), half_pack(y2, y3));
                 *reinterpret_cast<uint2 *>(q_s + at) = hi;
                 if constexpr (QT == 2) {
@@ -734,7 +720,8 @@ __global__ void __launch_bounds__(kWThreads, 1) kv4_mass_many_kernel(const Kv4At
         pdl_wait();                                                        /* lse */
         for (int t = 0; t < n_tiles; t++) {
             const int slot = t % kWSlots, p0 = first + t * kPRows + lw * 16;
-            float x[kBatch][4], lse = 0.0f;
+            ServeRaw4<T> raw[kBatch];
+            float lse = 0.0f;
             /* a place on from pair to pair: a division for each took longer than the rest */
             int in_row = (p0 + side) / a.group;
             const T *p = q.data + seq * q.seq + in_row * q.row + kv_head * a.group * q.head + d;
@@ -743,21 +730,8 @@ __global__ void __launch_bounds__(kWThreads, 1) kv4_mass_many_kernel(const Kv4At
 #pragma unroll
             for (int u = 0; u < kBatch; u++) {
                 const bool real = mine && p0 + u * kSide + side < pairs;
-#pragma unroll
-                for (int i = 0; i < 4; i++) x[u][i] = 0.0f;
-                if (real) {
-                    if (!a.wide) {
-#pragma unroll
-                        for (int i = 0; i < 4; i++) x[u][i] = serve_get(p + i);
-                    } else if constexpr (sizeof(T) == 4) {
-                        const float4 v = *reinterpret_cast<const float4 *>(p);
-                        x[u][0] = v.x; x[u][1] = v.y; x[u][2] = v.z; x[u][3] = v.w;
-                    } else {
-                        const uint2 v = *reinterpret_cast<const uint2 *>(p);
-                        const float2 lo = serve_pair(v.x, p), hi = serve_pair(v.y, p);
-                        x[u][0] = lo.x; x[u][1] = lo.y; x[u][2] = hi.x; x[u][3] = hi.y;
-                    }
-                }
+                raw[u].none();
+                if (real) raw[u].load(p, a.wide);
                 in_row += kSide;
                 p += kSide * q.head;
                 while (in_row >= a.group) {
@@ -774,9 +748,8 @@ __global__ void __launch_bounds__(kWThreads, 1) kv4_mass_many_kernel(const Kv4At
 #pragma unroll
             for (int u = 0; u < kBatch; u++) {
                 const int r = lw * 16 + u * kSide + side;
-                uint32_t most = 0;
-#pragma unroll
-                for (int i = 0; i < 4; i++) most = max(most, __float_as_uint(x[u][i]) & 0x7fffffffu);
+                const float4 x = raw[u].get();
+                uint32_t most = max(max(__float_as_uint(x.x) & 0x7fffffffu, __float_as_uint(x.y) & 0x7fffffffu), max(__float_as_uint(x.z) & 0x7fffffffu, __float_as_uint(x.w) & 0x7fffffffu));
                 if constexpr (kSide == 1) {
                     most = __reduce_max_sync(0xffffffffu, most);
                 } else {
@@ -788,7 +761,7 @@ __global__ void __launch_bounds__(kWThreads, 1) kv4_mass_many_kernel(const Kv4At
                 if (!mine) continue;
                 if (d == 0) pair_s[t % kWRing][r].x = a.scale * 1.44269504f * __uint_as_float((254u - field) << 23);
                 unsigned char *to = q_s + slot * (QT * Cfg::kSlot) + (d >> 6) * kPBlock + at_off(r, (d & 63) >> 3) + (d & 7) * 2;
-                const float y0 = x[u][0] * up, y1 = x[u][1] * up, y2 = x[u][2] * up, y3 = x[u][3] * up;
+                const float y0 = x.x * up, y1 = x.y * up, y2 = x.z * up, y3 = x.w * up;
                 const uint2 hi = make_uint2(half_pack(y0, y1), half_pack(y2, y3));
                 *reinterpret_cast<uint2 *>(to) = hi;
                 if constexpr (QT == 2) {
@@ -836,9 +809,10 @@ int prompt_launch(Kv4Attn a, const ServeRows<T> &q, const ServeRows<T> &out, int
     if (units > INT_MAX) return serve_fail("too many rows");
     a.row_tiles = (int)row_tiles;
     a.split = units < sm_count && a.c.capacity > kPLeast * kPKeys;
-    /* a part of at least four tiles: beginning and ending take as long as five */
-    const int rest = (int)(units % sm_count), most = std::min(kPTailParts, a.c.capacity / (4 * kPKeys));
-    a.tail_parts = !a.split && units > sm_count && rest > 0 ? std::min(sm_count / rest, most) : 1;
+    /* The units beyond the last whole round are cut where they are few and long: a part takes as long to begin and to end as five tiles, and
+     * the join 4 us (512 units of eight tiles, 68 of them in the last round, cut in two: 130 us, not 110). */
+    const int rest = (int)(units % sm_count), tiles = (a.c.capacity + kPKeys - 1) / kPKeys;
+    a.tail_parts = !a.split && units > sm_count && rest > 0 && rest <= sm_count / 4 && tiles >= 16 ? std::min({sm_count / rest, kPTailParts, tiles / 4}) : 1;
     a.tail_units = a.tail_parts > 1 ? rest : 1;
     a.tail0 = a.tail_parts > 1 ? (int)units - rest : INT_MAX;
     const unsigned tail = a.tail_parts > 1 ? (unsigned)(rest * a.tail_parts) : 0u;

@@ -168,6 +168,45 @@ VB_DEVINL void serve_store(T *p, bool wide, const float (&x)[N]) {
         for (int i = 0; i < N; i++) serve_put(p + i, x[i]);
     }
 }
+/* Four values side by side as they lie there, and what they are: a load whose result is not looked at yet waits for nothing. `wide`: they
+ * are aligned to their size */
+template <class T>
+struct ServeRaw4 {
+    uint32_t w[sizeof(T)];                                /* 16 bytes, or 8 */
+    VB_DEVINL void none() {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T); i++) w[i] = 0u;
+    }
+    VB_DEVINL void load(const T *p, bool wide) {
+        if constexpr (sizeof(T) == 4) {
+            const uint32_t *u = reinterpret_cast<const uint32_t *>(p);
+            if (wide) {
+                const uint4 v = *reinterpret_cast<const uint4 *>(p);
+                w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++) w[i] = u[i];
+            }
+        } else {
+            const uint16_t *u = reinterpret_cast<const uint16_t *>(p);
+            if (wide) {
+                const uint2 v = *reinterpret_cast<const uint2 *>(p);
+                w[0] = v.x; w[1] = v.y;
+            } else {
+                w[0] = u[0] | (uint32_t)u[1] << 16;
+                w[1] = u[2] | (uint32_t)u[3] << 16;
+            }
+        }
+    }
+    VB_DEVINL float4 get() const {
+        if constexpr (sizeof(T) == 4) {
+            return make_float4(__uint_as_float(w[0]), __uint_as_float(w[1]), __uint_as_float(w[2]), __uint_as_float(w[3]));
+        } else {
+            const float2 a = serve_pair(w[0], (const T *)nullptr), b = serve_pair(w[1], (const T *)nullptr);
+            return make_float4(a.x, a.y, b.x, b.y);
+        }
+    }
+};
 /* Whether every row of heads begins on a 16-byte boundary. */
 template <class T>
 bool serve_wide(const ServeRows<T> &r) {
