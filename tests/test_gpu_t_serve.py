@@ -496,6 +496,105 @@ def test_two_caches_at_once(pkg):
         assert all(torch.equal(x, m[3]) for x in o)
 
 
+# ---------------------------------------------------------------------------------------------- what is refused, and nothing at all
+
+def test_portions_of_no_rows(pkg):
+    s, h, d, n = 2, 2, 64, 40
+    k = _randn(_gen(1), s, n, h, d)
+    cache, at = _fill(pkg, k, k, n, [n, 7])
+    none = torch.empty(s, 0, h, d, device="cuda")
+    cache.append(none, none, at)
+    cache.read(none, none, at)
+    q, lse = torch.empty(s, 0, 4, d, device="cuda"), torch.empty(s, 0, 4, device="cuda")
+    cache.attention(q, q, at)
+    mass_in, mass = torch.rand(s, h, n, device="cuda"), torch.full((s, h, n), -1.0, device="cuda")
+    cache.attention(q, q, at, lse=lse, mass_in=mass_in, mass_out=mass)
+    assert torch.equal(mass[0], mass_in[0]) and torch.equal(mass[1, :, :7], mass_in[1, :, :7]) and (mass[1, :, 7:] == -1.0).all()
+    # rows there are, of which none is real
+    q, lse = torch.randn(s, 3, 4, d, device="cuda"), torch.full((s, 3, 4), 5.0, device="cuda")
+    out = torch.full_like(q, 5.0)
+    cache.attention(q, out, at, rows=_ints(0, 0), lse=lse, mass_in=mass_in, mass_out=mass)
+    assert (out == 5.0).all() and (lse == 5.0).all() and torch.equal(mass[0], mass_in[0])
+    cache.check()
+
+
+def test_calls_that_are_refused(pkg):
+    import ctypes as C
+    import sys
+    serve = sys.modules[pkg.__name__ + ".serve"]
+    L = serve.serve_lib()
+    cache, small = pkg.KV4Cache(2, 2, 64, 32), pkg.KV4Cache(2, 2, 64, 8)
+    k, at, q = torch.zeros(2, 3, 2, 64, device="cuda"), _ints(3, 3), torch.zeros(2, 3, 4, 64, device="cuda")
+    host = torch.zeros(2, 3, 2, 64)
+    p = lambda t: t.data_ptr()  # noqa: E731
+
+    def refused(fn, handles, args, word):
+        assert fn(*handles, C.byref(args), None) == -1
+        assert word in L.vb200_serve_error().decode(), L.vb200_serve_error()
+
+    rows = lambda t, kind=0: serve._Rows(p(t), kind, 384, 128, 64)  # noqa: E731
+    for args, word in ((serve._AppendArgs(None, None, 3, rows(k), rows(k)), "needed"), (serve._AppendArgs(p(at), None, -1, rows(k), rows(k)), "negative"),
+                       (serve._AppendArgs(p(at), None, 3, rows(k), rows(k, 1)), "one type"), (serve._AppendArgs(p(at), None, 3, rows(k, 7), rows(k, 7)), "one type"),
+                       (serve._AppendArgs(p(at), None, 3, rows(host), rows(host)), "does not lie"),
+                       (serve._AppendArgs(p(at), None, 3, serve._Rows(p(k) + 2, 0, 384, 128, 64), rows(k)), "aligned")):
+        refused(L.vb200_kv4_append, (cache.h,), args, word)
+        refused(L.vb200_kv4_read, (cache.h,), args, word)
+    att = dict(lengths=p(at), rows=None, max_rows=3, heads=4, scale=1.0, q=rows(q), out=rows(q), lse=None, mass_in=None, mass_out=None)
+    for change, word in (({"heads": 3}, "multiple"), ({"heads": 0}, "multiple"), ({"q": rows(q, 1)}, "one type"), ({"lengths": None}, "needed"), ({"max_rows": -2}, "negative"),
+                         ({"mass_out": p(k)}, "lse"), ({"mass_in": p(k)}, "without"), ({"scale": math.nan}, "finite"), ({"scale": math.inf}, "finite"),
+                         ({"q": rows(host), "out": rows(host)}, "does not lie"), ({"max_rows": 1 << 30, "heads": 8}, "too many")):
+        refused(L.vb200_kv4_attention, (cache.h,), serve._AttentionArgs(**dict(att, **change)), word)
+    mass, kept = torch.zeros(2, 2, 32, device="cuda"), torch.zeros(2, 2, 8, dtype=torch.int32, device="cuda")
+    ev = dict(lengths=p(at), new_lengths=p(at), mass=p(mass), new_mass=p(mass), new_mass_ld=32, kept=p(kept), keep=8, recent=2, first=1)
+    for change, word in (({"keep": 0}, "keep"), ({"recent": 8}, "together"), ({"first": -1}, "not negative"), ({"new_mass_ld": 7}, "new_mass_ld"), ({"kept": None}, "needed"),
+                         ({"new_mass_ld": 31}, "may be mass")):
+        refused(L.vb200_kv4_evict, (cache.h, cache.h), serve._EvictArgs(**dict(ev, **change)), word)
+    refused(L.vb200_kv4_evict, (cache.h, small.h), serve._EvictArgs(**dict(ev, keep=9)), "more than into")
+    refused(L.vb200_kv4_evict, (cache.h, small.h), serve._EvictArgs(**ev), "may be mass")
+    refused(L.vb200_kv4_evict, (cache.h, pkg.KV4Cache(2, 1, 64, 8).h), serve._EvictArgs(**ev), "other seqs")
+    call = cache.append_call(k, k, at)
+    call()
+    cache.close()
+    with pytest.raises(ValueError, match="closed"):
+        call()
+    x = torch.zeros(2, 5)
+    refused(L.vb200_token_logprobs, (), serve._LogprobsArgs(p(x), 0, 2, 5, 5, p(at), p(k), None, 0, None, None), "do not lie")
+
+
+def test_first_call_of_a_process_inside_a_capture():
+    import os
+    import subprocess
+    import sys
+    code = """
+import sys
+sys.path.insert(0, %r)
+import conftest, torch
+pkg = conftest.load_package()
+cache = pkg.KV4Cache(1, 1, 64, 100)
+k, q = torch.randn(1, 70, 1, 64, device="cuda"), torch.randn(1, 70, 2, 64, device="cuda")
+at, kept = torch.tensor([70], dtype=torch.int32, device="cuda"), torch.empty(1, 1, 20, dtype=torch.int32, device="cuda")
+new = torch.empty_like(at)
+out, lse, mass = torch.empty_like(q), torch.empty(1, 70, 2, device="cuda"), torch.zeros(1, 1, 100, device="cuda")
+x, tok, lp = torch.randn(3, 5000, device="cuda"), torch.tensor([1, 2, 3], dtype=torch.int32, device="cuda"), torch.empty(3, device="cuda")
+graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+with torch.cuda.graph(graph, stream=side):
+    st = torch.cuda.current_stream().cuda_stream
+    pkg.token_logprobs(x, tok, lp, stream=st)
+    cache.append(k, k, at, stream=st)
+    cache.attention(q, out, at, lse=lse, mass_out=mass, stream=st)
+    cache.attention(q[:, :1], out[:, :1], at, stream=st)
+    cache.evict(cache, at, new, mass, mass, kept, keep=20, stream=st)
+graph.replay()
+torch.cuda.synchronize()
+cache.check()
+assert torch.allclose(lp, torch.log_softmax(x, -1)[torch.arange(3), tok.long()], atol=1e-5)
+assert int(new) == 20 and abs(float(lse.exp().isfinite().all()) - 1) == 0
+print("OK")
+""" % os.path.dirname(os.path.abspath(__file__))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "OK" in r.stdout, (r.stdout[-2000:], r.stderr[-3000:])
+
+
 # ---------------------------------------------------------------------------------------------- log probabilities
 
 def _check_logprobs(pkg, x, tokens, top):

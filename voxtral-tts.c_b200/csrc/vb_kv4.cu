@@ -346,13 +346,13 @@ int load(int blocks) {
 
 int check_rows(const vb200_kv4 *h, const vb200_kv4_rows_t *a) {
     if (!h || !a) return serve_fail("no cache or no arguments");
-    if (!a->lengths || !a->k.data || !a->v.data) return serve_fail("lengths, k and v are needed");
     if (a->max_rows < 0) return serve_fail("max_rows is negative");
+    if (!a->lengths || (a->max_rows > 0 && (!a->k.data || !a->v.data))) return serve_fail("lengths, k and v are needed");
     if (a->k.type != a->v.type || a->k.type < VB200_F32 || a->k.type > VB200_F16) return serve_fail("k and v are of one type: fp32, bf16 or fp16");
     if (((uintptr_t)a->k.data | (uintptr_t)a->v.data) % serve_size(a->k.type)) return serve_fail("k and v have to be aligned to their elements");
     int now = -1;
     if (cudaGetDevice(&now) != cudaSuccess || now != h->device) return serve_fail("the cache lies on another device than the current one");
-    if (!serve_on_device(a->k.data)) return serve_fail("k does not lie on the current device");
+    if (a->max_rows > 0 && !serve_on_device(a->k.data)) return serve_fail("k does not lie on the current device");
     return 0;
 }
 
@@ -477,17 +477,17 @@ int vb200_kv4_evict(vb200_kv4_t *h, vb200_kv4_t *into, const vb200_kv4_evict_t *
 
 int vb200_kv4_attention(vb200_kv4_t *h, const vb200_kv4_attention_t *a, void *stream) {
     if (!h || !a) return serve_fail("no cache or no arguments");
-    if (!a->lengths || !a->q.data || !a->out.data) return serve_fail("lengths, q and out are needed");
     if (a->max_rows < 0) return serve_fail("max_rows is negative");
+    if (!a->lengths || (a->max_rows > 0 && (!a->q.data || !a->out.data))) return serve_fail("lengths, q and out are needed");
     if (a->heads < 1 || a->heads % h->c.kv_heads) return serve_fail("heads has to be a multiple of the cache's kv_heads");
     if (a->q.type != a->out.type || a->q.type < VB200_F32 || a->q.type > VB200_F16) return serve_fail("q and out are of one type: fp32, bf16 or fp16");
     if (((uintptr_t)a->q.data | (uintptr_t)a->out.data) % serve_size(a->q.type)) return serve_fail("q and out have to be aligned to their elements");
     if (a->mass_in && !a->mass_out) return serve_fail("mass_in without mass_out");
-    if (a->mass_out && !a->lse) return serve_fail("mass_out needs lse");
+    if (a->mass_out && a->max_rows > 0 && !a->lse) return serve_fail("mass_out needs lse");
     if (!(a->scale > -1e30f && a->scale < 1e30f)) return serve_fail("scale is not a finite number");
     int now = -1;
     if (cudaGetDevice(&now) != cudaSuccess || now != h->device) return serve_fail("the cache lies on another device than the current one");
-    if (!serve_on_device(a->q.data)) return serve_fail("q does not lie on the current device");
+    if (a->max_rows > 0 && !serve_on_device(a->q.data)) return serve_fail("q does not lie on the current device");
     if (a->max_rows == 0 && !a->mass_out) return 0;
     return kv4_attention(h->c, h->w, *a, (cudaStream_t)stream);
 }

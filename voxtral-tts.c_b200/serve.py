@@ -111,7 +111,7 @@ def _dense(a, name, shape, dtype):
         raise ValueError(f"{name} has to be {dtype} of shape {tuple(shape)}: got {_dtype(a)} of shape {tuple(a.shape)}")
     n = 1
     for size, stride in zip(reversed(tuple(a.shape)), reversed(tuple(a.stride()))):
-        if size > 1 and stride != n:
+        if size > 1 and stride != n and 0 not in shape:
             raise ValueError(f"{name} has to be dense")
         n *= size
     return a.data_ptr()
@@ -131,13 +131,16 @@ def _rows(a, name, seqs, rows, heads, head_dim):
 
 class Call:
     """A checked call: call(stream) queues it. It keeps the arrays that it is about."""
-    __slots__ = ("_fn", "_front", "_args", "_lib", "_keep")
+    __slots__ = ("_fn", "_caches", "_args", "_lib", "_keep")
 
-    def __init__(self, L, fn, front, args, keep):
-        self._lib, self._fn, self._front, self._args, self._keep = L, fn, front, C.byref(args), (args, keep)
+    def __init__(self, L, fn, caches, args, keep):
+        self._lib, self._fn, self._caches, self._args, self._keep = L, fn, caches, C.byref(args), (args, keep)
 
     def __call__(self, stream=0):
-        if self._fn(*self._front, self._args, stream) != 0:
+        handles = [c.h for c in self._caches]
+        if None in handles:
+            raise ValueError("the cache is closed")
+        if self._fn(*handles, self._args, stream) != 0:
             raise RuntimeError(self._lib.vb200_serve_error().decode())
 
 
@@ -165,7 +168,6 @@ class KV4Cache:
     def _open(self):
         if not self.h:
             raise ValueError("the cache is closed")
-        return self.h
 
     def _spans(self, lengths, rows, arrays):
         places = {_place(a) for a in arrays if a is not None} - {None}
@@ -174,14 +176,14 @@ class KV4Cache:
         return _dense(lengths, "lengths", (self.seqs,), "int32"), _dense(rows, "rows", (self.seqs,), "int32")
 
     def _move(self, fn, k, v, lengths, rows):
-        h = self._open()
+        self._open()
         if _dtype(k) != _dtype(v):
             raise ValueError("k and v have to be of one type")
         ln, rw = self._spans(lengths, rows, (k, v, lengths, rows))
         n = k.shape[1] if len(k.shape) == 4 else 0
         shape = (self.seqs, n, self.kv_heads, self.head_dim)
         a = _AppendArgs(ln, rw, n, _rows(k, "k", *shape), _rows(v, "v", *shape))
-        return Call(self.L, fn, (h,), a, (self, k, v, lengths, rows))
+        return Call(self.L, fn, (self,), a, (k, v, lengths, rows))
 
     def append_call(self, k, v, lengths, rows=None):
         return self._move(self.L.vb200_kv4_append, k, v, lengths, rows)
@@ -198,7 +200,7 @@ class KV4Cache:
         self.read_call(k, v, lengths, rows)(stream)
 
     def attention_call(self, q, out, lengths, scale=None, rows=None, lse=None, mass_in=None, mass_out=None):
-        h = self._open()
+        self._open()
         if len(q.shape) != 4:
             raise ValueError("q has to be [seqs, rows, heads, head_dim]")
         n, heads = q.shape[1], q.shape[2]
@@ -212,7 +214,7 @@ class KV4Cache:
             raise ValueError("mass_out needs lse")
         a = _AttentionArgs(ln, rw, n, heads, 1.0 / math.sqrt(self.head_dim) if scale is None else scale, _rows(q, "q", *shape), _rows(out, "out", *shape),
                            _dense(lse, "lse", shape[:3], "float32"), _dense(mass_in, "mass_in", mass, "float32"), _dense(mass_out, "mass_out", mass, "float32"))
-        return Call(self.L, self.L.vb200_kv4_attention, (h,), a, (self, q, out, lengths, rows, lse, mass_in, mass_out))
+        return Call(self.L, self.L.vb200_kv4_attention, (self,), a, (q, out, lengths, rows, lse, mass_in, mass_out))
 
     def attention(self, q, out, lengths, scale=None, rows=None, lse=None, mass_in=None, mass_out=None, stream=0):
         """Causal attention of q [seqs, rows, heads, head_dim], the queries of the last tokens, into out. scale: 1 / sqrt(head_dim) where
@@ -220,7 +222,7 @@ class KV4Cache:
         self.attention_call(q, out, lengths, scale, rows, lse, mass_in, mass_out)(stream)
 
     def evict_call(self, into, lengths, new_lengths, mass, new_mass, kept, keep, recent=0, first=0):
-        h = self._open()
+        self._open()
         into._open()
         self._spans(lengths, None, (lengths, new_lengths, mass, new_mass, kept))
         ln, nl = _dense(lengths, "lengths", (self.seqs,), "int32"), _dense(new_lengths, "new_lengths", (self.seqs,), "int32")
@@ -228,7 +230,7 @@ class KV4Cache:
         a = _EvictArgs(ln, nl, _dense(mass, "mass", (self.seqs, self.kv_heads, self.capacity), "float32"),
                        _dense(new_mass, "new_mass", (self.seqs, self.kv_heads, ld), "float32"), ld,
                        _dense(kept, "kept", (self.seqs, self.kv_heads, keep), "int32"), keep, recent, first)
-        return Call(self.L, self.L.vb200_kv4_evict, (h, into.h), a, (self, into, lengths, new_lengths, mass, new_mass, kept))
+        return Call(self.L, self.L.vb200_kv4_evict, (self, into), a, (lengths, new_lengths, mass, new_mass, kept))
 
     def evict(self, into, lengths, new_lengths, mass, new_mass, kept, keep, recent=0, first=0, stream=0):
         """Sequences of more than `keep` tokens are cut to that many, by mass; what stays goes into the first slots of `into` (a
