@@ -406,7 +406,7 @@ vb200_kv4_t *vb200_kv4_open(int seqs, int kv_heads, int head_dim, int capacity) 
     h->w.n_tickets = 2 * n_sm;
     h->w.part_floats = std::max((size_t)2 * n_sm * 8 * (head_dim + 2), kv4_prompt_floats(head_dim / 32, n_sm));
     const size_t rows = (size_t)seqs * kv_heads * c.slots, codes = rows * (size_t)(head_dim / 2), scales = rows * (size_t)c.blocks;
-    const size_t work = h->w.part_floats * sizeof(float), tickets = sizeof(unsigned) * (size_t)(h->w.n_tickets + 1);
+    const size_t aside = kv4_aside_floats(c.blocks, n_sm), work = (h->w.part_floats + aside) * sizeof(float), tickets = sizeof(unsigned) * (size_t)(h->w.n_tickets + n_sm + 1);
     h->bytes = 2 * codes + 2 * scales + work + tickets;
     void *p = nullptr;
     if (cudaMalloc(&p, h->bytes) != cudaSuccess || cudaMemset(p, 0, h->bytes) != cudaSuccess || cudaDeviceSynchronize() != cudaSuccess) {
@@ -422,8 +422,10 @@ vb200_kv4_t *vb200_kv4_open(int seqs, int kv_heads, int head_dim, int capacity) 
     c.ks = c.v + codes;
     c.vs = c.ks + scales;
     h->w.part = (float *)(c.vs + scales);
-    h->w.tickets = (unsigned *)(h->w.part + h->w.part_floats);
-    h->w.status = (int *)(h->w.tickets + h->w.n_tickets);
+    h->w.aside = h->w.part + h->w.part_floats;
+    h->w.tickets = (unsigned *)(h->w.aside + aside);
+    h->w.rooms = h->w.tickets + h->w.n_tickets;
+    h->w.status = (int *)(h->w.rooms + n_sm);
     return h;
 }
 

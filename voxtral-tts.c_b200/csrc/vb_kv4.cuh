@@ -36,8 +36,9 @@ struct Kv4Attn {
     float *lse;
     const float *mass_in;
     float *mass_out;
-    float *part;
-    unsigned *tickets;
+    float *part, *aside;
+    unsigned *tickets, *rooms;
+    int n_rooms;
     int *status;
 };
 
@@ -188,6 +189,7 @@ int kv4_mass_many(const Kv4Attn &a, const ServeRows<T> &q, cudaStream_t st);
 int kv4_prompt_load(int blocks);
 /* floats of partial results that it needs */
 size_t kv4_prompt_floats(int blocks, int sm_count);
+size_t kv4_aside_floats(int blocks, int sm_count);       /* and of sums put aside */
 
 } // namespace vb
 

@@ -782,7 +782,7 @@ int kv4_attention(const Kv4 &c, const Kv4Work &w, const vb200_kv4_attention_t &v
     a.c = c;
     a.lengths = v.lengths; a.rows = v.rows; a.max_rows = v.max_rows; a.heads = v.heads; a.group = v.heads / c.kv_heads;
     a.scale = v.scale; a.lse = v.lse; a.mass_in = v.mass_in; a.mass_out = v.mass_out;
-    a.part = w.part; a.tickets = w.tickets; a.status = w.status;
+    a.part = w.part; a.aside = w.aside; a.tickets = w.tickets; a.rooms = w.rooms; a.n_rooms = w.sm_count; a.status = w.status;
     if ((long long)a.max_rows * a.group > (1ll << 30)) return serve_fail("too many rows");
     if (v.q.type == VB200_F32) return attn_dims<float>(a, v, w, st);
     if (v.q.type == VB200_BF16) return attn_dims<__nv_bfloat16>(a, v, w, st);

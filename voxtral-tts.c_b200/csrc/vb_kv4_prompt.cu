@@ -6,11 +6,12 @@
  *   S [128 x 128]   = Q K^T    Q in shared memory, one FP16 term (bf16, fp16) or two (fp32), rows brought to [2^14, 2^15)
  *   O [128 x dim]  += P V      P in TMEM, in S's own columns, one term (bf16) or two; V rows [token][dim] are an MN-major operand
  *
- * Keys and values go from codes to FP16 on the way to shared memory, four warps for the keys and three for the values: keys times 2^(e - S + 13), S the largest
- * scale of a warp's 32 tokens, which the softmax undoes, values times 2^(e - E + 13), E the largest scale so far, on which the
- * accumulator is based (exact down to 2^-36 of the largest). Scores, weights, sums as in vb_kv4_attn.cu. Two warpgroups take
- * alternate tiles with a reference, sums and an accumulator each, merged at the end, so that the tensor pipe works on one tile while the
- * other is in its softmax.
+ * Keys and values go from codes to FP16 on the way to shared memory, four warps for the keys and three for the values: keys times
+ * 2^(e - S + 13), S the largest scale of a warp's 32 tokens, which the softmax undoes, values times 2^(e - E + 13), E the largest scale
+ * so far, on which the accumulator is based (exact down to 2^-36 of the largest). Scores, weights, sums as in vb_kv4_attn.cu. Two pairs of
+ * warpgroups take alternate tiles with a reference, sums and an accumulator each, merged at the end, so that the tensor pipe works on
+ * one tile while the other is in its softmax. A thread has half of a row's columns: with a whole row a thread, and half as many
+ * threads, 1203 rows took 206 us in place of 178.
  *
  * Warps: 0-7, 8-15 softmax, 16-19 keys, 20-22 values, 23 issues the MMAs. All waits are bounded.
  */
@@ -26,8 +27,14 @@ namespace {
 constexpr int kPRows = 128, kPKeys = 128, kPSoft = 512, kPMmaWarp = 23, kPThreads = 32 * (kPMmaWarp + 1), kPBlock = kPKeys * 128, kPStatus = 62, kPRing = 8;
 constexpr int kPLeast = 2, kPTailParts = 8;   /* tiles of a part at least; parts of a unit of the last round at most */
 constexpr uint32_t kPTmem = 512, kPO = 256;
+/* A sum in TMEM loses up to a unit of its last place with every product of 16 tokens that is added, towards zero: 224 of them, 28 tiles of two
+ * terms, left results of a portion of 1203 fp32 rows 3.4e-6 off 64 bits (elementary fp32 operations: 1.2e-6). So fp32 results put
+ * what six tiles of a warpgroup pair have made aside in global memory and add it up there, rounded to nearest. */
+constexpr int kPChain = 6;
+
 template <int NB, int QT>
 struct PCfg {
+    static constexpr bool kAside = QT == 2;
     static constexpr int kD64 = (NB + 1) / 2;                                  /* blocks of 64 columns */
     static constexpr int kSlot = kD64 * kPBlock;
     static constexpr int kSlots = kD64 >= 2 ? 2 : 3;
@@ -108,6 +115,27 @@ VB_DEVINL bool p_work(const Kv4Attn &a, int block, PWork &p) {
     return p.split < p.used;
 }
 
+/* Room for sums put aside, which a CTA takes for its time: as many as SMs, and a CTA has an SM to itself (its registers leave room for no
+ * other), so that one is free. The SM's number is only where the search begins. False: none found, which would be a fault. */
+VB_DEVINL bool p_take(const Kv4Attn &a, int &room) {
+    uint32_t sm;
+    asm("mov.u32 %0, %%smid;" : "=r"(sm));
+    room = (int)(sm % (uint32_t)a.n_rooms);
+    for (int i = 0; i < 1 << 16; i++) {
+        if (atomicCAS(&a.rooms[room], 0u, 1u) == 0u) {
+            __threadfence();
+            return true;
+        }
+        room = room + 1 == a.n_rooms ? 0 : room + 1;
+    }
+    return false;
+}
+/* In it 32 columns of a warpgroup pair: [four columns][row], a float4 each. */
+template <int NB>
+VB_DEVINL float4 *p_aside(const Kv4Attn &a, int room, int pair, int block) {
+    return reinterpret_cast<float4 *>(a.aside) + (((size_t)room * 2 + pair) * NB + block) * 8 * kPRows;
+}
+
 template <int NB, int PT, class T>
 __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn a, const ServeRows<T> q, const ServeRows<T> out) {
     constexpr int QT = sizeof(T) == 4 ? 2 : 1, kDim = NB * 32;
@@ -117,7 +145,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
     unsigned char *q_s = base, *k_s = q_s + Cfg::kQ, *v_s = k_s + Cfg::kSlots * Cfg::kSlot;
     __shared__ __align__(8) uint64_t k_full[Cfg::kSlots], k_empty[Cfg::kSlots], v_full[Cfg::kSlots], v_empty[Cfg::kSlots], s_full[2], p_full[2], o_done[2], q_full;
     __shared__ float key_up[kPRing][4], down_s[kPRows], top_s[2][2][kPRows];
-    __shared__ int value_top[kPRing], bad_s[NB], abort_s;
+    __shared__ float2 aside_s[2][2][kPRows];                       /* reference, scale of what is put aside */
+    __shared__ int value_top[kPRing], bad_s[NB], abort_s, room_s;
     __shared__ uint32_t tmem_slot;
     int *abort_flag = &abort_s;
 
@@ -145,6 +174,12 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
         vb_mbar_init_fence();
     }
     if (tid < NB) bad_s[tid] = 1 << 30;
+    const bool puts_aside = Cfg::kAside && n_tiles > 2 * kPChain;
+    if (puts_aside && tid == 32) {
+        int room;
+        if (!p_take(a, room)) atomicCAS(a.status, 0, kPStatus);
+        room_s = room;
+    }
     if (warp == kPMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(vb_smem_u32(&tmem_slot)), "r"(kPTmem) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -154,6 +189,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
     tc_fence_after();
     pdl_launch_dependents();       /* not before the allocation: a kernel that starts early must not take columns this one needs */
     const uint32_t tmem = *(volatile uint32_t *)&tmem_slot;
+    const int room = puts_aside ? room_s : 0;
     auto give_up = [&]() {
         atomicCAS(a.status, 0, kPStatus);
         *(volatile int *)abort_flag = 1;
@@ -215,9 +251,18 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
         const float mul = (a.scale != 0.0f ? fabsf(a.scale) * 1.44269504f : 1.0f) * down_s[r];
         float ref = -INFINITY, sum = 0.0f;
         int top_scale = 0, it = 0;
+        bool ok = true;                                            /* the pair's barrier is met in every round, given up or not */
+        auto wait = [&](uint64_t *bar, uint32_t phase) {
+            ok = ok && at_warp_wait(bar, phase, abort_flag);
+            if (!ok) give_up();
+            return ok;
+        };
         for (int t = w; t < n_tiles; t += 2, it++) {
             const int j0 = (first_tile + t) * kPKeys;
-            if (!at_warp_wait(&s_full[w], (uint32_t)it & 1u, abort_flag)) { give_up(); break; }
+            if (!wait(&s_full[w], (uint32_t)it & 1u)) {
+                vb_named_bar(2 + w, 256);
+                continue;
+            }
             tc_fence_after();
             const float *ups = key_up[t % kPRing];
             const int last = sees - j0;                            /* columns before this one are seen */
@@ -246,23 +291,57 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
             vb_named_bar(2 + w, 256);
             top = fmaxf(top, top_s[w][half ^ 1][r]);
             /* values: the scale that this tile is based on */
-            if (!at_warp_wait(&v_full[t % Cfg::kSlots], (uint32_t)(t / Cfg::kSlots) & 1u, abort_flag)) { give_up(); break; }
+            if (!wait(&v_full[t % Cfg::kSlots], (uint32_t)(t / Cfg::kSlots) & 1u)) continue;
             const int now_scale = value_top[t % kPRing];
             const bool rise = top > ref + 8.0f;
-            if (__any_sync(0xffffffffu, rise) || now_scale != top_scale) {
+            const bool put_aside = Cfg::kAside && it > 0 && it % kPChain == 0;
+            if (__any_sync(0xffffffffu, rise) || now_scale != top_scale || put_aside) {
                 const float now = rise ? top : ref, f = rise ? exp2_fast(ref - now) : 1.0f;      /* the first time: 0 */
                 if (it > 0) {
-                    if (!at_warp_wait(&o_done[w], (uint32_t)(it - 1) & 1u, abort_flag)) { give_up(); break; }
+                    if (!wait(&o_done[w], (uint32_t)(it - 1) & 1u)) continue;
                     tc_fence_after();
-                    const int fall = now_scale - top_scale;
-                    const float fo = fall > 126 ? 0.0f : f * __uint_as_float((uint32_t)(127 - fall) << 23);
+                    if (put_aside) {
+                        /* added at the reference of what is there, unless that has come to lie too far below */
+                        const float2 there = aside_s[w][half][r];
+                        const int rises = top_scale - __float_as_int(there.y);
+                        const bool first = it == kPChain, rebase = !first && (!(there.x > -INFINITY) || ref - there.x + (float)rises > 60.0f);
+                        const float g = first || rebase ? 1.0f : exp2_fast(ref - there.x) * __uint_as_float((uint32_t)(127 + rises) << 23);
+                        if (rebase) {
+                            const float fa = !(there.x > -INFINITY) || rises > 126 ? 0.0f : exp2_fast(there.x - ref) * __uint_as_float((uint32_t)(127 - rises) << 23);
 #pragma unroll 1
-                    for (int c = half; c < NB; c += 2) {
-                        uint32_t reg[32];
-                        at_ld32(tO + (uint32_t)(c * 32), reg);
+                            for (int c = half; c < NB; c += 2)
+#pragma unroll 1
+                                for (int k = 0; k < 8; k++) {
+                                    float4 *to = p_aside<NB>(a, room, w, c) + k * kPRows + r;
+                                    const float4 old = __ldcg(to);
+                                    *to = make_float4(old.x * fa, old.y * fa, old.z * fa, old.w * fa);
+                                }
+                        }
+                        if (first || rebase) aside_s[w][half][r] = make_float2(ref, __int_as_float(top_scale));
+#pragma unroll 1
+                        for (int c = half; c < NB; c += 2) {
+                            uint32_t reg[32];
+                            at_ld32(tO + (uint32_t)(c * 32), reg);
+                            float4 *to = p_aside<NB>(a, room, w, c) + r;
 #pragma unroll
-                        for (int k = 0; k < 32; k++) reg[k] = __float_as_uint(__uint_as_float(reg[k]) * fo);
-                        at_st32(tO + (uint32_t)(c * 32), reg);
+                            for (int k = 0; k < 8; k++) {
+                                const float4 v = make_float4(__uint_as_float(reg[4 * k]) * g, __uint_as_float(reg[4 * k + 1]) * g, __uint_as_float(reg[4 * k + 2]) * g,
+                                                             __uint_as_float(reg[4 * k + 3]) * g);
+                                if (first) to[k * kPRows] = v;
+                                else atomicAdd(to + k * kPRows, v);        /* this thread alone adds here, so in one order */
+                            }
+                        }
+                    } else {
+                        const int fall = now_scale - top_scale;
+                        const float fo = fall > 126 ? 0.0f : f * __uint_as_float((uint32_t)(127 - fall) << 23);
+#pragma unroll 1
+                        for (int c = half; c < NB; c += 2) {
+                            uint32_t reg[32];
+                            at_ld32(tO + (uint32_t)(c * 32), reg);
+#pragma unroll
+                            for (int k = 0; k < 32; k++) reg[k] = __float_as_uint(__uint_as_float(reg[k]) * fo);
+                            at_st32(tO + (uint32_t)(c * 32), reg);
+                        }
                     }
                 }
                 sum *= f;
@@ -305,12 +384,13 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
             tc_fence_before();
             vb_mbar_arrive(&p_full[w]);
         }
-        if (it > 0 && !at_warp_wait(&o_done[w], (uint32_t)(it - 1) & 1u, abort_flag)) give_up();
+        if (it > 0) wait(&o_done[w], (uint32_t)(it - 1) & 1u);
         /* the tiles of either pair of warpgroups, merged, a warpgroup a block of 32 columns, by way of shared memory */
         vb_named_bar(1, kPSoft);                                     /* every product is done: the rings are free */
         float4 *ends = reinterpret_cast<float4 *>(k_s);            /* 4 x 128 x (reference, sum, scale) */
         float *rows = reinterpret_cast<float *>(k_s + 4 * kPRows * 16);
         ends[wg * kPRows + r] = make_float4(ref, sum * 0x1p-15f, __int_as_float(top_scale), 0.0f);
+        if (puts_aside) __threadfence();
         tc_fence_before();
         vb_named_bar(1, kPSoft);
         tc_fence_after();
@@ -341,8 +421,30 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
                 float v = 0.0f;
                 if (n_tiles > 0) v = __uint_as_float(oa[k]) * a0 * fa * a1;
                 if (n_tiles > 1) v += __uint_as_float(ob[k]) * b0 * fb * b1;
-                if (total == 0.0f) v = 0.0f;               /* nothing seen */
-                oa[k] = nan ? 0x7fffffffu : __float_as_uint(v);
+                oa[k] = __float_as_uint(v);
+            }
+            if constexpr (Cfg::kAside) {
+#pragma unroll 1
+                for (int x = 0; x < 2 && n_tiles > 2 * kPChain + x; x++) {
+                    const float2 e = aside_s[x][0][r];
+                    const int scale = __float_as_int(e.y) - 155;
+                    const float f = e.x > -INFINITY ? exp2_fast(e.x - reference) * inv : 0.0f;
+                    const float s0 = __uint_as_float((uint32_t)(127 + (scale >> 1)) << 23), s1 = __uint_as_float((uint32_t)(127 + scale - (scale >> 1)) << 23);
+                    const float4 *from = p_aside<NB>(a, room, x, c) + r;
+#pragma unroll
+                    for (int k = 0; k < 32; k += 4) {
+                        const float4 o = __ldcg(from + k / 4 * kPRows);
+                        oa[k] = __float_as_uint(__uint_as_float(oa[k]) + o.x * s0 * f * s1);
+                        oa[k + 1] = __float_as_uint(__uint_as_float(oa[k + 1]) + o.y * s0 * f * s1);
+                        oa[k + 2] = __float_as_uint(__uint_as_float(oa[k + 2]) + o.z * s0 * f * s1);
+                        oa[k + 3] = __float_as_uint(__uint_as_float(oa[k + 3]) + o.w * s0 * f * s1);
+                    }
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 32; k++) {
+                if (total == 0.0f) oa[k] = 0u;                     /* nothing seen */
+                if (nan) oa[k] = 0x7fffffffu;
             }
 #pragma unroll
             for (int k = 0; k < 32; k += 4) *reinterpret_cast<uint4 *>(rows + r * Cfg::kLd + c * 32 + k) = make_uint4(oa[k], oa[k + 1], oa[k + 2], oa[k + 3]);
@@ -506,7 +608,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
             for (int ks = 0; ks < kPKeys / 16; ks++) {
                 const uint32_t p = tmem + (uint32_t)(w * kPKeys + (ks >> 1) * 32 + (ks & 1) * 8);
 #pragma unroll
-                for (int u = 0; u < PT; u++) at_mma_ts(d, p + u * 16, vd.at(ks * (2048 >> 4)), idesc_o, (t >> 1 | ks | u) != 0 ? 1u : 0u);
+                for (int u = 0; u < PT; u++) at_mma_ts(d, p + u * 16, vd.at(ks * (2048 >> 4)), idesc_o, ((Cfg::kAside ? (t >> 1) % kPChain : t >> 1) | ks | u) != 0 ? 1u : 0u);
             }
             umma_commit(&v_empty[slot]);
             umma_commit(&o_done[w]);
@@ -517,6 +619,10 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
     }
     tc_fence_before();
     __syncthreads();
+    if (puts_aside && tid == 32) {
+        __threadfence();
+        atomicExch(&a.rooms[room], 0u);
+    }
     if (warp == kPMmaWarp) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kPTmem) : "memory");
@@ -864,6 +970,7 @@ template int kv4_prompt<__nv_bfloat16>(const Kv4Attn &, const ServeRows<__nv_bfl
 template int kv4_prompt<__half>(const Kv4Attn &, const ServeRows<__half> &, const ServeRows<__half> &, int, cudaStream_t);
 
 size_t kv4_prompt_floats(int blocks, int sm_count) { return blocks <= 4 ? (size_t)sm_count * kPRows * (blocks * 32 + 2) : 0; }
+size_t kv4_aside_floats(int blocks, int sm_count) { return blocks <= 4 ? (size_t)sm_count * 2 * kPRows * blocks * 32 : 0; }
 
 int kv4_prompt_load(int blocks) {
     bool ok = true;

@@ -216,8 +216,8 @@ bool serve_wide(const ServeRows<T> &r) {
 
 /* ------------------------------------------------------------------ launchers (vb_kv4_attn.cu) */
 struct Kv4Work {
-    float *part;                 /* partial results of key splits */
-    unsigned *tickets;           /* zero between calls */
+    float *part, *aside;         /* partial results of key splits; sums put aside */
+    unsigned *tickets, *rooms;   /* zero between calls; rooms: which places of aside are taken, one an SM */
     int *status;                 /* set where a bounded wait ran out */
     size_t part_floats;
     int n_tickets, sm_count;
