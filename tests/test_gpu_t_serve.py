@@ -244,6 +244,38 @@ def test_values_of_very_different_magnitude(pkg, rows):
     _check_attention(out, lse, q, kk.transpose(1, 2), vv.transpose(1, 2), [n], [rows], d ** -0.5, torch.float32)
 
 
+@pytest.mark.parametrize("rise", [0, 20, 80])
+def test_many_rows_over_many_tokens(pkg, rise):
+    """More units than SMs and far more tokens than a sum stays in one place. Halfway the scores rise by `rise` binary orders while values
+    fall by 20: both halves count where the rise is 20."""
+    g = _gen(61)
+    n, h, d, rows = 7001, 160, 32, 100
+    half = 3500
+    k, v = torch.zeros(1, n, h, d, device="cuda"), _randn(g, 1, n, h, d).abs()
+    k[:, half:, :, 0] = 4.0
+    v[:, :half] *= 2.0 ** 20
+    cache, at = _fill(pkg, k, v, n, [n])
+    q = _randn(g, 1, rows, h, d) * 0.0
+    q[..., 0] = rise * math.log(2.0) / 4.0
+    out, lse = torch.full_like(q, 3.0), torch.full((1, rows, h), 4.0, device="cuda")
+    cache.attention(q, out, at, scale=1.0, lse=lse)
+    cache.check()
+    vv = _held(v, None)[0]                                               # [h, n, d]
+    seen = [half, n - rows - half + 1]                                   # of each half by the first row, one more of the second a row
+    early, late = vv[:, :half].sum(1), vv[:, half:].cumsum(1)[:, -rows:].transpose(0, 1)
+    rise_exact = float(q[0, 0, 0, 0].double()) * 4.0                     # natural
+    w = math.exp(-rise_exact)
+    count = torch.arange(rows, device="cuda", dtype=torch.float64)[:, None, None] + seen[1]
+    want = (early[None] * w + late) / (half * w + count)
+    # a score: queries as two terms, products and factors; a weight: twice that, exponentials and terms (2^-20), and FP16's smallest step of its
+    # second term, 2^-32 of the largest weight, for every early token; sums: a unit for each 16 tokens and term, and the scales' factors
+    score = rise_exact * (2.0 ** -22 + 10 * 2.0 ** -23)
+    limit = want * (2 * score + 2.0 ** -19 + (n / 8 + 16) * 2.0 ** -23) + early[None] * 2.0 ** -32 / count
+    assert ((out[0].double() - want).abs() <= limit).all()
+    total = torch.log(half * w + count[..., 0]) + rise_exact
+    assert ((lse[0].double() - total).abs() <= score + 2.0 ** -18 + total.abs() * 2.0 ** -23).all()
+
+
 @pytest.mark.parametrize("rows", [3, 90])
 def test_what_a_row_does_not_see_does_not_reach_it(pkg, rows):
     """NaN and infinities in later tokens, and in what an earlier sequence has left behind the last one."""

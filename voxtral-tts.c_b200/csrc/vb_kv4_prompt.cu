@@ -27,9 +27,9 @@ namespace {
 constexpr int kPRows = 128, kPKeys = 128, kPSoft = 512, kPMmaWarp = 23, kPThreads = 32 * (kPMmaWarp + 1), kPBlock = kPKeys * 128, kPStatus = 62, kPRing = 8;
 constexpr int kPLeast = 2, kPTailParts = 8;   /* tiles of a part at least; parts of a unit of the last round at most */
 constexpr uint32_t kPTmem = 512, kPO = 256;
-/* A sum in TMEM loses up to a unit of its last place with every product of 16 tokens that is added, towards zero: 224 of them, 28 tiles of two
- * terms, left results of a portion of 1203 fp32 rows 3.4e-6 off 64 bits (elementary fp32 operations: 1.2e-6). So fp32 results put
- * what six tiles of a warpgroup pair have made aside in global memory and add it up there, rounded to nearest. */
+/* A sum in TMEM loses up to a unit of its last place with every product of 16 tokens that is added, towards zero: 224 of them, 14 tiles of two
+ * terms, left results of a portion of 1203 fp32 rows 3.4e-6 off 64 bits (elementary fp32 operations: 1.2e-6). So for fp32 a warpgroup
+ * pair puts what six tiles have made aside in global memory, added up there rounded to nearest: 1.6e-6, 195 us in place of 177. */
 constexpr int kPChain = 6;
 
 template <int NB, int QT>
@@ -136,6 +136,41 @@ VB_DEVINL float4 *p_aside(const Kv4Attn &a, int room, int pair, int block) {
     return reinterpret_cast<float4 *>(a.aside) + (((size_t)room * 2 + pair) * NB + block) * 8 * kPRows;
 }
 
+/* What is in TMEM is added to what lies aside, at the reference and scale of what is there unless those have come to lie too far below. A
+ * function of its own: within the softmax its registers made that spill (1203 rows: 213 us in place of 207). */
+template <int NB>
+__device__ __noinline__ void p_put_aside(float4 *mine, float2 *base, uint32_t tO, int half, bool first, float ref, int top_scale) {
+    const float2 there = *base;
+    const int rises = top_scale - __float_as_int(there.y);
+    const bool rebase = !first && (!(there.x > -INFINITY) || ref - there.x + (float)rises > 60.0f);
+    const float g = first || rebase ? 1.0f : exp2_fast(ref - there.x) * __uint_as_float((uint32_t)(127 + rises) << 23);
+    if (rebase) {
+        const float fa = !(there.x > -INFINITY) || rises > 126 ? 0.0f : exp2_fast(there.x - ref) * __uint_as_float((uint32_t)(127 - rises) << 23);
+#pragma unroll 1
+        for (int c = half; c < NB; c += 2)
+#pragma unroll 1
+            for (int k = 0; k < 8; k++) {
+                float4 *to = mine + ((c - half) * 8 + k) * kPRows;
+                const float4 old = __ldcg(to);
+                *to = make_float4(old.x * fa, old.y * fa, old.z * fa, old.w * fa);
+            }
+    }
+    if (first || rebase) *base = make_float2(ref, __int_as_float(top_scale));
+#pragma unroll 1
+    for (int c = half; c < NB; c += 2) {
+        uint32_t reg[32];
+        at_ld32(tO + (uint32_t)(c * 32), reg);
+        float4 *to = mine + (c - half) * 8 * kPRows;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const float4 v = make_float4(__uint_as_float(reg[4 * k]) * g, __uint_as_float(reg[4 * k + 1]) * g, __uint_as_float(reg[4 * k + 2]) * g,
+                                         __uint_as_float(reg[4 * k + 3]) * g);
+            if (first) to[k * kPRows] = v;
+            else atomicAdd(to + k * kPRows, v);        /* this thread alone adds here, so in one order */
+        }
+    }
+}
+
 template <int NB, int PT, class T>
 __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn a, const ServeRows<T> q, const ServeRows<T> out) {
     constexpr int QT = sizeof(T) == 4 ? 2 : 1, kDim = NB * 32;
@@ -189,7 +224,6 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
     tc_fence_after();
     pdl_launch_dependents();       /* not before the allocation: a kernel that starts early must not take columns this one needs */
     const uint32_t tmem = *(volatile uint32_t *)&tmem_slot;
-    const int room = puts_aside ? room_s : 0;
     auto give_up = [&]() {
         atomicCAS(a.status, 0, kPStatus);
         *(volatile int *)abort_flag = 1;
@@ -250,20 +284,14 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
         /* positive, so that what is masked stays -inf: queries are zeros where the scale is */
         const float mul = (a.scale != 0.0f ? fabsf(a.scale) * 1.44269504f : 1.0f) * down_s[r];
         float ref = -INFINITY, sum = 0.0f;
-        int top_scale = 0, it = 0;
-        bool ok = true;                                            /* the pair's barrier is met in every round, given up or not */
-        auto wait = [&](uint64_t *bar, uint32_t phase) {
-            ok = ok && at_warp_wait(bar, phase, abort_flag);
-            if (!ok) give_up();
-            return ok;
-        };
-        for (int t = w; t < n_tiles; t += 2, it++) {
+        int top_scale = 0, it = 0, t = w;
+        for (; t < n_tiles; t += 2, it++) {
             const int j0 = (first_tile + t) * kPKeys;
-            if (!wait(&s_full[w], (uint32_t)it & 1u)) {
-                vb_named_bar(2 + w, 256);
-                continue;
-            }
+            if (!at_warp_wait(&s_full[w], (uint32_t)it & 1u, abort_flag)) { give_up(); break; }
             tc_fence_after();
+            if constexpr (Cfg::kAside) {       /* the products up to it - 1 were done before these scores were begun; the next starts from zero */
+                if (it > 0 && it % kPChain == 0) p_put_aside<NB>(p_aside<NB>(a, *(volatile int *)&room_s, w, half) + r, &aside_s[w][half][r], tO, half, it == kPChain, ref, top_scale);
+            }
             const float *ups = key_up[t % kPRing];
             const int last = sees - j0;                            /* columns before this one are seen */
             const bool masked = j0 + kPKeys > all_see;
@@ -291,57 +319,23 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
             vb_named_bar(2 + w, 256);
             top = fmaxf(top, top_s[w][half ^ 1][r]);
             /* values: the scale that this tile is based on */
-            if (!wait(&v_full[t % Cfg::kSlots], (uint32_t)(t / Cfg::kSlots) & 1u)) continue;
+            if (!at_warp_wait(&v_full[t % Cfg::kSlots], (uint32_t)(t / Cfg::kSlots) & 1u, abort_flag)) { give_up(); t += 2; break; }
             const int now_scale = value_top[t % kPRing];
             const bool rise = top > ref + 8.0f;
-            const bool put_aside = Cfg::kAside && it > 0 && it % kPChain == 0;
-            if (__any_sync(0xffffffffu, rise) || now_scale != top_scale || put_aside) {
+            if (__any_sync(0xffffffffu, rise) || now_scale != top_scale) {
                 const float now = rise ? top : ref, f = rise ? exp2_fast(ref - now) : 1.0f;      /* the first time: 0 */
                 if (it > 0) {
-                    if (!wait(&o_done[w], (uint32_t)(it - 1) & 1u)) continue;
+                    if (!at_warp_wait(&o_done[w], (uint32_t)(it - 1) & 1u, abort_flag)) { give_up(); t += 2; break; }
                     tc_fence_after();
-                    if (put_aside) {
-                        /* added at the reference of what is there, unless that has come to lie too far below */
-                        const float2 there = aside_s[w][half][r];
-                        const int rises = top_scale - __float_as_int(there.y);
-                        const bool first = it == kPChain, rebase = !first && (!(there.x > -INFINITY) || ref - there.x + (float)rises > 60.0f);
-                        const float g = first || rebase ? 1.0f : exp2_fast(ref - there.x) * __uint_as_float((uint32_t)(127 + rises) << 23);
-                        if (rebase) {
-                            const float fa = !(there.x > -INFINITY) || rises > 126 ? 0.0f : exp2_fast(there.x - ref) * __uint_as_float((uint32_t)(127 - rises) << 23);
+                    const int fall = now_scale - top_scale;
+                    const float fo = fall > 126 ? 0.0f : f * __uint_as_float((uint32_t)(127 - fall) << 23);
 #pragma unroll 1
-                            for (int c = half; c < NB; c += 2)
-#pragma unroll 1
-                                for (int k = 0; k < 8; k++) {
-                                    float4 *to = p_aside<NB>(a, room, w, c) + k * kPRows + r;
-                                    const float4 old = __ldcg(to);
-                                    *to = make_float4(old.x * fa, old.y * fa, old.z * fa, old.w * fa);
-                                }
-                        }
-                        if (first || rebase) aside_s[w][half][r] = make_float2(ref, __int_as_float(top_scale));
-#pragma unroll 1
-                        for (int c = half; c < NB; c += 2) {
-                            uint32_t reg[32];
-                            at_ld32(tO + (uint32_t)(c * 32), reg);
-                            float4 *to = p_aside<NB>(a, room, w, c) + r;
+                    for (int c = half; c < NB; c += 2) {
+                        uint32_t reg[32];
+                        at_ld32(tO + (uint32_t)(c * 32), reg);
 #pragma unroll
-                            for (int k = 0; k < 8; k++) {
-                                const float4 v = make_float4(__uint_as_float(reg[4 * k]) * g, __uint_as_float(reg[4 * k + 1]) * g, __uint_as_float(reg[4 * k + 2]) * g,
-                                                             __uint_as_float(reg[4 * k + 3]) * g);
-                                if (first) to[k * kPRows] = v;
-                                else atomicAdd(to + k * kPRows, v);        /* this thread alone adds here, so in one order */
-                            }
-                        }
-                    } else {
-                        const int fall = now_scale - top_scale;
-                        const float fo = fall > 126 ? 0.0f : f * __uint_as_float((uint32_t)(127 - fall) << 23);
-#pragma unroll 1
-                        for (int c = half; c < NB; c += 2) {
-                            uint32_t reg[32];
-                            at_ld32(tO + (uint32_t)(c * 32), reg);
-#pragma unroll
-                            for (int k = 0; k < 32; k++) reg[k] = __float_as_uint(__uint_as_float(reg[k]) * fo);
-                            at_st32(tO + (uint32_t)(c * 32), reg);
-                        }
+                        for (int k = 0; k < 32; k++) reg[k] = __float_as_uint(__uint_as_float(reg[k]) * fo);
+                        at_st32(tO + (uint32_t)(c * 32), reg);
                     }
                 }
                 sum *= f;
@@ -384,7 +378,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
             tc_fence_before();
             vb_mbar_arrive(&p_full[w]);
         }
-        if (it > 0) wait(&o_done[w], (uint32_t)(it - 1) & 1u);
+        for (; t < n_tiles; t += 2) vb_named_bar(2 + w, 256);         /* given up: the others of the pair meet its barrier all the same */
+        if (it > 0 && !at_warp_wait(&o_done[w], (uint32_t)(it - 1) & 1u, abort_flag)) give_up();
         /* the tiles of either pair of warpgroups, merged, a warpgroup a block of 32 columns, by way of shared memory */
         vb_named_bar(1, kPSoft);                                     /* every product is done: the rings are free */
         float4 *ends = reinterpret_cast<float4 *>(k_s);            /* 4 x 128 x (reference, sum, scale) */
@@ -430,7 +425,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
                     const int scale = __float_as_int(e.y) - 155;
                     const float f = e.x > -INFINITY ? exp2_fast(e.x - reference) * inv : 0.0f;
                     const float s0 = __uint_as_float((uint32_t)(127 + (scale >> 1)) << 23), s1 = __uint_as_float((uint32_t)(127 + scale - (scale >> 1)) << 23);
-                    const float4 *from = p_aside<NB>(a, room, x, c) + r;
+                    const float4 *from = p_aside<NB>(a, room_s, x, c) + r;
 #pragma unroll
                     for (int k = 0; k < 32; k += 4) {
                         const float4 o = __ldcg(from + k / 4 * kPRows);
@@ -621,7 +616,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
     __syncthreads();
     if (puts_aside && tid == 32) {
         __threadfence();
-        atomicExch(&a.rooms[room], 0u);
+        atomicExch(&a.rooms[room_s], 0u);
     }
     if (warp == kPMmaWarp) {
         tc_fence_after();
