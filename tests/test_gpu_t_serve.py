@@ -397,6 +397,12 @@ def test_eviction_of_every_row_size(pkg, dim):
     _check_eviction(pkg, [500, 299], 300, 20, 4, mass, dim=dim, in_place=True, alias=True)
 
 
+def test_eviction_in_place_of_more_heads_than_run_at_once(pkg):
+    """The new lengths over the old ones: the heads that come last find the new ones there."""
+    mass = torch.rand(2, 1100, 60, generator=_gen(71), device="cuda")
+    _check_eviction(pkg, [60, 57], 40, 8, 2, mass, dim=32, in_place=True, alias=True)
+
+
 @pytest.mark.parametrize("kind", ["equal", "zeros", "few values", "nan", "negative", "infinite", "tiny"])
 def test_eviction_where_masses_tie_or_are_no_numbers(pkg, kind):
     g = _gen(7)

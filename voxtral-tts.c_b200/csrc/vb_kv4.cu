@@ -43,7 +43,8 @@ constexpr int kRowThreads = 256, kRowUnroll = 4;
 
 /* ------------------------------------------------------------------ rows into the cache and out of it
  * A CTA has rows of one head, keys or values; a thread a word of 8 values of a row, four rows at a time with their loads together; four
- * lanes make a block of 32. Memory-bound, and at one row a launch bound by its latency. (With words of all heads side by side, indices
+ * lanes make a block of 32. Memory-bound, and at one row a launch bound by its latency: 4097 bf16 rows of two sequences and 8 heads of 128
+ * in and out again, 118 MB, 24 us, 4.8 TB/s; one row of eight sequences in and out 6.5 us, the host's time for two launches. (With words of all heads side by side, indices
  * worked out word by word, 4097 rows of two sequences took 22 us in and 16 out.) */
 template <class T>
 struct RowsArgs {
@@ -191,7 +192,7 @@ constexpr int kSelThreads = 1024, kSelBins = 2048, kSelHeld = 40960;
 /* Which tokens stay: a CTA per sequence and head. The need-th largest key of the middle by digits of 11, 11 and 10 bits (counts of a
  * digit among those that share the digits before it; the first holds sign, exponent and two bits, so that masses spread over it), then
  * the tokens in order: a thread has a stretch of them, an odd number so that threads' reads fall on different banks. Keys wait in shared
- * memory; of sequences too long for that they are read again. (With a thread's 32 keys in registers, loops unrolled over them:
+ * memory; of sequences too long for that they are read again. Bound by the latencies of its passes: 26 us for 128 heads of 32768 tokens. (With a thread's 32 keys in registers, loops unrolled over them:
  * 17 us for 1601 tokens and 44 for 32768, most of it for fetching the code.) */
 __global__ void __launch_bounds__(kSelThreads) kv4_select_kernel(const EvictArgs a) {
     extern __shared__ uint32_t held[];
@@ -283,7 +284,7 @@ size_t select_smem(int capacity) { return sizeof(uint32_t) * (size_t)std::min(ca
 
 /* The rows that stay into their places, in pieces of 16 bytes (codes) and a byte a block (scales). In place a CTA takes all of a
  * head, since a row's new slot may be another row's old one: rows move towards the front in order, so a stretch may be written once all
- * stretches up to it have been read. */
+ * stretches up to it have been read. 128 heads of 8192 rows of 128 dims out of 32768: 62 us, 4.6 TB/s read and written. */
 constexpr int kMoveThreads = 256;
 
 template <bool IN_PLACE>
@@ -292,7 +293,7 @@ __global__ void __launch_bounds__(kMoveThreads) kv4_move_kernel(const EvictArgs 
     pdl_launch_dependents();
     pdl_wait();
     const int n = min(max(a.lengths[s], 0), a.from.capacity), m = min(n, a.keep);
-    if (blockIdx.x == 0 && h == 0 && tid == 0) a.new_lengths[s] = m;     /* whoever reads it later finds the same m */
+    if (blockIdx.x == 0 && h == 0 && tid == 0) a.new_lengths[s] = m;     /* may be lengths: whoever reads it later finds another n but the same m */
     const int blocks = a.from.blocks, pieces = blocks;                   /* of 16 bytes a row and plane */
     const int per = kMoveThreads / (2 * pieces);                         /* rows at a time */
     const int r0 = tid / (2 * pieces), piece = tid - r0 * 2 * pieces;
@@ -300,7 +301,8 @@ __global__ void __launch_bounds__(kMoveThreads) kv4_move_kernel(const EvictArgs 
     const int *kept = a.kept + ((size_t)s * a.from.kv_heads + h) * a.keep;
     const size_t from0 = a.from.row(s, h, 0), into0 = a.into.row(s, h, 0), head = (size_t)s * a.from.kv_heads + h;
     const int first = IN_PLACE ? 0 : blockIdx.x * per, step = IN_PLACE ? per : gridDim.x * per;
-    if (IN_PLACE && m == n && (!a.new_mass || a.new_mass == a.mass)) return;      /* nothing moves */
+    /* nothing moves: tokens stay in order, so where the last one is at its place all are */
+    if (IN_PLACE && (m == 0 || kept[m - 1] == m - 1) && (!a.new_mass || a.new_mass == a.mass)) return;
     for (int i0 = first; i0 < m; i0 += step) {
         const int i = i0 + r0;
         const bool mine = r0 < per && i < m;
@@ -440,9 +442,13 @@ void vb200_kv4_close(vb200_kv4_t *h) {
 
 int vb200_kv4_status(const vb200_kv4_t *h) {
     if (!h) return serve_fail("no cache");
-    int s = 0;
-    if (cudaMemcpy(&s, h->w.status, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess) return serve_launched() ? -1 : serve_fail("the status could not be read");
-    return s;
+    int s = 0, now = -1;
+    if (cudaGetDevice(&now) == cudaSuccess && now != h->device) cudaSetDevice(h->device);
+    /* streams that do not wait for the default one have to be waited for by themselves */
+    const bool read = cudaDeviceSynchronize() == cudaSuccess && cudaMemcpy(&s, h->w.status, sizeof(int), cudaMemcpyDeviceToHost) == cudaSuccess;
+    if (!read && !serve_launched()) serve_fail("the status could not be read");
+    if (now >= 0 && now != h->device) cudaSetDevice(now);
+    return read ? s : -1;
 }
 
 size_t vb200_kv4_bytes(const vb200_kv4_t *h) { return h ? h->bytes : 0; }
