@@ -38,7 +38,7 @@ typedef struct {
  * ones to 6). A block with a value that is not finite reads as NaN throughout. (head_dim + head_dim / 16) bytes a token
  * and head, keys and values together, where fp32 takes 8 head_dim.
  *
- * The handle owns the rows and a small workspace on the device that was current when it was opened, and is used with that
+ * The handle owns the rows and a workspace (up to 30 MB) on the device that was current when it was opened, and is used with that
  * device current. Calls on one handle are made one after another: on one stream, or on streams that events put in order;
  * graphs that hold such calls likewise. Different handles are independent.
  *

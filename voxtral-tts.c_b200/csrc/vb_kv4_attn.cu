@@ -16,6 +16,10 @@
  * A warp walks tiles of 32 tokens with a maximum, sums and accumulators of its own, through a ring of its own that bulk copies
  * fill: no barrier between warps until the end. A sequence's tokens are split over CTAs where there are few of them; the CTA that
  * comes last at a ticket joins the parts.
+ *
+ * Bound by the issue of instructions where tokens are many: a warp's tile is 605 of them, of which 283, conversions and integer operations, go to a pipe of
+ * half the rate. One row of 32 heads over four sequences of 131072 tokens and 8 KV heads of 128, bf16: 102 us, 4.2 TB/s of codes and scales, 64 % of
+ * a plain copy's rate. Over 301 tokens 6.6 us: latencies that wait for one another.
  */
 #include <algorithm>
 #include <limits.h>
@@ -571,7 +575,8 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(co
 
 /* mass_out: the scores again, now that the rows' sums are known (in the attention kernel only the last CTA of a split sequence knows them,
  * and keeping scores takes memory for every row). A CTA has up to four tiles of tokens a warp, whose keys stay in shared memory while the
- * (row, head) pairs come by, 64 at a time, a column of eight by each warp. A token's weights are summed in one order: no atomics. */
+ * (row, head) pairs come by, 64 at a time, a column of eight by each warp. A token's weights are summed in one order: no atomics. One row of 32
+ * heads over eight sequences of 4608 tokens and 8 KV heads of 128, bf16: 13 us beside the attention's 14, latencies for the most part. */
 constexpr int kMTiles = 4, kMMostPairs = 64;      /* of a KV head: more take the kernel of vb_kv4_prompt.cu, heads up to 128 */
 
 template <int NB, class T>

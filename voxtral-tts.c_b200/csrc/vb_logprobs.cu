@@ -3,7 +3,8 @@
  *
  *   m = max x,  l = sum e^(x - m),  w = sum e^(x - m) (x - m);  lse = m + log l,  entropy = log l - w / l
  *
- * Bound by the logits' bytes where there are many rows, by latency where there is one. A row is split over the CTAs of a cluster;
+ * Bound by the logits' bytes where there are many rows (1024 fp32 rows of 100003: 80 us, 5.1 TB/s, 79 % of a plain copy's rate), by latency where
+ * there is one (131072: 7.4 us). A row is split over the CTAs of a cluster;
  * a thread keeps m, l, w of what it reads, rescaled when its maximum rises. The largest values: a threshold that `top` values are known to reach (the
  * top-th largest of the maxima that 32 groups of threads have in their first stretch) lets a few dozen values of a row through, which are
  * collected and put in order at the end. Values are compared with their index below them, so all are different. Where more come through than
