@@ -244,18 +244,17 @@ def test_values_of_very_different_magnitude(pkg, rows):
     _check_attention(out, lse, q, kk.transpose(1, 2), vv.transpose(1, 2), [n], [rows], d ** -0.5, torch.float32)
 
 
-@pytest.mark.parametrize("rise", [0, 20, 80])
-def test_many_rows_over_many_tokens(pkg, rise):
+@pytest.mark.parametrize("dtype,n,rise,fall", [("f32", 7001, 0, 20), ("f32", 7001, 20, 20), ("f32", 7001, 80, 20), ("f16", 33001, 4, 4), ("bf16", 33001, 20, 20)])
+def test_many_rows_over_many_tokens(pkg, dtype, n, rise, fall):
     """More units than SMs and far more tokens than a sum stays in one place. Halfway the scores rise by `rise` binary orders while values
-    fall by 20: both halves count where the rise is 20."""
+    fall by `fall`: both halves count where the two are alike."""
     g = _gen(61)
-    n, h, d, rows = 7001, 160, 32, 100
-    half = 3500
-    k, v = torch.zeros(1, n, h, d, device="cuda"), _randn(g, 1, n, h, d).abs()
+    h, d, rows, half, t = 160, 32, 100, n // 2, TYPES[dtype]
+    k, v = torch.zeros(1, n, h, d, device="cuda", dtype=t), _randn(g, 1, n, h, d, dtype=t).abs()
     k[:, half:, :, 0] = 4.0
-    v[:, :half] *= 2.0 ** 20
+    v[:, :half] *= 2.0 ** fall
     cache, at = _fill(pkg, k, v, n, [n])
-    q = _randn(g, 1, rows, h, d) * 0.0
+    q = _randn(g, 1, rows, h, d, dtype=t) * 0.0
     q[..., 0] = rise * math.log(2.0) / 4.0
     out, lse = torch.full_like(q, 3.0), torch.full((1, rows, h), 4.0, device="cuda")
     cache.attention(q, out, at, scale=1.0, lse=lse)
@@ -268,9 +267,10 @@ def test_many_rows_over_many_tokens(pkg, rise):
     count = torch.arange(rows, device="cuda", dtype=torch.float64)[:, None, None] + seen[1]
     want = (early[None] * w + late) / (half * w + count)
     # a score: queries as two terms, products and factors; a weight: twice that, exponentials and terms (2^-20), and FP16's smallest step of its
-    # second term, 2^-32 of the largest weight, for every early token; sums: a unit for each 16 tokens and term, and the scales' factors
+    # second term, 2^-32 of the largest weight, for every early token (one term for bf16: 2^-11, normal numbers here); sums: a unit for each 16
+    # tokens and term, and the scales' factors; the result's own rounding
     score = rise_exact * (2.0 ** -22 + 10 * 2.0 ** -23)
-    limit = want * (2 * score + 2.0 ** -19 + (n / 8 + 16) * 2.0 ** -23) + early[None] * 2.0 ** -32 / count
+    limit = want * (2 * score + 2.0 ** -19 + (n / 8 + 16) * 2.0 ** -23 + (2.0 ** -11 if dtype == "bf16" else 0.0) + torch.finfo(t).eps / 2) + early[None] * 2.0 ** -32 / count
     assert ((out[0].double() - want).abs() <= limit).all()
     total = torch.log(half * w + count[..., 0]) + rise_exact
     assert ((lse[0].double() - total).abs() <= score + 2.0 ** -18 + total.abs() * 2.0 ** -23).all()

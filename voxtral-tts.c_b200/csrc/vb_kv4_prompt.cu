@@ -29,14 +29,14 @@ namespace {
 constexpr int kPRows = 128, kPKeys = 128, kPSoft = 512, kPMmaWarp = 23, kPThreads = 32 * (kPMmaWarp + 1), kPBlock = kPKeys * 128, kPStatus = 62, kPRing = 8;
 constexpr int kPLeast = 2, kPTailParts = 8;   /* tiles of a part at least; parts of a unit of the last round at most */
 constexpr uint32_t kPTmem = 512, kPO = 256;
-/* A sum in TMEM loses up to a unit of its last place with every product of 16 tokens that is added, towards zero: 224 of them, 14 tiles of two
- * terms, left results of a portion of 1203 fp32 rows 3.4e-6 off 64 bits (elementary fp32 operations: 1.2e-6). So for fp32 a warpgroup
- * pair puts what six tiles have made aside in global memory, added up there rounded to nearest: 1.6e-6, 195 us in place of 177. */
-constexpr int kPChain = 6;
-
 template <int NB, int QT>
 struct PCfg {
-    static constexpr bool kAside = QT == 2;
+    /* A sum in TMEM loses up to a unit of its last place with every product of 16 tokens that is added, towards zero: 224 of them, 14 tiles of two
+     * terms, left results of a portion of 1203 fp32 rows 3.4e-6 off 64 bits (elementary fp32 operations: 1.2e-6). So a warpgroup pair puts what
+     * a few tiles have made aside in global memory, added up there rounded to nearest. fp32: three tiles (six: 1.5e-6 off over 2112
+     * tokens, where elementary operations are 0.7e-6 and three 0.9e-6). 1203 rows: 205 us, 195 with six, 177 without. Types that round
+     * their results to less: as many as stay far below that (64 * 16 * 2^-24). */
+    static constexpr int kChain = QT == 2 ? 3 : 64;
     static constexpr int kD64 = (NB + 1) / 2;                                  /* blocks of 64 columns */
     static constexpr int kSlot = kD64 * kPBlock;
     static constexpr int kSlots = kD64 >= 2 ? 2 : 3;
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
         vb_mbar_init_fence();
     }
     if (tid < NB) bad_s[tid] = 1 << 30;
-    const bool puts_aside = Cfg::kAside && n_tiles > 2 * kPChain;
+    const bool puts_aside = n_tiles > 2 * Cfg::kChain;
     if (puts_aside && tid == 32) {
         int room;
         if (!p_take(a, room)) atomicCAS(a.status, 0, kPStatus);
@@ -291,9 +291,9 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
             const int j0 = (first_tile + t) * kPKeys;
             if (!at_warp_wait(&s_full[w], (uint32_t)it & 1u, abort_flag)) { give_up(); break; }
             tc_fence_after();
-            if constexpr (Cfg::kAside) {       /* the products up to it - 1 were done before these scores were begun; the next starts from zero */
-                if (it > 0 && it % kPChain == 0) p_put_aside<NB>(p_aside<NB>(a, *(volatile int *)&room_s, w, half) + r, &aside_s[w][half][r], tO, half, it == kPChain, ref, top_scale);
-            }
+            /* the products up to it - 1 were done before these scores were begun; the next starts from zero */
+            if (it > 0 && it % Cfg::kChain == 0)
+                p_put_aside<NB>(p_aside<NB>(a, *(volatile int *)&room_s, w, half) + r, &aside_s[w][half][r], tO, half, it == Cfg::kChain, ref, top_scale);
             const float *ups = key_up[t % kPRing];
             const int last = sees - j0;                            /* columns before this one are seen */
             const bool masked = j0 + kPKeys > all_see;
@@ -420,22 +420,20 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
                 if (n_tiles > 1) v += __uint_as_float(ob[k]) * b0 * fb * b1;
                 oa[k] = __float_as_uint(v);
             }
-            if constexpr (Cfg::kAside) {
 #pragma unroll 1
-                for (int x = 0; x < 2 && n_tiles > 2 * kPChain + x; x++) {
-                    const float2 e = aside_s[x][0][r];
-                    const int scale = __float_as_int(e.y) - 155;
-                    const float f = e.x > -INFINITY ? exp2_fast(e.x - reference) * inv : 0.0f;
-                    const float s0 = __uint_as_float((uint32_t)(127 + (scale >> 1)) << 23), s1 = __uint_as_float((uint32_t)(127 + scale - (scale >> 1)) << 23);
-                    const float4 *from = p_aside<NB>(a, room_s, x, c) + r;
+            for (int x = 0; x < 2 && n_tiles > 2 * Cfg::kChain + x; x++) {
+                const float2 e = aside_s[x][0][r];
+                const int scale = __float_as_int(e.y) - 155;
+                const float f = e.x > -INFINITY ? exp2_fast(e.x - reference) * inv : 0.0f;
+                const float s0 = __uint_as_float((uint32_t)(127 + (scale >> 1)) << 23), s1 = __uint_as_float((uint32_t)(127 + scale - (scale >> 1)) << 23);
+                const float4 *from = p_aside<NB>(a, room_s, x, c) + r;
 #pragma unroll
-                    for (int k = 0; k < 32; k += 4) {
-                        const float4 o = __ldcg(from + k / 4 * kPRows);
-                        oa[k] = __float_as_uint(__uint_as_float(oa[k]) + o.x * s0 * f * s1);
-                        oa[k + 1] = __float_as_uint(__uint_as_float(oa[k + 1]) + o.y * s0 * f * s1);
-                        oa[k + 2] = __float_as_uint(__uint_as_float(oa[k + 2]) + o.z * s0 * f * s1);
-                        oa[k + 3] = __float_as_uint(__uint_as_float(oa[k + 3]) + o.w * s0 * f * s1);
-                    }
+                for (int k = 0; k < 32; k += 4) {
+                    const float4 o = __ldcg(from + k / 4 * kPRows);
+                    oa[k] = __float_as_uint(__uint_as_float(oa[k]) + o.x * s0 * f * s1);
+                    oa[k + 1] = __float_as_uint(__uint_as_float(oa[k + 1]) + o.y * s0 * f * s1);
+                    oa[k + 2] = __float_as_uint(__uint_as_float(oa[k + 2]) + o.z * s0 * f * s1);
+                    oa[k + 3] = __float_as_uint(__uint_as_float(oa[k + 3]) + o.w * s0 * f * s1);
                 }
             }
 #pragma unroll
@@ -605,7 +603,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
             for (int ks = 0; ks < kPKeys / 16; ks++) {
                 const uint32_t p = tmem + (uint32_t)(w * kPKeys + (ks >> 1) * 32 + (ks & 1) * 8);
 #pragma unroll
-                for (int u = 0; u < PT; u++) at_mma_ts(d, p + u * 16, vd.at(ks * (2048 >> 4)), idesc_o, ((Cfg::kAside ? (t >> 1) % kPChain : t >> 1) | ks | u) != 0 ? 1u : 0u);
+                for (int u = 0; u < PT; u++) at_mma_ts(d, p + u * 16, vd.at(ks * (2048 >> 4)), idesc_o, ((t >> 1) % Cfg::kChain | ks | u) != 0 ? 1u : 0u);
             }
             umma_commit(&v_empty[slot]);
             umma_commit(&o_done[w]);
