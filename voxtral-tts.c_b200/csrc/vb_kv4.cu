@@ -44,8 +44,8 @@ constexpr int kRowThreads = 256, kRowUnroll = 4;
 /* ------------------------------------------------------------------ rows into the cache and out of it
  * A CTA has rows of one head, keys or values; a thread a word of 8 values of a row, four rows at a time with their loads together; four
  * lanes make a block of 32. Memory-bound, and at one row a launch bound by its latency: 4097 bf16 rows of two sequences and 8 heads of 128
- * in and out again, 118 MB, 24 us, 4.8 TB/s; one row of eight sequences in and out 6.5 us, the host's time for two launches. (With words of all heads side by side, indices
- * worked out word by word, 4097 rows of two sequences took 22 us in and 16 out.) */
+ * in and out again as fp32, 118 MB, 24 us, 4.8 TB/s; one row of eight sequences in and out 6.5 us, the host's time for two launches. (With
+ * words of all heads side by side, indices worked out word by word, 4097 rows of two sequences took 22 us in and 16 out.) */
 template <class T>
 struct RowsArgs {
     Kv4 c;

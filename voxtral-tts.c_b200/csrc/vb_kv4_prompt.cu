@@ -11,9 +11,9 @@
  * so far, on which the accumulator is based (exact down to 2^-36 of the largest). Scores, weights, sums as in vb_kv4_attn.cu. Two pairs of
  * warpgroups take alternate tiles with a reference, sums and an accumulator each, merged at the end, so that the tensor pipe works on
  * one tile while the other is in its softmax. A thread has half of a row's columns: with a whole row a thread, and half as many
- * threads, 1203 rows took 206 us in place of 178.
+ * threads, 1203 rows took 206 us in place of 178 (before sums were put aside).
  * Bound by the chain of scores, softmax, results and scores again that a pair goes through: 4100 to 4300 clocks a tile, where the tensor pipe's
- * part of it is 2048 with two terms each. 1203 fp32 rows of 32 heads of 128 over 4208 tokens: 195 us, 360 TFLOP/s (twice that as executed).
+ * part of it is 2048 with two terms each. 1203 fp32 rows of 32 heads of 128 over 4208 tokens: 205 us, 347 TFLOP/s (twice that as executed).
  *
  * Warps: 0-7, 8-15 softmax, 16-19 keys, 20-22 values, 23 issues the MMAs. All waits are bounded.
  */
