@@ -512,6 +512,46 @@ def test_captured_and_replayed(pkg):
     assert torch.allclose(lp.double().cpu(), plain.logprobs(x, tokens, 0)[0], atol=1e-5)
 
 
+def test_portions_captured_and_replayed_side_by_side(pkg):
+    """Portions of many rows of two caches, in graphs on two streams at once, replayed with new lengths and queries: every time the bits of the
+    calls by themselves, which are right; the masses go on from what they were."""
+    g = _gen(67)
+    s, h, heads, d, cap, rows = 2, 4, 16, 128, 3000, 200
+    lengths = [[3000, 700], [200, 2999], [1500, 2200]]
+    base, v0 = _randn(g, s, cap, h, d), _randn(g, s, cap, h, d)
+    qs = [_randn(g, s, rows, heads, d) for _ in lengths]
+    kh, vh = _held(base, None), _held(v0, None)
+    alone, _ = _fill(pkg, base, v0, cap, [cap, cap])
+    want = []
+    for n, q in zip(lengths, qs):
+        out, lse, mass = torch.empty_like(q), torch.empty(s, rows, heads, device="cuda"), torch.ones(s, h, cap, device="cuda")
+        alone.attention(q, out, _ints(*n), lse=lse, mass_in=mass, mass_out=mass)
+        _check_attention(out, lse, q, kh, vh, n, [rows, rows], d ** -0.5, torch.float32, mass, torch.ones(s, h, cap, device="cuda"))
+        want.append((out, lse, mass))
+    sides = []
+    for _ in range(2):
+        cache, at = _fill(pkg, base, v0, cap, [cap, cap])
+        st, graph, q = torch.cuda.Stream(), torch.cuda.CUDAGraph(), qs[0].clone()
+        got = (torch.empty_like(q), torch.empty(s, rows, heads, device="cuda"), torch.ones(s, h, cap, device="cuda"))
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=st):
+            cache.attention(q, got[0], at, lse=got[1], mass_in=got[2], mass_out=got[2], stream=torch.cuda.current_stream().cuda_stream)
+        sides.append((cache, at, q, got, st, graph))
+    for i in range(6):
+        for _, at, q, got, _, _ in sides:
+            at.copy_(_ints(*lengths[i % 3]))
+            q.copy_(qs[i % 3])
+            got[2].fill_(1.0)
+        torch.cuda.synchronize()
+        for *_, st, graph in sides:
+            with torch.cuda.stream(st):
+                graph.replay()
+        torch.cuda.synchronize()
+        for cache, _, _, got, _, _ in sides:
+            cache.check()
+            assert all(torch.equal(x, y) for x, y in zip(got, want[i % 3]))
+
+
 def test_two_caches_at_once(pkg):
     """Attention of two caches on two streams side by side, many times: workspaces are a cache's own."""
     g = _gen(61)
