@@ -742,8 +742,8 @@ int attn_launch(const Kv4Attn &args, const vb200_kv4_attention_t &v, const Kv4Wo
     a.wide_out = serve_wide(out);
     /* Eight pairs against n tokens cost 32 ps n here and 128 pairs 181 ps n on the tensor cores' kernel, which takes 17 us more to begin
      * and to join (fp32, heads of 128; the other types and sizes cross at about the same place). Measured, here and there in us: 8 heads, 1024
-     * tokens, 128 and 512 pairs each 15, 30 and 29, 38; 8192 tokens, 64 and 128 pairs 30, 34 and 50, 40; 65536 tokens, 32 and 64 pairs 83, 100 and
-     * 168, 102; 64 heads, 1024 tokens, 64 and 128 pairs 30, 37 and 51, 47. The tokens are the cache's room for them: lengths are not
+     * tokens, 256 and 512 pairs each 17, 30 and 29, 39; 8192 tokens, 64 and 128 pairs 31, 52 and 33, 44; 65536 tokens, 32 and 64 pairs 86, 176 and
+     * 107, 110; 64 heads, 1024 tokens, 64 and 128 pairs 31, 52 and 35, 46. The tokens are the cache's room for them: lengths are not
      * known here. */
     const long long pairs = (long long)a.max_rows * a.group, room = (long long)a.c.capacity * a.c.kv_heads * a.c.seqs;
     if (NB <= 4 && (double)room * (double)((pairs + 7) / 8 - 6 * ((pairs + 127) / 128)) > 550e3) {
