@@ -295,6 +295,7 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(co
                     }
                 }
             }
+            __syncwarp();                                /* columns rise by themselves; a transposition takes the whole warp */
         }
         /* weights, turned into the B operand of V^T P^T */
         uint2 p[2][PT];
@@ -687,6 +688,7 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_mass_kernel(co
 #pragma unroll 1
             for (int r = 0; r < made; r++) {
                 float s[2][4];
+                __syncwarp();                            /* lanes differ in what they have added up */
 #pragma unroll
                 for (int b = 0; b < NB; b++) {
                     uint2 qf[2][QT];

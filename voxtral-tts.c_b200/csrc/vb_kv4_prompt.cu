@@ -158,6 +158,7 @@ __device__ __noinline__ void p_put_aside(float4 *mine, float2 *base, uint32_t tO
             }
     }
     if (first || rebase) *base = make_float2(ref, __int_as_float(top_scale));
+    __syncwarp();                                      /* rows of a warp differ in that; what follows takes all of them together */
 #pragma unroll 1
     for (int c = half; c < NB; c += 2) {
         uint32_t reg[32];
@@ -314,7 +315,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
 #pragma unroll
                 for (int k = 4; k < 32; k++) m4[k & 3] = fmaxf(m4[k & 3], __uint_as_float(reg[k]));
                 const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-                if (m > -INFINITY) top = fmaxf(top, m * (ups[half * 2 + c] * mul));
+                top = m > -INFINITY ? fmaxf(top, m * (ups[half * 2 + c] * mul)) : top;
+                __syncwarp();                          /* lanes are together where the next columns are read */
             }
             /* the other half's: it has been read by then when it is written again, since the next tile's scores wait for both halves */
             top_s[w][half][r] = top;
@@ -411,6 +413,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
         for (int c = wg; c < NB; c += kPSoft / 128) {
             uint32_t oa[32], ob[32];
             const bool nan = bad_s[c] < sees;
+            __syncwarp();
             if (n_tiles > 0) at_ld32(tmem + lanes + kPO + (uint32_t)(c * 32), oa);
             if (n_tiles > 1) at_ld32(tmem + lanes + kPO + 128u + (uint32_t)(c * 32), ob);
 #pragma unroll
@@ -787,6 +790,7 @@ __global__ void __launch_bounds__(kWThreads, 1) kv4_mass_many_kernel(const Kv4At
 #pragma unroll 1
             for (int c = 0; c < 4; c++) {
                 uint32_t s[32];
+                __syncwarp();
                 at_ld32(tS + (uint32_t)(c * 32), s);
                 const float4 *of = reinterpret_cast<const float4 *>(&pair_s[t % kWRing][c * 32]);
 #pragma unroll
