@@ -50,7 +50,7 @@ typedef struct {
  * does not count. */
 typedef struct vb200_kv4 vb200_kv4_t;
 
-/* head_dim: 32, 64, 96, 128, 192 or 256; at most 65535 seqs, 16384 kv_heads, 2^30 tokens. */
+/* head_dim: 32, 64, 96, 128, 192 or 256; at most 65535 seqs, 16384 kv_heads, 2^30 tokens, 2^40 bytes of rows. */
 vb200_kv4_t *vb200_kv4_open(int seqs, int kv_heads, int head_dim, int capacity);
 void vb200_kv4_close(vb200_kv4_t *cache);
 size_t vb200_kv4_bytes(const vb200_kv4_t *cache);      /* device memory it holds */

@@ -384,6 +384,11 @@ vb200_kv4_t *vb200_kv4_open(int seqs, int kv_heads, int head_dim, int capacity) 
         serve_fail("seqs have to be 1 to 65535, kv_heads 1 to 16384, capacity 1 to 2^30");
         return nullptr;
     }
+    /* in 128 bits: sizes within these limits can pass 64 */
+    if ((unsigned __int128)seqs * kv_heads * ((capacity + kKv4Tile - 1) / kKv4Tile * kKv4Tile) * (head_dim + head_dim / 16) > (unsigned __int128)1 << 40) {
+        serve_fail("seqs, kv_heads, capacity and head_dim have to be less: rows of more than 2^40 bytes");
+        return nullptr;
+    }
     int dev = 0, major = 0, minor = 0, n_sm = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess ||
         cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev) != cudaSuccess ||
