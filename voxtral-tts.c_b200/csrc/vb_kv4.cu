@@ -4,6 +4,7 @@
  */
 #include <algorithm>
 #include <limits.h>
+#include <stdio.h>
 #include <new>
 #include <string>
 
@@ -35,6 +36,23 @@ bool serve_on_device(const void *p) {
         return false;
     }
     return at.type == cudaMemoryTypeManaged || (at.type == cudaMemoryTypeDevice && at.device == now);
+}
+int serve_check(std::initializer_list<ServePointer> pointers) {
+    int now = -1;
+    cudaGetDevice(&now);
+    for (const ServePointer &x : pointers) {
+        if (!x.p) continue;
+        cudaPointerAttributes at;
+        if (cudaPointerGetAttributes(&at, x.p) != cudaSuccess) {
+            cudaGetLastError();
+            at.type = cudaMemoryTypeUnregistered;
+        }
+        if ((at.type == cudaMemoryTypeDevice && at.device == now) || at.type == cudaMemoryTypeManaged || (at.type == cudaMemoryTypeHost && at.devicePointer == x.p)) continue;
+        char what[96];
+        snprintf(what, sizeof what, "%s does not lie on the current device", x.name);
+        return serve_fail(what);
+    }
+    return 0;
 }
 
 namespace {
@@ -354,8 +372,9 @@ int check_rows(const vb200_kv4 *h, const vb200_kv4_rows_t *a) {
     if (((uintptr_t)a->k.data | (uintptr_t)a->v.data) % serve_size(a->k.type)) return serve_fail("k and v have to be aligned to their elements");
     int now = -1;
     if (cudaGetDevice(&now) != cudaSuccess || now != h->device) return serve_fail("the cache lies on another device than the current one");
-    if (a->max_rows > 0 && !serve_on_device(a->k.data)) return serve_fail("k does not lie on the current device");
-    return 0;
+    if (a->max_rows == 0) return 0;
+    if (!serve_on_device(a->k.data)) return serve_fail("k does not lie on the current device");
+    return serve_check({{a->v.data, "v"}, {a->lengths, "lengths"}, {a->rows, "rows"}});
 }
 
 int rows_call(const vb200_kv4 *h, const vb200_kv4_rows_t *a, bool read, cudaStream_t st) {
@@ -473,6 +492,7 @@ int vb200_kv4_evict(vb200_kv4_t *h, vb200_kv4_t *into, const vb200_kv4_evict_t *
     int now = -1;
     if (cudaGetDevice(&now) != cudaSuccess || now != h->device || into->device != h->device) return serve_fail("a cache lies on another device than the current one");
     if (!serve_on_device(a->mass)) return serve_fail("mass does not lie on the current device");
+    if (serve_check({{a->lengths, "lengths"}, {a->new_lengths, "new_lengths"}, {a->new_mass, "new_mass"}, {a->kept, "kept"}})) return -1;
     const cudaStream_t st = (cudaStream_t)stream;
     EvictArgs e = {h->c, into->c, a->lengths, a->new_lengths, a->mass, a->new_mass, a->new_mass_ld, a->kept, a->keep, a->recent, a->first, into == h};
     cudaError_t err = launch_pdl(kv4_select_kernel, dim3(h->c.kv_heads, h->c.seqs), dim3(kSelThreads), select_smem(h->c.capacity), st, e);
@@ -502,6 +522,8 @@ int vb200_kv4_attention(vb200_kv4_t *h, const vb200_kv4_attention_t *a, void *st
     if (cudaGetDevice(&now) != cudaSuccess || now != h->device) return serve_fail("the cache lies on another device than the current one");
     if (a->max_rows > 0 && !serve_on_device(a->q.data)) return serve_fail("q does not lie on the current device");
     if (a->max_rows == 0 && !a->mass_out) return 0;
+    if (a->max_rows > 0 && serve_check({{a->out.data, "out"}, {a->lse, "lse"}})) return -1;
+    if (serve_check({{a->lengths, "lengths"}, {a->rows, "rows"}, {a->mass_in, "mass_in"}, {a->mass_out, "mass_out"}})) return -1;
     return kv4_attention(h->c, h->w, *a, (cudaStream_t)stream);
 }
 

@@ -421,6 +421,7 @@ extern "C" int vb200_token_logprobs(const vb200_logprobs_t *a, void *stream) {
         return serve_fail("an sm_100 GPU is required (there is no CPU fallback)");
     }
     if (!serve_on_device(a->logits)) return serve_fail("logits do not lie on the current device");
+    if (serve_check({{a->tokens, "tokens"}, {a->logprobs, "logprobs"}, {a->entropy, "entropy"}, {a->top_ids, "top_ids"}, {a->top_logprobs, "top_logprobs"}})) return -1;
     const bool tops = a->top_ids || a->top_logprobs;
     const LpArgs l = {a->logits, a->row_stride, a->rows, a->vocab, tops ? a->top : 0, a->tokens, a->logprobs, a->entropy, a->top_ids, a->top_logprobs};
     const cudaStream_t st = (cudaStream_t)stream;

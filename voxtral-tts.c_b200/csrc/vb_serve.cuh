@@ -7,6 +7,8 @@
 
 #include <cuda_fp16.h>
 
+#include <initializer_list>
+
 #include "../../include/voxtral_b200_serve.h"
 #include "vb_common.cuh"
 
@@ -16,8 +18,15 @@ namespace vb {
 /* Says why a call failed; returns -1. */
 int serve_fail(const char *what);
 int serve_launched();                                     /* 0, or -1 with the launch's error */
-/* Whether `p` may be read by a kernel of the current device. */
+/* Whether `p` lies on the current device (or is managed memory). */
 bool serve_on_device(const void *p);
+/* 0 where all of them are NULL or memory that a kernel of the current device may use (host memory that is mapped, too); -1 with the name of the
+ * first that is not. What a kernel does with other pointers is a fault of the GPU's. */
+struct ServePointer {
+    const void *p;
+    const char *name;
+};
+int serve_check(std::initializer_list<ServePointer> pointers);
 
 template <class T>
 struct ServeRows {                                        /* vb200_rows_t with its type */
