@@ -75,3 +75,92 @@ def test_host_memory_is_refused_wherever_it_is_given(pkg):
     assert L.vb200_kv4_append(cache.h, C.byref(serve._AppendArgs(**dict(move, lengths=pinned.data_ptr()))), None) == 0
     torch.cuda.synchronize()
     cache.check()
+
+
+def _check_by_component(out, lse, q, k, v, rows, scale, dtype, mass=None):
+    """Against 64 bits, every result within its own roundings: those of sum p |v| and of sum |q k|, whatever the largest |v| and |k| of the
+    cache are. One sequence; k, v [H, n, D] as they are held."""
+    n, heads, h = k.shape[1], q.shape[2], k.shape[0]
+    g = heads // h
+    want, want_lse, want_mass = plain.attention(q[0], k, v, n, rows, scale)
+    d = k.shape[-1]
+    for u in range(heads):
+        kk, vv = k[u // g].double(), v[u // g].double()
+        for i in range(rows):
+            sees = n - rows + i + 1
+            if sees <= 0:
+                continue
+            p = torch.exp(kk[:sees] @ q[0, i, u].double() * scale - want_lse[i, u])
+            sums = float((kk[:sees].abs() @ q[0, i, u].double().abs() * abs(scale)).amax())
+            # as attention_bounds derives them, of this row's own largest sum of magnitudes
+            score = sums * ((2 * d // 32 + 4) * 2.0 ** -23 + 2.0 ** -22 + 4 * 2.0 ** -24 + 2.0 ** -21)
+            weight = 2 * score + 2.0 ** -19 + (2.0 ** -11 if dtype == torch.bfloat16 else 0.0) + (n / 8 + 16) * 2.0 ** -23
+            limit = (p @ vv[:sees].abs()) * weight + want[i, u].abs() * torch.finfo(dtype).eps / 2 + torch.finfo(dtype).tiny
+            err = (out[0, i, u].double() - want[i, u]).abs()
+            assert (err <= limit).all(), (u, i, float((err / limit).max()))
+            assert abs(float(lse[0, i, u].double() - want_lse[i, u])) <= score + 2.0 ** -18 + abs(float(want_lse[i, u])) * 2.0 ** -23
+    if mass is not None:
+        sums = float((k.abs().double() @ q[0, :rows].double().abs().flatten(0, 1).T * abs(scale)).amax())
+        score = sums * ((2 * d // 32 + 4) * 2.0 ** -23 + 2.0 ** -20)
+        assert ((mass[0, :, :n].double() - want_mass).abs() <= want_mass * (2 * score + 2.0 ** -18) + 1e-30).all()
+
+
+FAR = [(1, 4, 1, 64, 400), (5, 2, 1, 128, 300), (3, 4, 2, 96, 200)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,heads,kv_heads,dim,n", FAR)
+def test_large_values_of_tokens_that_weigh_little(pkg, rows, heads, kv_heads, dim, n, dtype):
+    """Every eighth token's values are 2^40 times the others' (2^14 in fp16, which has no more) and its weight 2^-45 (2^-19)."""
+    g, t = _gen(79), TYPES[dtype]
+    far = 14 if dtype == "f16" else 40
+    k, v = torch.zeros(1, n, kv_heads, dim, device="cuda"), _randn(g, 1, n, kv_heads, dim)
+    k[:, ::8, :, 0] = -4.0
+    k[:, ::8, :, 1] = 0.5
+    v = v / 64.0 if dtype == "f16" else v
+    v[:, ::8] = (v[:, ::8] * 2.0 ** far).clamp(-60000.0, 60000.0) if dtype == "f16" else v[:, ::8] * 2.0 ** far
+    k, v = k.to(t), v.to(t)
+    cache, at = _fill(pkg, k, v, n, [n])
+    q = (_randn(g, 1, rows, heads, dim) * 0.1).to(t)
+    q[..., 0] = (far + 5) * math.log(2.0) / 4.0
+    out, lse = torch.full_like(q, 3.0), torch.full((1, rows, heads), 4.0, device="cuda")
+    cache.attention(q, out, at, scale=1.0, lse=lse)
+    cache.check()
+    _check_by_component(out, lse, q, _held(k, None)[0], _held(v, None)[0], rows, 1.0, t)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("big", [20, 50, 100, 120])
+@pytest.mark.parametrize("rows,heads,kv_heads,dim,n", FAR)
+def test_large_values_that_a_row_does_not_see(pkg, rows, heads, kv_heads, dim, n, big, dtype):
+    """The portion's tokens have values 2^big times the cache's, each four times the one before: rows that see none of a token's have nothing of it."""
+    g, t = _gen(83), TYPES[dtype]
+    k, v = _randn(g, 1, n, kv_heads, dim), _randn(g, 1, n, kv_heads, dim)
+    for i in range(min(rows - 1, 3)):
+        v[:, n - 1 - i] *= 2.0 ** (big - 2 * i)
+    k, v = k.to(t), v.to(t)
+    cache, at = _fill(pkg, k, v, n, [n])
+    q = _randn(g, 1, rows, heads, dim, dtype=t)
+    out, lse = torch.full_like(q, 3.0), torch.full((1, rows, heads), 4.0, device="cuda")
+    cache.attention(q, out, at, lse=lse)
+    cache.check()
+    _check_by_component(out, lse, q, _held(k, None)[0], _held(v, None)[0], rows, dim ** -0.5, t)
+
+
+def test_blocks_of_zeros(pkg):
+    """Blocks of zeros beside others, and nothing but zeros: no scale of theirs stands in anything's way."""
+    g = _gen(89)
+    for rows in (1, 3):
+        n, h, heads, d = 300, 2, 4, 128
+        k, v = _randn(g, 1, n, h, d), _randn(g, 1, n, h, d)
+        k[:, ::3, :, :32], v[:, ::5, :, 64:], v[:, 7::11] = 0.0, 0.0, -0.0
+        v[:, :, 1, 32:64] = 0.0
+        cache, at = _fill(pkg, k, v, n, [n])
+        gk, gv = torch.empty_like(k), torch.empty_like(v)
+        cache.read(gk, gv, at)
+        assert torch.equal(gk.double(), plain.rounded(k)) and torch.equal(gv.double(), plain.rounded(v))
+        q = _randn(g, 1, rows, heads, d)
+        out, lse = torch.full_like(q, 3.0), torch.empty(1, rows, heads, device="cuda")
+        cache.attention(q, out, at, lse=lse)
+        _check_by_component(out, lse, q, _held(k, None)[0], _held(v, None)[0], rows, d ** -0.5, torch.float32)
+        assert (out[0, :, 2:, 32:64] == 0).all()

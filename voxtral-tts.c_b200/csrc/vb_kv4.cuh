@@ -181,6 +181,107 @@ VB_DEVINL Kv4Place kv4_place(const Kv4Attn &a, int round, int least, int most_sp
     return {a.c.seqs, 0, 0, share};
 }
 
+/* ------------------------------------------------------------------ scales too far apart
+ * The tensor cores take values as FP16, based on the largest scale: exact where scales lie within 2^36 of one another. A CTA that meets others
+ * (kv4_far; scales that have risen by more than kKv4Rise: what a row has of smaller ones fell with them) works its part out again here, in fp32 and
+ * with bases of a row's own, so that what a row does not see does not reach it and a large value that weighs little leaves the others as they are. A
+ * function of its own: inlined into vb_kv4_attn.cu's loop for a tile at a time it cost every call 5 % (four sequences of 131072 tokens
+ * 98 -> 104 us). 40 times slower than the tensor cores. */
+constexpr int kKv4Rise = 64;
+constexpr int kKv4Rest = 8;                   /* sums and results of a part are held times 2^-8 */
+
+/* 2^e, |e| up to 252, as a product of two */
+VB_DEVINL float2 kv4_power(int e) { return make_float2(__uint_as_float((uint32_t)(127 + (e >> 1)) << 23), __uint_as_float((uint32_t)(127 + e - (e >> 1)) << 23)); }
+
+/* A head's planes */
+struct Kv4Head {
+    const uint8_t *k, *v, *ks, *vs;
+};
+template <int NB>
+VB_DEVINL Kv4Head kv4_head(const Kv4 &c, size_t row0) { return {c.k + row0 * (NB * 16), c.v + row0 * (NB * 16), c.ks + row0 * NB, c.vs + row0 * NB}; }
+
+/* A query row over the rows tok0 .. tok1 of a head, by a warp: its reference and sum; results [NB * 32] in out_s. q_s has room for a row. (By
+ * value: a reference to a kernel's arguments has all of them copied to the stack first.) */
+template <int NB, class T>
+__device__ __noinline__ float2 kv4_plain_row(Kv4Head c, const T *q, float scale, int tok0, int tok1, float *q_s, float *out_s) {
+    constexpr int kDim = NB * 32;
+    const int lane = threadIdx.x & 31;
+    uint32_t most = 0;
+    for (int d = lane; d < kDim; d += 32) most = max(most, __float_as_uint(serve_get(q + d)) & 0x7fffffffu);
+    most = __reduce_max_sync(0xffffffffu, most);
+    /* the largest to [2^14, 2^15), as on the tensor cores: no product of finite numbers passes fp32 */
+    const uint32_t e = most >> 23, field = e == 0u || e == 255u ? 127u : min(268u - e, 253u);
+    const float up = __uint_as_float(field << 23), mul = scale * 1.44269504f * __uint_as_float((254u - field) << 23);
+    __syncwarp();
+    for (int d = lane; d < kDim; d += 32) q_s[d] = serve_get(q + d) * up;
+    __syncwarp();
+    float ref = -INFINITY, sum = 0.0f, o[NB];
+    int base[NB];
+    uint32_t nan = 0;
+#pragma unroll
+    for (int i = 0; i < NB; i++) o[i] = 0.0f, base[i] = 0;
+    for (int j0 = tok0; j0 < tok1; j0 += 32) {
+        /* scores: a lane a token */
+        const int j = j0 + lane, n = min(32, tok1 - j0);
+        const size_t row = min(j, tok1 - 1);
+        float s = 0.0f;
+#pragma unroll 1
+        for (int b = 0; b < NB; b++) {
+            float sums = 0.0f;
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                uint32_t h[4];
+                kv4_halves(*reinterpret_cast<const uint32_t *>(c.k + row * (NB * 16) + (t * NB + b) * 4), h);
+                const float4 x = *reinterpret_cast<const float4 *>(q_s + 32 * b + 8 * t), y = *reinterpret_cast<const float4 *>(q_s + 32 * b + 8 * t + 4);
+                const float2 k0 = kv4_f2(h[0]), k1 = kv4_f2(h[1]), k2 = kv4_f2(h[2]), k3 = kv4_f2(h[3]);
+                sums = fmaf(k0.x, x.x, fmaf(k0.y, x.y, fmaf(k1.x, x.z, fmaf(k1.y, x.w, sums))));
+                sums = fmaf(k2.x, y.x, fmaf(k2.y, y.y, fmaf(k3.x, y.z, fmaf(k3.y, y.w, sums))));
+            }
+            const uint32_t byte = c.ks[row * NB + b];
+            const float2 f = kv4_power((int)min(byte, 252u) - 127);
+            s += byte == 255u ? __uint_as_float(0x7fffffffu) : sums == 0.0f ? 0.0f : sums * f.x * mul * f.y;
+        }
+        if (j >= tok1) s = -INFINITY;
+        float top = s;
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        const float now = fmaxf(ref, top), fall = ref > -INFINITY ? exp2_fast(ref - now) : 0.0f;
+        ref = now;
+        const float p = j >= tok1 ? 0.0f : exp2_fast(s - (ref > -INFINITY ? ref : 0.0f));
+        float all = p;
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) all += __shfl_xor_sync(0xffffffffu, all, x);
+        sum = fmaf(sum, fall, all);
+        /* values: a lane one of every block */
+#pragma unroll
+        for (int i = 0; i < NB; i++) {
+            const uint32_t byte = j < tok1 ? c.vs[row * NB + i] : 0u;
+            if (__any_sync(0xffffffffu, byte == 255u)) nan |= 1u << i;
+            const int rise = max(0, (int)__reduce_max_sync(0xffffffffu, byte == 255u ? 0u : byte) - base[i]);
+            base[i] += rise;
+            o[i] *= rise > 126 ? 0.0f : fall * __uint_as_float((uint32_t)(127 - rise) << 23);
+            const int u = 8 * i + (lane >> 2), at = kv4_value_half(u, NB) * 2 + ((lane & 3) >> 1), shift = (lane & 1) * 4;
+            float part = 0.0f;
+#pragma unroll 4
+            for (int x = 0; x < n; x++) {
+                const uint32_t there = __shfl_sync(0xffffffffu, byte, x), w = (c.v[(size_t)(j0 + x) * (NB * 16) + at] >> shift) & 15u;
+                uint32_t h[4];
+                kv4_halves(w, h);
+                const float2 f = kv4_power(there == 255u ? 0 : (int)there - base[i]);
+                part += kv4_f2(h[0]).x * (__shfl_sync(0xffffffffu, p, x) * f.x) * f.y;
+            }
+            o[i] += part;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+        const float2 f = kv4_power(base[i] - 127 - kKv4Rest);
+        out_s[32 * i + lane] = nan >> i & 1 ? __uint_as_float(0x7fffffffu) : o[i] * f.x * f.y;
+    }
+    __syncwarp();
+    return make_float2(ref, sum * (1.0f / (1 << kKv4Rest)));
+}
+
 /* Many rows, heads up to 128 (vb_kv4_prompt.cu) */
 template <class T>
 int kv4_prompt(const Kv4Attn &a, const ServeRows<T> &q, const ServeRows<T> &out, int sm_count, cudaStream_t st);

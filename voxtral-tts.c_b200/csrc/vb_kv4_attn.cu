@@ -221,9 +221,10 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(co
     for (int i = 0; i < 2 * NB; i++)
 #pragma unroll
         for (int j = 0; j < 4; j++) o[i][j] = 0.0f;
-    int top_scale[kVS];
+    int top_scale[kVS], first_scale[kVS];
+    bool far = false;
 #pragma unroll
-    for (int i = 0; i < kVS; i++) top_scale[i] = 0;
+    for (int i = 0; i < kVS; i++) top_scale[i] = first_scale[i] = 0;
 
     int stage = 0;
     uint32_t parity = 0;
@@ -386,7 +387,9 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(co
                 const int up = most[i] - top_scale[i];
                 if (up > 0) {
                     const float fall = up > 126 ? 0.0f : __uint_as_float((uint32_t)(127 - up) << 23);
+                    if (top_scale[i] == 0) first_scale[i] = most[i];
                     top_scale[i] = most[i];
+                    far |= most[i] - first_scale[i] > kKv4Rise;
 #pragma unroll
                     for (int r = 0; r < 2 * NB; r++)
                         if (Cfg::kWhole || r / 2 == i) {
@@ -416,6 +419,7 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(co
                 for (int m = 0; m < 2; m++)
 #pragma unroll
                     for (int x = 0; x < 2; x++) {
+                        far |= kv4_far(vsc[m][x][i] & 0xffffu, top_scale[i]) || kv4_far(vsc[m][x][i] >> 16, top_scale[i]);
                         const int lo = (int)(vsc[m][x][i] & 0xffffu) + 140 - top_scale[i], hi = (int)(vsc[m][x][i] >> 16) + 140 - top_scale[i];
                         vsc[m][x][i] = half_pack(__uint_as_float((uint32_t)max(lo, 0) << 23), __uint_as_float((uint32_t)max(hi, 0) << 23));
                     }
@@ -470,7 +474,7 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(co
         for (int x = 4; x < 32; x <<= 1) sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], x);
         sum[u] *= 0x1p-15f;
     }
-    __syncthreads();                                     /* every ring is empty */
+    const bool plain = __syncthreads_or(far);            /* every ring is empty */
     constexpr int kUnits = 2 * NB * 32;                  /* of four results */
     float4 *mo = reinterpret_cast<float4 *>(a_smem);
     float2 *mm = reinterpret_cast<float2 *>(mo + kAWarps * kUnits), *ml = mm + kAWarps * 4;
@@ -512,7 +516,32 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(co
     };
     /* a part's factor against a reference; parts without weights have none */
     auto factor = [](float m, float reference) { return m > -INFINITY || m != m ? exp2_fast(m - reference) : 0.0f; };
-    {
+    if (plain) {
+        __syncthreads();
+        const int pair = pair0 + warp, row = pair / a.group, head = kv_head * a.group + pair - row * a.group;
+        const int tok0 = used == 1 ? 0 : split * share * kAKeys;
+        if (warp < n_pairs) {
+            float *q_row = reinterpret_cast<float *>(a_smem) + warp * 2 * kDim, *results = q_row + kDim;
+            const float2 end = kv4_plain_row<NB, T>(kv4_head<NB>(a.c, row0), q.data + seq * q.seq + row * q.row + head * q.head, a.scale, tok0,
+                                                    min(min(t_end * kAKeys, seen), before + row + 1), q_row, results);
+            float *part = parts + split * step;
+            const float inv = end.y == 0.0f ? 0.0f : 1.0f / end.y;
+            for (int d = lane; d < kDim; d += 32) {
+                if (used == 1) {
+                    serve_put(out.data + seq * out.seq + row * out.row + head * out.head + d, end.y == 0.0f ? 0.0f : results[d] * inv);
+                } else {                                 /* in the accumulators' order */
+                    const int gd = Cfg::kWhole ? d / (4 * NB) : d % 32 / 4, i = Cfg::kWhole ? d % (4 * NB) / 2 : d / 32 * 2 + d % 4 / 2;
+                    part[((i * 32 + gd * 4 + (warp >> 1)) * 2 + (d & 1)) * 2 + (warp & 1)] = results[d];
+                }
+            }
+            if (lane == 0 && used == 1 && a.lse) a.lse[((size_t)seq * a.max_rows + row) * a.heads + head] = end.y == 0.0f ? -INFINITY : (end.x + 8.0f + log2f(end.y)) * 0.69314718f;
+            if (lane == 0 && used > 1) {
+                part[kACols * kDim + warp] = end.x;
+                part[kACols * kDim + 8 + warp] = end.y;
+            }
+        }
+        if (used == 1) return;
+    } else {
         float2 reference = make_float2(-INFINITY, -INFINITY), total = make_float2(0.0f, 0.0f), f[kAWarps];
 #pragma unroll
         for (int w = 0; w < kAWarps; w++) {

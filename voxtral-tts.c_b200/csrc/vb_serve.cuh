@@ -72,12 +72,17 @@ VB_DEVINL Kv4Span kv4_span(const int *lengths, const int *rows, int max_rows, in
 }
 
 /* ------------------------------------------------------------------ the format */
-/* Scale byte of a block: `most` its largest magnitude, infinite or NaN where a value is. Subnormal numbers have the byte of 2^-126. */
+/* Scale byte of a block: `most` its largest magnitude, infinite or NaN where a value is. Subnormal numbers have the byte of 2^-126, a block of
+ * zeros 0: it is not far below any other. */
 VB_DEVINL uint32_t kv4_scale(float most) {
     const uint32_t e = __float_as_uint(most) >> 23;
-    return e == 255u ? 255u : e <= 3u ? 1u : e - 2u;
+    return e == 255u ? 255u : most == 0.0f ? 0u : e <= 3u ? 1u : e - 2u;
 }
-/* 1 / scale, for bytes 1 .. 252: exact */
+/* A block with this byte is not exact in FP16 based on the scale byte `top`: its least value, half a scale, lies below FP16's smallest step
+ * where `top` stands for 2^13. */
+constexpr int kKv4Range = 36;
+VB_DEVINL bool kv4_far(uint32_t byte, int top) { return byte != 0u && byte != 255u && (int)byte + kKv4Range < top; }
+/* 1 / scale, for bytes 1 .. 252: exact (0: any finite number does) */
 VB_DEVINL float kv4_inverse(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
 /* Eight values times `inv` as codes (byte i: values 2 i, 2 i + 1). */
 VB_DEVINL uint32_t kv4_codes(const float (&x)[8], float inv) {
