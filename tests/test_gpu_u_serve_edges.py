@@ -77,40 +77,43 @@ def test_host_memory_is_refused_wherever_it_is_given(pkg):
     cache.check()
 
 
-def _check_by_component(out, lse, q, k, v, rows, scale, dtype, mass=None):
+def _check_by_component(out, lse, q, k, v, rows, scale, dtype, mass=None, before=None):
     """Against 64 bits, every result within its own roundings: those of sum p |v| and of sum |q k|, whatever the largest |v| and |k| of the
     cache are. One sequence; k, v [H, n, D] as they are held."""
-    n, heads, h = k.shape[1], q.shape[2], k.shape[0]
+    n, heads, h, d = k.shape[1], q.shape[2], k.shape[0], k.shape[-1]
     g = heads // h
-    want, want_lse, want_mass = plain.attention(q[0], k, v, n, rows, scale)
-    d = k.shape[-1]
+    sees = torch.arange(n, device="cuda")[None] < torch.arange(n - rows + 1, n + 1, device="cuda")[:, None]
+    want_mass = torch.zeros(h, n, dtype=torch.float64, device="cuda")
+    mass_limit = torch.zeros_like(want_mass)
     for u in range(heads):
-        kk, vv = k[u // g].double(), v[u // g].double()
-        for i in range(rows):
-            sees = n - rows + i + 1
-            if sees <= 0:
-                continue
-            p = torch.exp(kk[:sees] @ q[0, i, u].double() * scale - want_lse[i, u])
-            sums = float((kk[:sees].abs() @ q[0, i, u].double().abs() * abs(scale)).amax())
-            # as attention_bounds derives them, of this row's own largest sum of magnitudes
-            score = sums * ((2 * d // 32 + 4) * 2.0 ** -23 + 2.0 ** -22 + 4 * 2.0 ** -24 + 2.0 ** -21)
-            weight = 2 * score + 2.0 ** -19 + (2.0 ** -11 if dtype == torch.bfloat16 else 0.0) + (n / 8 + 16) * 2.0 ** -23
-            limit = (p @ vv[:sees].abs()) * weight + want[i, u].abs() * torch.finfo(dtype).eps / 2 + torch.finfo(dtype).tiny
-            err = (out[0, i, u].double() - want[i, u]).abs()
-            assert (err <= limit).all(), (u, i, float((err / limit).max()))
-            assert abs(float(lse[0, i, u].double() - want_lse[i, u])) <= score + 2.0 ** -18 + abs(float(want_lse[i, u])) * 2.0 ** -23
+        kk, vv, qq = k[u // g].double(), v[u // g].double(), q[0, :rows, u].double()
+        s = torch.where(sees, qq @ kk.T * scale, -math.inf)
+        total = torch.logsumexp(s, 1, keepdim=True)
+        p = torch.exp(s - total)
+        want = p @ vv
+        sums = torch.where(sees, qq.abs() @ kk.abs().T * abs(scale), 0.0)
+        # as attention_bounds derives them, of the weights that count: those of a row by their own sums of magnitudes
+        score = sums * ((2 * d // 32 + 4) * 2.0 ** -23 + 2.0 ** -22 + 4 * 2.0 ** -24 + 2.0 ** -21)
+        of_sum = (p * score).sum(1, keepdim=True)
+        weight = p * (score + of_sum + 2.0 ** -19 + (2.0 ** -11 if dtype == torch.bfloat16 else 0.0) + (n / 8 + 16) * 2.0 ** -23)
+        limit = weight @ vv.abs() + want.abs() * torch.finfo(dtype).eps / 2 + torch.finfo(dtype).tiny
+        err = (out[0, :rows, u].double() - want).abs()
+        assert (err <= limit).all(), (u, float((err / limit).max()))
+        assert ((lse[0, :rows, u, None].double() - total).abs() <= of_sum + 2.0 ** -18 + total.abs() * 2.0 ** -23).all()
+        want_mass[u // g] += p.sum(0)
+        mass_limit[u // g] += (p * (score + of_sum + 2.0 ** -18)).sum(0)
     if mass is not None:
-        sums = float((k.abs().double() @ q[0, :rows].double().abs().flatten(0, 1).T * abs(scale)).amax())
-        score = sums * ((2 * d // 32 + 4) * 2.0 ** -23 + 2.0 ** -20)
-        assert ((mass[0, :, :n].double() - want_mass).abs() <= want_mass * (2 * score + 2.0 ** -18) + 1e-30).all()
+        assert ((mass[0, :, :n].double() - want_mass).abs() <= mass_limit + 2.0 ** -24 * (want_mass + before[0, :, :n])).all()
 
 
-FAR = [(1, 4, 1, 64, 400), (5, 2, 1, 128, 300), (3, 4, 2, 96, 200)]
+# rows, heads, KV heads, head_dim, tokens, capacity: a few rows; many, as a unit alone, in parts and in a last round of parts
+FAR = [(1, 4, 1, 64, 400, 400), (5, 2, 1, 128, 300, 300), (3, 4, 2, 96, 200, 200), (80, 2, 1, 64, 200, 200000), (70, 4, 2, 128, 5000, 120000), (90, 2, 2, 96, 9000, 120000),
+       (65, 150, 150, 32, 2100, 2100)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("rows,heads,kv_heads,dim,n", FAR)
-def test_large_values_of_tokens_that_weigh_little(pkg, rows, heads, kv_heads, dim, n, dtype):
+@pytest.mark.parametrize("rows,heads,kv_heads,dim,n,capacity", FAR)
+def test_large_values_of_tokens_that_weigh_little(pkg, rows, heads, kv_heads, dim, n, capacity, dtype):
     """Every eighth token's values are 2^40 times the others' (2^14 in fp16, which has no more) and its weight 2^-45 (2^-19)."""
     g, t = _gen(79), TYPES[dtype]
     far = 14 if dtype == "f16" else 40
@@ -120,7 +123,7 @@ def test_large_values_of_tokens_that_weigh_little(pkg, rows, heads, kv_heads, di
     v = v / 64.0 if dtype == "f16" else v
     v[:, ::8] = (v[:, ::8] * 2.0 ** far).clamp(-60000.0, 60000.0) if dtype == "f16" else v[:, ::8] * 2.0 ** far
     k, v = k.to(t), v.to(t)
-    cache, at = _fill(pkg, k, v, n, [n])
+    cache, at = _fill(pkg, k, v, capacity, [n])
     q = (_randn(g, 1, rows, heads, dim) * 0.1).to(t)
     q[..., 0] = (far + 5) * math.log(2.0) / 4.0
     out, lse = torch.full_like(q, 3.0), torch.full((1, rows, heads), 4.0, device="cuda")
@@ -131,20 +134,42 @@ def test_large_values_of_tokens_that_weigh_little(pkg, rows, heads, kv_heads, di
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("big", [20, 50, 100, 120])
-@pytest.mark.parametrize("rows,heads,kv_heads,dim,n", FAR)
-def test_large_values_that_a_row_does_not_see(pkg, rows, heads, kv_heads, dim, n, big, dtype):
+@pytest.mark.parametrize("rows,heads,kv_heads,dim,n,capacity", FAR)
+def test_large_values_that_a_row_does_not_see(pkg, rows, heads, kv_heads, dim, n, capacity, big, dtype):
     """The portion's tokens have values 2^big times the cache's, each four times the one before: rows that see none of a token's have nothing of it."""
     g, t = _gen(83), TYPES[dtype]
     k, v = _randn(g, 1, n, kv_heads, dim), _randn(g, 1, n, kv_heads, dim)
     for i in range(min(rows - 1, 3)):
         v[:, n - 1 - i] *= 2.0 ** (big - 2 * i)
     k, v = k.to(t), v.to(t)
-    cache, at = _fill(pkg, k, v, n, [n])
+    cache, at = _fill(pkg, k, v, capacity, [n])
     q = _randn(g, 1, rows, heads, dim, dtype=t)
     out, lse = torch.full_like(q, 3.0), torch.full((1, rows, heads), 4.0, device="cuda")
     cache.attention(q, out, at, lse=lse)
     cache.check()
     _check_by_component(out, lse, q, _held(k, None)[0], _held(v, None)[0], rows, dim ** -0.5, t)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,heads,kv_heads,dim,n,capacity", [x for x in FAR if x[3] >= 64])
+def test_keys_of_very_different_magnitude(pkg, rows, heads, kv_heads, dim, n, capacity, dtype):
+    """Every seventh token's keys are 2^45 in dims that the queries leave out and the last one's 2^100, so that scores are as the others' keys
+    make them. With masses, into what was there."""
+    g, t = _gen(97), TYPES[dtype]
+    k, v, q = _randn(g, 1, n, kv_heads, dim), _randn(g, 1, n, kv_heads, dim), _randn(g, 1, rows, heads, dim)
+    k[:, ::7, :, 32:] *= 2.0 ** 45
+    k[:, n - 1, :, 32:] *= 2.0 ** 55
+    q[..., 32:] = 0.0
+    k, v, q = k.to(t), v.to(t), q.to(t)
+    cache, at = _fill(pkg, k, v, capacity, [n])
+    out, lse = torch.full_like(q, 3.0), torch.full((1, rows, heads), 4.0, device="cuda")
+    mass = torch.rand(1, kv_heads, capacity, generator=g, device="cuda")
+    before = mass.clone()
+    cache.attention(q, out, at, lse=lse, mass_in=mass, mass_out=mass)
+    cache.check()
+    assert torch.equal(mass[..., n:], before[..., n:])
+    before[..., n - rows:] = 0.0
+    _check_by_component(out, lse, q, _held(k, None)[0], _held(v, None)[0], rows, dim ** -0.5, t, mass.double() - before.double(), before)
 
 
 def test_blocks_of_zeros(pkg):

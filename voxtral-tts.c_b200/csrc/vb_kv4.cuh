@@ -200,21 +200,48 @@ struct Kv4Head {
 template <int NB>
 VB_DEVINL Kv4Head kv4_head(const Kv4 &c, size_t row0) { return {c.k + row0 * (NB * 16), c.v + row0 * (NB * 16), c.ks + row0 * NB, c.vs + row0 * NB}; }
 
-/* A query row over the rows tok0 .. tok1 of a head, by a warp: its reference and sum; results [NB * 32] in out_s. q_s has room for a row. (By
+/* A query row into q_s, by a warp, the largest brought to [2^14, 2^15) as on the tensor cores: no product of finite numbers passes fp32. Returns what
+ * its scores are to be multiplied by to be powers of two. */
+template <int NB, class T>
+VB_DEVINL float kv4_plain_query(const T *q, float scale, float *q_s) {
+    const int lane = threadIdx.x & 31;
+    uint32_t most = 0;
+    for (int d = lane; d < NB * 32; d += 32) most = max(most, __float_as_uint(serve_get(q + d)) & 0x7fffffffu);
+    most = __reduce_max_sync(0xffffffffu, most);
+    const uint32_t e = most >> 23, field = e == 0u || e == 255u ? 127u : min(268u - e, 253u);
+    __syncwarp();
+    for (int d = lane; d < NB * 32; d += 32) q_s[d] = serve_get(q + d) * __uint_as_float(field << 23);
+    __syncwarp();
+    return scale * 1.44269504f * __uint_as_float((254u - field) << 23);
+}
+/* Its score with a row of the cache, by a lane. */
+template <int NB>
+VB_DEVINL float kv4_plain_score(const Kv4Head &c, size_t row, const float *q_s, float mul) {
+    float s = 0.0f;
+#pragma unroll 1
+    for (int b = 0; b < NB; b++) {
+        float sums = 0.0f;
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            uint32_t h[4];
+            kv4_halves(*reinterpret_cast<const uint32_t *>(c.k + row * (NB * 16) + (t * NB + b) * 4), h);
+            const float4 x = *reinterpret_cast<const float4 *>(q_s + 32 * b + 8 * t), y = *reinterpret_cast<const float4 *>(q_s + 32 * b + 8 * t + 4);
+            const float2 k0 = kv4_f2(h[0]), k1 = kv4_f2(h[1]), k2 = kv4_f2(h[2]), k3 = kv4_f2(h[3]);
+            sums = fmaf(k0.x, x.x, fmaf(k0.y, x.y, fmaf(k1.x, x.z, fmaf(k1.y, x.w, sums))));
+            sums = fmaf(k2.x, y.x, fmaf(k2.y, y.y, fmaf(k3.x, y.z, fmaf(k3.y, y.w, sums))));
+        }
+        const uint32_t byte = c.ks[row * NB + b];
+        const float2 f = kv4_power((int)min(byte, 252u) - 127);
+        s += byte == 255u ? __uint_as_float(0x7fffffffu) : sums == 0.0f ? 0.0f : sums * f.x * mul * f.y;
+    }
+    return s;
+}
+/* A query row over the rows tok0 .. tok1 of a head, by a warp: its reference and sum; results [NB * 32] in out_s. q_s has room for a row. (The head by
  * value: a reference to a kernel's arguments has all of them copied to the stack first.) */
 template <int NB, class T>
 __device__ __noinline__ float2 kv4_plain_row(Kv4Head c, const T *q, float scale, int tok0, int tok1, float *q_s, float *out_s) {
-    constexpr int kDim = NB * 32;
     const int lane = threadIdx.x & 31;
-    uint32_t most = 0;
-    for (int d = lane; d < kDim; d += 32) most = max(most, __float_as_uint(serve_get(q + d)) & 0x7fffffffu);
-    most = __reduce_max_sync(0xffffffffu, most);
-    /* the largest to [2^14, 2^15), as on the tensor cores: no product of finite numbers passes fp32 */
-    const uint32_t e = most >> 23, field = e == 0u || e == 255u ? 127u : min(268u - e, 253u);
-    const float up = __uint_as_float(field << 23), mul = scale * 1.44269504f * __uint_as_float((254u - field) << 23);
-    __syncwarp();
-    for (int d = lane; d < kDim; d += 32) q_s[d] = serve_get(q + d) * up;
-    __syncwarp();
+    const float mul = kv4_plain_query<NB>(q, scale, q_s);
     float ref = -INFINITY, sum = 0.0f, o[NB];
     int base[NB];
     uint32_t nan = 0;
@@ -224,23 +251,7 @@ __device__ __noinline__ float2 kv4_plain_row(Kv4Head c, const T *q, float scale,
         /* scores: a lane a token */
         const int j = j0 + lane, n = min(32, tok1 - j0);
         const size_t row = min(j, tok1 - 1);
-        float s = 0.0f;
-#pragma unroll 1
-        for (int b = 0; b < NB; b++) {
-            float sums = 0.0f;
-#pragma unroll
-            for (int t = 0; t < 4; t++) {
-                uint32_t h[4];
-                kv4_halves(*reinterpret_cast<const uint32_t *>(c.k + row * (NB * 16) + (t * NB + b) * 4), h);
-                const float4 x = *reinterpret_cast<const float4 *>(q_s + 32 * b + 8 * t), y = *reinterpret_cast<const float4 *>(q_s + 32 * b + 8 * t + 4);
-                const float2 k0 = kv4_f2(h[0]), k1 = kv4_f2(h[1]), k2 = kv4_f2(h[2]), k3 = kv4_f2(h[3]);
-                sums = fmaf(k0.x, x.x, fmaf(k0.y, x.y, fmaf(k1.x, x.z, fmaf(k1.y, x.w, sums))));
-                sums = fmaf(k2.x, y.x, fmaf(k2.y, y.y, fmaf(k3.x, y.z, fmaf(k3.y, y.w, sums))));
-            }
-            const uint32_t byte = c.ks[row * NB + b];
-            const float2 f = kv4_power((int)min(byte, 252u) - 127);
-            s += byte == 255u ? __uint_as_float(0x7fffffffu) : sums == 0.0f ? 0.0f : sums * f.x * mul * f.y;
-        }
+        float s = kv4_plain_score<NB>(c, row, q_s, mul);
         if (j >= tok1) s = -INFINITY;
         float top = s;
 #pragma unroll

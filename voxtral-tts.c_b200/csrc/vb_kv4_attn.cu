@@ -6,8 +6,8 @@
  * The codes are exact in FP16, so the products run on FP16 warp-level MMAs (m16n8k16), tokens along M, eight
  * (row, query head) pairs of a KV head along N:
  *   S^T [16 tokens x 8] += K Q^T    a block of 32 at a time, whose sum is multiplied by the token's scale in fp32
- *   O^T [16 dims x 8]   += V^T P^T  values times 2^(e - E + 13), E the largest scale of the block column so far: exact in FP16 unless a
- *                                   token's scale is under 2^-36 of the largest, where its values are rounded to 2^-38 of that
+ *   O^T [16 dims x 8]   += V^T P^T  values times 2^(e - E + 13), E the largest scale of the block column so far: exact in FP16 where no
+ *                                   token's scale is under 2^-36 of the largest; a CTA that meets one works in fp32 (kv4_plain_row)
  * Queries are brought to [2^14, 2^15) by a power of two a row (exact), then one FP16 term (bf16, fp16: exact down to 2^-29
  * of a row's largest) or two (fp32: 22 bits and a sign). Weights are taken against a running reference that trails the maximum by
  * at most 2^8, times 2^7, so that FP16 holds weights from 2^15 down to 2^-24 (2^-46 with the second term, as far as its exponent goes):

@@ -8,7 +8,8 @@
  *
  * Keys and values go from codes to FP16 on the way to shared memory, four warps for the keys and three for the values: keys times
  * 2^(e - S + 13), S the largest scale of a warp's 32 tokens, which the softmax undoes, values times 2^(e - E + 13), E the largest scale
- * so far, on which the accumulator is based (exact down to 2^-36 of the largest). Scores, weights, sums as in vb_kv4_attn.cu. Two pairs of
+ * so far, on which the accumulator is based: exact down to 2^-36 of the largest. A CTA that meets others works in fp32 (p_plain). Scores,
+ * weights, sums as in vb_kv4_attn.cu. Two pairs of
  * warpgroups take alternate tiles with a reference, sums and an accumulator each, merged at the end, so that the tensor pipe works on
  * one tile while the other is in its softmax. A thread has half of a row's columns: with a whole row a thread, and half as many
  * threads, 1203 rows took 206 us in place of 178 (before sums were put aside).
@@ -174,6 +175,35 @@ __device__ __noinline__ void p_put_aside(float4 *mine, float2 *base, uint32_t tO
     }
 }
 
+/* Scales too far apart: all that this CTA has, in fp32, over what was left by then. By itself, with arguments by value and places worked out
+ * again, so that nothing is kept for it in the kernel's registers (1203 rows: 212 us so, 211 now). */
+template <int NB, class T>
+__device__ __noinline__ void p_plain(const Kv4Attn a, const ServeRows<T> q, const ServeRows<T> out) {
+    constexpr int kDim = NB * 32, kPart = kPRows * (kDim + 2);
+    extern __shared__ unsigned char p_smem_raw[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    float *q_row = reinterpret_cast<float *>(((uintptr_t)p_smem_raw + 1023) & ~(uintptr_t)1023) + warp * 2 * kDim, *results = q_row + kDim;
+    PWork work;
+    p_work(a, blockIdx.x, work);
+    const Kv4Head cache = kv4_head<NB>(a.c, a.c.row(work.seq, work.kv_head, 0));
+    float *part = a.part + (size_t)work.slot * kPart;
+    for (int p = warp; p < work.n_pairs; p += kPThreads / 32) {
+        const int row = (work.pair0 + p) / a.group, head = work.kv_head * a.group + work.pair0 + p - row * a.group;
+        const float2 end = kv4_plain_row<NB, T>(cache, q.data + work.seq * q.seq + row * q.row + head * q.head, a.scale, work.first_tile * kPKeys,
+                                                min((work.first_tile + work.n_tiles) * kPKeys, work.before + row + 1), q_row, results);
+        const float inv = end.y == 0.0f ? 0.0f : 1.0f / end.y;
+        for (int d = lane; d < kDim; d += 32) {
+            if (work.used > 1) part[p * kDim + d] = results[d];
+            else serve_put(out.data + work.seq * out.seq + row * out.row + head * out.head + d, end.y == 0.0f ? 0.0f : results[d] * inv);
+        }
+        if (lane == 0) {
+            if (work.used > 1) reinterpret_cast<float2 *>(part + kPRows * kDim)[p] = end;
+            else if (a.lse) a.lse[((size_t)work.seq * a.max_rows + row) * a.heads + head] = end.y == 0.0f ? -INFINITY : (end.x + 8.0f + log2f(end.y)) * 0.69314718f;
+        }
+        __syncwarp();
+    }
+}
+
 template <int NB, int PT, class T>
 __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn a, const ServeRows<T> q, const ServeRows<T> out) {
     constexpr int QT = sizeof(T) == 4 ? 2 : 1, kDim = NB * 32;
@@ -184,7 +214,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
     __shared__ __align__(8) uint64_t k_full[Cfg::kSlots], k_empty[Cfg::kSlots], v_full[Cfg::kSlots], v_empty[Cfg::kSlots], s_full[2], p_full[2], o_done[2], q_full;
     __shared__ float key_up[kPRing][4], down_s[kPRows], top_s[2][2][kPRows];
     __shared__ float2 aside_s[2][2][kPRows];                       /* reference, scale of what is put aside */
-    __shared__ int value_top[kPRing], bad_s[NB], abort_s, room_s;
+    __shared__ int value_top[kPRing], bad_s[NB], abort_s, room_s, far_s;
     __shared__ uint32_t tmem_slot;
     int *abort_flag = &abort_s;
 
@@ -208,7 +238,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
             vb_mbar_init(&o_done[i], 1);
         }
         vb_mbar_init(&q_full, kPSoft);
-        abort_s = 0;
+        abort_s = far_s = 0;
         vb_mbar_init_fence();
     }
     if (tid < NB) bad_s[tid] = 1 << 30;
@@ -480,14 +510,22 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
         for (int t = 0; t < n_tiles; t++) {
             const int slot = t % Cfg::kSlots, j0 = (first_tile + t) * kPKeys + lw * 32;
             int most = 0;
+            uint32_t least = 255u;                     /* less one: zeros, which nothing is lost of, come last */
 #pragma unroll
             for (int i = 0; i < 4; i++)
 #pragma unroll
                 for (int b = 0; b < NB; b++) {
                     if (j0 + i * 8 + g >= seen) { words[i][b] = 0; bytes[i][b] = 0; }       /* whatever lies behind the last token */
-                    if (bytes[i][b] != 255u) most = max(most, (int)bytes[i][b]);
                 }
+            /* four lanes have the same tokens: each looks at one of them */
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                const uint32_t byte = tq < 2 ? (tq == 0 ? bytes[0][b] : bytes[1][b]) : tq == 2 ? bytes[2][b] : bytes[3][b];
+                if (byte != 255u) most = max(most, (int)byte);
+                least = min(least, byte - 1u);
+            }
             most = max((int)__reduce_max_sync(0xffffffffu, (unsigned)most), 14);          /* its undoing stays a normal number */
+            if (kv4_far(least + 1u, most)) *(volatile int *)&far_s = 1;
             if (!at_warp_wait(&k_empty[slot], ((uint32_t)(t / Cfg::kSlots) & 1u) ^ 1u, abort_flag)) { give_up(); break; }
             unsigned char *to = k_s + slot * Cfg::kSlot;
 #pragma unroll
@@ -531,7 +569,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
 #pragma unroll
             for (int i = 0; i < NB; i++) all[i] = four[i];
         };
-        int top = 0;
+        int top = 0, first_top = 0;
         const int tasks = n_tiles * 4;
         if (warp - 20 < tasks) fetch(warp - 20);
         for (int task = warp - 20; task < tasks; task += 3) {
@@ -552,6 +590,11 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
                     if (lane * 4 + i / NB < real && ((all[i / 4] >> (8 * (i % 4))) & 255u) == 255u) atomicMin(&bad_s[i % NB], j0 + lane * 4 + i / NB);
             }
             top = max(top, (int)__reduce_max_sync(0xffffffffu, (unsigned)most));
+            if (first_top == 0) first_top = top;
+            uint32_t least = 255u;
+#pragma unroll
+            for (int i = 0; i < NB; i++) least = min(least, (lw * 32 + (i * 32 + lane) / NB < real ? byte[i] : 0u) - 1u);
+            if (kv4_far(least + 1u, top) || top - first_top > kKv4Rise) *(volatile int *)&far_s = 1;
             if (!at_warp_wait(&v_empty[slot], ((uint32_t)(t / Cfg::kSlots) & 1u) ^ 1u, abort_flag)) { give_up(); break; }
             unsigned char *to = v_s + slot * Cfg::kSlot;
 #pragma unroll
@@ -617,6 +660,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
     }
     tc_fence_before();
     __syncthreads();
+    if (*(volatile int *)&far_s) p_plain<NB, T>(a, q, out);
     if (puts_aside && tid == 32) {
         __threadfence();
         atomicExch(&a.rooms[room_s], 0u);
@@ -697,7 +741,7 @@ __global__ void __launch_bounds__(kWThreads, 1) kv4_mass_many_kernel(const Kv4At
     __shared__ __align__(8) uint64_t q_full[kWSlots], q_empty[kWSlots], s_full[2], s_empty[2], k_full;
     __shared__ __align__(16) float2 pair_s[kWRing][kPRows];                 /* of a pair: what S is multiplied by, its lse in powers of two */
     __shared__ float sum_s[kPKeys];
-    __shared__ int abort_s;
+    __shared__ int abort_s, far_s;
     __shared__ uint32_t tmem_slot;
     int *abort_flag = &abort_s;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kv_head = blockIdx.y, seq = blockIdx.z, tok0 = blockIdx.x * kPKeys;
@@ -721,7 +765,7 @@ __global__ void __launch_bounds__(kWThreads, 1) kv4_mass_many_kernel(const Kv4At
             vb_mbar_init(&s_empty[i], 128);
         }
         vb_mbar_init(&k_full, 8);
-        abort_s = 0;
+        abort_s = far_s = 0;
         vb_mbar_init_fence();
     }
     if (warp == kWMmaWarp) {
@@ -742,7 +786,7 @@ __global__ void __launch_bounds__(kWThreads, 1) kv4_mass_many_kernel(const Kv4At
         const int g = lane >> 2, tq = lane & 3;
         const size_t row0 = a.c.row(seq, kv_head, 0);
         __shared__ float key_up[8];
-        uint32_t words[2][NB], bytes[2][NB];
+        uint32_t words[2][NB], bytes[2][NB], least = 255u;
         int most = 0;
 #pragma unroll
         for (int i = 0; i < 2; i++) {
@@ -754,9 +798,11 @@ __global__ void __launch_bounds__(kWThreads, 1) kv4_mass_many_kernel(const Kv4At
             for (int b = 0; b < NB; b++) {
                 if (j >= span.length) { words[i][b] = 0; bytes[i][b] = 0; }
                 if (bytes[i][b] != 255u) most = max(most, (int)bytes[i][b]);
+                least = min(least, bytes[i][b] - 1u);
             }
         }
         most = max((int)__reduce_max_sync(0xffffffffu, (unsigned)most), 14);              /* its undoing stays a normal number */
+        if (kv4_far(least + 1u, most)) *(volatile int *)&far_s = 1;
 #pragma unroll
         for (int i = 0; i < 2; i++)
 #pragma unroll
@@ -812,7 +858,7 @@ __global__ void __launch_bounds__(kWThreads, 1) kv4_mass_many_kernel(const Kv4At
         const float sum = both.x + both.y;
         if (w == 1) sum_s[r] = sum;
         vb_named_bar(1, 256);
-        if (w == 0 && j < span.length) {
+        if (w == 0 && j < span.length && !*(volatile int *)&far_s) {
             pdl_wait();
             const size_t at = ((size_t)seq * a.c.kv_heads + kv_head) * a.c.capacity + j;
             a.mass_out[at] = sum + sum_s[r] + (a.mass_in && j < before ? a.mass_in[at] : 0.0f);
@@ -902,6 +948,30 @@ __global__ void __launch_bounds__(kWThreads, 1) kv4_mass_many_kernel(const Kv4At
     }
     tc_fence_before();
     __syncthreads();
+    if (*(volatile int *)&far_s) {
+        /* scales too far apart: in fp32, a lane a token, four warps the pairs of 32 tokens in turn */
+        pdl_wait();
+        const Kv4Head head = kv4_head<NB>(a.c, a.c.row(seq, kv_head, 0));
+        float *q_row = reinterpret_cast<float *>(base) + warp * NB * 32, *sums = reinterpret_cast<float *>(base) + 16 * NB * 32;
+        const int j = tok0 + (warp & 3) * 32 + lane;
+        if (warp < 16) {
+            float sum = 0.0f;
+            for (int p = first + (warp >> 2); p < pairs; p += 4) {
+                const int row = p / a.group, h = kv_head * a.group + p - row * a.group;
+                const float mul = kv4_plain_query<NB>(q.data + seq * q.seq + row * q.row + h * q.head, a.scale, q_row);
+                const float lse = a.lse[((size_t)seq * a.max_rows + row) * a.heads + h], s = kv4_plain_score<NB>(head, min(j, span.length - 1), q_row, mul);
+                if (j < before + row + 1 && lse != -INFINITY) sum += exp2_fast(s - lse * 1.44269504f);
+                __syncwarp();
+            }
+            sums[warp * 32 + lane] = sum;
+        }
+        __syncthreads();
+        if (warp < 4 && j < span.length) {
+            const size_t at = ((size_t)seq * a.c.kv_heads + kv_head) * a.c.capacity + j;
+            a.mass_out[at] = sums[warp * 32 + lane] + sums[(warp + 4) * 32 + lane] + sums[(warp + 8) * 32 + lane] + sums[(warp + 12) * 32 + lane] +
+                             (a.mass_in && j < before ? a.mass_in[at] : 0.0f);
+        }
+    }
     if (warp == kWMmaWarp) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kWTmem) : "memory");
