@@ -189,3 +189,18 @@ def test_blocks_of_zeros(pkg):
         cache.attention(q, out, at, lse=lse)
         _check_by_component(out, lse, q, _held(k, None)[0], _held(v, None)[0], rows, d ** -0.5, torch.float32)
         assert (out[0, :, 2:, 32:64] == 0).all()
+
+
+@pytest.mark.parametrize("dtype,small", [("f32", 8), ("f32", 20), ("f32", 90), ("bf16", 8), ("bf16", 40), ("f16", 8)])
+@pytest.mark.parametrize("rows,heads,kv_heads,dim,n,capacity", FAR)
+def test_small_queries(pkg, rows, heads, kv_heads, dim, n, capacity, dtype, small):
+    """Queries of 2^-small, of a model that normalises them or far smaller: weights come out nearly even, in tiles that end inside a sequence too."""
+    g, t = _gen(103), TYPES[dtype]
+    k, v, q = _randn(g, 1, n, kv_heads, dim, dtype=t), _randn(g, 1, n, kv_heads, dim, dtype=t), (_randn(g, 1, rows, heads, dim) * 2.0 ** -small).to(t)
+    cache, at = _fill(pkg, k, v, capacity, [n])
+    for scale in (dim ** -0.5, 2.0 ** -60):
+        out, lse = torch.full_like(q, 3.0), torch.full((1, rows, heads), 4.0, device="cuda")
+        mass = torch.zeros(1, kv_heads, capacity, device="cuda")
+        cache.attention(q, out, at, scale=scale, lse=lse, mass_out=mass)
+        cache.check()
+        _check_by_component(out, lse, q, _held(k, None)[0], _held(v, None)[0], rows, scale, t, mass, torch.zeros_like(mass))

@@ -112,7 +112,7 @@ struct QueryColumn {
         const float down = __uint_as_float((254u - field) << 23);
         float up = __uint_as_float(field << 23);
         if (a.scale <= 0.0f) up = a.scale < 0.0f ? -up : 0.0f;       /* the factor is positive: the largest score is the largest product */
-        if (lane == 0) mul_s[n] = (a.scale != 0.0f ? fabsf(a.scale) * 1.44269504f : 1.0f) * down;
+        if (lane == 0) mul_s[n] = fmaxf((a.scale != 0.0f ? fabsf(a.scale) * 1.44269504f : 1.0f) * down, 0x1p-149f);      /* not 0: what is masked stays -inf */
 #pragma unroll
         for (int i = 0; i < kEach; i++) {
             const int at = lane + 32 * i;                             /* 8 blocks + 2 t + half */

@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
 #pragma unroll
             for (int c = 0; c < 2; c++) {
                 const int column = half * 64 + c * 32;
-                const float up = ups[half * 2 + c] * mul;
+                const float up = fmaxf(ups[half * 2 + c] * mul, 0x1p-149f);      /* not 0, whatever the scales: what is masked stays -inf */
                 const uint64_t up2 = vb_f2_pack(up, up);
                 uint32_t s[32], second[PT == 2 ? 16 : 1];
                 at_ld32(tS + (uint32_t)column, s);
