@@ -204,3 +204,17 @@ def test_small_queries(pkg, rows, heads, kv_heads, dim, n, capacity, dtype, smal
         cache.attention(q, out, at, scale=scale, lse=lse, mass_out=mass)
         cache.check()
         _check_by_component(out, lse, q, _held(k, None)[0], _held(v, None)[0], rows, scale, t, mass, torch.zeros_like(mass))
+
+
+@pytest.mark.parametrize("rows,heads,kv_heads,dim,n,capacity,large", [
+    (3, 4, 2, 96, 200, 200, 95), (3, 4, 2, 96, 200, 200, -80), (80, 2, 1, 64, 200, 200000, 115), (80, 2, 1, 64, 200, 200000, -80), (70, 4, 2, 128, 5000, 120000, 115)])
+def test_masses_of_large_keys_and_small_queries(pkg, rows, heads, kv_heads, dim, n, capacity, large):
+    """Keys of 2^large, queries of 2^-large: scores are ordinary numbers, and so are all of their parts where factors meet first."""
+    g = _gen(101)
+    k, v, q = _randn(g, 1, n, kv_heads, dim) * 2.0 ** large, _randn(g, 1, n, kv_heads, dim), _randn(g, 1, rows, heads, dim) * 2.0 ** -large
+    cache, at = _fill(pkg, k, v, capacity, [n])
+    out, lse = torch.full_like(q, 3.0), torch.full((1, rows, heads), 4.0, device="cuda")
+    mass = torch.zeros(1, kv_heads, capacity, device="cuda")
+    cache.attention(q, out, at, lse=lse, mass_out=mass)
+    cache.check()
+    _check_by_component(out, lse, q, _held(k, None)[0], _held(v, None)[0], rows, dim ** -0.5, torch.float32, mass, torch.zeros_like(mass))

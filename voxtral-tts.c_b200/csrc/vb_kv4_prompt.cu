@@ -842,7 +842,7 @@ __global__ void __launch_bounds__(kWThreads, 1) kv4_mass_many_kernel(const Kv4At
 #pragma unroll
                 for (int k = 0; k < 32; k += 2) {
                     const float4 p = of[k / 2];
-                    const float2 x = vb_f2_get(vb_f2_fma(vb_f2_mul(vb_f2_pack(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), up2), vb_f2_pack(p.x, p.z), vb_f2_pack(-p.y, -p.w)));
+                    const float2 x = vb_f2_get(vb_f2_fma(vb_f2_pack(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), vb_f2_mul(up2, vb_f2_pack(p.x, p.z)), vb_f2_pack(-p.y, -p.w)));
                     float e0 = exp2_fast(x.x), e1 = exp2_fast(x.y);
                     if (masked) {
                         if (c * 32 + k < c0 || c * 32 + k >= c1) e0 = 0.0f;
