@@ -218,3 +218,28 @@ def test_masses_of_large_keys_and_small_queries(pkg, rows, heads, kv_heads, dim,
     cache.attention(q, out, at, lse=lse, mass_out=mass)
     cache.check()
     _check_by_component(out, lse, q, _held(k, None)[0], _held(v, None)[0], rows, dim ** -0.5, torch.float32, mass, torch.zeros_like(mass))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,heads", [(1, 300), (100, 160)])
+def test_weights_far_below_the_largest(pkg, rows, heads, dtype):
+    """Eight tokens at the front and 65528 that are 20 below them: together they count, each of them 2^-29. More heads than CTAs that run at
+    once: a warp or two goes through a whole sequence."""
+    t, n, d, tops = TYPES[dtype], 65536, 32, 8
+    k, v = torch.zeros(1, n, 1, d, device="cuda", dtype=t), torch.ones(1, n, 1, d, device="cuda", dtype=t)
+    k[:, 0:32 * tops:32, :, 0], v[:, 0:32 * tops:32] = 4.0, 0.0
+    cache, at = _fill(pkg, k.expand(1, n, heads, d), v.expand(1, n, heads, d), n, [n])
+    q = torch.zeros(1, rows, heads, d, device="cuda", dtype=t)
+    q[..., 0] = 5.0
+    out, lse = torch.full_like(q, 3.0), torch.empty(1, rows, heads, device="cuda")
+    cache.attention(q, out, at, scale=1.0, lse=lse)
+    cache.check()
+    count = torch.arange(n - rows + 1, n + 1, device="cuda", dtype=torch.float64)[:, None, None] - tops
+    low = math.exp(-20.0)
+    want = (count * low / (tops + count * low)).expand(rows, heads, d)
+    # a weight: half of FP16's smallest step, 2^-25 of 2^13 (the reference, which the first tokens are); a score's roundings (20 times 10 of 2^-24)
+    # twice, an exponential and terms; sums: a unit for each 16 tokens and term; the result's own rounding
+    relative = 2 * 20 * 10 * 2.0 ** -24 + 2.0 ** -19 + (n / 8 + 16) * 2.0 ** -23 + (2.0 ** -11 if dtype == "bf16" else 0.0)
+    limit = count * 2.0 ** -38 / tops + want * (relative + torch.finfo(t).eps / 2) + (2.0 ** -25 if dtype == "f16" else 0.0)      # fp16: its smallest step
+    err = (out[0].double() - want).abs()
+    assert (err <= limit).all(), float((err / limit).max())

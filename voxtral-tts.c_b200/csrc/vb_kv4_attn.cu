@@ -9,9 +9,9 @@
  *   O^T [16 dims x 8]   += V^T P^T  values times 2^(e - E + 13), E the largest scale of the block column so far: exact in FP16 where no
  *                                   token's scale is under 2^-36 of the largest; a CTA that meets one works in fp32 (kv4_plain_row)
  * Queries are brought to [2^14, 2^15) by a power of two a row (exact), then one FP16 term (bf16, fp16: exact down to 2^-29
- * of a row's largest) or two (fp32: 22 bits and a sign). Weights are taken against a running reference that trails the maximum by
- * at most 2^8, times 2^7, so that FP16 holds weights from 2^15 down to 2^-24 (2^-46 with the second term, as far as its exponent goes):
- * one term for bf16 results (11 bits against the 8 of the result), two otherwise.
+ * of a row's largest) or two (fp32: 22 bits and a sign, down to 2^-39 of the largest). Weights are taken against a running reference that
+ * trails the maximum by at most 2^2, times 2^13, so that FP16 holds them from 2^15 down in steps of 2^-24: one term for bf16 results (11 bits against
+ * the 8 of the result, 2^-38 of the largest weight at least), two otherwise (22 bits down to 2^-15 of the largest, below that to within 2^-38 of it).
  *
  * A warp walks tiles of 32 tokens with a maximum, sums and accumulators of its own, through a ring of its own that bulk copies
  * fill: no barrier between warps until the end. A sequence's tokens are split over CTAs where there are few of them; the CTA that
@@ -280,12 +280,12 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(co
         float top[2];
 #pragma unroll
         for (int u = 0; u < 2; u++) top[u] = fmaxf(fmaxf(s[0][u], s[0][2 + u]), fmaxf(s[1][u], s[1][2 + u])) * mul[u];      /* the factors are positive */
-        if (__any_sync(0xffffffffu, top[0] > ref[0] + 8.0f || top[1] > ref[1] + 8.0f)) {
+        if (__any_sync(0xffffffffu, top[0] > ref[0] + kKv4Trail || top[1] > ref[1] + kKv4Trail)) {
 #pragma unroll
             for (int u = 0; u < 2; u++) {
 #pragma unroll
                 for (int x = 4; x < 32; x <<= 1) top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], x));
-                if (top[u] > ref[u] + 8.0f) {
+                if (top[u] > ref[u] + kKv4Trail) {
                     const float fall = exp2_fast(ref[u] - top[u]);      /* the first time: 0 */
                     ref[u] = top[u];
                     sum[u] *= fall;
@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(co
     for (int u = 0; u < 2; u++) {
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], x);
-        sum[u] *= 0x1p-15f;
+        sum[u] *= kKv4Out;
     }
     const bool plain = __syncthreads_or(far);            /* every ring is empty */
     constexpr int kUnits = 2 * NB * 32;                  /* of four results */
@@ -484,7 +484,7 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(co
     }
 #pragma unroll
     for (int i = 0; i < 2 * NB; i++) {
-        const int e = top_scale[Cfg::kWhole ? 0 : i / 2] - 155, e0 = e >> 1;      /* in two steps: 2^e may not be a normal number */
+        const int e = top_scale[Cfg::kWhole ? 0 : i / 2] - kKv4Down, e0 = e >> 1;      /* in two steps: 2^e may not be a normal number */
         const float f0 = __uint_as_float((uint32_t)(127 + e0) << 23), f1 = __uint_as_float((uint32_t)(127 + e - e0) << 23);
         mo[(warp * 2 * NB + i) * 32 + lane] = make_float4(o[i][0] * f0 * f1, o[i][1] * f0 * f1, o[i][2] * f0 * f1, o[i][3] * f0 * f1);
     }
@@ -511,7 +511,7 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(co
                 serve_put(to, x);
                 serve_put(to + 1, y);
             }
-            if (d == 0 && a.lse) a.lse[((size_t)seq * a.max_rows + row) * a.heads + head] = l == 0.0f ? -INFINITY : (r + 8.0f + log2f(l)) * 0.69314718f;
+            if (d == 0 && a.lse) a.lse[((size_t)seq * a.max_rows + row) * a.heads + head] = l == 0.0f ? -INFINITY : (r + (float)kKv4Rest + log2f(l)) * 0.69314718f;
         }
     };
     /* a part's factor against a reference; parts without weights have none */
@@ -534,7 +534,7 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(co
                     part[((i * 32 + gd * 4 + (warp >> 1)) * 2 + (d & 1)) * 2 + (warp & 1)] = results[d];
                 }
             }
-            if (lane == 0 && used == 1 && a.lse) a.lse[((size_t)seq * a.max_rows + row) * a.heads + head] = end.y == 0.0f ? -INFINITY : (end.x + 8.0f + log2f(end.y)) * 0.69314718f;
+            if (lane == 0 && used == 1 && a.lse) a.lse[((size_t)seq * a.max_rows + row) * a.heads + head] = end.y == 0.0f ? -INFINITY : (end.x + (float)kKv4Rest + log2f(end.y)) * 0.69314718f;
             if (lane == 0 && used > 1) {
                 part[kACols * kDim + warp] = end.x;
                 part[kACols * kDim + 8 + warp] = end.y;

@@ -198,7 +198,7 @@ __device__ __noinline__ void p_plain(const Kv4Attn a, const ServeRows<T> q, cons
         }
         if (lane == 0) {
             if (work.used > 1) reinterpret_cast<float2 *>(part + kPRows * kDim)[p] = end;
-            else if (a.lse) a.lse[((size_t)work.seq * a.max_rows + row) * a.heads + head] = end.y == 0.0f ? -INFINITY : (end.x + 8.0f + log2f(end.y)) * 0.69314718f;
+            else if (a.lse) a.lse[((size_t)work.seq * a.max_rows + row) * a.heads + head] = end.y == 0.0f ? -INFINITY : (end.x + (float)kKv4Rest + log2f(end.y)) * 0.69314718f;
         }
         __syncwarp();
     }
@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
             /* values: the scale that this tile is based on */
             if (!at_warp_wait(&v_full[t % Cfg::kSlots], (uint32_t)(t / Cfg::kSlots) & 1u, abort_flag)) { give_up(); t += 2; break; }
             const int now_scale = value_top[t % kPRing];
-            const bool rise = top > ref + 8.0f;
+            const bool rise = top > ref + kKv4Trail;
             if (__any_sync(0xffffffffu, rise) || now_scale != top_scale) {
                 const float now = rise ? top : ref, f = rise ? exp2_fast(ref - now) : 1.0f;      /* the first time: 0 */
                 if (it > 0) {
@@ -418,7 +418,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
         vb_named_bar(1, kPSoft);                                     /* every product is done: the rings are free */
         float4 *ends = reinterpret_cast<float4 *>(k_s);            /* 4 x 128 x (reference, sum, scale) */
         float *rows = reinterpret_cast<float *>(k_s + 4 * kPRows * 16);
-        ends[wg * kPRows + r] = make_float4(ref, sum * 0x1p-15f, __int_as_float(top_scale), 0.0f);
+        ends[wg * kPRows + r] = make_float4(ref, sum * kKv4Out, __int_as_float(top_scale), 0.0f);
         if (puts_aside) __threadfence();
         tc_fence_before();
         vb_named_bar(1, kPSoft);
@@ -433,10 +433,10 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
         if (used > 1) {
             if (wg == 0) reinterpret_cast<float2 *>(part + kPRows * kDim)[r] = make_float2(reference, total);
         } else if (wg == 0 && valid && a.lse)
-            a.lse[((size_t)seq * a.max_rows + row) * a.heads + head] = total == 0.0f ? -INFINITY : (reference + 8.0f + log2f(total)) * 0.69314718f;
+            a.lse[((size_t)seq * a.max_rows + row) * a.heads + head] = total == 0.0f ? -INFINITY : (reference + (float)kKv4Rest + log2f(total)) * 0.69314718f;
         fa *= inv;
         fb *= inv;
-        const int ea = __float_as_int(A.z) - 155, eb = __float_as_int(B.z) - 155;      /* in two steps: 2^e may not be a normal number */
+        const int ea = __float_as_int(A.z) - kKv4Down, eb = __float_as_int(B.z) - kKv4Down;      /* in two steps: 2^e may not be a normal number */
         const float a0 = __uint_as_float((uint32_t)(127 + (ea >> 1)) << 23), a1 = __uint_as_float((uint32_t)(127 + ea - (ea >> 1)) << 23);
         const float b0 = __uint_as_float((uint32_t)(127 + (eb >> 1)) << 23), b1 = __uint_as_float((uint32_t)(127 + eb - (eb >> 1)) << 23);
 #pragma unroll 1
@@ -456,7 +456,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
 #pragma unroll 1
             for (int x = 0; x < 2 && n_tiles > 2 * Cfg::kChain + x; x++) {
                 const float2 e = aside_s[x][0][r];
-                const int scale = __float_as_int(e.y) - 155;
+                const int scale = __float_as_int(e.y) - kKv4Down;
                 const float f = e.x > -INFINITY ? exp2_fast(e.x - reference) * inv : 0.0f;
                 const float s0 = __uint_as_float((uint32_t)(127 + (scale >> 1)) << 23), s1 = __uint_as_float((uint32_t)(127 + scale - (scale >> 1)) << 23);
                 const float4 *from = p_aside<NB>(a, room_s, x, c) + r;
@@ -713,7 +713,7 @@ __global__ void __launch_bounds__(kJThreads) kv4_join_kernel(const Kv4Attn a, co
         T *to = out.data + seq * out.seq + row * out.row + head * out.head + lane * NB;
 #pragma unroll
         for (int i = 0; i < NB; i++) serve_put(to + i, total == 0.0f ? 0.0f : v[i] * inv);
-        if (lane == 0 && a.lse) a.lse[((size_t)seq * a.max_rows + row) * a.heads + head] = total == 0.0f ? -INFINITY : (reference + 8.0f + log2f(total)) * 0.69314718f;
+        if (lane == 0 && a.lse) a.lse[((size_t)seq * a.max_rows + row) * a.heads + head] = total == 0.0f ? -INFINITY : (reference + (float)kKv4Rest + log2f(total)) * 0.69314718f;
     }
 }
 
