@@ -23,8 +23,8 @@ namespace vb {
     }
 
 /* Weights are taken against a reference that trails the largest by at most 2^2 and held times 2^13, so that the largest are 2^15 and FP16's smallest
- * step, 2^-24, is 2^-37 of the reference. (2^8 and 2^7 need fewer changes of the reference, and lost a tenth of weights of 2^-29: 204
- * us for 1203 rows, 211 with these.) */
+ * step, 2^-24, is 2^-37 of the reference. (2^8 and 2^7 need fewer changes of the reference, and lost a tenth of weights of 2^-29; level
+ * in time with a few rows.) */
 constexpr float kKv4Trail = 2.0f, kKv4Bias = 13.0f;
 constexpr int kKv4Rest = 8;                   /* sums and results of a part leave the accumulators times 2^-8: */
 constexpr float kKv4Out = 0x1p-21f;           /* 2^-13 2^-8, sums */

@@ -30,6 +30,10 @@ namespace {
 constexpr int kPRows = 128, kPKeys = 128, kPSoft = 512, kPMmaWarp = 23, kPThreads = 32 * (kPMmaWarp + 1), kPBlock = kPKeys * 128, kPStatus = 62, kPRing = 8;
 constexpr int kPLeast = 2, kPTailParts = 8;   /* tiles of a part at least; parts of a unit of the last round at most */
 constexpr uint32_t kPTmem = 512, kPO = 256;
+/* A row's reference trails by at most 2^4 here, weights are held times 2^11. With 2^2 and 2^13, as in vb_kv4_attn.cu, more tiles change a reference of
+ * one of a warp's 32 rows: 1024 bf16 rows over 4096 tokens 133 us in place of 126, 1203 fp32 rows over 4208 213 in place of 207. */
+constexpr float kPTrail = 4.0f, kPBias = 11.0f, kPOut = 0x1p-19f;
+constexpr int kPDown = 127 + 13 + 19;
 template <int NB, int QT>
 struct PCfg {
     /* A sum in TMEM loses up to a unit of its last place with every product of 16 tokens that is added, towards zero: 224 of them, 14 tiles of two
@@ -355,7 +359,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
             /* values: the scale that this tile is based on */
             if (!at_warp_wait(&v_full[t % Cfg::kSlots], (uint32_t)(t / Cfg::kSlots) & 1u, abort_flag)) { give_up(); t += 2; break; }
             const int now_scale = value_top[t % kPRing];
-            const bool rise = top > ref + kKv4Trail;
+            const bool rise = top > ref + kPTrail;
             if (__any_sync(0xffffffffu, rise) || now_scale != top_scale) {
                 const float now = rise ? top : ref, f = rise ? exp2_fast(ref - now) : 1.0f;      /* the first time: 0 */
                 if (it > 0) {
@@ -376,7 +380,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
                 ref = now;
                 top_scale = now_scale;
             }
-            const float low = ref > -INFINITY ? ref - kKv4Bias : 0.0f;      /* nothing seen yet: every weight is 2^-inf */
+            const float low = ref > -INFINITY ? ref - kPBias : 0.0f;      /* nothing seen yet: every weight is 2^-inf */
             uint64_t sums[2] = {0, 0};
             const uint64_t low2 = vb_f2_pack(-low, -low);
 #pragma unroll
@@ -418,7 +422,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
         vb_named_bar(1, kPSoft);                                     /* every product is done: the rings are free */
         float4 *ends = reinterpret_cast<float4 *>(k_s);            /* 4 x 128 x (reference, sum, scale) */
         float *rows = reinterpret_cast<float *>(k_s + 4 * kPRows * 16);
-        ends[wg * kPRows + r] = make_float4(ref, sum * kKv4Out, __int_as_float(top_scale), 0.0f);
+        ends[wg * kPRows + r] = make_float4(ref, sum * kPOut, __int_as_float(top_scale), 0.0f);
         if (puts_aside) __threadfence();
         tc_fence_before();
         vb_named_bar(1, kPSoft);
@@ -436,7 +440,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
             a.lse[((size_t)seq * a.max_rows + row) * a.heads + head] = total == 0.0f ? -INFINITY : (reference + (float)kKv4Rest + log2f(total)) * 0.69314718f;
         fa *= inv;
         fb *= inv;
-        const int ea = __float_as_int(A.z) - kKv4Down, eb = __float_as_int(B.z) - kKv4Down;      /* in two steps: 2^e may not be a normal number */
+        const int ea = __float_as_int(A.z) - kPDown, eb = __float_as_int(B.z) - kPDown;      /* in two steps: 2^e may not be a normal number */
         const float a0 = __uint_as_float((uint32_t)(127 + (ea >> 1)) << 23), a1 = __uint_as_float((uint32_t)(127 + ea - (ea >> 1)) << 23);
         const float b0 = __uint_as_float((uint32_t)(127 + (eb >> 1)) << 23), b1 = __uint_as_float((uint32_t)(127 + eb - (eb >> 1)) << 23);
 #pragma unroll 1
@@ -456,7 +460,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
 #pragma unroll 1
             for (int x = 0; x < 2 && n_tiles > 2 * Cfg::kChain + x; x++) {
                 const float2 e = aside_s[x][0][r];
-                const int scale = __float_as_int(e.y) - kKv4Down;
+                const int scale = __float_as_int(e.y) - kPDown;
                 const float f = e.x > -INFINITY ? exp2_fast(e.x - reference) * inv : 0.0f;
                 const float s0 = __uint_as_float((uint32_t)(127 + (scale >> 1)) << 23), s1 = __uint_as_float((uint32_t)(127 + scale - (scale >> 1)) << 23);
                 const float4 *from = p_aside<NB>(a, room_s, x, c) + r;
@@ -575,26 +579,33 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Attn 
         for (int task = warp - 20; task < tasks; task += 3) {
             const int t = task / 4, lw = task % 4, slot = t % Cfg::kSlots, j0 = (first_tile + t) * kPKeys;
             const int real = seen - j0;                            /* tokens of the tile that are seen */
-            int most = 0;
-            bool bad = false;
+            /* the largest and the smallest byte of the tile, two at a time; by themselves where some do not count */
+            uint32_t hi = 0u, lo = 0x00ff00ffu;
 #pragma unroll
-            for (int i = 0; i < NB * 4; i++) {
-                const int byte_i = (int)((all[i / 4] >> (8 * (i % 4))) & 255u);
-                const bool there = lane * 4 + i / NB < real;
-                if (there && byte_i != 255) most = max(most, byte_i);
-                bad |= there && byte_i == 255;
+            for (int i = 0; i < NB; i++) {
+                const uint32_t even = all[i] & 0x00ff00ffu, odd = (all[i] >> 8) & 0x00ff00ffu;
+                hi = __vmaxu2(hi, __vmaxu2(even, odd));
+                lo = __vminu2(lo, __vminu2(even, odd));
             }
-            if (__any_sync(0xffffffffu, bad)) {                    /* blocks that are NaN: the rows that see them; their codes are zeros */
+            int most = (int)max(hi & 0xffffu, hi >> 16);
+            uint32_t least = min(lo & 0xffffu, lo >> 16);
+            if (__any_sync(0xffffffffu, real < kPKeys || most == 255 || least == 0u)) {
+                most = 0;
+                least = 255u;
 #pragma unroll
-                for (int i = 0; i < NB * 4; i++)
-                    if (lane * 4 + i / NB < real && ((all[i / 4] >> (8 * (i % 4))) & 255u) == 255u) atomicMin(&bad_s[i % NB], j0 + lane * 4 + i / NB);
+                for (int i = 0; i < NB * 4; i++) {
+                    const uint32_t byte_i = (all[i / 4] >> (8 * (i % 4))) & 255u;
+                    if (lane * 4 + i / NB >= real) continue;
+                    if (byte_i == 255u) atomicMin(&bad_s[i % NB], j0 + lane * 4 + i / NB);      /* a block that is NaN: the rows that see it; its codes are zeros */
+                    else most = max(most, (int)byte_i);
+                    least = min(least, byte_i - 1u);       /* zeros, which nothing is lost of, come last */
+                }
+                least = least < 254u ? least + 1u : 255u;
+                __syncwarp();
             }
             top = max(top, (int)__reduce_max_sync(0xffffffffu, (unsigned)most));
             if (first_top == 0) first_top = top;
-            uint32_t least = 255u;
-#pragma unroll
-            for (int i = 0; i < NB; i++) least = min(least, (lw * 32 + (i * 32 + lane) / NB < real ? byte[i] : 0u) - 1u);
-            if (kv4_far(least + 1u, top) || top - first_top > kKv4Rise) *(volatile int *)&far_s = 1;
+            if (kv4_far(least, top) || top - first_top > kKv4Rise) *(volatile int *)&far_s = 1;
             if (!at_warp_wait(&v_empty[slot], ((uint32_t)(t / Cfg::kSlots) & 1u) ^ 1u, abort_flag)) { give_up(); break; }
             unsigned char *to = v_s + slot * Cfg::kSlot;
 #pragma unroll
