@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import serve_plain as plain
-from test_gpu_t_serve import TYPES, _fill, _gen, _held, _ints, _randn
+from test_gpu_t_serve import TYPES, _check_logprobs, _fill, _gen, _held, _ints, _randn
 
 pytestmark = pytest.mark.gpu
 
@@ -244,3 +244,20 @@ def test_weights_far_below_the_largest(pkg, rows, heads, dtype):
     limit = count * (2.0 ** -38 if rows == 1 else 2.0 ** -36) / tops + want * (relative + torch.finfo(t).eps / 2) + (2.0 ** -25 if dtype == "f16" else 0.0)      # fp16: its smallest step
     err = (out[0].double() - want).abs()
     assert (err <= limit).all(), float((err / limit).max())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("vocab", [777, 20011, 131072])
+def test_entropy_of_logits_further_apart_than_the_largest_number(pkg, vocab, dtype):
+    """A mask's lowest value beside logits of 1e38, in every place of a row: finite numbers, so finite entropies."""
+    t = TYPES[dtype]
+    x = torch.full((4, vocab), torch.finfo(t).min, device="cuda", dtype=t)
+    x[0, 5] = 1e38
+    x[1, vocab - 3] = 1e38
+    x[2, vocab // 2:] = 1e38
+    x[3, ::2] = 1e38
+    ent, lp = torch.full((4,), 5.0, device="cuda"), torch.full((4,), 5.0, device="cuda")
+    tokens = _ints(5, vocab - 3, vocab - 1, 0)
+    pkg.token_logprobs(x, tokens, lp, ent)
+    many = torch.tensor([1.0, 1.0, vocab - vocab // 2, (vocab + 1) // 2], dtype=torch.float64, device="cuda").log()
+    assert torch.allclose(ent.double(), many, rtol=0.0, atol=1e-4) and torch.allclose(lp.double(), -many, rtol=0.0, atol=1e-4)

@@ -198,8 +198,8 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const LpArgs a)
         }
         raise(top);
         if (first) add(extra);
-        if (low > -INFINITY) {
-            /* two at a time; nothing is infinitely far below the reference */
+        if (low - sums.m > -INFINITY) {
+            /* two at a time; nothing is infinitely far below the reference, finite numbers more than fp32's largest apart neither */
             const uint64_t m2 = vb_f2_pack(-sums.m, -sums.m), log2e = vb_f2_pack(1.44269504f, 1.44269504f);
             uint64_t l2 = 0, w2 = 0;
 #pragma unroll
