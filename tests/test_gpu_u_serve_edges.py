@@ -261,3 +261,25 @@ def test_entropy_of_logits_further_apart_than_the_largest_number(pkg, vocab, dty
     pkg.token_logprobs(x, tokens, lp, ent)
     many = torch.tensor([1.0, 1.0, vocab - vocab // 2, (vocab + 1) // 2], dtype=torch.float64, device="cuda").log()
     assert torch.allclose(ent.double(), many, rtol=0.0, atol=1e-4) and torch.allclose(lp.double(), -many, rtol=0.0, atol=1e-4)
+
+
+@pytest.mark.parametrize("vocab,base", [(20000, -200.0), (9001, -math.inf), (131072, -60.0)])
+def test_logprobs_of_peaked_rows(pkg, vocab, base):
+    """The maximum far into a row, up to 30 above the largest before it, which the same thread has read: log probabilities near 0 to fp32's own
+    step, never above 0, entropies never below."""
+    rows = 600
+    d = torch.linspace(0.01, 30.0, rows, device="cuda")
+    x = torch.full((rows, vocab), base, device="cuda")
+    x[:, 0], x[:, 8192] = 0.0, d
+    lp, ent, top = (torch.full(s, 5.0, device="cuda") for s in ((rows,), (rows,), (rows, 1)))
+    pkg.token_logprobs(x, torch.full((rows,), 8192, dtype=torch.int32, device="cuda"), lp, ent, None, top)
+    # the sum is 1 + e, e below 1: exponentials (2^-21, and 2^-23 of their argument) count with e, the sum and its logarithm with half a step each
+    rest = torch.exp(-d.double()) + (vocab - 2) * torch.exp(base - d.double())
+    limit = 2.0 ** -23 + rest * (2.0 ** -21 + d.double() * 2.0 ** -23)
+    want = -torch.log1p(rest)
+    assert ((lp.double() - want).abs() <= limit).all(), float(((lp.double() - want).abs() / limit).max())
+    assert torch.equal(top[:, 0], lp) and (lp <= 0).all() and (ent >= 0).all()
+    p = torch.exp(-d.double()) / (1 + rest)
+    low = 0.0 if base == -math.inf else (vocab - 2) * torch.exp(base - d.double()) / (1 + rest) * (d.double() - base)
+    want_ent = -want + p * d.double() + low
+    assert ((ent.double() - want_ent).abs() <= limit + (p * d.double() + low) * (2.0 ** -20 + d.double() * 2.0 ** -22)).all()

@@ -156,9 +156,9 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const LpArgs a)
 
     LpSums sums = {-INFINITY, 0.0f, 0.0f};
     bool bad = false;                         /* NaN or +inf */
-    /* a reference that trails the maximum by at most 8 */
+    /* the reference is the maximum: one that trailed by up to 8 left log probabilities near 0 differences of two numbers up to 8 */
     auto raise = [&](float top) {
-        if (!(top <= sums.m + 8.0f)) {
+        if (!(top <= sums.m)) {
             if (top < INFINITY) {
                 lp_rebase(sums, top);
             } else {
