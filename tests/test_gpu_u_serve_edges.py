@@ -283,3 +283,33 @@ def test_logprobs_of_peaked_rows(pkg, vocab, base):
     low = 0.0 if base == -math.inf else (vocab - 2) * torch.exp(base - d.double()) / (1 + rest) * (d.double() - base)
     want_ent = -want + p * d.double() + low
     assert ((ent.double() - want_ent).abs() <= limit + (p * d.double() + low) * (2.0 ** -20 + d.double() * 2.0 ** -22)).all()
+
+
+@pytest.mark.parametrize("capacity", [60, 300])
+def test_eviction_into_a_cache_of_another_size_and_on(pkg, capacity):
+    """Masses go along into the layout of the other cache, whose attention adds to them."""
+    g = _gen(107)
+    s, h, heads, d, cap, keep = 2, 2, 8, 64, 200, 50
+    lengths = [200, 45]
+    k, v, mass = _randn(g, s, cap, h, d), _randn(g, s, cap, h, d), torch.rand(s, h, cap, generator=g, device="cuda")
+    cache, at = _fill(pkg, k, v, cap, lengths)
+    into, new = pkg.KV4Cache(s, h, d, capacity), torch.empty_like(at)
+    new_mass, kept = torch.full((s, h, capacity), -1.0, device="cuda"), torch.empty(s, h, keep, dtype=torch.int32, device="cuda")
+    cache.evict(into, at, new, mass, new_mass, kept, keep=keep, recent=10, first=2)
+    assert new.tolist() == [50, 45]
+    q, nk, nv = _randn(g, s, 1, heads, d), _randn(g, s, 1, h, d), _randn(g, s, 1, h, d)
+    new += 1
+    into.append(nk, nv, new)
+    out, lse, after = torch.empty_like(q), torch.empty(s, 1, heads, device="cuda"), new_mass.clone()
+    into.attention(q, out, new, lse=lse, mass_in=after, mass_out=after)
+    into.check()
+    for i in range(s):
+        n = int(new[i])
+        which = [plain.kept(mass[i, j], lengths[i], keep, 10, 2) for j in range(h)]
+        hk, hv = (torch.stack([torch.cat((plain.rounded(x)[i, which[j], j], plain.rounded(y)[i, :, j])) for j in range(h)]) for x, y in ((k, nk), (v, nv)))
+        was = torch.stack([torch.cat((mass[i, j, which[j]], torch.zeros(1, device="cuda"))) for j in range(h)])
+        want, want_lse, want_mass = plain.attention(q[i], hk, hv, n, 1, d ** -0.5, was)
+        score, result = plain.attention_bounds(q[i], hk, hv, d ** -0.5, torch.float32)
+        assert ((out[i].double() - want).abs() <= result + 2.0 ** -24 * want.abs()).all()
+        assert ((after[i, :, :n].double() - want_mass).abs() <= want_mass * (2 * score + 2.0 ** -20)).all()
+        assert (after[i, :, n:] == -1.0).all()

@@ -226,7 +226,9 @@ class KV4Cache:
         into._open()
         self._spans(lengths, None, (lengths, new_lengths, mass, new_mass, kept))
         ln, nl = _dense(lengths, "lengths", (self.seqs,), "int32"), _dense(new_lengths, "new_lengths", (self.seqs,), "int32")
-        ld = self.capacity if new_mass is not None and tuple(new_mass.shape) == (self.seqs, self.kv_heads, self.capacity) else keep
+        ld = keep
+        if new_mass is not None and new_mass.shape[-1] in (self.capacity, into.capacity):
+            ld = max(keep, new_mass.shape[-1])
         a = _EvictArgs(ln, nl, _dense(mass, "mass", (self.seqs, self.kv_heads, self.capacity), "float32"),
                        _dense(new_mass, "new_mass", (self.seqs, self.kv_heads, ld), "float32"), ld,
                        _dense(kept, "kept", (self.seqs, self.kv_heads, keep), "int32"), keep, recent, first)
@@ -234,8 +236,8 @@ class KV4Cache:
 
     def evict(self, into, lengths, new_lengths, mass, new_mass, kept, keep, recent=0, first=0, stream=0):
         """Sequences of more than `keep` tokens are cut to that many, by mass; what stays goes into the first slots of `into` (a
-        cache like this one, or this one). new_lengths, new_mass ([.., keep] or [.., capacity], or None) and kept [seqs, kv_heads, keep] are
-        results."""
+        cache like this one, or this one). new_lengths, new_mass ([.., keep], or [.., the capacity of either cache], or None) and kept [seqs,
+        kv_heads, keep] are results."""
         self.evict_call(into, lengths, new_lengths, mass, new_mass, kept, keep, recent, first)(stream)
 
     def close(self):
