@@ -54,7 +54,8 @@ typedef struct vb200_kv4 vb200_kv4_t;
 vb200_kv4_t *vb200_kv4_open(int seqs, int kv_heads, int head_dim, int capacity);
 void vb200_kv4_close(vb200_kv4_t *cache);
 size_t vb200_kv4_bytes(const vb200_kv4_t *cache);      /* device memory it holds */
-/* Waits for the device; 0, or the code of a bounded wait inside the attention kernels that ran out (its results are wrong). */
+/* Waits for the device; 0, or the code of a bounded wait inside the attention kernels that ran out since the last time this was asked (results since
+ * then are not to be relied on; later ones are sound again). */
 int vb200_kv4_status(const vb200_kv4_t *cache);
 
 typedef struct {

@@ -313,3 +313,24 @@ def test_eviction_into_a_cache_of_another_size_and_on(pkg, capacity):
         assert ((out[i].double() - want).abs() <= result + 2.0 ** -24 * want.abs()).all()
         assert ((after[i, :, :n].double() - want_mass).abs() <= want_mass * (2 * score + 2.0 ** -20)).all()
         assert (after[i, :, n:] == -1.0).all()
+
+
+def test_status_is_said_once(pkg):
+    """A code where a wait that ran out leaves it (written there by another call; no wait is made to run out): check raises, then the cache goes on."""
+    import ctypes as C
+    cache = pkg.KV4Cache(1, 1, 64, 70)
+    # the handle: planes, five sizes, workspace pointers, of which the status is the fifth; the base of it all behind two sizes
+    planes, status = C.c_void_p.from_address(cache.h).value, C.c_void_p.from_address(cache.h + 56 + 32).value
+    assert planes < status < planes + cache.bytes() and status % 4 == 0
+    x = torch.zeros(1, 100, device="cuda")
+    x[0, 61] = 1.0
+    pkg.token_logprobs(x, None, None, None, pkg.DeviceArray(status, (1, 1), "int32"))
+    with pytest.raises(RuntimeError, match="status 61"):
+        cache.check()
+    cache.check()
+    k, at = _randn(_gen(1), 1, 70, 1, 64), _ints(70)
+    cache.append(k, k, at)
+    out = torch.empty(1, 1, 1, 64, device="cuda")
+    cache.attention(k[:, :1], out, at)
+    cache.check()
+    assert torch.isfinite(out).all()

@@ -469,7 +469,9 @@ int vb200_kv4_status(const vb200_kv4_t *h) {
     int s = 0, now = -1;
     if (cudaGetDevice(&now) == cudaSuccess && now != h->device) cudaSetDevice(h->device);
     /* streams that do not wait for the default one have to be waited for by themselves */
-    const bool read = cudaDeviceSynchronize() == cudaSuccess && cudaMemcpy(&s, h->w.status, sizeof(int), cudaMemcpyDeviceToHost) == cudaSuccess;
+    bool read = cudaDeviceSynchronize() == cudaSuccess && cudaMemcpy(&s, h->w.status, sizeof(int), cudaMemcpyDeviceToHost) == cudaSuccess;
+    /* said once: what is queued from here on begins anew (tickets and rooms are given back where a wait runs out too) */
+    if (read && s) read = cudaMemset(h->w.status, 0, sizeof(int)) == cudaSuccess && cudaDeviceSynchronize() == cudaSuccess;
     if (!read && !serve_launched()) serve_fail("the status could not be read");
     if (now >= 0 && now != h->device) cudaSetDevice(now);
     return read ? s : -1;

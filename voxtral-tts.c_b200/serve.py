@@ -160,7 +160,7 @@ class KV4Cache:
         return self.L.vb200_kv4_bytes(self.h)
 
     def check(self):
-        """Waits for the device; raises where a bounded wait inside a kernel has run out."""
+        """Waits for the device; raises where a bounded wait inside a kernel has run out since the last check."""
         s = self.L.vb200_kv4_status(self.h)
         if s:
             raise RuntimeError(f"a bounded wait ran out on the device (status {s})" if s > 0 else self.L.vb200_serve_error().decode())
