@@ -334,3 +334,114 @@ def test_status_is_said_once(pkg):
     cache.attention(k[:, :1], out, at)
     cache.check()
     assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("dtype,chain", [("f16", 64 * 16), ("bf16", 64 * 8)])
+def test_sums_of_16_bit_portions_over_many_tokens(pkg, dtype, chain):
+    """Weights of a few magnitudes over 32800 tokens of positive values: sums that lose up to a unit towards zero all lose it the same way."""
+    g, t = _gen(109), TYPES[dtype]
+    n, h, d, rows = 32800, 160, 32, 100
+    k, v = torch.zeros(1, n, 1, d, device="cuda", dtype=t), (_randn(g, 1, n, 1, d).abs() + 0.5).to(t)
+    k[..., 0] = torch.randint(-4, 5, (1, n, 1), generator=g, device="cuda").to(t)
+    cache, at = _fill(pkg, k.expand(1, n, h, d), v.expand(1, n, h, d), n, [n])
+    q = torch.zeros(1, rows, h, d, device="cuda", dtype=t)
+    q[..., 0] = 0.3
+    out = torch.full_like(q, 3.0)
+    cache.attention(q, out, at, scale=1.0)
+    cache.check()
+    vv, s = plain.rounded(v)[0, :, 0], plain.rounded(k)[0, :, 0, 0] * q[0, 0, 0, 0].double()
+    p = torch.exp(s)[:, None]
+    want = ((p * vv).cumsum(0)[-rows:] / p.cumsum(0)[-rows:])[:, None]
+    # a score is one product, exact, times a factor and against a reference (4 * 2^-24 of at most 1.2, twice in a weight); an exponential and terms
+    # (2^-20; one term for bf16: 2^-12 each, either way); a sum in tensor memory loses up to 2^-23 with each of its `chain` products, less while it
+    # is small: half of that on the whole; what is put aside is added up to nearest, (n / 128) times 2^-24 at most, and the result rounded
+    terms = 2.0 ** -12 if dtype == "bf16" else 0.0
+    limit = want * (2 * 1.2 * 4 * 2.0 ** -24 + 2.0 ** -20 + terms + chain * 2.0 ** -24 + n / 128 * 2.0 ** -24 + torch.finfo(t).eps / 2)
+    err = (out[0].double() - want).abs()
+    assert (err <= limit).all(), float((err / limit).max())
+
+
+# ---------------------------------------------------------------------------------------------- around the borders between schemes
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("seqs,rows,heads,kv_heads,dim,capacity", [
+    (70, 1, 4, 2, 64, 1500), (33, 2, 8, 1, 128, 3000), (64, 1, 2, 2, 256, 700), (128, 1, 4, 1, 96, 2000),      # a few rows, sequences cut
+    (70, 100, 2, 2, 64, 1500), (40, 120, 3, 3, 32, 2000),                                                       # many rows, cut
+    (40, 1, 32, 8, 64, 500), (300, 1, 1, 1, 32, 400)])                                                          # a CTA a unit
+def test_more_sequences_than_lanes(pkg, seqs, rows, heads, kv_heads, dim, capacity, dtype):
+    """Sequences of very unequal lengths, some of no token, some shorter than their portion: every one has its place among the CTAs."""
+    g, t = _gen(seqs + rows), TYPES[dtype]
+    cuts = [0, 1, 31, 33, capacity, capacity // 7, capacity // 2 + 1, rows // 2, 129, capacity - 1]
+    lengths = [min(capacity, cuts[(7 * i + i // 10) % len(cuts)]) for i in range(seqs)]
+    real = [(rows, rows // 3, 0, rows)[i % 4] if rows > 1 else i % 9 != 4 for i in range(seqs)]
+    real = [int(x) for x in real]
+    k, v = (_randn(g, seqs, capacity, kv_heads, dim, dtype=t) for _ in range(2))
+    cache, at = _fill(pkg, k, v, capacity, lengths)
+    q = _randn(g, seqs, rows, heads, dim, dtype=t)
+    mass = torch.full((seqs, kv_heads, capacity), -1.0, device="cuda")
+    out, lse = torch.full_like(q, 3.0), torch.full((seqs, rows, heads), 4.0, device="cuda")
+    for _ in range(3):                                                   # tickets and rooms are as they were each time
+        cache.attention(q, out, at, rows=_ints(*real), lse=lse, mass_out=mass)
+    cache.check()
+    kk, vv = _held(k, None), _held(v, None)
+    for i in range(seqs):
+        n, m = lengths[i], real[i]
+        assert (out[i, m:] == 3.0).all() and (lse[i, m:] == 4.0).all() and (mass[i, :, n:] == -1.0).all()
+        empty = max(0, m - n)                                            # rows before token 0
+        assert (out[i, :empty] == 0).all() and (lse[i, :empty] == -math.inf).all()
+        if m == 0 or n == 0:
+            assert (mass[i, :, :n] == 0).all()
+            continue
+        _check_by_component(out[i:i + 1, empty:], lse[i:i + 1, empty:], q[i:i + 1, empty:], kk[i, :, :n], vv[i, :, :n], m - empty, dim ** -0.5, t, mass[i:i + 1],
+                            torch.zeros_like(mass[i:i + 1]))
+
+
+@pytest.mark.parametrize("rows,heads,kv_heads,dim", [(1, 8, 2, 128), (16, 8, 2, 64), (5, 4, 1, 192), (150, 4, 2, 96)])
+def test_a_cache_with_far_more_room_than_tokens(pkg, rows, heads, kv_heads, dim):
+    """Rules on sizes see the room, kernels the lengths."""
+    g, seqs, capacity, lengths = _gen(127), 3, 1 << 18, [1000, 150, 1]
+    k, v = (_randn(g, seqs, 1000, kv_heads, dim) for _ in range(2))
+    cache, at = _fill(pkg, k, v, capacity, lengths)
+    q = _randn(g, seqs, rows, heads, dim)
+    out, lse = torch.full_like(q, 3.0), torch.full((seqs, rows, heads), 4.0, device="cuda")
+    mass = torch.full((seqs, kv_heads, capacity), -1.0, device="cuda")
+    cache.attention(q, out, at, lse=lse, mass_out=mass)
+    cache.check()
+    kk, vv = _held(k, None), _held(v, None)
+    for i, n in enumerate(lengths):
+        empty = max(0, rows - n)
+        assert (out[i, :empty] == 0).all() and (mass[i, :, n:] == -1.0).all()
+        _check_by_component(out[i:i + 1, empty:], lse[i:i + 1, empty:], q[i:i + 1, empty:], kk[i, :, :n], vv[i, :, :n], rows - empty, dim ** -0.5, torch.float32, mass[i:i + 1],
+                            torch.zeros_like(mass[i:i + 1]))
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("kind", ["random", "few values", "nan"])
+def test_eviction_of_more_tokens_than_keys_are_held(pkg, kind, in_place):
+    """Sequences on both sides of the 40960 tokens whose keys wait in shared memory."""
+    g = _gen(131)
+    lengths, keep, recent, first, h, d = [70001, 40960, 41003, 12000], 12345, 1000, 4, 2, 32
+    s, capacity = len(lengths), 70001
+    mass = torch.rand(s, h, capacity, generator=g, device="cuda")
+    if kind == "few values":
+        mass = (mass * 5).floor()
+    elif kind == "nan":
+        mass = torch.where(mass < 0.9, math.nan, mass)
+    k = _randn(g, s, capacity, h, d, dtype=torch.bfloat16)
+    cache, at = _fill(pkg, k, -k, capacity, lengths)
+    into = cache if in_place else pkg.KV4Cache(s, h, d, keep)
+    old, held = mass.clone(), plain.rounded(k)
+    new_mass = mass if in_place else torch.full((s, h, keep), -1.0, device="cuda")
+    new, kept = at if in_place else torch.empty_like(at), torch.full((s, h, keep), -7, dtype=torch.int32, device="cuda")
+    cache.evict(into, at, new, mass, new_mass, kept, keep=keep, recent=recent, first=first)
+    assert new.tolist() == [min(n, keep) for n in lengths]
+    gk, gv = (torch.empty(s, keep, h, d, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    into.read(gk, gv, new, rows=new)
+    for i, n in enumerate(lengths):
+        for j in range(h):
+            want = plain.kept(old[i, j], n, keep, recent, first)
+            m = len(want)
+            assert kept[i, j, :m].tolist() == want
+            assert torch.equal(gk[i, :m, j].double(), held[i, want, j]) and torch.equal(gv[i, :m, j].double(), -held[i, want, j])
+            a, b = new_mass[i, j, :m], old[i, j, want]
+            assert torch.equal(torch.nan_to_num(a, nan=-2.0), torch.nan_to_num(b, nan=-2.0))

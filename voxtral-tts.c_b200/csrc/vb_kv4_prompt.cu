@@ -40,7 +40,8 @@ struct PCfg {
      * terms, left results of a portion of 1203 fp32 rows 3.4e-6 off 64 bits (elementary fp32 operations: 1.2e-6). So a warpgroup pair puts what
      * a few tiles have made aside in global memory, added up there rounded to nearest. fp32: three tiles (six: 1.5e-6 off over 2112
      * tokens, where elementary operations are 0.7e-6 and three 0.9e-6). 1203 rows: 205 us, 195 with six, 177 without. Types that round
-     * their results to less: as many as stay far below that (64 * 16 * 2^-24). */
+     * their results to less: 64. That leaves fp16 results over 32800 tokens 2.4e-5 lower than eight tiles do, a twentieth of half a unit (with
+     * eight, 1024 rows over 4096 tokens take 157 us in place of 143); bf16 has half as many products, and a half unit eight times as large. */
     static constexpr int kChain = QT == 2 ? 3 : 64;
     static constexpr int kD64 = (NB + 1) / 2;                                  /* blocks of 64 columns */
     static constexpr int kSlot = kD64 * kPBlock;
