@@ -192,7 +192,7 @@ VB_DEVINL Kv4Place kv4_place(const Kv4Attn &a, int round, int least, int most_sp
  * (kv4_far; scales that have risen by more than kKv4Rise: what a row has of smaller ones fell with them) works its part out again here, in fp32 and
  * with bases of a row's own, so that what a row does not see does not reach it and a large value that weighs little leaves the others as they are. A
  * function of its own: inlined into vb_kv4_attn.cu's loop for a tile at a time it cost every call 5 % (four sequences of 131072 tokens
- * 98 -> 104 us). 40 times slower than the tensor cores. */
+ * 98 -> 104 us). One row over 4208 tokens 14 us -> 126, over 131072 133 -> 4960, 1203 fp32 rows 0.2 ms -> 19. */
 constexpr int kKv4Rise = 64;
 
 /* 2^e, |e| up to 252, as a product of two */
@@ -222,22 +222,28 @@ VB_DEVINL float kv4_plain_query(const T *q, float scale, float *q_s) {
 /* Its score with a row of the cache, by a lane. */
 template <int NB>
 VB_DEVINL float kv4_plain_score(const Kv4Head &c, size_t row, const float *q_s, float mul) {
-    float s = 0.0f;
-#pragma unroll 1
-    for (int b = 0; b < NB; b++) {
-        float sums = 0.0f;
+    float sums[NB], s = 0.0f;
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
+    for (int b = 0; b < NB; b++) sums[b] = 0.0f;
+#pragma unroll 1
+    for (int t = 0; t < 4; t++) {
+        uint32_t w[NB];
+        get_words<NB>(c.k + row * (NB * 16) + t * (NB * 4), w);
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
             uint32_t h[4];
-            kv4_halves(*reinterpret_cast<const uint32_t *>(c.k + row * (NB * 16) + (t * NB + b) * 4), h);
+            kv4_halves(w[b], h);
             const float4 x = *reinterpret_cast<const float4 *>(q_s + 32 * b + 8 * t), y = *reinterpret_cast<const float4 *>(q_s + 32 * b + 8 * t + 4);
             const float2 k0 = kv4_f2(h[0]), k1 = kv4_f2(h[1]), k2 = kv4_f2(h[2]), k3 = kv4_f2(h[3]);
-            sums = fmaf(k0.x, x.x, fmaf(k0.y, x.y, fmaf(k1.x, x.z, fmaf(k1.y, x.w, sums))));
-            sums = fmaf(k2.x, y.x, fmaf(k2.y, y.y, fmaf(k3.x, y.z, fmaf(k3.y, y.w, sums))));
+            sums[b] = fmaf(k0.x, x.x, fmaf(k0.y, x.y, fmaf(k1.x, x.z, fmaf(k1.y, x.w, sums[b]))));
+            sums[b] = fmaf(k2.x, y.x, fmaf(k2.y, y.y, fmaf(k3.x, y.z, fmaf(k3.y, y.w, sums[b]))));
         }
+    }
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
         const uint32_t byte = c.ks[row * NB + b];
         const float2 f = kv4_power((int)min(byte, 252u) - 127);
-        s += byte == 255u ? __uint_as_float(0x7fffffffu) : sums == 0.0f ? 0.0f : sums * f.x * mul * f.y;
+        s += byte == 255u ? __uint_as_float(0x7fffffffu) : sums[b] == 0.0f ? 0.0f : sums[b] * f.x * mul * f.y;
     }
     return s;
 }
@@ -276,15 +282,23 @@ __device__ __noinline__ float2 kv4_plain_row(Kv4Head c, const T *q, float scale,
             const int rise = max(0, (int)__reduce_max_sync(0xffffffffu, byte == 255u ? 0u : byte) - base[i]);
             base[i] += rise;
             o[i] *= rise > 126 ? 0.0f : fall * __uint_as_float((uint32_t)(127 - rise) << 23);
-            const int u = 8 * i + (lane >> 2), at = kv4_value_half(u, NB) * 2 + ((lane & 3) >> 1), shift = (lane & 1) * 4;
+            /* a lane's own token: its weight times its scale against the base */
+            const float2 f = kv4_power(byte == 255u ? 0 : min((int)byte - base[i], 0));
+            const float weight = p * f.x * f.y;
+            const uint8_t *values = c.v + (size_t)j0 * (NB * 16) + kv4_value_half(8 * i + (lane >> 2), NB) * 2 + ((lane & 3) >> 1);
             float part = 0.0f;
-#pragma unroll 4
-            for (int x = 0; x < n; x++) {
-                const uint32_t there = __shfl_sync(0xffffffffu, byte, x), w = (c.v[(size_t)(j0 + x) * (NB * 16) + at] >> shift) & 15u;
-                uint32_t h[4];
-                kv4_halves(w, h);
-                const float2 f = kv4_power(there == 255u ? 0 : (int)there - base[i]);
-                part += kv4_f2(h[0]).x * (__shfl_sync(0xffffffffu, p, x) * f.x) * f.y;
+#pragma unroll 2
+            for (int x0 = 0; x0 < n; x0 += 4) {        /* what is behind the last token weighs nothing; four conversions of a word together (one byte
+                                                        * of a word alone, in an unrolled loop, came out as zeros) */
+                uint32_t four = 0, h[4];
+#pragma unroll
+                for (int x = 0; x < 4; x++) four |= (uint32_t)values[(size_t)min(x0 + x, n - 1) * (NB * 16)] << (8 * x);
+                kv4_halves(four, h);
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    const float2 pair = kv4_f2(h[x]);
+                    part = fmaf(lane & 1 ? pair.y : pair.x, __shfl_sync(0xffffffffu, weight, x0 + x), part);
+                }
             }
             o[i] += part;
         }

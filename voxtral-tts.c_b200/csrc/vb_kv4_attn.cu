@@ -17,9 +17,11 @@
  * fill: no barrier between warps until the end. A sequence's tokens are split over CTAs where there are few of them; the CTA that
  * comes last at a ticket joins the parts.
  *
- * Bound by the issue of instructions where tokens are many: a warp's tile is 605 of them, of which 283, conversions and integer operations, go to a pipe of
- * half the rate. One row of 32 heads over four sequences of 131072 tokens and 8 KV heads of 128, bf16: 102 us, 4.2 TB/s of codes and scales, 64 % of
- * a plain copy's rate. Over 301 tokens 6.6 us: latencies that wait for one another.
+ * Where tokens are many nothing is saturated: a warp's tile is 607 instructions, of which 283, conversions and integer operations, go to a pipe of half
+ * the rate; that pipe is 58 % busy, the issue slots 61, the tensor pipe 26, memory at 63 % of a plain copy's rate. Four warps a scheduler with
+ * chains of dependent instructions leave the rest. One row of 32 heads over four sequences of 65536 to 131072 tokens and 8 KV heads of 128, bf16:
+ * 104 us, 4.1 TB/s of codes and scales. Over 301 tokens 7.2 us: latencies that wait for one another. Several groups of eight pairs of a KV head
+ * each decode its keys and values again: 32 rows and heads of it over 65536 tokens 70 us.
  */
 #include <algorithm>
 #include <limits.h>
@@ -619,7 +621,7 @@ __global__ void __launch_bounds__(kAThreads, NB <= 4 ? 2 : 1) kv4_attn_kernel(co
 /* mass_out: the scores again, now that the rows' sums are known (in the attention kernel only the last CTA of a split sequence knows them,
  * and keeping scores takes memory for every row). A CTA has up to four tiles of tokens a warp, whose keys stay in shared memory while the
  * (row, head) pairs come by, 64 at a time, a column of eight by each warp. A token's weights are summed in one order: no atomics. One row of 32
- * heads over eight sequences of 4608 tokens and 8 KV heads of 128, bf16: 13 us beside the attention's 14, latencies for the most part. */
+ * heads over eight sequences of 4608 tokens and 8 KV heads of 128, bf16: 17 us by itself where the attention takes 20, 32 both, whose ends overlap. */
 constexpr int kMTiles = 4, kMMostPairs = 64;      /* of a KV head: more take the kernel of vb_kv4_prompt.cu, heads up to 128 */
 
 template <int NB, class T>
@@ -775,7 +777,8 @@ int attn_launch(const Kv4Attn &args, const vb200_kv4_attention_t &v, const Kv4Wo
      * and to join (fp32, heads of 128; the other types and sizes cross at about the same place). Measured, here and there in us: 8 heads, 1024
      * tokens, 256 and 512 pairs each 17, 30 and 29, 39; 8192 tokens, 64 and 128 pairs 31, 52 and 33, 44; 65536 tokens, 32 and 64 pairs 86, 176 and
      * 107, 110; 64 heads, 1024 tokens, 64 and 128 pairs 31, 52 and 35, 46. The tokens are the cache's room for them: lengths are not
-     * known here. */
+     * known here, and those figures are of full caches. Where most of the room is empty the other kernel is taken from fewer tokens on than it
+     * pays for: its 17 us. */
     const long long pairs = (long long)a.max_rows * a.group, room = (long long)a.c.capacity * a.c.kv_heads * a.c.seqs;
     if (NB <= 4 && (double)room * (double)((pairs + 7) / 8 - 6 * ((pairs + 127) / 128)) > 550e3) {
         if (kv4_prompt(a, q, out, work.sm_count, st)) return -1;

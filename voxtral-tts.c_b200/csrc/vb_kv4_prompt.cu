@@ -13,8 +13,10 @@
  * warpgroups take alternate tiles with a reference, sums and an accumulator each, merged at the end, so that the tensor pipe works on
  * one tile while the other is in its softmax. A thread has half of a row's columns: with a whole row a thread, and half as many
  * threads, 1203 rows took 206 us in place of 178 (before sums were put aside).
- * Bound by the chain of scores, softmax, results and scores again that a pair goes through: 4100 to 4300 clocks a tile, where the tensor pipe's
- * part of it is 2048 with two terms each. 1203 fp32 rows of 32 heads of 128 over 4208 tokens: 205 us, 347 TFLOP/s (twice that as executed).
+ * Nothing is saturated: a tile of 128 x 128 takes an SM 5800 clocks with two terms each, of which the tensor pipe needs 2048 (36 %; 26 % for bf16); issue
+ * slots are 50 % busy, the integer pipe 41. The roles wait for one another: scores for keys, the softmax for scores and for the other half of its
+ * rows, results for all of a tile's weights. 1203 fp32 rows of 32 heads of 128 over 4208 tokens: 204 us, 349 TFLOP/s (twice that as executed);
+ * 1024 bf16 rows over 4096 tokens 123 us.
  *
  * Warps: 0-7, 8-15 softmax, 16-19 keys, 20-22 values, 23 issues the MMAs. All waits are bounded.
  */
@@ -733,7 +735,8 @@ __global__ void __launch_bounds__(kJThreads) kv4_join_kernel(const Kv4Attn a, co
  *   S^T [128 tokens x 128 pairs] = K Q^T,  mass_j = sum over pairs of exp(S_j - lse), a thread per token
  * A CTA has 128 tokens of a KV head, whose keys stay in shared memory; the pairs that see them come by 128 at a time: eight warps bring
  * queries to FP16, one issues the products, two warpgroups take alternate tiles of pairs. A token's weights are summed in one order.
- * 1024 rows of 32 heads over 4096 tokens: 840 us on warp-level MMAs (vb_kv4_attn.cu), whose keys are decoded again for every eight pairs. */
+ * 1024 rows of 32 heads over 4096 tokens, 256 CTAs on 148 SMs: 197 us by itself (840 on warp-level MMAs, whose keys are decoded again for every
+ * eight pairs), issue slots 58 % busy, the tensor pipe 9: every CTA brings the queries to FP16 again, and eight warps take the exponentials. */
 constexpr int kWMmaWarp = 16, kWThreads = 32 * (kWMmaWarp + 1), kWSlots = 2, kWStatus = 63, kWRing = 4;
 constexpr uint32_t kWTmem = 256;
 
