@@ -73,7 +73,7 @@ int vb200_kv4_read(const vb200_kv4_t *cache, const vb200_kv4_rows_t *a, void *st
  *   out = sum_j softmax_j(scale q . k_j) v_j   over tokens j <= the row's own
  * heads is a multiple of kv_heads; query head h reads KV head h / (heads / kv_heads). A row that sees no key is zeros with
  * lse = -inf. Scores, weights and sums are fp32, keys and values exact: what a row does not see does not reach it, whatever its size. (Where the
- * scales of a head's blocks lie more than 2^36 apart, blocks of zeros aside, the call is exact on a path of its own that takes tens of times as long.) Queries and
+ * scales of a head's blocks lie more than 2^36 apart, blocks of zeros aside, the call is exact on a path of its own that takes ten to a hundred times as long.) Queries and
  * weights go through the tensor cores as two FP16 terms each for fp32 (22 bits), queries exactly otherwise, and weights as two terms for fp16,
  * one (11 bits) for bf16: a query's values below 2^-39 (fp32) or 2^-29 of its largest, and weights below 2^-36 of a row's largest, round
  * to steps of about that. Keys of 2^100 and more may pass fp32 on the way to a score.

@@ -836,6 +836,7 @@ __global__ void __launch_bounds__(kWThreads, 1) kv4_mass_many_kernel(const Kv4At
         /* ---- sums: warpgroup w takes tiles w, w + 2, ... of pairs, a thread token tok0 + r ---- */
         const int w = warp >> 2, r = tid & 127, j = tok0 + r;
         const uint32_t tS = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(w * kPRows);
+        pdl_wait();                                                        /* bounded waits begin when the kernels before are done, however long they take */
         const float up = key_up[r >> 4];
         const uint64_t up2 = vb_f2_pack(up, up);
         uint64_t sums[2] = {0, 0};
@@ -943,6 +944,7 @@ __global__ void __launch_bounds__(kWThreads, 1) kv4_mass_many_kernel(const Kv4At
         /* ---- MMA issuer ---- */
         const uint32_t idesc = p_idesc(kPRows, false);
         const AtDesc k_desc(umma_desc_k_sw128(k_s)), q_desc(umma_desc_k_sw128(q_s));
+        pdl_wait();
         bool ok = vb_mbar_wait(&k_full, 0u, abort_flag);
         for (int t = 0; t < n_tiles && ok; t++) {
             const int slot = t % kWSlots, w = t & 1;
